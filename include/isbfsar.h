@@ -438,6 +438,105 @@ int isb_dist_info(const isb_dist* d, int32_t* rank, int32_t* world);
  * host-side helper isbfsar_amd/dist.py does). d_send may alias its own slot of d_recv. */
 int isb_dist_all_gather(isb_dist* d, const void* d_send, void* d_recv, size_t bytes_per_rank, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Layer operators: a cross-attention layer over feature sequences -- e.g. isb_ar_infer's embeddings of the query windows
+ * against the frames of a support set (isb_ar_get_support_features) -- with the gradients that fine-tuning needs. The
+ * tuple attention of isb_ar_* is the reference's own operator (a softmax over the QUERY tuples); these are its
+ * conventional neighbours and use no handle.
+ *   - every call is asynchronous on `stream`, allocates nothing and keeps nothing: the caller owns outputs and the
+ *     workspace (isb_*_workspace gives its bytes for the same arguments; 0 bytes: NULL is fine). Two calls that may run at
+ *     the same time need a workspace each. All calls may be captured into a hipGraph.
+ *   - `device` is the ordinal that owns every pointer; the calling thread's current device is left as it was.
+ *   - sums, softmax statistics and norms are 32-bit; 16-bit results are rounded to nearest, fp16 ones saturate at +-65504.
+ *   - the results of a call do not depend on the schedule (no atomics): the same call gives the same bits.
+ *   - strides are in elements; the innermost dimension is contiguous. 16-bit tensors: pointers on 16 bytes, strides and
+ *     inner sizes multiples of 8 (else ISB_ERR_INVALID). Outputs must not overlap inputs.
+ * ---------------------------------------------------------------------------------------------- */
+#define ISB_T_F32 0
+#define ISB_T_F16 1
+#define ISB_T_BF16 2
+
+/* Cross attention: query rows attend to an encoder's states of another length.
+ *   q [B,Lq,Hq,D], k, v [Bk,Lk,Hk,D], 16-bit; D a multiple of 8, at most 128; Hq a multiple of Hk (grouped heads: head h reads
+ *   state head h / (Hq / Hk)); B a multiple of Bk (sample b reads the states of b / (B / Bk): Bk = 1 is one support set that
+ *   every window shares).
+ *   State j of states b takes part iff j < kv_len[b] (NULL: Lk; values outside 0 .. Lk are clamped) and key_mask[b, j] != 0
+ *   (NULL: all). What masked states hold is never used (NaN and infinities included).
+ *   out [B,Lq,Hq,D] = softmax(scale q k^T) v, lse [B,Hq,Lq] f32 = log sum exp(scale q k^T) (natural logarithm). A row with no
+ *   state gets out = 0, lse = -inf and passes no gradient. scale > 0.
+ * Backward: dout [B,Lq,Hq,D], out and lse of the forward call -> dq, dk, dv (contiguous, shapes of q, k, v; gradients of
+ * shared heads and shared states are summed in 32 bits; masked states get zeros). */
+typedef struct isb_xattn_args {
+    int32_t device, dtype;                              /* ISB_T_F16 or ISB_T_BF16 */
+    int32_t B, Bk, Lq, Lk, Hq, Hk, D;
+    float scale;
+    const void *q, *k, *v;
+    int64_t q_stride[3], k_stride[3], v_stride[3];      /* of sample, position, head */
+    const int32_t* kv_len;                              /* [Bk] or NULL */
+    const uint8_t* key_mask;                            /* [Bk,Lk] or NULL */
+    int64_t mask_stride;                                /* of sample */
+    void* out;                                          /* contiguous; forward: written, backward: read */
+    float* lse;
+    const void* dout;                                   /* backward only, from here */
+    int64_t dout_stride[3];
+    void *dq, *dk, *dv;
+} isb_xattn_args;
+int isb_xattn_workspace(const isb_xattn_args* a, int32_t backward, size_t* bytes);
+int isb_xattn_forward(const isb_xattn_args* a, void* d_workspace, size_t bytes, void* stream);
+int isb_xattn_backward(const isb_xattn_args* a, void* d_workspace, size_t bytes, void* stream);
+
+/* Gated feed-forward block: y = (act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd, 16-bit, torch Linear weights.
+ *   x [M,D] (row stride x_stride), w_gate, w_up [F,D], w_down [D,F], b_gate, b_up [F], b_down [D] or NULL, y [M,D].
+ *   D, F multiples of 8; M >= 1.
+ *   For the backward pass forward also fills pre_gate, pre_up [M,F] f32 (both or neither) and hidden [M,F] (needed with them,
+ *   else NULL: it lives in the workspace).
+ * Backward: dy [M,D] (row stride dy_stride) and those three -> dx [M,D], dw_gate_up [2F,D] (the gate's rows first), dw_down [D,F],
+ * db_gate, db_up (both or neither) [F], db_down [D] or NULL. */
+#define ISB_ACT_SILU 0
+#define ISB_ACT_GELU 1       /* the exact one: x Phi(x) */
+#define ISB_ACT_RELU 2
+#define ISB_ACT_SIGMOID 3
+typedef struct isb_ffn_args {
+    int32_t device, dtype;                              /* ISB_T_F16 or ISB_T_BF16 */
+    int32_t M, D, F, act;
+    int64_t x_stride, dy_stride;
+    const void *x, *w_gate, *w_up, *w_down, *b_gate, *b_up, *b_down;
+    void* y;
+    float *pre_gate, *pre_up;
+    void* hidden;
+    const void* dy;                                     /* backward only, from here */
+    void *dx, *dw_gate_up, *dw_down, *db_gate, *db_up, *db_down;
+} isb_ffn_args;
+int isb_ffn_workspace(const isb_ffn_args* a, int32_t backward, size_t* bytes);
+int isb_ffn_forward(const isb_ffn_args* a, void* d_workspace, size_t bytes, void* stream);
+int isb_ffn_backward(const isb_ffn_args* a, void* d_workspace, size_t bytes, void* stream);
+
+/* The norms around a block with its gate and residual scale: r = x + scale * gate * N_post(y), z = N_pre(r).
+ *   x, y, r, z [B,L,D] contiguous, f32, fp16 or bf16; gate [B,D] of the same type or NULL (1); scale [D] f32 or NULL (1).
+ *   post, pre: ISB_NORM_*; weights and biases [D] f32 or NULL (1 and 0; a bias or weight needs its norm, an RMS norm takes no bias).
+ *   y NULL: r is x (not written), only z = N_pre(x). pre NONE: z is not written. D at most 8192.
+ *   z is the norm of r before r is rounded. stats [B,L,4] f32 or NULL: what the backward pass needs of the row's statistics.
+ * Backward: dr (NULL: zeros) and dz (with a pre norm), x, y, stats -> dx, dy (unless y is NULL), dgate (gate's type, if gate),
+ * dscale, dpost_weight, dpost_bias, dpre_weight, dpre_bias f32 (each may be NULL). */
+#define ISB_NORM_NONE 0
+#define ISB_NORM_LAYER 1
+#define ISB_NORM_RMS 2
+typedef struct isb_norm_args {
+    int32_t device, dtype;
+    int32_t B, L, D, post, pre;
+    float eps;
+    const void *x, *y, *gate;
+    const float *scale, *post_weight, *post_bias, *pre_weight, *pre_bias;
+    void *r, *z;
+    float* stats;                                       /* forward: written if not NULL; backward: read */
+    const void *dr, *dz;                                /* backward only, from here */
+    void *dx, *dy, *dgate;
+    float *dscale, *dpost_weight, *dpost_bias, *dpre_weight, *dpre_bias;
+} isb_norm_args;
+int isb_norm_workspace(const isb_norm_args* a, size_t* bytes);                        /* of the backward pass; forward needs none */
+int isb_norm_forward(const isb_norm_args* a, void* stream);
+int isb_norm_backward(const isb_norm_args* a, void* d_workspace, size_t bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -40,6 +40,29 @@ class isb_det_cfg(C.Structure):
     _fields_ = [("width", C.c_int32), ("height", C.c_int32), ("device", C.c_int32), ("max_batch", C.c_int32)]
 
 
+_I3 = C.c_int64 * 3
+
+
+class isb_xattn_args(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("device", "dtype", "B", "Bk", "Lq", "Lk", "Hq", "Hk", "D")] + [("scale", C.c_float)]
+                + [(n, C.c_void_p) for n in ("q", "k", "v")] + [(n, _I3) for n in ("q_stride", "k_stride", "v_stride")]
+                + [("kv_len", C.c_void_p), ("key_mask", C.c_void_p), ("mask_stride", C.c_int64), ("out", C.c_void_p), ("lse", C.c_void_p),
+                   ("dout", C.c_void_p), ("dout_stride", _I3)] + [(n, C.c_void_p) for n in ("dq", "dk", "dv")])
+
+
+class isb_ffn_args(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("device", "dtype", "M", "D", "F", "act")] + [("x_stride", C.c_int64), ("dy_stride", C.c_int64)]
+                + [(n, C.c_void_p) for n in ("x", "w_gate", "w_up", "w_down", "b_gate", "b_up", "b_down", "y", "pre_gate", "pre_up", "hidden",
+                                             "dy", "dx", "dw_gate_up", "dw_down", "db_gate", "db_up", "db_down")])
+
+
+class isb_norm_args(C.Structure):
+    _fields_ = ([(n, C.c_int32) for n in ("device", "dtype", "B", "L", "D", "post", "pre")] + [("eps", C.c_float)]
+                + [(n, C.c_void_p) for n in ("x", "y", "gate", "scale", "post_weight", "post_bias", "pre_weight", "pre_bias", "r", "z", "stats",
+                                             "dr", "dz", "dx", "dy", "dgate", "dscale", "dpost_weight", "dpost_bias", "dpre_weight",
+                                             "dpre_bias")])
+
+
 _lib = None
 
 # name -> (restype, argtypes); every symbol include/isbfsar.h declares
@@ -106,6 +129,15 @@ SIGNATURES = {
     "isb_det_forward": (C.c_int, [_P, _P, C.c_int32, _P, _P, _P]),
     "isb_det_forward_host": (C.c_int, [_P, _P, C.c_int32, _P, _P]),
     "isb_det_debug_host": (C.c_int, [_P, _P, C.c_int32, _P, _P, _P, _P]),
+    "isb_xattn_workspace": (C.c_int, [C.POINTER(isb_xattn_args), C.c_int32, C.POINTER(C.c_size_t)]),
+    "isb_xattn_forward": (C.c_int, [C.POINTER(isb_xattn_args), _P, C.c_size_t, _P]),
+    "isb_xattn_backward": (C.c_int, [C.POINTER(isb_xattn_args), _P, C.c_size_t, _P]),
+    "isb_ffn_workspace": (C.c_int, [C.POINTER(isb_ffn_args), C.c_int32, C.POINTER(C.c_size_t)]),
+    "isb_ffn_forward": (C.c_int, [C.POINTER(isb_ffn_args), _P, C.c_size_t, _P]),
+    "isb_ffn_backward": (C.c_int, [C.POINTER(isb_ffn_args), _P, C.c_size_t, _P]),
+    "isb_norm_workspace": (C.c_int, [C.POINTER(isb_norm_args), C.POINTER(C.c_size_t)]),
+    "isb_norm_forward": (C.c_int, [C.POINTER(isb_norm_args), _P]),
+    "isb_norm_backward": (C.c_int, [C.POINTER(isb_norm_args), _P, C.c_size_t, _P]),
     "isb_debug_fused_mb": (C.c_int, [C.c_int32] + [_P] * 8 + [C.c_int32] * 7 + [_P, C.POINTER(C.c_float)]),
     "isb_debug_hpe_mb8_stamps": (C.c_int, [_P, C.c_int32, _P]),
     "isb_debug_ar_stamps": (C.c_int, [_P, C.c_int32, _P]),

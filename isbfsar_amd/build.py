@@ -42,7 +42,16 @@ SOURCES = [
     "dist_api.cpp",
     "rgb_kernels.hip",
     "rgb_api.cpp",
+    # the stand-alone layer operators
+    "xattn_kernels.hip",
+    "ffn_kernels.hip",
+    "norm_kernels.hip",
+    "blocks_api.cpp",
 ]
+# compiled without packed f32 instructions: some of their forms have given wrong results on gfx950 parts now and then (the units before
+# these are written for them and are held by their bit-identity tests)
+NO_PACKED_F32 = {"xattn_kernels.hip", "ffn_kernels.hip", "norm_kernels.hip"}
+NO_PACKED_F32_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # optional units appear as they are written
 for _extra in ("conv_mb8.hip", "conv_mb16.hip"):
     if os.path.exists(os.path.join(CSRC, _extra)):
@@ -249,7 +258,7 @@ def build(force: bool = False, verbose: bool = True) -> str:
         o = os.path.join(OBJ, src.replace(".", "_") + ".o")
         objs.append(o)
         if force or not os.path.exists(o) or os.path.getmtime(o) < max(os.path.getmtime(s), hdr_m):
-            cmd = [hipcc, *FLAGS, "-x", "hip", "-c", s, "-o", o]
+            cmd = [hipcc, *FLAGS, *(NO_PACKED_F32_FLAGS if src in NO_PACKED_F32 else []), "-x", "hip", "-c", s, "-o", o]
             jobs.append(cmd)
 
     def run(cmd):
@@ -258,8 +267,10 @@ def build(force: bool = False, verbose: bool = True) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError("hipcc failed:\n" + " ".join(cmd) + "\n" + r.stdout + r.stderr)
-        if verbose and r.stderr.strip():
-            print(r.stderr.strip())
+        # (hipcc's host pass does not know the feature of NO_PACKED_F32_FLAGS and says so)
+        err = "\n".join(ln for ln in r.stderr.splitlines() if "'-packed-fp32-ops' is not a recognized feature" not in ln).strip()
+        if verbose and err:
+            print(err)
 
     if jobs:
         with ThreadPoolExecutor(max_workers=min(int(os.environ.get("ISB_BUILD_JOBS", "8")), len(jobs))) as ex:

@@ -1,0 +1,499 @@
+// Gated feed-forward block y = (act(x Wg^T + bg) o (x Wu^T + bu)) Wd^T + bd and its gradients.
+//
+// One matrix-product kernel carries all of it: C[m][n] = sum_k A(m, k) B(n, k), 16-bit operands, f32 sums, each operand either with k
+// contiguous (layout 0: LDS rows are m or n, fragments are 16-byte reads) or with m / n contiguous (layout 1: LDS rows are k, fragments
+// are transposing reads), so no operand is ever transposed in memory. The product is formed transposed (accumulator rows = n), so a lane
+// owns four neighbouring n of one m. The epilogues:
+//   GATE  both projections at once: every wave holds the gate and the up columns of the same features; h = act(g) o u (g, u kept in f32
+//         for the backward pass: rounded to 16 bits they would put a second rounding into every gradient);
+//   OUT   + bias, rounded (or the f32 partial sums of a split of k);
+//   DH    dh stays in registers: dG = dh o u o act'(g) and dU = dh o act(g) are what is stored.
+#include <algorithm>
+#include <cmath>
+
+#include "blocks.h"
+
+namespace isb {
+namespace {
+
+enum { EPI_GATE = 0, EPI_OUT = 1, EPI_DH = 2 };
+enum { FFN_SILU = 0, FFN_GELU = 1, FFN_RELU = 2, FFN_SIGMOID = 3 };
+constexpr int BK = 64;
+
+struct MmArgs {
+    const uint16_t *A, *B, *B2;          // B2: GATE: the up weights; else the operand of the second k segment
+    int64_t lda, ldb;
+    int M, N, K;                         // GATE: N = 2 F (32 gate columns, 32 up columns, ...)
+    int nseg;                            // segments of K (A continues at column K)
+    int splits, kt_per_split;
+    const uint16_t *bias, *bias2;
+    uint16_t* C;
+    int64_t ldc;
+    float *g, *u;                        // GATE: saved (or null); DH: read
+    float* part;                         // OUT with splits > 1: [split][M][N]
+    int F, act;
+    int tiles_m, tiles_n, n_items;
+};
+
+__device__ __forceinline__ float sigmoid_(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-LOG2E * x)); }
+__device__ __forceinline__ float act_of(int act, float g) {
+    if (act == FFN_SILU) return g * sigmoid_(g);
+    if (act == FFN_GELU) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
+    if (act == FFN_RELU) return fmaxf(g, 0.f);
+    return sigmoid_(g);
+}
+__device__ __forceinline__ void act_and_slope(int act, float g, float& f, float& d) {
+    if (act == FFN_GELU) {
+        const float phi = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+        f = g * phi;
+        d = phi + g * 0.3989422804014327f * __builtin_amdgcn_exp2f(-0.5f * LOG2E * g * g);
+    } else if (act == FFN_RELU) {
+        f = fmaxf(g, 0.f);
+        d = g > 0.f ? 1.f : 0.f;
+    } else {
+        const float s = sigmoid_(g), c = 1.0f - s;
+        f = act == FFN_SILU ? g * s : s;
+        d = act == FFN_SILU ? s * __builtin_fmaf(g, c, 1.0f) : s * c;
+    }
+}
+
+// requests of one operand tile. Layout 0: ROWS rows of 64 k (row valid below `rows`); layout 1: 64 k rows of ROWS values (value valid
+// below `rows`). PAIR: rows 0-31 gate, 32-63 up, ... of ROWS / 2 features.
+template <int LAY, int ROWS, int NW, bool PAIR>
+struct OpLoad {
+    static constexpr int PIECES = ROWS * BK * 2 / 1024 / NW, W = LAY == 0 ? BK : ROWS;
+    static_assert(PIECES >= 1 && PIECES * NW * 1024 == ROWS * BK * 2 && W >= 64, "whole pieces per wave, rows that tile_xor covers");
+    uint32_t voff[PIECES];
+    int kk[PIECES];                                   // first k (layout 0) or k (layout 1) of the lane's chunk
+    __device__ __forceinline__ void init(int wave, int lane, int64_t ld, int rows) {
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            const int byte = (wave * PIECES + j) * 1024 + lane * 16, r = byte / (W * 2);
+            const int c = ((byte % (W * 2)) >> 4) ^ tile_xor<W>(r);
+            if constexpr (LAY == 0) {
+                const int row = PAIR ? (r >> 6) * 32 + (r & 31) : r;
+                kk[j] = 8 * c;
+                voff[j] = row < rows ? (uint32_t)(row * (int)ld * 2 + c * 16) : DMA_NONE;
+            } else {
+                kk[j] = r;
+                voff[j] = 8 * c < rows ? (uint32_t)(r * (int)ld * 2 + c * 16) : DMA_NONE;
+            }
+        }
+    }
+    __device__ __forceinline__ void request(const uint16_t* base, const uint16_t* base2, int k_left, uint32_t lds, int wave) const {
+        const i32x4 d = dma_desc(base);
+        const i32x4 d2 = PAIR ? dma_desc(base2) : d;
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            const uint32_t v = kk[j] < k_left ? voff[j] : DMA_NONE;
+            const bool up = PAIR && (((wave * PIECES + j) >> 2) & 1);      // a piece is 8 rows: 4 pieces per 32-row group (wave-uniform)
+            dma16_desc(up ? d2 : d, v, lds + (wave * PIECES + j) * 1024);
+        }
+    }
+};
+
+// ROWS x 64 operand tile in LDS -> fragment of 32 rows (columns) at r0, k-step ks
+template <int LAY, int ROWS>
+__device__ __forceinline__ uint4 op_frag(const unsigned char* t, int r0, int ks, int lane) {
+    if constexpr (LAY == 0) return frag_rows<BK>(t, r0, ks, lane);
+    else return frag_cols<ROWS, 8, 4>(t, 16 * ks, r0, lane);
+}
+
+template <bool F16, int BM, int BN, int NWM, int NWN, int LA, int LB, int EPI>
+__global__ __launch_bounds__(NWM * NWN * 64, NWM * NWN >= 8 ? 2 : 1) void ffn_mm_kernel(MmArgs p) {
+    T16<F16>::enter();
+    constexpr int NW = NWM * NWN, WM = BM / NWM, WN = BN / NWN, IM = WM / 32, IN = WN / 32;
+    constexpr bool PAIR = EPI == EPI_GATE;
+    static_assert(!PAIR || (IN % 2 == 0 && LB == 0), "a wave owns gate and up columns of the same features");
+    constexpr int ABYTES = BM * BK * 2, STAGE = ABYTES + BN * BK * 2;
+    const int item = xcd_item(blockIdx.x, p.n_items);
+    if (item >= p.n_items) return;
+    // the m tiles of one n tile run side by side on an XCD: they read the same weights
+    const int tm = item % p.tiles_m, tn = item / p.tiles_m % p.tiles_n, split = item / p.tiles_m / p.tiles_n;
+    const int m0 = tm * BM, n0 = tn * BN;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
+    const int wm = wave % NWM, wn = wave / NWM;
+
+    const int kts = (p.K + BK - 1) / BK, total = kts * p.nseg;
+    const int t0 = split * p.kt_per_split, t1 = min(total, t0 + p.kt_per_split);
+    OpLoad<LA, BM, NW, false> la;
+    OpLoad<LB, BN, NW, PAIR> lb;
+    la.init(wave, lane, p.lda, p.M - m0);
+    lb.init(wave, lane, p.ldb, PAIR ? p.F - n0 / 2 : p.N - n0);
+    const uint32_t lds0 = lds_addr_of(conv_lds_dyn);
+    auto request = [&](int t, int buf) {
+        const int seg = t >= kts, kt = t - seg * kts;
+        const int k0 = kt * BK;
+        const uint16_t* a = LA == 0 ? p.A + (int64_t)m0 * p.lda + seg * p.K + k0 : p.A + (int64_t)k0 * p.lda + m0;
+        const uint16_t* bb = PAIR || !seg ? p.B : p.B2;
+        const int64_t off = LB == 0 ? (int64_t)(PAIR ? n0 / 2 : n0) * p.ldb + k0 : (int64_t)k0 * p.ldb + n0;
+        la.request(a, nullptr, p.K - k0, lds0 + buf * STAGE, wave);
+        lb.request(bb + off, PAIR ? p.B2 + off : nullptr, p.K - k0, lds0 + buf * STAGE + ABYTES, wave);
+    };
+    f32x16 acc[IM][IN];
+#pragma unroll
+    for (int i = 0; i < IM; ++i)
+#pragma unroll
+        for (int j = 0; j < IN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    if (t0 < t1) request(t0, 0);
+    for (int t = t0; t < t1; ++t) {
+        wait_all_and_meet();
+        const int buf = (t - t0) & 1;
+        if (t + 1 < t1) request(t + 1, buf ^ 1);
+        const unsigned char* at = conv_lds_dyn + buf * STAGE;
+        const unsigned char* bt = at + ABYTES;
+#pragma unroll
+        for (int ks = 0; ks < BK / 16; ++ks) {
+            uint4 a[IM], b[IN];
+#pragma unroll
+            for (int i = 0; i < IM; ++i) a[i] = op_frag<LA, BM>(at, wm * WM + 32 * i, ks, lane);
+#pragma unroll
+            for (int j = 0; j < IN; ++j) b[j] = op_frag<LB, BN>(bt, wn * WN + 32 * j, ks, lane);
+#pragma unroll
+            for (int j = 0; j < IN; ++j)
+#pragma unroll
+                for (int i = 0; i < IM; ++i) acc[i][j] = T16<F16>::mfma32(b[j], a[i], acc[i][j]);
+        }
+    }
+
+#pragma unroll
+    for (int i = 0; i < IM; ++i) {
+        const int m = m0 + wm * WM + 32 * i + (lane & 31);
+        if (m >= p.M) continue;
+        if constexpr (EPI == EPI_GATE) {
+#pragma unroll
+            for (int j = 0; j < IN; j += 2)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int f = (n0 + wn * WN + 32 * j) / 2 + 8 * q + 4 * h;
+                    if (f >= p.F) continue;
+                    float g[4], u[4], o[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) { g[e] = acc[i][j][4 * q + e]; u[e] = acc[i][j + 1][4 * q + e]; }
+                    if (p.bias) {
+                        const uint2 w = *reinterpret_cast<const uint2*>(p.bias + f);
+                        g[0] += T16<F16>::lo(w.x); g[1] += T16<F16>::hi(w.x); g[2] += T16<F16>::lo(w.y); g[3] += T16<F16>::hi(w.y);
+                    }
+                    if (p.bias2) {
+                        const uint2 w = *reinterpret_cast<const uint2*>(p.bias2 + f);
+                        u[0] += T16<F16>::lo(w.x); u[1] += T16<F16>::hi(w.x); u[2] += T16<F16>::lo(w.y); u[3] += T16<F16>::hi(w.y);
+                    }
+                    const int64_t at = (int64_t)m * p.F + f;
+                    if (p.g) {
+                        *reinterpret_cast<float4*>(p.g + at) = make_float4(g[0], g[1], g[2], g[3]);
+                        *reinterpret_cast<float4*>(p.u + at) = make_float4(u[0], u[1], u[2], u[3]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = act_of(p.act, g[e]) * u[e];
+                    *reinterpret_cast<uint2*>(p.C + at) = make_uint2(T16<F16>::pack2(o[0], o[1]), T16<F16>::pack2(o[2], o[3]));
+                }
+        } else {
+#pragma unroll
+            for (int j = 0; j < IN; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int n = n0 + wn * WN + 32 * j + 8 * q + 4 * h;
+                    if (n >= p.N) continue;
+                    float o[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = acc[i][j][4 * q + e];
+                    if constexpr (EPI == EPI_DH) {
+                        const int64_t at = (int64_t)m * p.F + n;
+                        const float4 g4 = *reinterpret_cast<const float4*>(p.g + at), u4 = *reinterpret_cast<const float4*>(p.u + at);
+                        const float g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
+                        float dg[4], du[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float f, s;
+                            act_and_slope(p.act, g[e], f, s);
+                            dg[e] = o[e] * u[e] * s;
+                            du[e] = o[e] * f;
+                        }
+                        uint16_t* c = p.C + (int64_t)m * p.ldc + n;
+                        *reinterpret_cast<uint2*>(c) = make_uint2(T16<F16>::pack2(dg[0], dg[1]), T16<F16>::pack2(dg[2], dg[3]));
+                        *reinterpret_cast<uint2*>(c + p.F) = make_uint2(T16<F16>::pack2(du[0], du[1]), T16<F16>::pack2(du[2], du[3]));
+                    } else if (p.splits > 1) {
+                        *reinterpret_cast<float4*>(p.part + ((int64_t)split * p.M + m) * p.N + n) = make_float4(o[0], o[1], o[2], o[3]);
+                    } else {
+                        if (p.bias) {
+                            const uint2 w = *reinterpret_cast<const uint2*>(p.bias + n);
+                            o[0] += T16<F16>::lo(w.x); o[1] += T16<F16>::hi(w.x); o[2] += T16<F16>::lo(w.y); o[3] += T16<F16>::hi(w.y);
+                        }
+                        *reinterpret_cast<uint2*>(p.C + (int64_t)m * p.ldc + n) = make_uint2(T16<F16>::pack2(o[0], o[1]), T16<F16>::pack2(o[2], o[3]));
+                    }
+                }
+        }
+    }
+}
+
+// sums of the splits of k in their order, + bias; four values per thread
+template <bool F16>
+__global__ __launch_bounds__(256) void ffn_sum_kernel(const float* part, int splits, int64_t n4, int N, const uint16_t* bias, uint16_t* C) {
+    T16<F16>::enter();
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n4) return;
+    float o[4] = {};
+    for (int s = 0; s < splits; ++s) {
+        const float4 v = *reinterpret_cast<const float4*>(part + (s * n4 + i) * 4);
+        o[0] += v.x; o[1] += v.y; o[2] += v.z; o[3] += v.w;
+    }
+    if (bias) {
+        const uint2 w = *reinterpret_cast<const uint2*>(bias + i * 4 % N);
+        o[0] += T16<F16>::lo(w.x); o[1] += T16<F16>::hi(w.x); o[2] += T16<F16>::lo(w.y); o[3] += T16<F16>::hi(w.y);
+    }
+    *reinterpret_cast<uint2*>(C + i * 4) = make_uint2(T16<F16>::pack2(o[0], o[1]), T16<F16>::pack2(o[2], o[3]));
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------------
+// At most TOKENS rows: the weights are the work, each read once in whole 1-KiB rows of a wave; dot products on the vector ALU.
+// PER waves share a weight row (pair of rows); their sums are added in wave order.
+// ------------------------------------------------------------------------------------------------------------------------------------
+constexpr int TOKENS = 4;
+template <bool F16, int MT, int PER, bool GATE>
+__global__ __launch_bounds__(256) void ffn_token_kernel(MmArgs p) {
+    T16<F16>::enter();
+    __shared__ float sums[4][2 * MT];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int n = blockIdx.x * (4 / PER) + wave / PER, part = wave % PER;
+    const int N = GATE ? p.F : p.N;
+    float s[GATE ? 2 : 1][MT] = {};
+    if (n < N) {
+        const uint16_t* w0 = p.B + (int64_t)n * p.ldb;
+        const uint16_t* w1 = GATE ? p.B2 + (int64_t)n * p.ldb : nullptr;
+#pragma unroll 4
+        for (int k = (part * 64 + lane) * 8; k < p.K; k += PER * 512) {
+            const uint4 a = *reinterpret_cast<const uint4*>(w0 + k);
+            uint4 b = a;
+            if constexpr (GATE) b = *reinterpret_cast<const uint4*>(w1 + k);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const uint4 x = *reinterpret_cast<const uint4*>(p.A + (int64_t)min(t, p.M - 1) * p.lda + k);
+                s[0][t] = T16<F16>::dot2(x.w, a.w, T16<F16>::dot2(x.z, a.z, T16<F16>::dot2(x.y, a.y, T16<F16>::dot2(x.x, a.x, s[0][t]))));
+                if constexpr (GATE) s[1][t] = T16<F16>::dot2(x.w, b.w, T16<F16>::dot2(x.z, b.z, T16<F16>::dot2(x.y, b.y, T16<F16>::dot2(x.x, b.x, s[1][t]))));
+            }
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < (GATE ? 2 : 1); ++j)
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int o = 32; o; o >>= 1) s[j][t] += __shfl_xor(s[j][t], o);
+    if constexpr (PER > 1) {
+        if (lane == 0) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) { sums[wave][t] = s[0][t]; if constexpr (GATE) sums[wave][MT + t] = s[1][t]; }
+        }
+        __syncthreads();
+        if (part != 0) return;
+#pragma unroll
+        for (int w = 1; w < PER; ++w)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) { s[0][t] += sums[wave + w][t]; if constexpr (GATE) s[1][t] += sums[wave + w][MT + t]; }
+    }
+    if (n >= N || lane != 0) return;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        if (t >= p.M) break;
+        float o = s[0][t] + (p.bias ? T16<F16>::to_f32(p.bias[n]) : 0.f);
+        if constexpr (GATE) {
+            const float u = s[1][t] + (p.bias2 ? T16<F16>::to_f32(p.bias2[n]) : 0.f);
+            if (p.g) { p.g[(int64_t)t * p.F + n] = o; p.u[(int64_t)t * p.F + n] = u; }
+            o = act_of(p.act, o) * u;
+        }
+        p.C[(int64_t)t * (GATE ? p.F : p.ldc) + n] = T16<F16>::from_f32(o);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------------
+// column sums (bias gradients): 256 columns x ROWS rows per workgroup, partial sums joined in order
+// ------------------------------------------------------------------------------------------------------------------------------------
+template <bool F16>
+__global__ __launch_bounds__(256) void ffn_colsum_kernel(const uint16_t* x, int64_t ld, int M, int N, int rows, float* part) {
+    __shared__ float red[8][256];
+    const int c = threadIdx.x & 31, rl = threadIdx.x >> 5, n = blockIdx.x * 256 + 8 * c, m0 = blockIdx.y * rows, m1 = min(M, m0 + rows);
+    float s[8] = {};
+    if (n < N)
+        for (int m = m0 + rl; m < m1; m += 8) {
+            const uint4 v = *reinterpret_cast<const uint4*>(x + m * ld + n);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { s[2 * e] += T16<F16>::lo(w[e]); s[2 * e + 1] += T16<F16>::hi(w[e]); }
+        }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) red[rl][8 * c + e] = s[e];
+    __syncthreads();
+    const int col = blockIdx.x * 256 + threadIdx.x;
+    if (col >= N) return;
+    float t = 0.f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) t += red[r][threadIdx.x];
+    part[(int64_t)blockIdx.y * N + col] = t;
+}
+template <bool F16>
+__global__ __launch_bounds__(256) void ffn_colsum_join_kernel(const float* part, int parts, int N, uint16_t* out, uint16_t* out2, int n1) {
+    T16<F16>::enter();
+    const int n = blockIdx.x * 256 + threadIdx.x;
+    if (n >= N) return;
+    float t = 0.f;
+    for (int i = 0; i < parts; ++i) t += part[(int64_t)i * N + n];
+    uint16_t* o = n < n1 ? out + n : out2 + (n - n1);
+    *o = T16<F16>::from_f32(t);
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------------------------------------------
+// tile shapes: thin (at most 64 rows: weights are read once or twice), mid (two workgroups per CU), big (one workgroup of eight waves;
+// half the LDS and L2 bytes per product, but only where its tiles fill the 256 CUs)
+enum { TILE_THIN, TILE_MID, TILE_BIG };
+int tile_of(int la, int M, int N) {
+    if (M <= 64 && la == 0) return TILE_THIN;         // (layout 1 keeps whole 128-byte rows of m in LDS: no thin form)
+    return (int64_t)cdiv(M, 256) * cdiv(N, 256) >= 200 ? TILE_BIG : TILE_MID;
+}
+int splits_of(int la, int M, int N, int kts) {            // k splits of an OUT product whose tiles do not fill the chip
+    const int t = tile_of(la, M, N), bm = t == TILE_THIN ? 32 : t == TILE_MID ? 128 : 256, bn = t == TILE_BIG ? 256 : 128;
+    const int64_t tiles = (int64_t)cdiv(M, bm) * cdiv(N, bn);
+    const int64_t want = t == TILE_BIG ? 1 : (512 + tiles - 1) / tiles;
+    int s = (int)std::min<int64_t>(want, std::max(1, kts / 4));
+    s = std::max(1, std::min(s, 16));
+    return cdiv(kts, cdiv(kts, s));
+}
+
+template <bool F16, int BM, int BN, int NWM, int NWN, int LA, int LB, int EPI>
+int mm_run(MmArgs p, const char* name, hipStream_t st) {
+    constexpr size_t lds = 2 * (BM + BN) * BK * 2;
+    p.tiles_m = cdiv(p.M, BM);
+    p.tiles_n = cdiv(p.N, BN);
+    const int64_t n = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+    ISB_REQUIRE(n < (1ll << 30), ISB_ERR_INVALID, "gated feed-forward: %lld workgroups are more than one launch holds", (long long)n);
+    p.n_items = (int)n;
+    p.kt_per_split = cdiv(cdiv(p.K, BK) * p.nseg, p.splits);
+    static DevMax attr;
+    if (attr.below((int)lds)) {
+        ISB_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(ffn_mm_kernel<F16, BM, BN, NWM, NWN, LA, LB, EPI>),
+                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        attr.set((int)lds);
+    }
+    ffn_mm_kernel<F16, BM, BN, NWM, NWN, LA, LB, EPI><<<(unsigned)(8 * ((n + 7) / 8)), NWM * NWN * 64, lds, st>>>(p);
+    ISB_LAUNCHED(name, st);
+    return ISB_OK;
+}
+template <bool F16, int LA, int LB, int EPI>
+int mm(const MmArgs& p, const char* name, hipStream_t st) {
+    const int t = tile_of(LA, p.M, p.N);
+    if constexpr (LA == 0)
+        if (t == TILE_THIN) return mm_run<F16, 32, 128, 1, 2, LA, LB, EPI>(p, name, st);
+    if (t == TILE_MID) return mm_run<F16, 128, 128, 2, 2, LA, LB, EPI>(p, name, st);
+    return mm_run<F16, 256, 256, 2, 4, LA, LB, EPI>(p, name, st);
+}
+// C = A B^T (+ bias), k split where the tiles alone leave CUs idle
+template <bool F16, int LA, int LB>
+int mm_out(MmArgs p, float* part, const char* name, hipStream_t st) {
+    p.splits = splits_of(LA, p.M, p.N, cdiv(p.K, BK) * p.nseg);
+    p.part = part;
+    ISB_TRY((mm<F16, LA, LB, EPI_OUT>(p, name, st)));
+    if (p.splits > 1) {
+        const int64_t n4 = (int64_t)p.M * p.N / 4;
+        ffn_sum_kernel<F16><<<(unsigned)((n4 + 255) / 256), 256, 0, st>>>(part, p.splits, n4, p.N, p.bias, p.C);
+        ISB_LAUNCHED("ffn_sum", st);
+    }
+    return ISB_OK;
+}
+size_t part_bytes(int la, int M, int N, int kts) {
+    const int s = splits_of(la, M, N, kts);
+    return s > 1 ? (size_t)s * M * N * 4 : 0;
+}
+constexpr int COLSUM_ROWS = 128;
+
+template <bool F16, int MT, bool GATE>
+int token(const MmArgs& p, hipStream_t st) {
+    const int n = GATE ? p.F : p.N;
+    if (p.K > 2048) ffn_token_kernel<F16, MT, 4, GATE><<<n, 256, 0, st>>>(p);
+    else ffn_token_kernel<F16, MT, 1, GATE><<<cdiv(n, 4), 256, 0, st>>>(p);
+    ISB_LAUNCHED("ffn_token", st);
+    return ISB_OK;
+}
+
+template <bool F16>
+int fwd(const FfnArgs& a, unsigned char* ws, hipStream_t st) {
+    uint16_t* h = a.h;
+    if (!h) {
+        h = reinterpret_cast<uint16_t*>(ws);
+        ws += ((size_t)a.M * a.F * 2 + 255) / 256 * 256;
+    }
+    MmArgs g{};
+    g.A = a.x; g.B = a.wg; g.B2 = a.wu; g.lda = a.x_s; g.ldb = a.D;
+    g.M = a.M; g.N = 64 * cdiv(a.F, 32); g.K = a.D; g.F = a.F; g.nseg = 1; g.splits = 1;
+    g.bias = a.bg; g.bias2 = a.bu; g.C = h; g.g = a.g; g.u = a.u; g.act = a.act;
+    MmArgs d{};
+    d.A = h; d.B = a.wd; d.lda = a.F; d.ldb = a.F;
+    d.M = a.M; d.N = a.D; d.K = a.F; d.nseg = 1; d.splits = 1;
+    d.bias = a.bd; d.C = a.y; d.ldc = a.D;
+    if (a.M <= TOKENS) {
+        if (a.M == 1) {
+            ISB_TRY((token<F16, 1, true>(g, st)));
+            return token<F16, 1, false>(d, st);
+        }
+        ISB_TRY((token<F16, TOKENS, true>(g, st)));
+        return token<F16, TOKENS, false>(d, st);
+    }
+    ISB_TRY((mm<F16, 0, 0, EPI_GATE>(g, "ffn gate + up", st)));
+    return mm_out<F16, 0, 0>(d, reinterpret_cast<float*>(ws), "ffn down", st);
+}
+
+template <bool F16>
+int bwd(const FfnArgs& a, unsigned char* ws, hipStream_t st) {
+    uint16_t* dgu = reinterpret_cast<uint16_t*>(ws);
+    float* part = reinterpret_cast<float*>(ws + ((size_t)a.M * 2 * a.F * 2 + 255) / 256 * 256);
+    MmArgs p{};
+    // dG, dU from dh = dy Wd
+    p.A = a.dy; p.B = a.wd; p.lda = a.dy_s; p.ldb = a.F; p.M = a.M; p.N = a.F; p.K = a.D; p.nseg = 1; p.splits = 1;
+    p.g = a.g; p.u = a.u; p.F = a.F; p.act = a.act; p.C = dgu; p.ldc = 2 * (int64_t)a.F;
+    ISB_TRY((mm<F16, 0, 1, EPI_DH>(p, "ffn dh", st)));
+    // dx = dG Wg + dU Wu
+    p = MmArgs{};
+    p.A = dgu; p.B = a.wg; p.B2 = a.wu; p.lda = 2 * (int64_t)a.F; p.ldb = a.D; p.M = a.M; p.N = a.D; p.K = a.F; p.nseg = 2;
+    p.C = a.dx; p.ldc = a.D;
+    ISB_TRY((mm_out<F16, 0, 1>(p, part, "ffn dx", st)));
+    // [dWg; dWu] = [dG | dU]^T x
+    p = MmArgs{};
+    p.A = dgu; p.B = a.x; p.lda = 2 * (int64_t)a.F; p.ldb = a.x_s; p.M = 2 * a.F; p.N = a.D; p.K = a.M; p.nseg = 1;
+    p.C = a.dwgu; p.ldc = a.D;
+    ISB_TRY((mm_out<F16, 1, 1>(p, part, "ffn dW gate, up", st)));
+    // dWd = dy^T h
+    p = MmArgs{};
+    p.A = a.dy; p.B = a.h; p.lda = a.dy_s; p.ldb = a.F; p.M = a.D; p.N = a.F; p.K = a.M; p.nseg = 1;
+    p.C = a.dwd; p.ldc = a.F;
+    ISB_TRY((mm_out<F16, 1, 1>(p, part, "ffn dW down", st)));
+    auto colsum = [&](const uint16_t* x, int64_t ld, int N, uint16_t* o, uint16_t* o2, int n1) -> int {
+        const int parts = cdiv(a.M, COLSUM_ROWS);
+        ffn_colsum_kernel<F16><<<dim3(cdiv(N, 256), parts), 256, 0, st>>>(x, ld, a.M, N, COLSUM_ROWS, part);
+        ISB_LAUNCHED("ffn_colsum", st);
+        ffn_colsum_join_kernel<F16><<<cdiv(N, 256), 256, 0, st>>>(part, parts, N, o, o2, n1);
+        ISB_LAUNCHED("ffn_colsum_join", st);
+        return ISB_OK;
+    };
+    if (a.dbg) ISB_TRY(colsum(dgu, 2 * (int64_t)a.F, 2 * a.F, a.dbg, a.dbu, a.F));
+    if (a.dbd) ISB_TRY(colsum(a.dy, a.dy_s, a.D, a.dbd, a.dbd, a.D));
+    return ISB_OK;
+}
+}  // namespace
+
+size_t ffn_workspace(const FfnArgs& a, bool backward) {
+    const size_t M = a.M, F = a.F;
+    if (!backward) {
+        const size_t h = a.h ? 0 : (M * F * 2 + 255) / 256 * 256;
+        return h + (a.M <= TOKENS ? 0 : part_bytes(0, a.M, a.D, cdiv(a.F, BK)));
+    }
+    size_t part = std::max(part_bytes(0, a.M, a.D, 2 * cdiv(a.F, BK)),
+                           std::max(part_bytes(1, 2 * a.F, a.D, cdiv(a.M, BK)), part_bytes(1, a.D, a.F, cdiv(a.M, BK))));
+    if (a.dbg || a.dbd) part = std::max(part, (size_t)cdiv(a.M, COLSUM_ROWS) * std::max(2 * F, (size_t)a.D) * 4);
+    return (M * 2 * F * 2 + 255) / 256 * 256 + part;
+}
+int launch_ffn_fwd(const FfnArgs& a, bool f16, unsigned char* ws, hipStream_t st) { return f16 ? fwd<true>(a, ws, st) : fwd<false>(a, ws, st); }
+int launch_ffn_bwd(const FfnArgs& a, bool f16, unsigned char* ws, hipStream_t st) { return f16 ? bwd<true>(a, ws, st) : bwd<false>(a, ws, st); }
+
+}  // namespace isb

@@ -1,0 +1,340 @@
+// The norms around a block in one pass: r = x + scale o gate o N_post(y) (what leaves the block before) and z = N_pre(r) (what enters the
+// next one), with the gradients of everything. N: LayerNorm, RMS norm or none. Both are bound by HBM: every row is read once, kept in
+// registers and written once; r is normalised before it is rounded.
+//
+// A workgroup of ceil(D / 512) waves owns a row, eight neighbouring columns per lane. Backward, it walks the rows of one sample with four
+// column sums in registers -- dR, dR o y^, dz, dz o r^ -- from which all parameter gradients follow, because gate and scale do not vary
+// within a sample:
+//   dgate_b = scale o sum t,  dscale = sum_b gate_b o sum t,  t = w o (dR o y^) + bias o dR;   dw_post = sum_b f_b o sum (dR o y^),
+//   dbias_post = sum_b f_b o sum dR  (f_b = scale o gate_b);   dw_pre = sum dz o r^,  dbias_pre = sum dz.
+// The partial sums of the workgroups are added in their order: the results do not depend on the schedule.
+#include <algorithm>
+
+#include "blocks.h"
+
+namespace isb {
+namespace {
+
+enum { NONE = 0, LAYER = 1, RMS = 2 };
+
+// eight neighbouring values at p + c (c < D; VEC: D % 8 == 0 and 16-byte rows), zeros past D
+template <int DT, bool VEC>
+__device__ __forceinline__ void load8(const void* base, int64_t row, int c, int D, float (&v)[8]) {
+    if constexpr (DT == 0) {
+        const float* p = static_cast<const float*>(base) + row * D + c;
+        if constexpr (VEC) {
+            const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = c + i < D ? p[i] : 0.f;
+        }
+    } else {
+        using T = T16<DT == 1>;
+        const uint16_t* p = static_cast<const uint16_t*>(base) + row * D + c;
+        if constexpr (VEC) {
+            const uint4 a = *reinterpret_cast<const uint4*>(p);
+            v[0] = T::lo(a.x); v[1] = T::hi(a.x); v[2] = T::lo(a.y); v[3] = T::hi(a.y); v[4] = T::lo(a.z); v[5] = T::hi(a.z); v[6] = T::lo(a.w); v[7] = T::hi(a.w);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = c + i < D ? T::to_f32(p[i]) : 0.f;
+        }
+    }
+}
+template <int DT, bool VEC>
+__device__ __forceinline__ void store8(void* base, int64_t row, int c, int D, const float (&v)[8]) {
+    if constexpr (DT == 0) {
+        float* p = static_cast<float*>(base) + row * D + c;
+        if constexpr (VEC) {
+            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) if (c + i < D) p[i] = v[i];
+        }
+    } else {
+        using T = T16<DT == 1>;
+        uint16_t* p = static_cast<uint16_t*>(base) + row * D + c;
+        if constexpr (VEC) {
+            *reinterpret_cast<uint4*>(p) = make_uint4(T::pack2(v[0], v[1]), T::pack2(v[2], v[3]), T::pack2(v[4], v[5]), T::pack2(v[6], v[7]));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) if (c + i < D) p[i] = T::from_f32(v[i]);
+        }
+    }
+}
+__device__ __forceinline__ void param8(const float* p, int c, int D, float fill, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = p && c + i < D ? p[c + i] : fill;
+}
+
+// sums of one or two values over the workgroup, the same bits in every lane. `slot` alternates between two halves of the buffer, so one
+// barrier per call is enough.
+struct Meet {
+    float* buf;
+    int waves, wave, lane, slot;
+    __device__ __forceinline__ void sum2(float& a, float& b) {
+#pragma unroll
+        for (int o = 32; o; o >>= 1) { a += __shfl_xor(a, o); b += __shfl_xor(b, o); }
+        if (waves == 1) return;
+        float* s = buf + slot * 32;
+        slot ^= 1;
+        if (lane == 0) { s[2 * wave] = a; s[2 * wave + 1] = b; }
+        __syncthreads();
+        a = b = 0.f;
+        for (int w = 0; w < waves; ++w) { a += s[2 * w]; b += s[2 * w + 1]; }
+    }
+    __device__ __forceinline__ float sum(float a) { float b = 0.f; sum2(a, b); return a; }
+};
+
+// v -> (v - mean) inv for `kind`; columns past D stay zero
+__device__ __forceinline__ void normalise(int kind, float (&v)[8], int c, int D, float eps, float& mean, float& inv, Meet& meet) {
+    mean = 0.f;
+    inv = 1.f;
+    if (kind == NONE) return;
+    if (kind == LAYER) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += v[i];
+        mean = meet.sum(s) / (float)D;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < D ? v[i] - mean : 0.f;
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s = __builtin_fmaf(v[i], v[i], s);
+    inv = 1.0f / sqrtf(meet.sum(s) / (float)D + eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= inv;
+}
+
+template <int DT, bool VEC>
+__global__ __launch_bounds__(1024) void norm_fwd_kernel(NormArgs a, int64_t rows) {
+    if constexpr (DT == 1) T16<true>::enter();
+    __shared__ float buf[64];
+    const int tid = threadIdx.x, c = tid * 8, D = a.D;
+    const bool in = c < D;
+    Meet meet{buf, (int)blockDim.x >> 6, tid >> 6, tid & 63, 0};
+    float qw[8], qb[8], pw[8], pb[8], sc[8];
+    param8(a.post_w, c, D, 1.f, qw);
+    param8(a.post_b, c, D, 0.f, qb);
+    param8(a.pre_w, c, D, 1.f, pw);
+    param8(a.pre_b, c, D, 0.f, pb);
+    param8(a.scale, c, D, 1.f, sc);
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        float r[8] = {}, y[8] = {}, g[8];
+        if (in) load8<DT, VEC>(a.x, row, c, D, r);
+        float my = 0.f, iy = 1.f, mr = 0.f, ir = 1.f;
+        if (a.y) {
+            if (in) load8<DT, VEC>(a.y, row, c, D, y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) g[i] = 1.f;
+            if (a.gate && in) load8<DT, VEC>(a.gate, row / a.L, c, D, g);
+            normalise(a.post, y, c, D, a.eps, my, iy, meet);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r[i] = c + i < D ? __builtin_fmaf(sc[i] * g[i], __builtin_fmaf(y[i], qw[i], qb[i]), r[i]) : 0.f;
+            if (in) store8<DT, VEC>(a.r, row, c, D, r);
+        }
+        if (a.pre) {
+            normalise(a.pre, r, c, D, a.eps, mr, ir, meet);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r[i] = __builtin_fmaf(r[i], pw[i], pb[i]);
+            if (in) store8<DT, VEC>(a.z, row, c, D, r);
+        }
+        if (a.stats && tid == 0) *reinterpret_cast<float4*>(a.stats + 4 * row) = make_float4(my, iy, mr, ir);
+    }
+}
+
+template <int DT, bool VEC>
+__global__ __launch_bounds__(1024) void norm_bwd_kernel(NormArgs a) {
+    if constexpr (DT == 1) T16<true>::enter();
+    __shared__ float buf[64];
+    const int tid = threadIdx.x, c = tid * 8, D = a.D;
+    const bool in = c < D;
+    Meet meet{buf, (int)blockDim.x >> 6, tid >> 6, tid & 63, 0};
+    const int b = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+    const int l0 = chunk * a.rows_per_chunk, l1 = min(a.L, l0 + a.rows_per_chunk);
+    float qw[8], qb[8], pw[8], f[8], g[8];
+    param8(a.post_w, c, D, 1.f, qw);
+    param8(a.post_b, c, D, 0.f, qb);
+    param8(a.pre_w, c, D, 1.f, pw);
+    param8(a.scale, c, D, 1.f, f);
+    if (a.gate && in) {
+        load8<DT, VEC>(a.gate, b, c, D, g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] *= g[i];
+    }
+    const float rD = 1.0f / (float)D;
+    float s0[8] = {}, s1[8] = {}, s2[8] = {}, s3[8] = {};
+    for (int l = l0; l < l1; ++l) {
+        const int64_t row = (int64_t)b * a.L + l;
+        float x[8] = {}, y[8] = {}, dr[8] = {}, dz[8] = {};
+        if (in) {
+            load8<DT, VEC>(a.x, row, c, D, x);
+            if (a.y) load8<DT, VEC>(a.y, row, c, D, y);
+            if (a.dr) load8<DT, VEC>(a.dr, row, c, D, dr);
+            if (a.pre) load8<DT, VEC>(a.dz, row, c, D, dz);
+        }
+        const float4 st = *reinterpret_cast<const float4*>(a.stats + 4 * row);
+        if (a.y) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                y[i] = c + i < D ? (y[i] - st.x) * st.y : 0.f;
+                x[i] = __builtin_fmaf(f[i], __builtin_fmaf(y[i], qw[i], qb[i]), x[i]);
+            }
+        }
+        if (a.pre) {
+            float t0 = 0.f, t1 = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[i] = c + i < D ? (x[i] - st.z) * st.w : 0.f;                 // r^
+                const float d = dz[i] * pw[i];
+                t0 += d;
+                t1 = __builtin_fmaf(d, x[i], t1);
+                s2[i] += dz[i];
+                s3[i] = __builtin_fmaf(dz[i], x[i], s3[i]);
+            }
+            meet.sum2(t0, t1);
+            const float m0 = a.pre == LAYER ? t0 * rD : 0.f, m1 = t1 * rD;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dr[i] = c + i < D ? __builtin_fmaf(st.w, dz[i] * pw[i] - m0 - x[i] * m1, dr[i]) : 0.f;
+        }
+        if (in) store8<DT, VEC>(a.dx, row, c, D, dr);
+        if (a.y) {
+            float d[8], t0 = 0.f, t1 = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                s0[i] += dr[i];
+                s1[i] = __builtin_fmaf(dr[i], y[i], s1[i]);
+                d[i] = c + i < D ? dr[i] * f[i] * qw[i] : 0.f;
+                t0 += d[i];
+                t1 = __builtin_fmaf(d[i], y[i], t1);
+            }
+            if (a.post) {
+                meet.sum2(t0, t1);
+                const float m0 = a.post == LAYER ? t0 * rD : 0.f, m1 = t1 * rD;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) d[i] = st.y * (d[i] - m0 - y[i] * m1);
+            }
+            if (in) store8<DT, VEC>(a.dy, row, c, D, d);
+        }
+    }
+    float* p = a.part + (int64_t)blockIdx.x * 4 * D;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (c + i < D) { p[c + i] = s0[i]; p[D + c + i] = s1[i]; p[2 * D + c + i] = s2[i]; p[3 * D + c + i] = s3[i]; }
+}
+
+// sums over the chunks of a sample: part [B, chunks, 4, D] -> joint [B, 4, D], and the sample's dgate. 64 columns x 4 chunk lanes.
+template <int DT>
+__global__ __launch_bounds__(256) void norm_join_kernel(NormArgs a, float* joint) {
+    if constexpr (DT == 1) T16<true>::enter();
+    __shared__ float red[4][4][64];
+    const int cl = threadIdx.x & 63, kl = threadIdx.x >> 6, b = blockIdx.y, c = blockIdx.x * 64 + cl, D = a.D;
+    float s[4] = {};
+    if (c < D)
+        for (int k = kl; k < a.chunks; k += 4) {
+            const float* p = a.part + ((int64_t)b * a.chunks + k) * 4 * D + c;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j] += p[j * D];
+        }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) red[kl][j][cl] = s[j];
+    __syncthreads();
+    if (c >= D) return;
+    joint[((int64_t)b * 4 + kl) * D + c] = red[0][kl][cl] + red[1][kl][cl] + red[2][kl][cl] + red[3][kl][cl];
+    if (kl == 0 && a.dgate) {
+        float t[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) t[j] = red[0][j][cl] + red[1][j][cl] + red[2][j][cl] + red[3][j][cl];
+        const float w = a.post_w ? a.post_w[c] : 1.f, q = a.post_b ? a.post_b[c] : 0.f;
+        const float v = (a.scale ? a.scale[c] : 1.f) * (w * t[1] + q * t[0]);
+        if constexpr (DT == 0) static_cast<float*>(a.dgate)[(int64_t)b * D + c] = v;
+        else static_cast<uint16_t*>(a.dgate)[(int64_t)b * D + c] = T16<DT == 1>::from_f32(v);
+    }
+}
+// joint [B, 4, D] -> the parameters' gradients: 32 columns x 8 sample lanes
+template <int DT>
+__global__ __launch_bounds__(256) void norm_params_kernel(NormArgs a, const float* joint) {
+    __shared__ float red[8][5][32];
+    const int cl = threadIdx.x & 31, bl = threadIdx.x >> 5, c = blockIdx.x * 32 + cl, D = a.D;
+    float s[5] = {};                         // dscale, dw_post, dbias_post, dw_pre, dbias_pre
+    if (c < D) {
+        const float w = a.post_w ? a.post_w[c] : 1.f, q = a.post_b ? a.post_b[c] : 0.f, sc = a.scale ? a.scale[c] : 1.f;
+        for (int b = bl; b < a.B; b += 8) {
+            const float* p = joint + (int64_t)b * 4 * D + c;
+            float g = 1.f;
+            if (a.gate) {
+                if constexpr (DT == 0) g = static_cast<const float*>(a.gate)[(int64_t)b * D + c];
+                else g = T16<DT == 1>::to_f32(static_cast<const uint16_t*>(a.gate)[(int64_t)b * D + c]);
+            }
+            const float a0 = p[0], a1 = p[D];
+            s[0] += g * (w * a1 + q * a0);
+            s[1] += sc * g * a1;
+            s[2] += sc * g * a0;
+            s[3] += p[3 * D];
+            s[4] += p[2 * D];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 5; ++j) red[bl][j][cl] = s[j];
+    __syncthreads();
+    if (c >= D || bl >= 5) return;
+    float t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) t += red[k][bl][cl];
+    float* out[5] = {a.d_scale, a.d_post_w, a.d_post_b, a.d_pre_w, a.d_pre_b};
+    float* o = bl == 0 ? out[0] : bl == 1 ? out[1] : bl == 2 ? out[2] : bl == 3 ? out[3] : out[4];
+    if (o) o[c] = t;
+}
+
+constexpr int TEAMS = 1024;               // workgroups of the backward pass: enough to fill the chip, few enough for small partial sums
+
+bool vec_ok(const NormArgs& a) {
+    uintptr_t m = 0;
+    for (const void* p : {a.x, a.y, a.gate, a.dr, a.dz, (const void*)a.r, (const void*)a.z, (const void*)a.dx, (const void*)a.dy}) m |= (uintptr_t)p;
+    return a.D % 8 == 0 && m % 16 == 0;
+}
+// chunks of rows per sample; without a gate all rows are one sample
+void plan(NormArgs& a) {
+    if (!a.gate) { a.L *= a.B; a.B = 1; }
+    const int want = std::max(1, TEAMS / a.B);
+    a.rows_per_chunk = cdiv(a.L, std::min(want, a.L));
+    a.chunks = cdiv(a.L, a.rows_per_chunk);
+}
+template <int DT>
+int fwd(const NormArgs& a, hipStream_t st) {
+    const int64_t rows = (int64_t)a.B * a.L;
+    const int threads = 64 * cdiv(a.D, 512);
+    const unsigned grid = (unsigned)std::min<int64_t>(rows, 4096);
+    if (vec_ok(a)) norm_fwd_kernel<DT, true><<<grid, threads, 0, st>>>(a, rows);
+    else norm_fwd_kernel<DT, false><<<grid, threads, 0, st>>>(a, rows);
+    ISB_LAUNCHED("norm_fwd", st);
+    return ISB_OK;
+}
+template <int DT>
+int bwd(NormArgs a, float* ws, hipStream_t st) {
+    plan(a);
+    a.part = ws;
+    float* joint = ws + (int64_t)a.B * a.chunks * 4 * a.D;
+    const int threads = 64 * cdiv(a.D, 512);
+    if (vec_ok(a)) norm_bwd_kernel<DT, true><<<a.B * a.chunks, threads, 0, st>>>(a);
+    else norm_bwd_kernel<DT, false><<<a.B * a.chunks, threads, 0, st>>>(a);
+    ISB_LAUNCHED("norm_bwd", st);
+    norm_join_kernel<DT><<<dim3(cdiv(a.D, 64), a.B), 256, 0, st>>>(a, joint);
+    ISB_LAUNCHED("norm_join", st);
+    norm_params_kernel<DT><<<cdiv(a.D, 32), 256, 0, st>>>(a, joint);
+    ISB_LAUNCHED("norm_params", st);
+    return ISB_OK;
+}
+}  // namespace
+
+size_t norm_workspace(const NormArgs& a0) {
+    NormArgs a = a0;
+    plan(a);
+    return ((size_t)a.B * a.chunks + a.B) * 4 * a.D * sizeof(float);
+}
+int launch_norm_fwd(const NormArgs& a, int dtype, hipStream_t st) { return dtype == 0 ? fwd<0>(a, st) : dtype == 1 ? fwd<1>(a, st) : fwd<2>(a, st); }
+int launch_norm_bwd(NormArgs a, int dtype, float* ws, hipStream_t st) { return dtype == 0 ? bwd<0>(a, ws, st) : dtype == 1 ? bwd<1>(a, ws, st) : bwd<2>(a, ws, st); }
+
+}  // namespace isb

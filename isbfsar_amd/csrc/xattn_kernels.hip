@@ -1,0 +1,798 @@
+// Cross attention of query rows to an encoder's states of another length: forward (rows in tiles, or few rows with the states split over
+// waves and workgroups) and backward. Softmax statistics, sums and partial results are 32-bit; the attention weights and dS are rounded to
+// the tensors' 16-bit type where they enter a matrix product (half a step, the same size as the rounding of the results).
+//
+// One identity carries all kernels: a 32x32x16 product's accumulator holds, per lane, ONE column and the 16 rows 8 (i / 4) + 4 h + i % 4
+// (h = lane / 32). Computing S^T = K Q^T (column = query row) makes the softmax lane-local, and its registers 8 s ... 8 s + 7 ARE the B
+// operand of the next product over the states if the other operand lists the summed index in the same order -- which the transposing LDS
+// read does for free (frag_cols<W, 4, 8>). P never leaves its registers.
+#include <algorithm>
+#include <cmath>
+
+#include "blocks.h"
+
+namespace isb {
+namespace {
+
+constexpr int KT = 64;                    // states per tile
+constexpr float NEG_INF = -__builtin_inff();
+
+// element offset of row r of group (bk, hk) in a [B, Lq, Hq, .] tensor with strides sb, sl, sh
+struct RowAt { int b, i, hq; };
+__device__ __forceinline__ RowAt row_at(const XattnArgs& a, int bk, int hk, int r) {
+    const uint32_t s = a.by_lqg.div(r), rem = r - s * a.by_lqg.d, i = a.by_g.div(rem);
+    return {bk * a.nb + (int)s, (int)i, hk * a.G + (int)(rem - i * a.by_g.d)};
+}
+__device__ __forceinline__ int64_t off_at(const RowAt& p, int64_t sb, int64_t sl, int64_t sh) { return p.b * sb + p.i * sl + p.hq * sh; }
+__device__ __forceinline__ int64_t off_out(const XattnArgs& a, const RowAt& p) { return (((int64_t)p.b * a.Lq + p.i) * a.Hq + p.hq) * a.D; }
+__device__ __forceinline__ int64_t off_lse(const XattnArgs& a, const RowAt& p) { return ((int64_t)p.b * a.Hq + p.hq) * a.Lq + p.i; }
+
+__device__ __forceinline__ int states_of(const XattnArgs& a, int bk) { return a.kv_len ? min(max(a.kv_len[bk], 0), a.Lk) : a.Lk; }
+
+// byte of lane's state in the mask (0 = masked or absent); the ballot of tile_bits makes the tile's validity one scalar
+__device__ __forceinline__ uint32_t mask_byte(const XattnArgs& a, int bk, int key, int k1) {
+    if (key >= k1) return 0;
+    return a.mask ? a.mask[bk * a.mask_sb + key] : 1u;
+}
+
+// fragment of a row held in global memory (zeros past D): lane half h, k-step ks
+__device__ __forceinline__ uint4 row_frag(const uint16_t* p, int ks, int h, int D, bool ok) {
+    const int c = 16 * ks + 8 * h;
+    return ok && c < D ? *reinterpret_cast<const uint4*>(p + c) : make_uint4(0, 0, 0, 0);
+}
+
+// ---- requests of one tile of ROWS states x DT values by NW waves; voff[] holds the lane's byte offsets (DMA_NONE past D)
+template <int DT, int ROWS, int NW>
+struct TileLoad {
+    static constexpr int PIECES = ROWS * DT * 2 / 1024 / NW;      // 1-KiB requests per wave
+    uint32_t voff[PIECES];
+    int row[PIECES];
+    __device__ __forceinline__ void init(int wave, int lane, int64_t sl, int D) {
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            const int byte = (wave * PIECES + j) * 1024 + lane * 16, r = byte / (DT * 2);
+            const int c = ((byte % (DT * 2)) >> 4) ^ tile_xor<DT>(r);
+            row[j] = r;
+            voff[j] = c * 8 < D ? (uint32_t)(r * (int)sl * 2 + c * 16) : DMA_NONE;
+        }
+    }
+    __device__ __forceinline__ void request(const uint16_t* base, uint64_t bits, uint32_t lds, int wave) const {
+        const i32x4 d = dma_desc(base);
+        const bool full = bits == ~0ull;
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) {
+            const uint32_t v = full || ((bits >> row[j]) & 1) ? voff[j] : DMA_NONE;
+            dma16_desc(d, v, lds + (wave * PIECES + j) * 1024);
+        }
+    }
+};
+
+// masked scores become -inf; bits: validity of the 32 states of the block
+__device__ __forceinline__ void mask_scores(f32x16& s, uint32_t bits, int h) {
+    const uint32_t w = bits >> (4 * h);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s[i] = (w >> (8 * (i / 4) + i % 4)) & 1 ? s[i] : NEG_INF;
+}
+
+// One block of NB x 32 states for 32 rows (a column of S^T each): scores, running maximum and sum, O^T += V^T P^T.
+// The maximum follows lazily: O^T is rescaled only when a row's maximum grows by more than 8 (base-2 units), so P <= 2^8.
+template <bool F16, int DT, int NB>
+__device__ __forceinline__ void attend(const unsigned char* kt, const unsigned char* vt, const uint4 (&qf)[DT / 16], f32x16 (&acc)[DT / 32],
+                                       float& m, float& l, float c, uint64_t bits, int lane) {
+    const int h = lane >> 5;
+    f32x16 s[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < DT / 16; ++ks) s[b] = T16<F16>::mfma32(frag_rows<DT>(kt, 32 * b, ks, lane), qf[ks], s[b]);
+    }
+    constexpr uint64_t ALL = NB == 2 ? ~0ull : 0xffffffffull;
+    if (bits != ALL) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) mask_scores(s[b], (uint32_t)(bits >> (32 * b)), h);
+    }
+    float mx = NEG_INF;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
+    mx = max_halves(mx) * c;
+    if (__any(mx > m + 8.0f)) {
+        const float mn = fmaxf(m, mx);
+        const float al = __builtin_amdgcn_exp2f(m - (mn == NEG_INF ? 0.f : mn));
+        l *= al;
+#pragma unroll
+        for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[d][i] *= al;
+        m = mn;
+    }
+    const float mu = m == NEG_INF ? 0.f : m;
+    uint4 p[2 * NB];
+    float sum = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            float e[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][8 * t + i], c, -mu));
+                sum += e[i];
+            }
+            p[2 * b + t] = make_uint4(T16<F16>::pack2(e[0], e[1]), T16<F16>::pack2(e[2], e[3]), T16<F16>::pack2(e[4], e[5]), T16<F16>::pack2(e[6], e[7]));
+        }
+    l += sum;
+#pragma unroll
+    for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+        for (int t = 0; t < 2 * NB; ++t) acc[d] = T16<F16>::mfma32(frag_cols<DT, 4, 8>(vt, 16 * t, 32 * d, lane), p[t], acc[d]);
+}
+
+// results of a row: out and lse, or (splits) its unnormalised sums with maximum and sum
+template <bool F16, int DT>
+__device__ __forceinline__ void store_row(const XattnArgs& a, int bk, int hk, int split, int r, const f32x16 (&acc)[DT / 32], float m, float l, int h) {
+    if (r >= a.M) return;
+    if (a.splits > 1) {
+        const int64_t at = ((int64_t)split * a.Bk * a.Hk + bk * a.Hk + hk) * a.M + r;
+        float* p = a.part + at * DT;
+#pragma unroll
+        for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<float4*>(p + 32 * d + 8 * q + 4 * h) = make_float4(acc[d][4 * q], acc[d][4 * q + 1], acc[d][4 * q + 2], acc[d][4 * q + 3]);
+        if (h == 0) *reinterpret_cast<float2*>(a.part2 + at * 2) = make_float2(m, l);
+        return;
+    }
+    const RowAt w = row_at(a, bk, hk, r);
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    uint16_t* o = a.out + off_out(a, w);
+#pragma unroll
+    for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int at = 32 * d + 8 * q + 4 * h;
+            if (at < a.D)
+                *reinterpret_cast<uint2*>(o + at) = make_uint2(T16<F16>::pack2(acc[d][4 * q] * inv, acc[d][4 * q + 1] * inv),
+                                                               T16<F16>::pack2(acc[d][4 * q + 2] * inv, acc[d][4 * q + 3] * inv));
+        }
+    if (h == 0) a.lse[off_lse(a, w)] = l == 0.f ? NEG_INF : (m + __builtin_amdgcn_logf(l)) * LN2;
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------------
+// Forward, many rows: a workgroup takes 128 rows (32 per wave) of one group and walks the states in tiles of 64; K and V tiles arrive by
+// LDS-DMA, the next ones while this one is used (two buffers, one barrier per tile).
+// ------------------------------------------------------------------------------------------------------------------------------------
+template <bool F16, int DT>
+__global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XattnArgs a) {
+    T16<F16>::enter();
+    const int item = xcd_item(blockIdx.x, a.n_items);
+    if (item >= a.n_items) return;
+    const int rt = item % a.tiles, split = item / a.tiles % a.splits, grp = item / a.tiles / a.splits, bk = grp / a.Hk, hk = grp % a.Hk;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
+    const int r = rt * 128 + wave * 32 + (lane & 31);
+    constexpr int TB = KT * DT * 2;
+
+    const int len = states_of(a, bk), k0 = split * a.chunk, k1 = min(len, k0 + a.chunk);
+    const int nt = k1 > k0 ? (k1 - k0 + KT - 1) / KT : 0;
+
+    uint4 qf[DT / 16];
+    {
+        const RowAt w = row_at(a, bk, hk, min(r, a.M - 1));
+        const uint16_t* q = a.q + off_at(w, a.q_sb, a.q_sl, a.q_sh);
+#pragma unroll
+        for (int ks = 0; ks < DT / 16; ++ks) qf[ks] = row_frag(q, ks, h, a.D, r < a.M);
+    }
+    f32x16 acc[DT / 32];
+#pragma unroll
+    for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+    float m = NEG_INF, l = 0.f;
+
+    const uint16_t* kb = a.k + bk * a.k_sb + hk * a.k_sh + (int64_t)k0 * a.k_sl;
+    const uint16_t* vb = a.v + bk * a.v_sb + hk * a.v_sh + (int64_t)k0 * a.v_sl;
+    const uint32_t lds0 = lds_addr_of(conv_lds_dyn);
+    TileLoad<DT, KT, 4> lk, lv;
+    lk.init(wave, lane, a.k_sl, a.D);
+    lv.init(wave, lane, a.v_sl, a.D);
+    uint64_t bits = 0, next = 0;
+    uint32_t byte = 0;
+    if (nt > 0) {
+        bits = __ballot(mask_byte(a, bk, k0 + lane, k1) != 0);
+        lk.request(kb, bits, lds0, wave);
+        lv.request(vb, bits, lds0 + TB, wave);
+        byte = mask_byte(a, bk, k0 + KT + lane, k1);
+    }
+    for (int t = 0; t < nt; ++t) {
+        next = __ballot(byte != 0);
+        wait_all_and_meet();
+        const uint32_t cur = (t & 1) * 2 * TB, oth = 2 * TB - cur;
+        if (t + 1 < nt) {
+            const int64_t at = (int64_t)(t + 1) * KT;
+            lk.request(kb + at * a.k_sl, next, lds0 + oth, wave);
+            lv.request(vb + at * a.v_sl, next, lds0 + oth + TB, wave);
+            byte = mask_byte(a, bk, k0 + (t + 2) * KT + lane, k1);
+        }
+        if (bits != 0) attend<F16, DT, 2>(conv_lds_dyn + cur, conv_lds_dyn + cur + TB, qf, acc, m, l, a.c, bits, lane);
+        bits = next;
+    }
+    l = sum_halves(l);
+    store_row<F16, DT>(a, bk, hk, split, r, acc, m, l, h);
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------------
+// Forward, at most 32 rows in a group (single tokens, grouped heads): the states are the work. Every wave walks its own blocks of 32
+// states through its own LDS (no barrier in the loop, the next block always in flight), the four waves' sums meet at the end.
+// ------------------------------------------------------------------------------------------------------------------------------------
+template <bool F16, int DT>
+__global__ __launch_bounds__(256, 1) void xattn_token_kernel(XattnArgs a) {
+    T16<F16>::enter();
+    const int item = xcd_item(blockIdx.x, a.n_items);
+    if (item >= a.n_items) return;
+    const int split = item % a.splits, grp = item / a.splits, bk = grp / a.Hk, hk = grp % a.Hk;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5, r = lane & 31;
+    constexpr int TB = 32 * DT * 2, PIECES = TB / 1024;
+
+    const int len = states_of(a, bk), k0 = split * a.chunk, k1 = min(len, k0 + a.chunk);
+    const int nt = k1 > k0 ? (k1 - k0 + 31) / 32 : 0;                        // blocks of the workgroup; wave w takes w, w + 4, ...
+    uint4 qf[DT / 16];
+    {
+        const RowAt w = row_at(a, bk, hk, min(r, a.M - 1));
+        const uint16_t* q = a.q + off_at(w, a.q_sb, a.q_sl, a.q_sh);
+#pragma unroll
+        for (int ks = 0; ks < DT / 16; ++ks) qf[ks] = row_frag(q, ks, h, a.D, r < a.M);
+    }
+    f32x16 acc[DT / 32];
+#pragma unroll
+    for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+    float m = NEG_INF, l = 0.f;
+
+    const uint16_t* kb = a.k + bk * a.k_sb + hk * a.k_sh + (int64_t)k0 * a.k_sl;
+    const uint16_t* vb = a.v + bk * a.v_sb + hk * a.v_sh + (int64_t)k0 * a.v_sl;
+    unsigned char* own = conv_lds_dyn + wave * 4 * TB;
+    const uint32_t lds0 = lds_addr_of(own);
+    TileLoad<DT, 32, 1> lk, lv;
+    lk.init(0, lane, a.k_sl, a.D);
+    lv.init(0, lane, a.v_sl, a.D);
+    auto valid = [&](int t) -> uint32_t { return t < nt ? mask_byte(a, bk, k0 + 32 * t + (lane & 31), k1) : 0u; };
+    auto request = [&](int t, uint32_t bits, int buf) {
+        const int64_t at = (int64_t)t * 32;
+        lk.request(kb + at * a.k_sl, bits, lds0 + buf * 2 * TB, 0);
+        lv.request(vb + at * a.v_sl, bits, lds0 + buf * 2 * TB + TB, 0);
+    };
+    uint32_t bits = (uint32_t)__ballot(valid(wave) != 0), byte = valid(wave + 4);
+    if (wave < nt) request(wave, bits, 0);
+    for (int t = wave, buf = 0; t < nt; t += 4, buf ^= 1) {
+        const uint32_t next = (uint32_t)__ballot(byte != 0);
+        byte = valid(t + 8);
+        // this block's 2 * PIECES requests are the oldest; everything requested behind them may stay in flight
+        if (t + 4 < nt) {
+            request(t + 4, next, buf ^ 1);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PIECES) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        if (bits != 0) attend<F16, DT, 1>(own + buf * 2 * TB, own + buf * 2 * TB + TB, qf, acc, m, l, a.c, bits, lane);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                    // the buffer is read before it is requested again
+        bits = next;
+    }
+    l = sum_halves(l);
+    // join the waves: (m, l) of all four, then every wave scales its sums to the common maximum and they are added in wave order
+    wait_all_and_meet();
+    float* ml = reinterpret_cast<float*>(conv_lds_dyn);
+    float* sums = ml + 256;                                                   // [4][32][DT + 4]
+    constexpr int SW = DT + 4;
+    if (h == 0) { ml[(wave * 32 + r) * 2] = m; ml[(wave * 32 + r) * 2 + 1] = l; }
+    __syncthreads();
+    float mm = NEG_INF, ll = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[(w * 32 + r) * 2]);
+    const float mu = mm == NEG_INF ? 0.f : mm;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) ll += ml[(w * 32 + r) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * 32 + r) * 2] - mu);
+    const float al = __builtin_amdgcn_exp2f(m - mu);
+#pragma unroll
+    for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<float4*>(sums + (wave * 32 + r) * SW + 32 * d + 8 * q + 4 * h) =
+                make_float4(acc[d][4 * q] * al, acc[d][4 * q + 1] * al, acc[d][4 * q + 2] * al, acc[d][4 * q + 3] * al);
+    __syncthreads();
+    if (wave != 0) return;
+#pragma unroll
+    for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float4 u = *reinterpret_cast<const float4*>(sums + (w * 32 + r) * SW + 32 * d + 8 * q + 4 * h);
+                t.x += u.x; t.y += u.y; t.z += u.z; t.w += u.w;
+            }
+            acc[d][4 * q] = t.x; acc[d][4 * q + 1] = t.y; acc[d][4 * q + 2] = t.z; acc[d][4 * q + 3] = t.w;
+        }
+    store_row<F16, DT>(a, bk, hk, split, r, acc, mm, ll, h);
+}
+
+// join the splits of a row in their order: one wave per row
+template <bool F16, int DT>
+__global__ __launch_bounds__(256) void xattn_join_kernel(XattnArgs a) {
+    T16<F16>::enter();
+    const int64_t rows = (int64_t)a.Bk * a.Hk * a.M, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= rows) return;
+    const int lane = threadIdx.x & 63;
+    constexpr int E = DT / 64;
+    float mm = NEG_INF;
+    for (int s = 0; s < a.splits; ++s) mm = fmaxf(mm, a.part2[(s * rows + row) * 2]);
+    const float mu = mm == NEG_INF ? 0.f : mm;
+    float l = 0.f, o[E] = {};
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 ml = *reinterpret_cast<const float2*>(a.part2 + (s * rows + row) * 2);
+        const float w = __builtin_amdgcn_exp2f(ml.x - mu);
+        l += w * ml.y;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] += w * a.part[(s * rows + row) * DT + lane * E + e];
+    }
+    const int grp = (int)(row / a.M);
+    const RowAt w = row_at(a, grp / a.Hk, grp % a.Hk, (int)(row % a.M));
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    uint16_t* out = a.out + off_out(a, w);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (lane * E + e < a.D) out[lane * E + e] = T16<F16>::from_f32(o[e] * inv);
+    if (lane == 0) a.lse[off_lse(a, w)] = l == 0.f ? NEG_INF : (mm + __builtin_amdgcn_logf(l)) * LN2;
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------------
+// Backward. delta = rowsum(dout * out); then dK, dV (a workgroup keeps 128 states, 32 per wave, and walks the rows) and dQ (a workgroup
+// keeps 128 rows and walks the states). Every sum has a fixed order: no atomics.
+//
+// fp16: P is formed as 2^12 P (<= 4096), so that weights of 1 / 16384 stay normal numbers, and dS carries a power of two chosen from what
+// the wave meets: it starts so that the first tile's largest |dS| lies in [2^10, 2^11) and is lowered, with the sums so far, when a tile
+// passes 2^14. bf16 has f32's range and needs neither.
+// ------------------------------------------------------------------------------------------------------------------------------------
+template <bool F16> constexpr float P_UP = F16 ? 12.0f : 0.0f;              // log2 of the factor on P
+
+template <bool F16>
+__global__ __launch_bounds__(256) void xattn_delta_kernel(XattnArgs a) {
+    const int64_t rows = (int64_t)a.Bk * a.Hk * a.M, row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (row >= rows) return;
+    const int l = threadIdx.x & 15, grp = (int)(row / a.M);
+    const RowAt w = row_at(a, grp / a.Hk, grp % a.Hk, (int)(row % a.M));
+    float s = 0.f;
+    if (8 * l < a.D) {
+        const uint4 x = *reinterpret_cast<const uint4*>(a.out + off_out(a, w) + 8 * l);
+        const uint4 y = *reinterpret_cast<const uint4*>(a.dout + off_at(w, a.d_sb, a.d_sl, a.d_sh) + 8 * l);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s += T16<F16>::lo(xs[i]) * T16<F16>::lo(ys[i]) + T16<F16>::hi(xs[i]) * T16<F16>::hi(ys[i]);
+    }
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o);
+    if (l == 0) a.delta[row] = s;
+}
+
+// the power of two on dS (see above); NB blocks of scores. Returns with ds scaled.
+template <bool F16, int NB, int NA>
+__device__ __forceinline__ void scale_ds(f32x16 (&ds)[NB], f32x16 (&acc)[NA], float& sc) {
+    if constexpr (F16) {
+        float mx = 0.f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fabsf(ds[b][i]));
+        if (__any(mx * sc > 16384.0f || (sc == 0.f && mx > 0.f))) {
+#pragma unroll
+            for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+            const int e = min(max(10 - (int)__builtin_amdgcn_frexp_expf(mx) + 1, -100), 100);      // mx = f 2^x, f in [1/2, 1): mx 2^e in [2^10, 2^11)
+            const float ns = __builtin_ldexpf(1.0f, e);
+            const float f = sc == 0.f ? 1.0f : ns / sc;
+#pragma unroll
+            for (int d = 0; d < NA; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[d][i] *= f;
+            sc = ns;
+        }
+        const float by = sc == 0.f ? 1.0f : sc;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) ds[b][i] *= by;
+    }
+}
+template <bool F16>
+__device__ __forceinline__ uint4 pack8(const f32x16& x, int t) {
+    return t == 0 ? make_uint4(T16<F16>::pack2(x[0], x[1]), T16<F16>::pack2(x[2], x[3]), T16<F16>::pack2(x[4], x[5]), T16<F16>::pack2(x[6], x[7]))
+                  : make_uint4(T16<F16>::pack2(x[8], x[9]), T16<F16>::pack2(x[10], x[11]), T16<F16>::pack2(x[12], x[13]), T16<F16>::pack2(x[14], x[15]));
+}
+
+// dK, dV: S = Q K^T with the rows in the accumulator's rows and a state per lane; P and dS are then operands over the rows.
+template <bool F16, int DT>
+__global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnArgs a) {
+    T16<F16>::enter();
+    const int item = xcd_item(blockIdx.x, a.n_items);
+    if (item >= a.n_items) return;
+    const int kt = item % a.tiles, split = item / a.tiles % a.splits, grp = item / a.tiles / a.splits, bk = grp / a.Hk, hk = grp % a.Hk;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5, tid = threadIdx.x;
+    const int key = kt * 128 + wave * 32 + (lane & 31);
+    const int len = states_of(a, bk);
+    const bool ok = mask_byte(a, bk, key, len) != 0;
+    constexpr int TB = 32 * DT * 2, STAGE = 2 * TB + 256, CH = DT / 8;       // a tile of 32 rows of Q, of dout, 32 lse, 32 delta
+    constexpr int PC = 32 * CH / 256;                                         // 16-byte chunks per thread and tensor (DT 64: 1, DT 128: 2)
+    const int r0 = split * a.chunk, r1 = min(a.M, r0 + a.chunk), nt = __syncthreads_or(ok) ? (r1 - r0 + 31) / 32 : 0;
+
+    uint4 kf[DT / 16], vf[DT / 16];
+    {
+        const int kc = min(key, a.Lk - 1);
+        const uint16_t* k = a.k + bk * a.k_sb + hk * a.k_sh + (int64_t)kc * a.k_sl;
+        const uint16_t* v = a.v + bk * a.v_sb + hk * a.v_sh + (int64_t)kc * a.v_sl;
+#pragma unroll
+        for (int ks = 0; ks < DT / 16; ++ks) { kf[ks] = row_frag(k, ks, h, a.D, ok); vf[ks] = row_frag(v, ks, h, a.D, ok); }
+    }
+    f32x16 dk[DT / 32], dv[DT / 32];
+#pragma unroll
+    for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { dk[d][i] = 0.f; dv[d][i] = 0.f; }
+    float sc = F16 ? 0.f : 1.0f;
+
+    uint4 gq[PC], gd[PC];
+    float gs = 0.f;
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int j = 0; j < PC; ++j) {
+            const int ch = tid + 256 * j, r = r0 + t * 32 + ch / CH, c = 8 * (ch % CH);
+            const bool in = r < r1 && c < a.D;
+            gq[j] = gd[j] = make_uint4(0, 0, 0, 0);
+            if (in) {
+                const RowAt w = row_at(a, bk, hk, r);
+                gq[j] = *reinterpret_cast<const uint4*>(a.q + off_at(w, a.q_sb, a.q_sl, a.q_sh) + c);
+                gd[j] = *reinterpret_cast<const uint4*>(a.dout + off_at(w, a.d_sb, a.d_sl, a.d_sh) + c);
+            }
+        }
+        if (tid < 64) {                                                        // 32 x -lse (base 2), 32 x delta; absent rows: P = exp2(-inf) = 0
+            const int r = r0 + t * 32 + (tid & 31);
+            if (r >= r1) gs = tid < 32 ? NEG_INF : 0.f;
+            else if (tid < 32) gs = P_UP<F16> - a.lse[off_lse(a, row_at(a, bk, hk, r))] * LOG2E;
+            else gs = a.delta[(int64_t)grp * a.M + r];
+        }
+    };
+    auto put = [&](int buf) {
+        unsigned char* s = conv_lds_dyn + buf * STAGE;
+#pragma unroll
+        for (int j = 0; j < PC; ++j) {
+            const int ch = tid + 256 * j, at = tile_at<DT>(ch / CH, ch % CH);
+            *reinterpret_cast<uint4*>(s + at) = gq[j];
+            *reinterpret_cast<uint4*>(s + TB + at) = gd[j];
+        }
+        if (tid < 64) reinterpret_cast<float*>(s + 2 * TB)[tid] = gs;
+    };
+    if (nt > 0) { fetch(0); put(0); }
+    __syncthreads();
+    for (int t = 0; t < nt; ++t) {
+        const unsigned char* qt = conv_lds_dyn + (t & 1) * STAGE;
+        const unsigned char* dt = qt + TB;
+        const float* st = reinterpret_cast<const float*>(qt + 2 * TB);
+        if (t + 1 < nt) fetch(t + 1);
+        f32x16 s, dp[1];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[0][i] = 0.f; }
+#pragma unroll
+        for (int ks = 0; ks < DT / 16; ++ks) s = T16<F16>::mfma32(frag_rows<DT>(qt, 0, ks, lane), kf[ks], s);
+#pragma unroll
+        for (int ks = 0; ks < DT / 16; ++ks) dp[0] = T16<F16>::mfma32(frag_rows<DT>(dt, 0, ks, lane), vf[ks], dp[0]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float4 nl = *reinterpret_cast<const float4*>(st + 8 * q + 4 * h), de = *reinterpret_cast<const float4*>(st + 32 + 8 * q + 4 * h);
+            const float n4[4] = {nl.x, nl.y, nl.z, nl.w}, d4[4] = {de.x, de.y, de.z, de.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[4 * q + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + i], a.c, n4[i]));
+                dp[0][4 * q + i] = s[4 * q + i] * (dp[0][4 * q + i] - d4[i]);
+            }
+        }
+        if constexpr (F16) {            // a masked state's column is not stored, but must not set the power of two either
+            if (!ok) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) dp[0][i] = 0.f;
+            }
+        }
+        scale_ds<F16, 1, DT / 32>(dp, dk, sc);
+        uint4 p[2], ds[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) { p[u] = pack8<F16>(s, u); ds[u] = pack8<F16>(dp[0], u); }
+#pragma unroll
+        for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                dv[d] = T16<F16>::mfma32(frag_cols<DT, 4, 8>(dt, 16 * u, 32 * d, lane), p[u], dv[d]);
+                dk[d] = T16<F16>::mfma32(frag_cols<DT, 4, 8>(qt, 16 * u, 32 * d, lane), ds[u], dk[d]);
+            }
+        if (t + 1 < nt) put((t + 1) & 1);
+        __syncthreads();
+    }
+    if (key >= a.Lk) return;
+    const float fv = ok ? __builtin_amdgcn_exp2f(-P_UP<F16>) : 0.f;
+    const float fk = ok ? a.scale * fv / (sc == 0.f ? 1.0f : sc) : 0.f;
+    const int64_t at = a.splits > 1 ? (((int64_t)split * a.Bk * a.Hk + grp) * a.Lk + key) * DT : (((int64_t)bk * a.Lk + key) * a.Hk + hk) * a.D;
+#pragma unroll
+    for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int e = 32 * d + 8 * q + 4 * h;
+            float4 x, y;
+            float* xs = &x.x;
+            float* ys = &y.x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                xs[i] = ok ? dk[d][4 * q + i] * fk : 0.f;
+                ys[i] = ok ? dv[d][4 * q + i] * fv : 0.f;
+            }
+            if (a.splits > 1) {
+                *reinterpret_cast<float4*>(a.part + at + e) = x;
+                *reinterpret_cast<float4*>(a.part2 + at + e) = y;
+            } else if (e < a.D) {
+                *reinterpret_cast<uint2*>(a.dk + at + e) = make_uint2(T16<F16>::pack2(x.x, x.y), T16<F16>::pack2(x.z, x.w));
+                *reinterpret_cast<uint2*>(a.dv + at + e) = make_uint2(T16<F16>::pack2(y.x, y.y), T16<F16>::pack2(y.z, y.w));
+            }
+        }
+}
+
+// dQ: as the forward kernel; dS^T has a row per lane, dQ^T += K^T dS^T reads the K tile a second time, transposed
+template <bool F16, int DT>
+__global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
+    T16<F16>::enter();
+    const int item = xcd_item(blockIdx.x, a.n_items);
+    if (item >= a.n_items) return;
+    const int rt = item % a.tiles, split = item / a.tiles % a.splits, grp = item / a.tiles / a.splits, bk = grp / a.Hk, hk = grp % a.Hk;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
+    const int r = rt * 128 + wave * 32 + (lane & 31);
+    constexpr int TB = KT * DT * 2;
+    const int len = states_of(a, bk), k0 = split * a.chunk, k1 = min(len, k0 + a.chunk);
+    const int nt = k1 > k0 ? (k1 - k0 + KT - 1) / KT : 0;
+
+    uint4 qf[DT / 16], df[DT / 16];
+    const RowAt w = row_at(a, bk, hk, min(r, a.M - 1));
+    float nl, de;
+    {
+        const uint16_t* q = a.q + off_at(w, a.q_sb, a.q_sl, a.q_sh);
+        const uint16_t* d = a.dout + off_at(w, a.d_sb, a.d_sl, a.d_sh);
+#pragma unroll
+        for (int ks = 0; ks < DT / 16; ++ks) { qf[ks] = row_frag(q, ks, h, a.D, r < a.M); df[ks] = row_frag(d, ks, h, a.D, r < a.M); }
+        nl = r < a.M ? P_UP<F16> - a.lse[off_lse(a, w)] * LOG2E : NEG_INF;
+        de = r < a.M ? a.delta[(int64_t)grp * a.M + r] : 0.f;
+    }
+    f32x16 acc[DT / 32];
+#pragma unroll
+    for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+    float sc = F16 ? 0.f : 1.0f;
+
+    const uint16_t* kb = a.k + bk * a.k_sb + hk * a.k_sh + (int64_t)k0 * a.k_sl;
+    const uint16_t* vb = a.v + bk * a.v_sb + hk * a.v_sh + (int64_t)k0 * a.v_sl;
+    const uint32_t lds0 = lds_addr_of(conv_lds_dyn);
+    TileLoad<DT, KT, 4> lk, lv;
+    lk.init(wave, lane, a.k_sl, a.D);
+    lv.init(wave, lane, a.v_sl, a.D);
+    uint64_t bits = 0, next = 0;
+    uint32_t byte = 0;
+    if (nt > 0) {
+        bits = __ballot(mask_byte(a, bk, k0 + lane, k1) != 0);
+        lk.request(kb, bits, lds0, wave);
+        lv.request(vb, bits, lds0 + TB, wave);
+        byte = mask_byte(a, bk, k0 + KT + lane, k1);
+    }
+    for (int t = 0; t < nt; ++t) {
+        next = __ballot(byte != 0);
+        wait_all_and_meet();
+        const uint32_t cur = (t & 1) * 2 * TB, oth = 2 * TB - cur;
+        if (t + 1 < nt) {
+            const int64_t at = (int64_t)(t + 1) * KT;
+            lk.request(kb + at * a.k_sl, next, lds0 + oth, wave);
+            lv.request(vb + at * a.v_sl, next, lds0 + oth + TB, wave);
+            byte = mask_byte(a, bk, k0 + (t + 2) * KT + lane, k1);
+        }
+        const unsigned char* ktile = conv_lds_dyn + cur;
+        const unsigned char* vtile = ktile + TB;
+        if (bits != 0) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                f32x16 s, ds[1];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) { s[i] = 0.f; ds[0][i] = 0.f; }
+#pragma unroll
+                for (int ks = 0; ks < DT / 16; ++ks) {
+                    s = T16<F16>::mfma32(frag_rows<DT>(ktile, 32 * b, ks, lane), qf[ks], s);
+                    ds[0] = T16<F16>::mfma32(frag_rows<DT>(vtile, 32 * b, ks, lane), df[ks], ds[0]);
+                }
+                if (bits != ~0ull) mask_scores(s, (uint32_t)(bits >> (32 * b)), h);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) ds[0][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, nl)) * (ds[0][i] - de);
+                scale_ds<F16, 1, DT / 32>(ds, acc, sc);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const uint4 f = pack8<F16>(ds[0], u);
+#pragma unroll
+                    for (int d = 0; d < DT / 32; ++d) acc[d] = T16<F16>::mfma32(frag_cols<DT, 4, 8>(ktile, 32 * b + 16 * u, 32 * d, lane), f, acc[d]);
+                }
+            }
+        }
+        bits = next;
+    }
+    if (r >= a.M) return;
+    const float f = a.scale * __builtin_amdgcn_exp2f(-P_UP<F16>) / (sc == 0.f ? 1.0f : sc);
+    const int64_t at = a.splits > 1 ? (((int64_t)split * a.Bk * a.Hk + grp) * a.M + r) * DT : off_out(a, w);
+#pragma unroll
+    for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int e = 32 * d + 8 * q + 4 * h;
+            const float4 x = make_float4(acc[d][4 * q] * f, acc[d][4 * q + 1] * f, acc[d][4 * q + 2] * f, acc[d][4 * q + 3] * f);
+            if (a.splits > 1) *reinterpret_cast<float4*>(a.part + at + e) = x;
+            else if (e < a.D) *reinterpret_cast<uint2*>(a.dq + at + e) = make_uint2(T16<F16>::pack2(x.x, x.y), T16<F16>::pack2(x.z, x.w));
+        }
+}
+
+// sums of the splits in their order: dst row = KEYS ? state of [Bk, Lk, Hk, D] : row of [B, Lq, Hq, D]; 16 lanes per row
+template <bool F16, int DT, bool KEYS>
+__global__ __launch_bounds__(256) void xattn_sum_kernel(XattnArgs a, const float* part, uint16_t* dst, int n) {
+    T16<F16>::enter();
+    const int64_t rows = (int64_t)a.Bk * a.Hk * n, row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (row >= rows) return;
+    const int grp = (int)(row / n), i = (int)(row % n), l = threadIdx.x & 15;
+    constexpr int E = DT / 16;
+    float o[E] = {};
+    for (int s = 0; s < a.splits; ++s) {
+        const float* p = part + (s * rows + row) * DT + l * E;
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p + e);
+            o[e] += v.x; o[e + 1] += v.y; o[e + 2] += v.z; o[e + 3] += v.w;
+        }
+    }
+    const int64_t at = KEYS ? (((int64_t)(grp / a.Hk) * a.Lk + i) * a.Hk + grp % a.Hk) * a.D : off_out(a, row_at(a, grp / a.Hk, grp % a.Hk, i));
+#pragma unroll
+    for (int e = 0; e < E; e += 4)
+        if (l * E + e < a.D) *reinterpret_cast<uint2*>(dst + at + l * E + e) = make_uint2(T16<F16>::pack2(o[e], o[e + 1]), T16<F16>::pack2(o[e + 2], o[e + 3]));
+}
+
+// ------------------------------------------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------------------------------------------
+constexpr int WANTED = 512;               // workgroups that fill the chip: two on each of the 256 CUs
+
+// splits of `len` (in units of `unit`) so that base * splits reaches WANTED, each split at least `least` units long
+void choose_splits(int64_t base, int len, int unit, int least, int& splits, int& chunk) {
+    const int64_t units = cdiv(std::max(len, 1), unit);
+    int64_t s = std::min<int64_t>((WANTED + base - 1) / base, std::max<int64_t>(1, units / least));
+    s = std::min<int64_t>(std::max<int64_t>(s, 1), 64);
+    const int64_t per = (units + s - 1) / s;
+    splits = (int)((units + per - 1) / per);
+    chunk = (int)(per * unit);
+}
+int dt_of(const XattnArgs& a) { return a.D <= 64 ? 64 : 128; }
+bool few_rows(const XattnArgs& a) { return a.M <= 32; }
+
+struct Plan { int tiles, splits, chunk; };
+Plan plan_fwd(const XattnArgs& a) {
+    Plan p{};
+    const int64_t groups = (int64_t)a.Bk * a.Hk;
+    if (few_rows(a)) {
+        p.tiles = 1;
+        choose_splits(groups, a.Lk, 128, 1, p.splits, p.chunk);
+    } else {
+        p.tiles = cdiv(a.M, 128);
+        choose_splits(groups * p.tiles, a.Lk, KT, 4, p.splits, p.chunk);
+    }
+    return p;
+}
+Plan plan_dkv(const XattnArgs& a) {
+    Plan p{};
+    p.tiles = cdiv(a.Lk, 128);
+    choose_splits((int64_t)a.Bk * a.Hk * p.tiles, a.M, 32, 8, p.splits, p.chunk);
+    return p;
+}
+Plan plan_dq(const XattnArgs& a) {
+    Plan p{};
+    p.tiles = cdiv(a.M, 128);
+    choose_splits((int64_t)a.Bk * a.Hk * p.tiles, a.Lk, KT, 4, p.splits, p.chunk);
+    return p;
+}
+int items(XattnArgs& a, const Plan& p, unsigned& grid) {
+    const int64_t n = (int64_t)a.Bk * a.Hk * p.tiles * p.splits;
+    ISB_REQUIRE(n < (1ll << 30), ISB_ERR_INVALID, "cross attention: %lld workgroups are more than one launch holds", (long long)n);
+    a.tiles = p.tiles;
+    a.splits = p.splits;
+    a.chunk = p.chunk;
+    a.n_items = (int)n;
+    grid = (unsigned)(8 * ((n + 7) / 8));
+    return ISB_OK;
+}
+template <auto Kernel>
+int launch(const char* name, unsigned grid, size_t lds, const XattnArgs& a, hipStream_t st) {
+    static DevMax attr;
+    if (attr.below((int)lds)) {
+        ISB_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+        attr.set((int)lds);
+    }
+    Kernel<<<grid, 256, lds, st>>>(a);
+    ISB_LAUNCHED(name, st);
+    return ISB_OK;
+}
+
+template <bool F16, int DT>
+int fwd(XattnArgs a, float* ws, hipStream_t st) {
+    const Plan p = plan_fwd(a);
+    unsigned grid = 0;
+    ISB_TRY(items(a, p, grid));
+    const int64_t rows = (int64_t)a.Bk * a.Hk * a.M;
+    a.part = ws;
+    a.part2 = ws + (int64_t)p.splits * rows * DT;
+    if (few_rows(a)) ISB_TRY((launch<xattn_token_kernel<F16, DT>>("xattn_token", grid, 4 * 4 * 32 * DT * 2, a, st)));
+    else ISB_TRY((launch<xattn_fwd_kernel<F16, DT>>("xattn_fwd", grid, 4 * KT * DT * 2, a, st)));
+    if (p.splits > 1) {
+        xattn_join_kernel<F16, DT><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a);
+        ISB_LAUNCHED("xattn_join", st);
+    }
+    return ISB_OK;
+}
+
+template <bool F16, int DT>
+int bwd(XattnArgs a, float* ws, hipStream_t st) {
+    const int64_t rows = (int64_t)a.Bk * a.Hk * a.M;
+    a.delta = ws;
+    float* part = ws + (rows + 63) / 64 * 64;
+    xattn_delta_kernel<F16><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(a);
+    ISB_LAUNCHED("xattn_delta", st);
+    unsigned grid = 0;
+    const int64_t states = (int64_t)a.Bk * a.Hk * a.Lk;
+    Plan p = plan_dkv(a);
+    ISB_TRY(items(a, p, grid));
+    a.part = part;
+    a.part2 = part + (int64_t)p.splits * states * DT;
+    ISB_TRY((launch<xattn_dkv_kernel<F16, DT>>("xattn_dkv", grid, 2 * (2 * 32 * DT * 2 + 256), a, st)));
+    if (p.splits > 1) {
+        const unsigned g = (unsigned)((states + 15) / 16);
+        xattn_sum_kernel<F16, DT, true><<<g, 256, 0, st>>>(a, a.part, a.dk, a.Lk);
+        ISB_LAUNCHED("xattn_sum dk", st);
+        xattn_sum_kernel<F16, DT, true><<<g, 256, 0, st>>>(a, a.part2, a.dv, a.Lk);
+        ISB_LAUNCHED("xattn_sum dv", st);
+    }
+    p = plan_dq(a);
+    ISB_TRY(items(a, p, grid));
+    ISB_TRY((launch<xattn_dq_kernel<F16, DT>>("xattn_dq", grid, 4 * KT * DT * 2, a, st)));
+    if (p.splits > 1) {
+        xattn_sum_kernel<F16, DT, false><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(a, a.part, a.dq, a.M);
+        ISB_LAUNCHED("xattn_sum dq", st);
+    }
+    return ISB_OK;
+}
+}  // namespace
+
+// bytes of workspace; the partial results of dK / dV and of dQ take turns in the same place (one stream orders them)
+size_t xattn_workspace(const XattnArgs& a, bool backward) {
+    const size_t rows = (size_t)a.Bk * a.Hk * a.M, states = (size_t)a.Bk * a.Hk * a.Lk, dt = dt_of(a);
+    if (!backward) {
+        const Plan p = plan_fwd(a);
+        return p.splits > 1 ? p.splits * rows * (dt + 2) * 4 : 0;
+    }
+    const Plan k = plan_dkv(a), q = plan_dq(a);
+    const size_t pk = k.splits > 1 ? 2 * k.splits * states * dt : 0, pq = q.splits > 1 ? q.splits * rows * dt : 0;
+    return ((rows + 63) / 64 * 64 + std::max(pk, pq)) * 4;
+}
+int launch_xattn_fwd(XattnArgs a, bool f16, float* ws, hipStream_t st) {
+    if (dt_of(a) == 64) return f16 ? fwd<true, 64>(a, ws, st) : fwd<false, 64>(a, ws, st);
+    return f16 ? fwd<true, 128>(a, ws, st) : fwd<false, 128>(a, ws, st);
+}
+int launch_xattn_bwd(XattnArgs a, bool f16, float* ws, hipStream_t st) {
+    if (dt_of(a) == 64) return f16 ? bwd<true, 64>(a, ws, st) : bwd<false, 64>(a, ws, st);
+    return f16 ? bwd<true, 128>(a, ws, st) : bwd<false, 128>(a, ws, st);
+}
+
+}  // namespace isb
