@@ -57,7 +57,7 @@ struct NormArgs {
     float *d_scale, *d_post_w, *d_post_b, *d_pre_w, *d_pre_b;
     float* part;                                         // [B, chunks, 4, D]
     int B, L, D, chunks, rows_per_chunk;
-    int post, pre;                                       // 0 none, 1 layer, 2 rms
+    int post, post_centred, pre, pre_centred;            // is there a norm; does it take the mean off (LayerNorm)
     float eps;
 };
 size_t norm_workspace(const NormArgs& a);

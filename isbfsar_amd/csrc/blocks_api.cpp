@@ -178,7 +178,9 @@ int norm_shape(const isb_norm_args* u, NormArgs& a) {
                     (u->pre == ISB_NORM_LAYER || !u->pre_bias),
                 ISB_ERR_INVALID, "block norm: a weight needs its norm, a bias a LayerNorm");
     ISB_REQUIRE(std::isfinite(u->eps) && u->eps >= 0, ISB_ERR_INVALID, "block norm: eps %g", (double)u->eps);
-    a.B = u->B; a.L = u->L; a.D = u->D; a.post = u->post; a.pre = u->pre; a.eps = u->eps;
+    a.B = u->B; a.L = u->L; a.D = u->D; a.eps = u->eps;
+    a.post = u->post != ISB_NORM_NONE; a.post_centred = u->post == ISB_NORM_LAYER;
+    a.pre = u->pre != ISB_NORM_NONE; a.pre_centred = u->pre == ISB_NORM_LAYER;
     a.x = u->x; a.y = u->y; a.gate = u->gate;
     a.scale = u->scale; a.post_w = u->post_weight; a.post_b = u->post_bias; a.pre_w = u->pre_weight; a.pre_b = u->pre_bias;
     a.stats = u->stats;

@@ -15,8 +15,6 @@
 namespace isb {
 namespace {
 
-enum { NONE = 0, LAYER = 1, RMS = 2 };
-
 // eight neighbouring values at p + c (c < D; VEC: D % 8 == 0 and 16-byte rows), zeros past D
 template <int DT, bool VEC>
 __device__ __forceinline__ void load8(const void* base, int64_t row, int c, int D, float (&v)[8]) {
@@ -68,90 +66,131 @@ __device__ __forceinline__ void param8(const float* p, int c, int D, float fill,
     for (int i = 0; i < 8; ++i) v[i] = p && c + i < D ? p[c + i] : fill;
 }
 
-// sums of one or two values over the workgroup, the same bits in every lane. `slot` alternates between two halves of the buffer, so one
-// barrier per call is enough.
+// sums of N values over the workgroup, the same bits in every lane. The buffer's two halves take turns, so one barrier per call is enough.
+template <int MOST>
 struct Meet {
-    float* buf;
+    float* buf;                              // [2][16 waves][MOST]
     int waves, wave, lane, slot;
-    __device__ __forceinline__ void sum2(float& a, float& b) {
+    template <int N>
+    __device__ __forceinline__ void sum(float (&v)[N]) {
+        static_assert(N <= MOST, "buffer");
 #pragma unroll
-        for (int o = 32; o; o >>= 1) { a += __shfl_xor(a, o); b += __shfl_xor(b, o); }
+        for (int o = 32; o; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o);
         if (waves == 1) return;
-        float* s = buf + slot * 32;
+        float* s = buf + slot * 16 * MOST;
         slot ^= 1;
-        if (lane == 0) { s[2 * wave] = a; s[2 * wave + 1] = b; }
+        if (lane == 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) s[wave * MOST + i] = v[i];
+        }
         __syncthreads();
-        a = b = 0.f;
-        for (int w = 0; w < waves; ++w) { a += s[2 * w]; b += s[2 * w + 1]; }
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = 0.f;
+        for (int w = 0; w < waves; ++w)
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] += s[w * MOST + i];
     }
-    __device__ __forceinline__ float sum(float a) { float b = 0.f; sum2(a, b); return a; }
 };
 
-// v -> (v - mean) inv for `kind`; columns past D stay zero
-__device__ __forceinline__ void normalise(int kind, float (&v)[8], int c, int D, float eps, float& mean, float& inv, Meet& meet) {
-    mean = 0.f;
-    inv = 1.f;
-    if (kind == NONE) return;
-    if (kind == LAYER) {
-        float s = 0.f;
+// R rows v -> (v - mean) inv (RMS: no mean); columns past D stay zero. Which of the norms runs comes as separate flags: the compiler of
+// ROCm 7.2 makes ONE three-way switch of tests on a single `kind` and lowers its default case (uniform, a loop around it) wrongly -- the
+// copies into the merged registers are skipped.
+template <int R>
+__device__ __forceinline__ void normalise(bool centred, float (&v)[R][8], int c, int D, float eps, float (&mean)[R], float (&inv)[R], Meet<2 * R>& meet) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s += v[i];
-        mean = meet.sum(s) / (float)D;
+    for (int k = 0; k < R; ++k) mean[k] = 0.f;
+    if (centred) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < D ? v[i] - mean : 0.f;
+        for (int k = 0; k < R; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) mean[k] += v[k][i];
+        meet.sum(mean);
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            mean[k] = mean[k] / (float)D;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[k][i] = c + i < D ? v[k][i] - mean[k] : 0.f;
+        }
     }
-    float s = 0.f;
+    float s[R] = {};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s = __builtin_fmaf(v[i], v[i], s);
-    inv = 1.0f / sqrtf(meet.sum(s) / (float)D + eps);
+    for (int k = 0; k < R; ++k)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= inv;
+        for (int i = 0; i < 8; ++i) s[k] = __builtin_fmaf(v[k][i], v[k][i], s[k]);
+    meet.sum(s);
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        inv[k] = 1.0f / sqrtf(s[k] / (float)D + eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[k][i] *= inv[k];
+    }
 }
 
-template <int DT, bool VEC>
-__global__ __launch_bounds__(1024) void norm_fwd_kernel(NormArgs a, int64_t rows) {
+// R rows at a time: their loads are in flight together and they share the barriers
+template <int DT, bool VEC, int R, int MOST>
+__global__ __launch_bounds__(MOST) void norm_fwd_kernel(NormArgs a, int64_t rows) {
     if constexpr (DT == 1) T16<true>::enter();
-    __shared__ float buf[64];
+    __shared__ float buf[2 * 16 * 2 * R];
     const int tid = threadIdx.x, c = tid * 8, D = a.D;
     const bool in = c < D;
-    Meet meet{buf, (int)blockDim.x >> 6, tid >> 6, tid & 63, 0};
+    Meet<2 * R> meet{buf, (int)blockDim.x >> 6, tid >> 6, tid & 63, 0};
     float qw[8], qb[8], pw[8], pb[8], sc[8];
     param8(a.post_w, c, D, 1.f, qw);
     param8(a.post_b, c, D, 0.f, qb);
     param8(a.pre_w, c, D, 1.f, pw);
     param8(a.pre_b, c, D, 0.f, pb);
     param8(a.scale, c, D, 1.f, sc);
-    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-        float r[8] = {}, y[8] = {}, g[8];
-        if (in) load8<DT, VEC>(a.x, row, c, D, r);
-        float my = 0.f, iy = 1.f, mr = 0.f, ir = 1.f;
+    for (int64_t row = (int64_t)blockIdx.x * R; row < rows; row += (int64_t)gridDim.x * R) {
+        const int n = (int)min((int64_t)R, rows - row);
+        float r[R][8] = {}, y[R][8] = {};
+#pragma unroll
+        for (int k = 0; k < R; ++k)
+            if (in && k < n) {
+                load8<DT, VEC>(a.x, row + k, c, D, r[k]);
+                if (a.y) load8<DT, VEC>(a.y, row + k, c, D, y[k]);
+            }
+        float my[R] = {}, iy[R], mr[R] = {}, ir[R];
+#pragma unroll
+        for (int k = 0; k < R; ++k) iy[k] = ir[k] = 1.f;
         if (a.y) {
-            if (in) load8<DT, VEC>(a.y, row, c, D, y);
+            if (a.post) normalise<R>(a.post_centred, y, c, D, a.eps, my, iy, meet);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) g[i] = 1.f;
-            if (a.gate && in) load8<DT, VEC>(a.gate, row / a.L, c, D, g);
-            normalise(a.post, y, c, D, a.eps, my, iy, meet);
+            for (int k = 0; k < R; ++k) {
+                float g[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) r[i] = c + i < D ? __builtin_fmaf(sc[i] * g[i], __builtin_fmaf(y[i], qw[i], qb[i]), r[i]) : 0.f;
-            if (in) store8<DT, VEC>(a.r, row, c, D, r);
+                for (int i = 0; i < 8; ++i) g[i] = 1.f;
+                if (a.gate && in && k < n) load8<DT, VEC>(a.gate, (row + k) / a.L, c, D, g);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) r[k][i] = c + i < D ? __builtin_fmaf(sc[i] * g[i], __builtin_fmaf(y[k][i], qw[i], qb[i]), r[k][i]) : 0.f;
+                if (in && k < n) store8<DT, VEC>(a.r, row + k, c, D, r[k]);
+            }
         }
         if (a.pre) {
-            normalise(a.pre, r, c, D, a.eps, mr, ir, meet);
+            normalise<R>(a.pre_centred, r, c, D, a.eps, mr, ir, meet);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) r[i] = __builtin_fmaf(r[i], pw[i], pb[i]);
-            if (in) store8<DT, VEC>(a.z, row, c, D, r);
+            for (int k = 0; k < R; ++k) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) r[k][i] = __builtin_fmaf(r[k][i], pw[i], pb[i]);
+                if (in && k < n) store8<DT, VEC>(a.z, row + k, c, D, r[k]);
+            }
         }
-        if (a.stats && tid == 0) *reinterpret_cast<float4*>(a.stats + 4 * row) = make_float4(my, iy, mr, ir);
+        if (a.stats && tid == 0) {
+#pragma unroll
+            for (int k = 0; k < R; ++k)
+                if (k < n) *reinterpret_cast<float4*>(a.stats + 4 * (row + k)) = make_float4(my[k], iy[k], mr[k], ir[k]);
+        }
     }
 }
 
-template <int DT, bool VEC>
-__global__ __launch_bounds__(1024) void norm_bwd_kernel(NormArgs a) {
+template <int DT, bool VEC, int R, int MOST>
+__global__ __launch_bounds__(MOST) void norm_bwd_kernel(NormArgs a) {
     if constexpr (DT == 1) T16<true>::enter();
-    __shared__ float buf[64];
+    __shared__ float buf[2 * 16 * 2 * R];
     const int tid = threadIdx.x, c = tid * 8, D = a.D;
     const bool in = c < D;
-    Meet meet{buf, (int)blockDim.x >> 6, tid >> 6, tid & 63, 0};
+    Meet<2 * R> meet{buf, (int)blockDim.x >> 6, tid >> 6, tid & 63, 0};
     const int b = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
     const int l0 = chunk * a.rows_per_chunk, l1 = min(a.L, l0 + a.rows_per_chunk);
     float qw[8], qb[8], pw[8], f[8], g[8];
@@ -166,57 +205,82 @@ __global__ __launch_bounds__(1024) void norm_bwd_kernel(NormArgs a) {
     }
     const float rD = 1.0f / (float)D;
     float s0[8] = {}, s1[8] = {}, s2[8] = {}, s3[8] = {};
-    for (int l = l0; l < l1; ++l) {
+    for (int l = l0; l < l1; l += R) {
         const int64_t row = (int64_t)b * a.L + l;
-        float x[8] = {}, y[8] = {}, dr[8] = {}, dz[8] = {};
-        if (in) {
-            load8<DT, VEC>(a.x, row, c, D, x);
-            if (a.y) load8<DT, VEC>(a.y, row, c, D, y);
-            if (a.dr) load8<DT, VEC>(a.dr, row, c, D, dr);
-            if (a.pre) load8<DT, VEC>(a.dz, row, c, D, dz);
+        const int n = min(R, l1 - l);
+        float x[R][8] = {}, y[R][8] = {}, dr[R][8] = {}, dz[R][8] = {};
+        float4 st[R];
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+            st[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k < n) {
+                if (in) {
+                    load8<DT, VEC>(a.x, row + k, c, D, x[k]);
+                    if (a.y) load8<DT, VEC>(a.y, row + k, c, D, y[k]);
+                    if (a.dr) load8<DT, VEC>(a.dr, row + k, c, D, dr[k]);
+                    if (a.pre) load8<DT, VEC>(a.dz, row + k, c, D, dz[k]);
+                }
+                st[k] = *reinterpret_cast<const float4*>(a.stats + 4 * (row + k));
+            }
         }
-        const float4 st = *reinterpret_cast<const float4*>(a.stats + 4 * row);
+        // (rows past the chunk: dr, dz and 1 / sd are zero, so they add nothing to any sum)
         if (a.y) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                y[i] = c + i < D ? (y[i] - st.x) * st.y : 0.f;
-                x[i] = __builtin_fmaf(f[i], __builtin_fmaf(y[i], qw[i], qb[i]), x[i]);
-            }
+            for (int k = 0; k < R; ++k)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    y[k][i] = c + i < D ? (y[k][i] - st[k].x) * st[k].y : 0.f;
+                    x[k][i] = __builtin_fmaf(f[i], __builtin_fmaf(y[k][i], qw[i], qb[i]), x[k][i]);
+                }
         }
         if (a.pre) {
-            float t0 = 0.f, t1 = 0.f;
+            float t[2 * R] = {};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[i] = c + i < D ? (x[i] - st.z) * st.w : 0.f;                 // r^
-                const float d = dz[i] * pw[i];
-                t0 += d;
-                t1 = __builtin_fmaf(d, x[i], t1);
-                s2[i] += dz[i];
-                s3[i] = __builtin_fmaf(dz[i], x[i], s3[i]);
+            for (int k = 0; k < R; ++k)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    x[k][i] = c + i < D ? (x[k][i] - st[k].z) * st[k].w : 0.f;                 // r^
+                    const float d = dz[k][i] * pw[i];
+                    t[2 * k] += d;
+                    t[2 * k + 1] = __builtin_fmaf(d, x[k][i], t[2 * k + 1]);
+                    s2[i] += dz[k][i];
+                    s3[i] = __builtin_fmaf(dz[k][i], x[k][i], s3[i]);
+                }
+            meet.sum(t);
+#pragma unroll
+            for (int k = 0; k < R; ++k) {
+                const float m0 = a.pre_centred ? t[2 * k] * rD : 0.f, m1 = t[2 * k + 1] * rD;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) dr[k][i] = c + i < D ? __builtin_fmaf(st[k].w, dz[k][i] * pw[i] - m0 - x[k][i] * m1, dr[k][i]) : 0.f;
             }
-            meet.sum2(t0, t1);
-            const float m0 = a.pre == LAYER ? t0 * rD : 0.f, m1 = t1 * rD;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) dr[i] = c + i < D ? __builtin_fmaf(st.w, dz[i] * pw[i] - m0 - x[i] * m1, dr[i]) : 0.f;
         }
-        if (in) store8<DT, VEC>(a.dx, row, c, D, dr);
+#pragma unroll
+        for (int k = 0; k < R; ++k)
+            if (in && k < n) store8<DT, VEC>(a.dx, row + k, c, D, dr[k]);
         if (a.y) {
-            float d[8], t0 = 0.f, t1 = 0.f;
+            float t[2 * R] = {};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                s0[i] += dr[i];
-                s1[i] = __builtin_fmaf(dr[i], y[i], s1[i]);
-                d[i] = c + i < D ? dr[i] * f[i] * qw[i] : 0.f;
-                t0 += d[i];
-                t1 = __builtin_fmaf(d[i], y[i], t1);
-            }
+            for (int k = 0; k < R; ++k)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    s0[i] += dr[k][i];
+                    s1[i] = __builtin_fmaf(dr[k][i], y[k][i], s1[i]);
+                    dr[k][i] = c + i < D ? dr[k][i] * f[i] * qw[i] : 0.f;
+                    t[2 * k] += dr[k][i];
+                    t[2 * k + 1] = __builtin_fmaf(dr[k][i], y[k][i], t[2 * k + 1]);
+                }
             if (a.post) {
-                meet.sum2(t0, t1);
-                const float m0 = a.post == LAYER ? t0 * rD : 0.f, m1 = t1 * rD;
+                meet.sum(t);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] = st.y * (d[i] - m0 - y[i] * m1);
+                for (int k = 0; k < R; ++k) {
+                    const float m0 = a.post_centred ? t[2 * k] * rD : 0.f, m1 = t[2 * k + 1] * rD;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) dr[k][i] = st[k].y * (dr[k][i] - m0 - y[k][i] * m1);
+                }
             }
-            if (in) store8<DT, VEC>(a.dy, row, c, D, d);
+#pragma unroll
+            for (int k = 0; k < R; ++k)
+                if (in && k < n) store8<DT, VEC>(a.dy, row + k, c, D, dr[k]);
         }
     }
     float* p = a.part + (int64_t)blockIdx.x * 4 * D;
@@ -306,9 +370,9 @@ template <int DT>
 int fwd(const NormArgs& a, hipStream_t st) {
     const int64_t rows = (int64_t)a.B * a.L;
     const int threads = 64 * cdiv(a.D, 512);
-    const unsigned grid = (unsigned)std::min<int64_t>(rows, 4096);
-    if (vec_ok(a)) norm_fwd_kernel<DT, true><<<grid, threads, 0, st>>>(a, rows);
-    else norm_fwd_kernel<DT, false><<<grid, threads, 0, st>>>(a, rows);
+    if (vec_ok(a) && threads <= 512 && rows >= 4096) norm_fwd_kernel<DT, true, 4, 512><<<2048, threads, 0, st>>>(a, rows);
+    else if (vec_ok(a)) norm_fwd_kernel<DT, true, 1, 1024><<<(unsigned)std::min<int64_t>(rows, 8192), threads, 0, st>>>(a, rows);
+    else norm_fwd_kernel<DT, false, 1, 1024><<<(unsigned)std::min<int64_t>(rows, 8192), threads, 0, st>>>(a, rows);
     ISB_LAUNCHED("norm_fwd", st);
     return ISB_OK;
 }
@@ -318,8 +382,9 @@ int bwd(NormArgs a, float* ws, hipStream_t st) {
     a.part = ws;
     float* joint = ws + (int64_t)a.B * a.chunks * 4 * a.D;
     const int threads = 64 * cdiv(a.D, 512);
-    if (vec_ok(a)) norm_bwd_kernel<DT, true><<<a.B * a.chunks, threads, 0, st>>>(a);
-    else norm_bwd_kernel<DT, false><<<a.B * a.chunks, threads, 0, st>>>(a);
+    if (vec_ok(a) && threads <= 512) norm_bwd_kernel<DT, true, 2, 512><<<a.B * a.chunks, threads, 0, st>>>(a);
+    else if (vec_ok(a)) norm_bwd_kernel<DT, true, 1, 1024><<<a.B * a.chunks, threads, 0, st>>>(a);
+    else norm_bwd_kernel<DT, false, 1, 1024><<<a.B * a.chunks, threads, 0, st>>>(a);
     ISB_LAUNCHED("norm_bwd", st);
     norm_join_kernel<DT><<<dim3(cdiv(a.D, 64), a.B), 256, 0, st>>>(a, joint);
     ISB_LAUNCHED("norm_join", st);

@@ -319,32 +319,43 @@ __global__ __launch_bounds__(256, 1) void xattn_token_kernel(XattnArgs a) {
     store_row<F16, DT>(a, bk, hk, split, r, acc, mm, ll, h);
 }
 
-// join the splits of a row in their order: one wave per row
+// join the splits of a row in their order: DT / 4 lanes per row, four columns each; a lane weighs one split (or two, ...) and hands its
+// weight round, so the loads of the partial sums do not wait for each other
 template <bool F16, int DT>
 __global__ __launch_bounds__(256) void xattn_join_kernel(XattnArgs a) {
     T16<F16>::enter();
-    const int64_t rows = (int64_t)a.Bk * a.Hk * a.M, row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    constexpr int L = DT / 4;
+    const int64_t rows = (int64_t)a.Bk * a.Hk * a.M, row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
     if (row >= rows) return;
-    const int lane = threadIdx.x & 63;
-    constexpr int E = DT / 64;
+    const int lane = threadIdx.x % L;
     float mm = NEG_INF;
-    for (int s = 0; s < a.splits; ++s) mm = fmaxf(mm, a.part2[(s * rows + row) * 2]);
-    const float mu = mm == NEG_INF ? 0.f : mm;
-    float l = 0.f, o[E] = {};
-    for (int s = 0; s < a.splits; ++s) {
-        const float2 ml = *reinterpret_cast<const float2*>(a.part2 + (s * rows + row) * 2);
-        const float w = __builtin_amdgcn_exp2f(ml.x - mu);
-        l += w * ml.y;
+    for (int s = lane; s < a.splits; s += L) mm = fmaxf(mm, a.part2[(s * rows + row) * 2]);
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] += w * a.part[(s * rows + row) * DT + lane * E + e];
+    for (int o = 1; o < L; o <<= 1) mm = fmaxf(mm, __shfl_xor(mm, o));
+    const float mu = mm == NEG_INF ? 0.f : mm;
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = 0; s0 < a.splits; s0 += L) {
+        float w = 0.f, wl = 0.f;
+        if (s0 + lane < a.splits) {
+            const float2 ml = *reinterpret_cast<const float2*>(a.part2 + ((s0 + lane) * rows + row) * 2);
+            w = __builtin_amdgcn_exp2f(ml.x - mu);
+            wl = w * ml.y;
+        }
+        const int n = min(L, a.splits - s0);
+#pragma unroll 4
+        for (int s = 0; s < n; ++s) {
+            const float4 p = *reinterpret_cast<const float4*>(a.part + ((s0 + s) * rows + row) * DT + 4 * lane);
+            const float ws = __shfl(w, s, L);
+            l += __shfl(wl, s, L);
+            o.x = __builtin_fmaf(ws, p.x, o.x); o.y = __builtin_fmaf(ws, p.y, o.y); o.z = __builtin_fmaf(ws, p.z, o.z); o.w = __builtin_fmaf(ws, p.w, o.w);
+        }
     }
     const int grp = (int)(row / a.M);
     const RowAt w = row_at(a, grp / a.Hk, grp % a.Hk, (int)(row % a.M));
     const float inv = l == 0.f ? 0.f : 1.0f / l;
-    uint16_t* out = a.out + off_out(a, w);
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-        if (lane * E + e < a.D) out[lane * E + e] = T16<F16>::from_f32(o[e] * inv);
+    if (4 * lane < a.D)
+        *reinterpret_cast<uint2*>(a.out + off_out(a, w) + 4 * lane) = make_uint2(T16<F16>::pack2(o.x * inv, o.y * inv), T16<F16>::pack2(o.z * inv, o.w * inv));
     if (lane == 0) a.lse[off_lse(a, w)] = l == 0.f ? NEG_INF : (mm + __builtin_amdgcn_logf(l)) * LN2;
 }
 
@@ -639,10 +650,13 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
         }
 }
 
-// sums of the splits in their order: dst row = KEYS ? state of [Bk, Lk, Hk, D] : row of [B, Lq, Hq, D]; 16 lanes per row
+// sums of the splits in their order: the states' rows of [Bk, Lk, Hk, D] (KEYS: grid.y = dk, dv) or the query rows of [B, Lq, Hq, D]; 16
+// lanes per row
 template <bool F16, int DT, bool KEYS>
-__global__ __launch_bounds__(256) void xattn_sum_kernel(XattnArgs a, const float* part, uint16_t* dst, int n) {
+__global__ __launch_bounds__(256) void xattn_sum_kernel(XattnArgs a, int n) {
     T16<F16>::enter();
+    const float* part = blockIdx.y ? a.part2 : a.part;
+    uint16_t* dst = !KEYS ? a.dq : blockIdx.y ? a.dv : a.dk;
     const int64_t rows = (int64_t)a.Bk * a.Hk * n, row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
     if (row >= rows) return;
     const int grp = (int)(row / n), i = (int)(row % n), l = threadIdx.x & 15;
@@ -665,17 +679,20 @@ __global__ __launch_bounds__(256) void xattn_sum_kernel(XattnArgs a, const float
 // ------------------------------------------------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------------------------------------------------
-constexpr int WANTED = 512;               // workgroups that fill the chip: two on each of the 256 CUs
-
-// splits of `len` (in units of `unit`) so that base * splits reaches WANTED, each split at least `least` units long
-void choose_splits(int64_t base, int len, int unit, int least, int& splits, int& chunk) {
+// splits of `len` (in units of `unit`) so that base * splits comes up to, not over, `wanted` workgroups; each at least `least` units long
+void choose_splits(int64_t base, int wanted, int len, int unit, int least, int& splits, int& chunk) {
     const int64_t units = cdiv(std::max(len, 1), unit);
-    int64_t s = std::min<int64_t>((WANTED + base - 1) / base, std::max<int64_t>(1, units / least));
+    int64_t s = std::min<int64_t>(wanted / base, units / least);
     s = std::min<int64_t>(std::max<int64_t>(s, 1), 64);
     const int64_t per = (units + s - 1) / s;
     splits = (int)((units + per - 1) / per);
     chunk = (int)(per * unit);
 }
+// One workgroup per CU is where splitting stops to pay (us, forward / dK dV / dQ alone, 1 split .. more; 120 workgroups without a split:
+// 46.1, 42.4 (2), 50.8 (5); 30: 37.3, 22.9 (4), 24.3 (8), 31.7 (15); 416: 27.7, 46.1 (2); dK dV with 30: 153 -> 64.3 (8), 75.7 (12); with
+// 192: 78.4, 96.5 (2)): the partial results cost more than the idle half of a CU. Single tokens read instead of compute: two workgroups
+// per CU, and no split under 3 x 128 states (tick of 1800 states: 9.8 with 5, 11.7 with 15).
+constexpr int CUS = 256;
 int dt_of(const XattnArgs& a) { return a.D <= 64 ? 64 : 128; }
 bool few_rows(const XattnArgs& a) { return a.M <= 32; }
 
@@ -685,23 +702,23 @@ Plan plan_fwd(const XattnArgs& a) {
     const int64_t groups = (int64_t)a.Bk * a.Hk;
     if (few_rows(a)) {
         p.tiles = 1;
-        choose_splits(groups, a.Lk, 128, 1, p.splits, p.chunk);
+        choose_splits(groups, 2 * CUS, a.Lk, 128, 3, p.splits, p.chunk);
     } else {
         p.tiles = cdiv(a.M, 128);
-        choose_splits(groups * p.tiles, a.Lk, KT, 4, p.splits, p.chunk);
+        choose_splits(groups * p.tiles, CUS, a.Lk, KT, 2, p.splits, p.chunk);
     }
     return p;
 }
 Plan plan_dkv(const XattnArgs& a) {
     Plan p{};
     p.tiles = cdiv(a.Lk, 128);
-    choose_splits((int64_t)a.Bk * a.Hk * p.tiles, a.M, 32, 8, p.splits, p.chunk);
+    choose_splits((int64_t)a.Bk * a.Hk * p.tiles, CUS, a.M, 32, 4, p.splits, p.chunk);
     return p;
 }
 Plan plan_dq(const XattnArgs& a) {
     Plan p{};
     p.tiles = cdiv(a.M, 128);
-    choose_splits((int64_t)a.Bk * a.Hk * p.tiles, a.Lk, KT, 4, p.splits, p.chunk);
+    choose_splits((int64_t)a.Bk * a.Hk * p.tiles, CUS, a.Lk, KT, 2, p.splits, p.chunk);
     return p;
 }
 int items(XattnArgs& a, const Plan& p, unsigned& grid) {
@@ -737,7 +754,8 @@ int fwd(XattnArgs a, float* ws, hipStream_t st) {
     if (few_rows(a)) ISB_TRY((launch<xattn_token_kernel<F16, DT>>("xattn_token", grid, 4 * 4 * 32 * DT * 2, a, st)));
     else ISB_TRY((launch<xattn_fwd_kernel<F16, DT>>("xattn_fwd", grid, 4 * KT * DT * 2, a, st)));
     if (p.splits > 1) {
-        xattn_join_kernel<F16, DT><<<(unsigned)((rows + 3) / 4), 256, 0, st>>>(a);
+        constexpr int per = 1024 / DT;
+        xattn_join_kernel<F16, DT><<<(unsigned)((rows + per - 1) / per), 256, 0, st>>>(a);
         ISB_LAUNCHED("xattn_join", st);
     }
     return ISB_OK;
@@ -758,17 +776,14 @@ int bwd(XattnArgs a, float* ws, hipStream_t st) {
     a.part2 = part + (int64_t)p.splits * states * DT;
     ISB_TRY((launch<xattn_dkv_kernel<F16, DT>>("xattn_dkv", grid, 2 * (2 * 32 * DT * 2 + 256), a, st)));
     if (p.splits > 1) {
-        const unsigned g = (unsigned)((states + 15) / 16);
-        xattn_sum_kernel<F16, DT, true><<<g, 256, 0, st>>>(a, a.part, a.dk, a.Lk);
-        ISB_LAUNCHED("xattn_sum dk", st);
-        xattn_sum_kernel<F16, DT, true><<<g, 256, 0, st>>>(a, a.part2, a.dv, a.Lk);
-        ISB_LAUNCHED("xattn_sum dv", st);
+        xattn_sum_kernel<F16, DT, true><<<dim3((unsigned)((states + 15) / 16), 2), 256, 0, st>>>(a, a.Lk);
+        ISB_LAUNCHED("xattn_sum dk, dv", st);
     }
     p = plan_dq(a);
     ISB_TRY(items(a, p, grid));
     ISB_TRY((launch<xattn_dq_kernel<F16, DT>>("xattn_dq", grid, 4 * KT * DT * 2, a, st)));
     if (p.splits > 1) {
-        xattn_sum_kernel<F16, DT, false><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(a, a.part, a.dq, a.M);
+        xattn_sum_kernel<F16, DT, false><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(a, a.M);
         ISB_LAUNCHED("xattn_sum dq", st);
     }
     return ISB_OK;
