@@ -31,6 +31,7 @@ struct MmArgs {
     int64_t ldc;
     float *g, *u;                        // GATE: saved (or null); DH: read
     float* part;                         // OUT with splits > 1: [split][M][N]
+    float* cs;                           // DH: column sums of dG | dU over 32 rows, [ceil(M / 32)][2 F], or null
     int F, act;
     int tiles_m, tiles_n, n_items;
 };
@@ -99,6 +100,9 @@ __device__ __forceinline__ uint4 op_frag(const unsigned char* t, int r0, int ks,
     else return frag_cols<ROWS, 8, 4>(t, 16 * ks, r0, lane);
 }
 
+// what this wave's lanes wrote to LDS is there for its other lanes (a wave's LDS accesses are done in order; this keeps the compiler to it)
+__device__ __forceinline__ void corner_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 template <bool F16, int BM, int BN, int NWM, int NWN, int LA, int LB, int EPI>
 __global__ __launch_bounds__(NWM * NWN * 64, NWM * NWN >= 8 ? 2 : 1) void ffn_mm_kernel(MmArgs p) {
     T16<F16>::enter();
@@ -137,94 +141,147 @@ __global__ __launch_bounds__(NWM * NWN * 64, NWM * NWN >= 8 ? 2 : 1) void ffn_mm
         for (int j = 0; j < IN; ++j)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
-    if (t0 < t1) request(t0, 0);
-    for (int t = t0; t < t1; ++t) {
-        wait_all_and_meet();
-        const int buf = (t - t0) & 1;
-        if (t + 1 < t1) request(t + 1, buf ^ 1);
+    // Fragments run one k-step ahead of the products, also over the edge of a tile: the workgroup meets BEFORE the last k-step's products, when
+    // every wave holds its fragments of the old tile; the buffer is then free for the tile after next, whose requests have a whole tile's
+    // products to land, and the first fragments of the next tile arrive behind the last products of this one.
+    uint4 fa[2][IM], fb[2][IN];
+    auto fetch = [&](int buf, int ks, int into) {
         const unsigned char* at = conv_lds_dyn + buf * STAGE;
-        const unsigned char* bt = at + ABYTES;
 #pragma unroll
-        for (int ks = 0; ks < BK / 16; ++ks) {
-            uint4 a[IM], b[IN];
+        for (int i = 0; i < IM; ++i) fa[into][i] = op_frag<LA, BM>(at, wm * WM + 32 * i, ks, lane);
 #pragma unroll
-            for (int i = 0; i < IM; ++i) a[i] = op_frag<LA, BM>(at, wm * WM + 32 * i, ks, lane);
+        for (int j = 0; j < IN; ++j) fb[into][j] = op_frag<LB, BN>(at + ABYTES, wn * WN + 32 * j, ks, lane);
+    };
+    constexpr int KS = BK / 16;
+    if (t0 < t1) {
+        request(t0, 0);
+        wait_all_and_meet();
+        if (t0 + 1 < t1) request(t0 + 1, 1);
+        fetch(0, 0, 0);
+    }
+    for (int t = t0; t < t1; ++t) {
+        const int buf = (t - t0) & 1;
 #pragma unroll
-            for (int j = 0; j < IN; ++j) b[j] = op_frag<LB, BN>(bt, wn * WN + 32 * j, ks, lane);
+        for (int ks = 0; ks < KS; ++ks) {
+            if (ks + 1 < KS) {
+                fetch(buf, ks + 1, (ks + 1) & 1);
+            } else if (t + 1 < t1) {
+                wait_all_and_meet();
+                if (t + 2 < t1) request(t + 2, buf);
+                fetch(buf ^ 1, 0, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int j = 0; j < IN; ++j)
 #pragma unroll
-                for (int i = 0; i < IM; ++i) acc[i][j] = T16<F16>::mfma32(b[j], a[i], acc[i][j]);
+                for (int i = 0; i < IM; ++i) acc[i][j] = T16<F16>::mfma32(fb[ks & 1][j], fa[ks & 1][i], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 
+    // The accumulators hold 32 rows m a lane column each; memory wants whole rows. Each wave turns its 32 x WN blocks round in its own corner of
+    // the operand buffers (free now), so that WN / 4 lanes write one row: full lines instead of 32-byte pieces.
+    constexpr int LN = WN / 4, RS = WN + 4, STEP = 64 / LN;           // lanes per row, LDS row (floats), rows per step
+    static_assert(NW * 32 * RS * 4 <= 2 * STAGE, "the corners fit");
+    wait_all_and_meet();
+    float* corner = reinterpret_cast<float*>(conv_lds_dyn) + wave * 32 * RS;
+    const int cl = lane % LN, rl = lane / LN;
 #pragma unroll
     for (int i = 0; i < IM; ++i) {
-        const int m = m0 + wm * WM + 32 * i + (lane & 31);
-        if (m >= p.M) continue;
+#pragma unroll
+        for (int j = 0; j < IN; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *reinterpret_cast<float4*>(corner + (lane & 31) * RS + 32 * j + 8 * q + 4 * h) =
+                    make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+        corner_done();
+        const int mb = m0 + wm * WM + 32 * i;
+        float sg[4] = {}, su[4] = {};                                         // DH: column sums over the block's rows
         if constexpr (EPI == EPI_GATE) {
-#pragma unroll
-            for (int j = 0; j < IN; j += 2)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int f = (n0 + wn * WN + 32 * j) / 2 + 8 * q + 4 * h;
-                    if (f >= p.F) continue;
-                    float g[4], u[4], o[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) { g[e] = acc[i][j][4 * q + e]; u[e] = acc[i][j + 1][4 * q + e]; }
-                    if (p.bias) {
-                        const uint2 w = *reinterpret_cast<const uint2*>(p.bias + f);
-                        g[0] += T16<F16>::lo(w.x); g[1] += T16<F16>::hi(w.x); g[2] += T16<F16>::lo(w.y); g[3] += T16<F16>::hi(w.y);
-                    }
-                    if (p.bias2) {
-                        const uint2 w = *reinterpret_cast<const uint2*>(p.bias2 + f);
-                        u[0] += T16<F16>::lo(w.x); u[1] += T16<F16>::hi(w.x); u[2] += T16<F16>::lo(w.y); u[3] += T16<F16>::hi(w.y);
-                    }
-                    const int64_t at = (int64_t)m * p.F + f;
-                    if (p.g) {
-                        *reinterpret_cast<float4*>(p.g + at) = make_float4(g[0], g[1], g[2], g[3]);
-                        *reinterpret_cast<float4*>(p.u + at) = make_float4(u[0], u[1], u[2], u[3]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = act_of(p.act, g[e]) * u[e];
-                    *reinterpret_cast<uint2*>(p.C + at) = make_uint2(T16<F16>::pack2(o[0], o[1]), T16<F16>::pack2(o[2], o[3]));
+            // half the lanes of a row: 4 features each, gate columns in the first 32 of every 64, up columns 32 further on
+            constexpr int LF = LN / 2, SF = 64 / LF;
+            const int c2 = lane % LF, r2 = lane / LF;
+            const int gc = (c2 >> 3) * 64 + (c2 & 7) * 4, f = (n0 + wn * WN) / 2 + 4 * c2;
+            float bg[4] = {}, bu[4] = {};
+            if (f < p.F) {
+                if (p.bias) {
+                    const uint2 w = *reinterpret_cast<const uint2*>(p.bias + f);
+                    bg[0] = T16<F16>::lo(w.x); bg[1] = T16<F16>::hi(w.x); bg[2] = T16<F16>::lo(w.y); bg[3] = T16<F16>::hi(w.y);
                 }
+                if (p.bias2) {
+                    const uint2 w = *reinterpret_cast<const uint2*>(p.bias2 + f);
+                    bu[0] = T16<F16>::lo(w.x); bu[1] = T16<F16>::hi(w.x); bu[2] = T16<F16>::lo(w.y); bu[3] = T16<F16>::hi(w.y);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 32; r += SF) {
+                const float4 g4 = *reinterpret_cast<const float4*>(corner + (r + r2) * RS + gc), u4 = *reinterpret_cast<const float4*>(corner + (r + r2) * RS + gc + 32);
+                const int m = mb + r + r2;
+                if (m >= p.M || f >= p.F) continue;
+                const float g[4] = {g4.x + bg[0], g4.y + bg[1], g4.z + bg[2], g4.w + bg[3]}, u[4] = {u4.x + bu[0], u4.y + bu[1], u4.z + bu[2], u4.w + bu[3]};
+                const int64_t at = (int64_t)m * p.F + f;
+                if (p.g) {
+                    *reinterpret_cast<float4*>(p.g + at) = make_float4(g[0], g[1], g[2], g[3]);
+                    *reinterpret_cast<float4*>(p.u + at) = make_float4(u[0], u[1], u[2], u[3]);
+                }
+                float o[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = act_of(p.act, g[e]) * u[e];
+                *reinterpret_cast<uint2*>(p.C + at) = make_uint2(T16<F16>::pack2(o[0], o[1]), T16<F16>::pack2(o[2], o[3]));
+            }
         } else {
-#pragma unroll
-            for (int j = 0; j < IN; ++j)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int n = n0 + wn * WN + 32 * j + 8 * q + 4 * h;
-                    if (n >= p.N) continue;
-                    float o[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o[e] = acc[i][j][4 * q + e];
-                    if constexpr (EPI == EPI_DH) {
-                        const int64_t at = (int64_t)m * p.F + n;
-                        const float4 g4 = *reinterpret_cast<const float4*>(p.g + at), u4 = *reinterpret_cast<const float4*>(p.u + at);
-                        const float g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w};
-                        float dg[4], du[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float f, s;
-                            act_and_slope(p.act, g[e], f, s);
-                            dg[e] = o[e] * u[e] * s;
-                            du[e] = o[e] * f;
-                        }
-                        uint16_t* c = p.C + (int64_t)m * p.ldc + n;
-                        *reinterpret_cast<uint2*>(c) = make_uint2(T16<F16>::pack2(dg[0], dg[1]), T16<F16>::pack2(dg[2], dg[3]));
-                        *reinterpret_cast<uint2*>(c + p.F) = make_uint2(T16<F16>::pack2(du[0], du[1]), T16<F16>::pack2(du[2], du[3]));
-                    } else if (p.splits > 1) {
-                        *reinterpret_cast<float4*>(p.part + ((int64_t)split * p.M + m) * p.N + n) = make_float4(o[0], o[1], o[2], o[3]);
-                    } else {
-                        if (p.bias) {
-                            const uint2 w = *reinterpret_cast<const uint2*>(p.bias + n);
-                            o[0] += T16<F16>::lo(w.x); o[1] += T16<F16>::hi(w.x); o[2] += T16<F16>::lo(w.y); o[3] += T16<F16>::hi(w.y);
-                        }
-                        *reinterpret_cast<uint2*>(p.C + (int64_t)m * p.ldc + n) = make_uint2(T16<F16>::pack2(o[0], o[1]), T16<F16>::pack2(o[2], o[3]));
-                    }
+            const int n = n0 + wn * WN + 4 * cl;
+            float bias[4] = {};
+            if constexpr (EPI == EPI_OUT)
+                if (p.bias && p.splits == 1 && n < p.N) {
+                    const uint2 w = *reinterpret_cast<const uint2*>(p.bias + n);
+                    bias[0] = T16<F16>::lo(w.x); bias[1] = T16<F16>::hi(w.x); bias[2] = T16<F16>::lo(w.y); bias[3] = T16<F16>::hi(w.y);
                 }
+#pragma unroll
+            for (int r = 0; r < 32; r += STEP) {
+                const float4 o = *reinterpret_cast<const float4*>(corner + (r + rl) * RS + 4 * cl);
+                const int m = mb + r + rl;
+                if (m >= p.M || n >= p.N) continue;
+                if constexpr (EPI == EPI_DH) {
+                    const int64_t at = (int64_t)m * p.F + n;
+                    const float4 g4 = *reinterpret_cast<const float4*>(p.g + at), u4 = *reinterpret_cast<const float4*>(p.u + at);
+                    const float g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w}, d[4] = {o.x, o.y, o.z, o.w};
+                    float dg[4], du[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float f, s;
+                        act_and_slope(p.act, g[e], f, s);
+                        dg[e] = d[e] * u[e] * s;
+                        du[e] = d[e] * f;
+                        sg[e] += dg[e];
+                        su[e] += du[e];
+                    }
+                    uint16_t* c = p.C + (int64_t)m * p.ldc + n;
+                    *reinterpret_cast<uint2*>(c) = make_uint2(T16<F16>::pack2(dg[0], dg[1]), T16<F16>::pack2(dg[2], dg[3]));
+                    *reinterpret_cast<uint2*>(c + p.F) = make_uint2(T16<F16>::pack2(du[0], du[1]), T16<F16>::pack2(du[2], du[3]));
+                } else if (p.splits > 1) {
+                    *reinterpret_cast<float4*>(p.part + ((int64_t)split * p.M + m) * p.N + n) = o;
+                } else {
+                    *reinterpret_cast<uint2*>(p.C + (int64_t)m * p.ldc + n) =
+                        make_uint2(T16<F16>::pack2(o.x + bias[0], o.y + bias[1]), T16<F16>::pack2(o.z + bias[2], o.w + bias[3]));
+                }
+            }
         }
+        if constexpr (EPI == EPI_DH) {
+            if (p.cs) {                                       // the block's column sums: the STEP lanes of a column, then one row of cs per 32 rows
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int o = LN; o < 64; o <<= 1) { sg[e] += __shfl_xor(sg[e], o); su[e] += __shfl_xor(su[e], o); }
+                const int n = n0 + wn * WN + 4 * cl;
+                if (rl == 0 && mb < p.M && n < p.N) {
+                    float* c = p.cs + (int64_t)(mb / 32) * 2 * p.F + n;
+                    *reinterpret_cast<float4*>(c) = make_float4(sg[0], sg[1], sg[2], sg[3]);
+                    *reinterpret_cast<float4*>(c + p.F) = make_float4(su[0], su[1], su[2], su[3]);
+                }
+            }
+        }
+        corner_done();
     }
 }
 
@@ -307,40 +364,52 @@ __global__ __launch_bounds__(256) void ffn_token_kernel(MmArgs p) {
     }
 }
 
-// ------------------------------------------------------------------------------------------------------------------------------------
-// column sums (bias gradients): 256 columns x ROWS rows per workgroup, partial sums joined in order
-// ------------------------------------------------------------------------------------------------------------------------------------
+// column sums over 32 rows of a 16-bit matrix: part [ceil(M / 32)][N]; 64 columns x 8 at a time, 4 row lanes
 template <bool F16>
-__global__ __launch_bounds__(256) void ffn_colsum_kernel(const uint16_t* x, int64_t ld, int M, int N, int rows, float* part) {
-    __shared__ float red[8][256];
-    const int c = threadIdx.x & 31, rl = threadIdx.x >> 5, n = blockIdx.x * 256 + 8 * c, m0 = blockIdx.y * rows, m1 = min(M, m0 + rows);
+__global__ __launch_bounds__(256) void ffn_colsum_kernel(const uint16_t* x, int64_t ld, int M, int N, float* part) {
+    __shared__ float red[4][512];
+    const int c = threadIdx.x & 63, rl = threadIdx.x >> 6, n = blockIdx.y * 512 + 8 * c, m0 = blockIdx.x * 32;
     float s[8] = {};
-    if (n < N)
-        for (int m = m0 + rl; m < m1; m += 8) {
+    if (n < N) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const int m = m0 + 4 * r + rl;
+            if (m >= M) continue;
             const uint4 v = *reinterpret_cast<const uint4*>(x + m * ld + n);
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) { s[2 * e] += T16<F16>::lo(w[e]); s[2 * e + 1] += T16<F16>::hi(w[e]); }
         }
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) red[rl][8 * c + e] = s[e];
     __syncthreads();
-    const int col = blockIdx.x * 256 + threadIdx.x;
-    if (col >= N) return;
-    float t = 0.f;
 #pragma unroll
-    for (int r = 0; r < 8; ++r) t += red[r][threadIdx.x];
-    part[(int64_t)blockIdx.y * N + col] = t;
+    for (int k = 0; k < 2; ++k) {
+        const int l = threadIdx.x + 256 * k, col = blockIdx.y * 512 + l;
+        if (col < N) part[(int64_t)blockIdx.x * N + col] = red[0][l] + red[1][l] + red[2][l] + red[3][l];
+    }
 }
+// bias gradients from the sums over 32 rows: columns of cs [parts][2 F] (gate, up), then of cd [parts][D] (down); 16 columns x 16 part lanes
 template <bool F16>
-__global__ __launch_bounds__(256) void ffn_colsum_join_kernel(const float* part, int parts, int N, uint16_t* out, uint16_t* out2, int n1) {
+__global__ __launch_bounds__(256) void ffn_bias_kernel(const float* cs, const float* cd, int parts, int F, int D, uint16_t* dbg, uint16_t* dbu, uint16_t* dbd) {
     T16<F16>::enter();
-    const int n = blockIdx.x * 256 + threadIdx.x;
-    if (n >= N) return;
+    __shared__ float red[16][16];
+    const int cl = threadIdx.x & 15, pl = threadIdx.x >> 4, i = blockIdx.x * 16 + cl, n2 = dbg ? 2 * F : 0;
+    const bool down = i >= n2;
+    const int n = down ? D : 2 * F, c = down ? i - n2 : i;
+    const float* p = (down ? cd : cs) + c;
+    const bool in = c < n && (!down || dbd);
     float t = 0.f;
-    for (int i = 0; i < parts; ++i) t += part[(int64_t)i * N + n];
-    uint16_t* o = n < n1 ? out + n : out2 + (n - n1);
-    *o = T16<F16>::from_f32(t);
+    if (in)
+        for (int k = pl; k < parts; k += 16) t += p[(int64_t)k * n];
+    red[pl][cl] = t;
+    __syncthreads();
+    if (pl != 0 || !in) return;
+    t = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) t += red[k][cl];
+    (down ? dbd[c] : c < F ? dbg[c] : dbu[c - F]) = T16<F16>::from_f32(t);
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------------
@@ -356,7 +425,7 @@ int tile_of(int la, int M, int N) {
 int splits_of(int la, int M, int N, int kts) {            // k splits of an OUT product whose tiles do not fill the chip
     const int t = tile_of(la, M, N), bm = t == TILE_THIN ? 32 : t == TILE_MID ? 128 : 256, bn = t == TILE_BIG ? 256 : 128;
     const int64_t tiles = (int64_t)cdiv(M, bm) * cdiv(N, bn);
-    const int64_t want = t == TILE_BIG ? 1 : (512 + tiles - 1) / tiles;
+    const int64_t want = t == TILE_BIG ? 1 : 512 / tiles;
     int s = (int)std::min<int64_t>(want, std::max(1, kts / 4));
     s = std::max(1, std::min(s, 16));
     return cdiv(kts, cdiv(kts, s));
@@ -406,8 +475,6 @@ size_t part_bytes(int la, int M, int N, int kts) {
     const int s = splits_of(la, M, N, kts);
     return s > 1 ? (size_t)s * M * N * 4 : 0;
 }
-constexpr int COLSUM_ROWS = 128;
-
 template <bool F16, int MT, bool GATE>
 int token(const MmArgs& p, hipStream_t st) {
     const int n = GATE ? p.F : p.N;
@@ -452,7 +519,20 @@ int bwd(const FfnArgs& a, unsigned char* ws, hipStream_t st) {
     // dG, dU from dh = dy Wd
     p.A = a.dy; p.B = a.wd; p.lda = a.dy_s; p.ldb = a.F; p.M = a.M; p.N = a.F; p.K = a.D; p.nseg = 1; p.splits = 1;
     p.g = a.g; p.u = a.u; p.F = a.F; p.act = a.act; p.C = dgu; p.ldc = 2 * (int64_t)a.F;
+    // (the bias gradients' partial sums use the place of the products' partial results before those need it)
+    const int parts = cdiv(a.M, 32);
+    float* down = part + (a.dbg ? (int64_t)parts * 2 * a.F : 0);
+    p.cs = a.dbg ? part : nullptr;
     ISB_TRY((mm<F16, 0, 1, EPI_DH>(p, "ffn dh", st)));
+    if (a.dbd) {
+        ffn_colsum_kernel<F16><<<dim3(parts, cdiv(a.D, 512)), 256, 0, st>>>(a.dy, a.dy_s, a.M, a.D, down);
+        ISB_LAUNCHED("ffn_colsum", st);
+    }
+    if (a.dbg || a.dbd) {
+        const int cols = (a.dbg ? 2 * a.F : 0) + (a.dbd ? a.D : 0);
+        ffn_bias_kernel<F16><<<cdiv(cols, 16), 256, 0, st>>>(part, down, parts, a.F, a.D, a.dbg, a.dbu, a.dbd);
+        ISB_LAUNCHED("ffn_bias", st);
+    }
     // dx = dG Wg + dU Wu
     p = MmArgs{};
     p.A = dgu; p.B = a.wg; p.B2 = a.wu; p.lda = 2 * (int64_t)a.F; p.ldb = a.D; p.M = a.M; p.N = a.D; p.K = a.F; p.nseg = 2;
@@ -467,18 +547,7 @@ int bwd(const FfnArgs& a, unsigned char* ws, hipStream_t st) {
     p = MmArgs{};
     p.A = a.dy; p.B = a.h; p.lda = a.dy_s; p.ldb = a.F; p.M = a.D; p.N = a.F; p.K = a.M; p.nseg = 1;
     p.C = a.dwd; p.ldc = a.F;
-    ISB_TRY((mm_out<F16, 1, 1>(p, part, "ffn dW down", st)));
-    auto colsum = [&](const uint16_t* x, int64_t ld, int N, uint16_t* o, uint16_t* o2, int n1) -> int {
-        const int parts = cdiv(a.M, COLSUM_ROWS);
-        ffn_colsum_kernel<F16><<<dim3(cdiv(N, 256), parts), 256, 0, st>>>(x, ld, a.M, N, COLSUM_ROWS, part);
-        ISB_LAUNCHED("ffn_colsum", st);
-        ffn_colsum_join_kernel<F16><<<cdiv(N, 256), 256, 0, st>>>(part, parts, N, o, o2, n1);
-        ISB_LAUNCHED("ffn_colsum_join", st);
-        return ISB_OK;
-    };
-    if (a.dbg) ISB_TRY(colsum(dgu, 2 * (int64_t)a.F, 2 * a.F, a.dbg, a.dbu, a.F));
-    if (a.dbd) ISB_TRY(colsum(a.dy, a.dy_s, a.D, a.dbd, a.dbd, a.D));
-    return ISB_OK;
+    return mm_out<F16, 1, 1>(p, part, "ffn dW down", st);
 }
 }  // namespace
 
@@ -488,9 +557,9 @@ size_t ffn_workspace(const FfnArgs& a, bool backward) {
         const size_t h = a.h ? 0 : (M * F * 2 + 255) / 256 * 256;
         return h + (a.M <= TOKENS ? 0 : part_bytes(0, a.M, a.D, cdiv(a.F, BK)));
     }
-    size_t part = std::max(part_bytes(0, a.M, a.D, 2 * cdiv(a.F, BK)),
-                           std::max(part_bytes(1, 2 * a.F, a.D, cdiv(a.M, BK)), part_bytes(1, a.D, a.F, cdiv(a.M, BK))));
-    if (a.dbg || a.dbd) part = std::max(part, (size_t)cdiv(a.M, COLSUM_ROWS) * std::max(2 * F, (size_t)a.D) * 4);
+    const size_t sums = (size_t)cdiv(a.M, 32) * ((a.dbg ? 2 * F : 0) + (a.dbd ? a.D : 0)) * 4;
+    const size_t part = std::max(std::max(sums, part_bytes(0, a.M, a.D, 2 * cdiv(a.F, BK))),
+                                 std::max(part_bytes(1, 2 * a.F, a.D, cdiv(a.M, BK)), part_bytes(1, a.D, a.F, cdiv(a.M, BK))));
     return (M * 2 * F * 2 + 255) / 256 * 256 + part;
 }
 int launch_ffn_fwd(const FfnArgs& a, bool f16, unsigned char* ws, hipStream_t st) { return f16 ? fwd<true>(a, ws, st) : fwd<false>(a, ws, st); }

@@ -15,30 +15,47 @@
 namespace isb {
 namespace {
 
-// eight neighbouring values at p + c (c < D; VEC: D % 8 == 0 and 16-byte rows), zeros past D
+// eight neighbouring values of a row at column c, as they lie in memory (VEC: D % 8 == 0 and 16-byte rows; else zeros past D): a row is
+// requested one row ahead and unpacked when its turn comes
 template <int DT, bool VEC>
-__device__ __forceinline__ void load8(const void* base, int64_t row, int c, int D, float (&v)[8]) {
-    if constexpr (DT == 0) {
-        const float* p = static_cast<const float*>(base) + row * D + c;
-        if constexpr (VEC) {
-            const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-        } else {
+struct Row8 {
+    uint4 a = make_uint4(0, 0, 0, 0), b = make_uint4(0, 0, 0, 0);            // b: f32's second half
+    __device__ __forceinline__ void load(const void* base, int64_t row, int c, int D) {
+        if constexpr (DT == 0) {
+            const uint32_t* p = static_cast<const uint32_t*>(base) + row * D + c;
+            if constexpr (VEC) {
+                a = reinterpret_cast<const uint4*>(p)[0];
+                b = reinterpret_cast<const uint4*>(p)[1];
+            } else {
+                uint32_t w[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = c + i < D ? p[i] : 0.f;
-        }
-    } else {
-        using T = T16<DT == 1>;
-        const uint16_t* p = static_cast<const uint16_t*>(base) + row * D + c;
-        if constexpr (VEC) {
-            const uint4 a = *reinterpret_cast<const uint4*>(p);
-            v[0] = T::lo(a.x); v[1] = T::hi(a.x); v[2] = T::lo(a.y); v[3] = T::hi(a.y); v[4] = T::lo(a.z); v[5] = T::hi(a.z); v[6] = T::lo(a.w); v[7] = T::hi(a.w);
+                for (int i = 0; i < 8; ++i) w[i] = c + i < D ? p[i] : 0u;
+                a = make_uint4(w[0], w[1], w[2], w[3]);
+                b = make_uint4(w[4], w[5], w[6], w[7]);
+            }
         } else {
+            const uint16_t* p = static_cast<const uint16_t*>(base) + row * D + c;
+            if constexpr (VEC) {
+                a = *reinterpret_cast<const uint4*>(p);
+            } else {
+                uint32_t w[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = c + i < D ? T::to_f32(p[i]) : 0.f;
+                for (int i = 0; i < 8; ++i) w[i] = c + i < D ? p[i] : 0u;
+                a = make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+            }
         }
     }
-}
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        if constexpr (DT == 0) {
+            v[0] = __uint_as_float(a.x); v[1] = __uint_as_float(a.y); v[2] = __uint_as_float(a.z); v[3] = __uint_as_float(a.w);
+            v[4] = __uint_as_float(b.x); v[5] = __uint_as_float(b.y); v[6] = __uint_as_float(b.z); v[7] = __uint_as_float(b.w);
+        } else {
+            using T = T16<DT == 1>;
+            v[0] = T::lo(a.x); v[1] = T::hi(a.x); v[2] = T::lo(a.y); v[3] = T::hi(a.y);
+            v[4] = T::lo(a.z); v[5] = T::hi(a.z); v[6] = T::lo(a.w); v[7] = T::hi(a.w);
+        }
+    }
+};
 template <int DT, bool VEC>
 __device__ __forceinline__ void store8(void* base, int64_t row, int c, int D, const float (&v)[8]) {
     if constexpr (DT == 0) {
@@ -66,131 +83,131 @@ __device__ __forceinline__ void param8(const float* p, int c, int D, float fill,
     for (int i = 0; i < 8; ++i) v[i] = p && c + i < D ? p[c + i] : fill;
 }
 
-// sums of N values over the workgroup, the same bits in every lane. The buffer's two halves take turns, so one barrier per call is enough.
-template <int MOST>
+// sum over the 64 lanes, in every lane, on the vector ALU alone (lane exchanges of 1, 2, 4, 8 as DPP, of 16 and 32 as row swaps)
+__device__ __forceinline__ float lanes_sum(float v) {
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xf, 0xf, true));      // quad_perm 1 0 3 2
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xf, 0xf, true));      // quad_perm 2 3 0 1
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xf, 0xf, true));     // half a row mirrored
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xf, 0xf, true));     // a row of 16 mirrored
+    const u32x2 r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return sum_halves(__uint_as_float(r.x) + __uint_as_float(r.y));
+}
+
+// sums over the workgroup, the same bits in every lane. The buffer's two halves take turns, so one barrier per call is enough.
 struct Meet {
-    float* buf;                              // [2][16 waves][MOST]
+    float* buf;                              // [2][16 waves][2]
     int waves, wave, lane, slot;
-    template <int N>
-    __device__ __forceinline__ void sum(float (&v)[N]) {
-        static_assert(N <= MOST, "buffer");
-#pragma unroll
-        for (int o = 32; o; o >>= 1)
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], o);
+    __device__ __forceinline__ void sum2(float& a, float& b) {
+        a = lanes_sum(a);
+        b = lanes_sum(b);
         if (waves == 1) return;
-        float* s = buf + slot * 16 * MOST;
+        float* s = buf + slot * 32;
         slot ^= 1;
-        if (lane == 0) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) s[wave * MOST + i] = v[i];
-        }
+        if (lane == 0) *reinterpret_cast<float2*>(s + 2 * wave) = make_float2(a, b);
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = 0.f;
-        for (int w = 0; w < waves; ++w)
-#pragma unroll
-            for (int i = 0; i < N; ++i) v[i] += s[w * MOST + i];
+        a = b = 0.f;
+        for (int w = 0; w < waves; ++w) {
+            const float2 t = *reinterpret_cast<const float2*>(s + 2 * w);
+            a += t.x;
+            b += t.y;
+        }
+    }
+    __device__ __forceinline__ float sum(float a) {
+        a = lanes_sum(a);
+        if (waves == 1) return a;
+        float* s = buf + slot * 32;
+        slot ^= 1;
+        if (lane == 0) s[wave] = a;
+        __syncthreads();
+        a = 0.f;
+        for (int w = 0; w < waves; ++w) a += s[w];
+        return a;
     }
 };
 
-// R rows v -> (v - mean) inv (RMS: no mean); columns past D stay zero. Which of the norms runs comes as separate flags: the compiler of
-// ROCm 7.2 makes ONE three-way switch of tests on a single `kind` and lowers its default case (uniform, a loop around it) wrongly -- the
-// copies into the merged registers are skipped.
-template <int R>
-__device__ __forceinline__ void normalise(bool centred, float (&v)[R][8], int c, int D, float eps, float (&mean)[R], float (&inv)[R], Meet<2 * R>& meet) {
-#pragma unroll
-    for (int k = 0; k < R; ++k) mean[k] = 0.f;
+// v -> (v - mean) inv (RMS: no mean); columns past D stay zero. Which of the norms runs comes as separate flags: the compiler of ROCm 7.2
+// makes ONE three-way switch of tests on a single `kind` and lowers its default case (uniform, a loop around it) wrongly -- the copies into
+// the merged registers are skipped.
+__device__ __forceinline__ void normalise(bool centred, float (&v)[8], int c, int D, float eps, float& mean, float& inv, Meet& meet) {
+    mean = 0.f;
     if (centred) {
+        float s = 0.f;
 #pragma unroll
-        for (int k = 0; k < R; ++k)
+        for (int i = 0; i < 8; ++i) s += v[i];
+        mean = meet.sum(s) / (float)D;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) mean[k] += v[k][i];
-        meet.sum(mean);
-#pragma unroll
-        for (int k = 0; k < R; ++k) {
-            mean[k] = mean[k] / (float)D;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[k][i] = c + i < D ? v[k][i] - mean[k] : 0.f;
-        }
+        for (int i = 0; i < 8; ++i) v[i] = c + i < D ? v[i] - mean : 0.f;
     }
-    float s[R] = {};
+    float s = 0.f;
 #pragma unroll
-    for (int k = 0; k < R; ++k)
+    for (int i = 0; i < 8; ++i) s = __builtin_fmaf(v[i], v[i], s);
+    inv = 1.0f / sqrtf(meet.sum(s) / (float)D + eps);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s[k] = __builtin_fmaf(v[k][i], v[k][i], s[k]);
-    meet.sum(s);
-#pragma unroll
-    for (int k = 0; k < R; ++k) {
-        inv[k] = 1.0f / sqrtf(s[k] / (float)D + eps);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[k][i] *= inv[k];
-    }
+    for (int i = 0; i < 8; ++i) v[i] *= inv;
 }
 
-// R rows at a time: their loads are in flight together and they share the barriers
-template <int DT, bool VEC, int R, int MOST>
-__global__ __launch_bounds__(MOST) void norm_fwd_kernel(NormArgs a, int64_t rows) {
+template <int DT, bool VEC, int MOST>
+__global__ __launch_bounds__(MOST, MOST <= 256 ? 5 : 4) void norm_fwd_kernel(NormArgs a, int rows) {
     if constexpr (DT == 1) T16<true>::enter();
-    __shared__ float buf[2 * 16 * 2 * R];
+    __shared__ __attribute__((aligned(16))) float buf[64];
     const int tid = threadIdx.x, c = tid * 8, D = a.D;
     const bool in = c < D;
-    Meet<2 * R> meet{buf, (int)blockDim.x >> 6, tid >> 6, tid & 63, 0};
-    float qw[8], qb[8], pw[8], pb[8], sc[8];
+    Meet meet{buf, (int)blockDim.x >> 6, tid >> 6, tid & 63, 0};
+    float qw[8], qb[8], pw[8], pb[8];
     param8(a.post_w, c, D, 1.f, qw);
     param8(a.post_b, c, D, 0.f, qb);
     param8(a.pre_w, c, D, 1.f, pw);
     param8(a.pre_b, c, D, 0.f, pb);
-    param8(a.scale, c, D, 1.f, sc);
-    for (int64_t row = (int64_t)blockIdx.x * R; row < rows; row += (int64_t)gridDim.x * R) {
-        const int n = (int)min((int64_t)R, rows - row);
-        float r[R][8] = {}, y[R][8] = {};
+    if (a.scale) {
+        float sc[8];
+        param8(a.scale, c, D, 1.f, sc);
 #pragma unroll
-        for (int k = 0; k < R; ++k)
-            if (in && k < n) {
-                load8<DT, VEC>(a.x, row + k, c, D, r[k]);
-                if (a.y) load8<DT, VEC>(a.y, row + k, c, D, y[k]);
-            }
-        float my[R] = {}, iy[R], mr[R] = {}, ir[R];
-#pragma unroll
-        for (int k = 0; k < R; ++k) iy[k] = ir[k] = 1.f;
+        for (int i = 0; i < 8; ++i) { qw[i] *= sc[i]; qb[i] *= sc[i]; }
+    }
+    Row8<DT, VEC> nx, ny;
+    auto request = [&](int row) {
+        if (in && row < rows) {
+            nx.load(a.x, row, c, D);
+            if (a.y) ny.load(a.y, row, c, D);
+        }
+    };
+    request(blockIdx.x);
+    for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+        float r[8], y[8], g[8];
+        nx.get(r);
+        ny.get(y);
+        request(row + gridDim.x);
+        float my = 0.f, iy = 1.f, mr = 0.f, ir = 1.f;
         if (a.y) {
-            if (a.post) normalise<R>(a.post_centred, y, c, D, a.eps, my, iy, meet);
 #pragma unroll
-            for (int k = 0; k < R; ++k) {
-                float g[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) g[i] = 1.f;
-                if (a.gate && in && k < n) load8<DT, VEC>(a.gate, (row + k) / a.L, c, D, g);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) r[k][i] = c + i < D ? __builtin_fmaf(sc[i] * g[i], __builtin_fmaf(y[k][i], qw[i], qb[i]), r[k][i]) : 0.f;
-                if (in && k < n) store8<DT, VEC>(a.r, row + k, c, D, r[k]);
+            for (int i = 0; i < 8; ++i) g[i] = 1.f;
+            if (a.gate && in) {
+                Row8<DT, VEC> t;
+                t.load(a.gate, row / a.L, c, D);
+                t.get(g);
             }
+            if (a.post) normalise(a.post_centred, y, c, D, a.eps, my, iy, meet);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) r[i] = c + i < D ? __builtin_fmaf(g[i], __builtin_fmaf(y[i], qw[i], qb[i]), r[i]) : 0.f;
+            if (in) store8<DT, VEC>(a.r, row, c, D, r);
         }
         if (a.pre) {
-            normalise<R>(a.pre_centred, r, c, D, a.eps, mr, ir, meet);
+            normalise(a.pre_centred, r, c, D, a.eps, mr, ir, meet);
 #pragma unroll
-            for (int k = 0; k < R; ++k) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) r[k][i] = __builtin_fmaf(r[k][i], pw[i], pb[i]);
-                if (in && k < n) store8<DT, VEC>(a.z, row + k, c, D, r[k]);
-            }
+            for (int i = 0; i < 8; ++i) r[i] = __builtin_fmaf(r[i], pw[i], pb[i]);
+            if (in) store8<DT, VEC>(a.z, row, c, D, r);
         }
-        if (a.stats && tid == 0) {
-#pragma unroll
-            for (int k = 0; k < R; ++k)
-                if (k < n) *reinterpret_cast<float4*>(a.stats + 4 * (row + k)) = make_float4(my[k], iy[k], mr[k], ir[k]);
-        }
+        if (a.stats && tid == 0) *reinterpret_cast<float4*>(a.stats + 4 * (int64_t)row) = make_float4(my, iy, mr, ir);
     }
 }
 
-template <int DT, bool VEC, int R, int MOST>
-__global__ __launch_bounds__(MOST) void norm_bwd_kernel(NormArgs a) {
+template <int DT, bool VEC, int MOST>
+__global__ __launch_bounds__(MOST, MOST <= 256 ? 3 : 4) void norm_bwd_kernel(NormArgs a) {
     if constexpr (DT == 1) T16<true>::enter();
-    __shared__ float buf[2 * 16 * 2 * R];
+    __shared__ __attribute__((aligned(16))) float buf[64];
     const int tid = threadIdx.x, c = tid * 8, D = a.D;
     const bool in = c < D;
-    Meet<2 * R> meet{buf, (int)blockDim.x >> 6, tid >> 6, tid & 63, 0};
+    Meet meet{buf, (int)blockDim.x >> 6, tid >> 6, tid & 63, 0};
     const int b = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
     const int l0 = chunk * a.rows_per_chunk, l1 = min(a.L, l0 + a.rows_per_chunk);
     float qw[8], qb[8], pw[8], f[8], g[8];
@@ -199,88 +216,78 @@ __global__ __launch_bounds__(MOST) void norm_bwd_kernel(NormArgs a) {
     param8(a.pre_w, c, D, 1.f, pw);
     param8(a.scale, c, D, 1.f, f);
     if (a.gate && in) {
-        load8<DT, VEC>(a.gate, b, c, D, g);
+        Row8<DT, VEC> t;
+        t.load(a.gate, b, c, D);
+        t.get(g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] *= g[i];
     }
     const float rD = 1.0f / (float)D;
     float s0[8] = {}, s1[8] = {}, s2[8] = {}, s3[8] = {};
-    for (int l = l0; l < l1; l += R) {
+    Row8<DT, VEC> nx, ny, ndr, ndz;
+    float4 nst = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto request = [&](int l) {
+        if (l >= l1) return;
         const int64_t row = (int64_t)b * a.L + l;
-        const int n = min(R, l1 - l);
-        float x[R][8] = {}, y[R][8] = {}, dr[R][8] = {}, dz[R][8] = {};
-        float4 st[R];
-#pragma unroll
-        for (int k = 0; k < R; ++k) {
-            st[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (k < n) {
-                if (in) {
-                    load8<DT, VEC>(a.x, row + k, c, D, x[k]);
-                    if (a.y) load8<DT, VEC>(a.y, row + k, c, D, y[k]);
-                    if (a.dr) load8<DT, VEC>(a.dr, row + k, c, D, dr[k]);
-                    if (a.pre) load8<DT, VEC>(a.dz, row + k, c, D, dz[k]);
-                }
-                st[k] = *reinterpret_cast<const float4*>(a.stats + 4 * (row + k));
-            }
+        if (in) {
+            nx.load(a.x, row, c, D);
+            if (a.y) ny.load(a.y, row, c, D);
+            if (a.dr) ndr.load(a.dr, row, c, D);
+            if (a.pre) ndz.load(a.dz, row, c, D);
         }
-        // (rows past the chunk: dr, dz and 1 / sd are zero, so they add nothing to any sum)
+        nst = *reinterpret_cast<const float4*>(a.stats + 4 * row);
+    };
+    request(l0);
+    for (int l = l0; l < l1; ++l) {
+        const int64_t row = (int64_t)b * a.L + l;
+        float x[8], y[8], dr[8], dz[8];
+        nx.get(x);
+        ny.get(y);
+        ndr.get(dr);
+        ndz.get(dz);
+        const float4 st = nst;
+        request(l + 1);
         if (a.y) {
 #pragma unroll
-            for (int k = 0; k < R; ++k)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    y[k][i] = c + i < D ? (y[k][i] - st[k].x) * st[k].y : 0.f;
-                    x[k][i] = __builtin_fmaf(f[i], __builtin_fmaf(y[k][i], qw[i], qb[i]), x[k][i]);
-                }
+            for (int i = 0; i < 8; ++i) {
+                y[i] = c + i < D ? (y[i] - st.x) * st.y : 0.f;
+                x[i] = __builtin_fmaf(f[i], __builtin_fmaf(y[i], qw[i], qb[i]), x[i]);
+            }
         }
         if (a.pre) {
-            float t[2 * R] = {};
+            float t0 = 0.f, t1 = 0.f;
 #pragma unroll
-            for (int k = 0; k < R; ++k)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    x[k][i] = c + i < D ? (x[k][i] - st[k].z) * st[k].w : 0.f;                 // r^
-                    const float d = dz[k][i] * pw[i];
-                    t[2 * k] += d;
-                    t[2 * k + 1] = __builtin_fmaf(d, x[k][i], t[2 * k + 1]);
-                    s2[i] += dz[k][i];
-                    s3[i] = __builtin_fmaf(dz[k][i], x[k][i], s3[i]);
-                }
-            meet.sum(t);
-#pragma unroll
-            for (int k = 0; k < R; ++k) {
-                const float m0 = a.pre_centred ? t[2 * k] * rD : 0.f, m1 = t[2 * k + 1] * rD;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) dr[k][i] = c + i < D ? __builtin_fmaf(st[k].w, dz[k][i] * pw[i] - m0 - x[k][i] * m1, dr[k][i]) : 0.f;
+            for (int i = 0; i < 8; ++i) {
+                x[i] = c + i < D ? (x[i] - st.z) * st.w : 0.f;                 // r^
+                const float d = dz[i] * pw[i];
+                t0 += d;
+                t1 = __builtin_fmaf(d, x[i], t1);
+                s2[i] += dz[i];
+                s3[i] = __builtin_fmaf(dz[i], x[i], s3[i]);
             }
+            meet.sum2(t0, t1);
+            const float m0 = a.pre_centred ? t0 * rD : 0.f, m1 = t1 * rD;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dr[i] = c + i < D ? __builtin_fmaf(st.w, dz[i] * pw[i] - m0 - x[i] * m1, dr[i]) : 0.f;
         }
-#pragma unroll
-        for (int k = 0; k < R; ++k)
-            if (in && k < n) store8<DT, VEC>(a.dx, row + k, c, D, dr[k]);
+        if (in) store8<DT, VEC>(a.dx, row, c, D, dr);
         if (a.y) {
-            float t[2 * R] = {};
+            float t0 = 0.f, t1 = 0.f;
 #pragma unroll
-            for (int k = 0; k < R; ++k)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    s0[i] += dr[k][i];
-                    s1[i] = __builtin_fmaf(dr[k][i], y[k][i], s1[i]);
-                    dr[k][i] = c + i < D ? dr[k][i] * f[i] * qw[i] : 0.f;
-                    t[2 * k] += dr[k][i];
-                    t[2 * k + 1] = __builtin_fmaf(dr[k][i], y[k][i], t[2 * k + 1]);
-                }
-            if (a.post) {
-                meet.sum(t);
-#pragma unroll
-                for (int k = 0; k < R; ++k) {
-                    const float m0 = a.post_centred ? t[2 * k] * rD : 0.f, m1 = t[2 * k + 1] * rD;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) dr[k][i] = st[k].y * (dr[k][i] - m0 - y[k][i] * m1);
-                }
+            for (int i = 0; i < 8; ++i) {
+                s0[i] += dr[i];
+                s1[i] = __builtin_fmaf(dr[i], y[i], s1[i]);
+                dr[i] = c + i < D ? dr[i] * f[i] * qw[i] : 0.f;
+                t0 += dr[i];
+                t1 = __builtin_fmaf(dr[i], y[i], t1);
             }
+            if (a.post) {
+                meet.sum2(t0, t1);
+                const float m0 = a.post_centred ? t0 * rD : 0.f, m1 = t1 * rD;
 #pragma unroll
-            for (int k = 0; k < R; ++k)
-                if (in && k < n) store8<DT, VEC>(a.dy, row + k, c, D, dr[k]);
+                for (int i = 0; i < 8; ++i) dr[i] = st.y * (dr[i] - m0 - y[i] * m1);
+            }
+            if (in) store8<DT, VEC>(a.dy, row, c, D, dr);
         }
     }
     float* p = a.part + (int64_t)blockIdx.x * 4 * D;
@@ -317,15 +324,15 @@ __global__ __launch_bounds__(256) void norm_join_kernel(NormArgs a, float* joint
         else static_cast<uint16_t*>(a.dgate)[(int64_t)b * D + c] = T16<DT == 1>::from_f32(v);
     }
 }
-// joint [B, 4, D] -> the parameters' gradients: 32 columns x 8 sample lanes
+// joint [B, 4, D] -> the parameters' gradients: 32 columns x 32 sample lanes
 template <int DT>
-__global__ __launch_bounds__(256) void norm_params_kernel(NormArgs a, const float* joint) {
-    __shared__ float red[8][5][32];
+__global__ __launch_bounds__(1024) void norm_params_kernel(NormArgs a, const float* joint) {
+    __shared__ float red[32][5][32];
     const int cl = threadIdx.x & 31, bl = threadIdx.x >> 5, c = blockIdx.x * 32 + cl, D = a.D;
     float s[5] = {};                         // dscale, dw_post, dbias_post, dw_pre, dbias_pre
     if (c < D) {
         const float w = a.post_w ? a.post_w[c] : 1.f, q = a.post_b ? a.post_b[c] : 0.f, sc = a.scale ? a.scale[c] : 1.f;
-        for (int b = bl; b < a.B; b += 8) {
+        for (int b = bl; b < a.B; b += 32) {
             const float* p = joint + (int64_t)b * 4 * D + c;
             float g = 1.f;
             if (a.gate) {
@@ -346,13 +353,15 @@ __global__ __launch_bounds__(256) void norm_params_kernel(NormArgs a, const floa
     if (c >= D || bl >= 5) return;
     float t = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) t += red[k][bl][cl];
+    for (int k = 0; k < 32; ++k) t += red[k][bl][cl];
     float* out[5] = {a.d_scale, a.d_post_w, a.d_post_b, a.d_pre_w, a.d_pre_b};
     float* o = bl == 0 ? out[0] : bl == 1 ? out[1] : bl == 2 ? out[2] : bl == 3 ? out[3] : out[4];
     if (o) o[c] = t;
 }
 
-constexpr int TEAMS = 1024;               // workgroups of the backward pass: enough to fill the chip, few enough for small partial sums
+// Workgroups that walk the rows: what the 256 CUs hold at once (five waves per SIMD forward, three backward, as the registers allow), so
+// that no second round is left over (rows of 1280: 2048 workgroups instead of 1536 took 98 us instead of 85)
+int walkers(int threads, int waves_per_simd) { return 256 * std::max(1, 4 * waves_per_simd / (threads / 64)); }
 
 bool vec_ok(const NormArgs& a) {
     uintptr_t m = 0;
@@ -362,17 +371,20 @@ bool vec_ok(const NormArgs& a) {
 // chunks of rows per sample; without a gate all rows are one sample
 void plan(NormArgs& a) {
     if (!a.gate) { a.L *= a.B; a.B = 1; }
-    const int want = std::max(1, TEAMS / a.B);
+    const int want = std::max(1, walkers(64 * cdiv(a.D, 512), 3) / a.B);
     a.rows_per_chunk = cdiv(a.L, std::min(want, a.L));
     a.chunks = cdiv(a.L, a.rows_per_chunk);
 }
 template <int DT>
 int fwd(const NormArgs& a, hipStream_t st) {
-    const int64_t rows = (int64_t)a.B * a.L;
-    const int threads = 64 * cdiv(a.D, 512);
-    if (vec_ok(a) && threads <= 512 && rows >= 4096) norm_fwd_kernel<DT, true, 4, 512><<<2048, threads, 0, st>>>(a, rows);
-    else if (vec_ok(a)) norm_fwd_kernel<DT, true, 1, 1024><<<(unsigned)std::min<int64_t>(rows, 8192), threads, 0, st>>>(a, rows);
-    else norm_fwd_kernel<DT, false, 1, 1024><<<(unsigned)std::min<int64_t>(rows, 8192), threads, 0, st>>>(a, rows);
+    const int rows = a.B * a.L, threads = 64 * cdiv(a.D, 512);
+    const unsigned grid = (unsigned)std::min(rows, walkers(threads, threads <= 256 ? 5 : 4));
+    if (vec_ok(a)) {
+        if (threads <= 256) norm_fwd_kernel<DT, true, 256><<<grid, threads, 0, st>>>(a, rows);
+        else norm_fwd_kernel<DT, true, 1024><<<grid, threads, 0, st>>>(a, rows);
+    } else {
+        norm_fwd_kernel<DT, false, 1024><<<grid, threads, 0, st>>>(a, rows);
+    }
     ISB_LAUNCHED("norm_fwd", st);
     return ISB_OK;
 }
@@ -382,13 +394,16 @@ int bwd(NormArgs a, float* ws, hipStream_t st) {
     a.part = ws;
     float* joint = ws + (int64_t)a.B * a.chunks * 4 * a.D;
     const int threads = 64 * cdiv(a.D, 512);
-    if (vec_ok(a) && threads <= 512) norm_bwd_kernel<DT, true, 2, 512><<<a.B * a.chunks, threads, 0, st>>>(a);
-    else if (vec_ok(a)) norm_bwd_kernel<DT, true, 1, 1024><<<a.B * a.chunks, threads, 0, st>>>(a);
-    else norm_bwd_kernel<DT, false, 1, 1024><<<a.B * a.chunks, threads, 0, st>>>(a);
+    if (vec_ok(a)) {
+        if (threads <= 256) norm_bwd_kernel<DT, true, 256><<<a.B * a.chunks, threads, 0, st>>>(a);
+        else norm_bwd_kernel<DT, true, 1024><<<a.B * a.chunks, threads, 0, st>>>(a);
+    } else {
+        norm_bwd_kernel<DT, false, 1024><<<a.B * a.chunks, threads, 0, st>>>(a);
+    }
     ISB_LAUNCHED("norm_bwd", st);
     norm_join_kernel<DT><<<dim3(cdiv(a.D, 64), a.B), 256, 0, st>>>(a, joint);
     ISB_LAUNCHED("norm_join", st);
-    norm_params_kernel<DT><<<cdiv(a.D, 32), 256, 0, st>>>(a, joint);
+    norm_params_kernel<DT><<<cdiv(a.D, 32), 1024, 0, st>>>(a, joint);
     ISB_LAUNCHED("norm_params", st);
     return ISB_OK;
 }
