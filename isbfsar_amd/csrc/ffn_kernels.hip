@@ -81,15 +81,20 @@ struct OpLoad {
             }
         }
     }
-    __device__ __forceinline__ void request(const uint16_t* base, const uint16_t* base2, int k_left, uint32_t lds, int wave) const {
-        const i32x4 d = dma_desc(base);
-        const i32x4 d2 = PAIR ? dma_desc(base2) : d;
-#pragma unroll
-        for (int j = 0; j < PIECES; ++j) {
-            const uint32_t v = kk[j] < k_left ? voff[j] : DMA_NONE;
-            const bool up = PAIR && (((wave * PIECES + j) >> 2) & 1);      // a piece is 8 rows: 4 pieces per 32-row group (wave-uniform)
-            dma16_desc(up ? d2 : d, v, lds + (wave * PIECES + j) * 1024);
-        }
+    // where the next tile comes from and goes to; its pieces can then be requested one by one
+    i32x4 d, d2;
+    int k_left;
+    uint32_t to;
+    __device__ __forceinline__ void aim(const uint16_t* base, const uint16_t* base2, int left, uint32_t lds, int wave) {
+        d = dma_desc(base);
+        d2 = PAIR ? dma_desc(base2) : d;
+        k_left = left;
+        to = lds + wave * PIECES * 1024;
+    }
+    __device__ __forceinline__ void piece(int j, int wave) const {
+        const uint32_t v = kk[j] < k_left ? voff[j] : DMA_NONE;
+        const bool up = PAIR && (((wave * PIECES + j) >> 2) & 1);          // a piece is 8 rows: 4 pieces per 32-row group (wave-uniform)
+        dma16_desc(up ? d2 : d, v, to + j * 1024);
     }
 };
 
@@ -112,8 +117,12 @@ __global__ __launch_bounds__(NWM * NWN * 64, NWM * NWN >= 8 ? 2 : 1) void ffn_mm
     constexpr int ABYTES = BM * BK * 2, STAGE = ABYTES + BN * BK * 2;
     const int item = xcd_item(blockIdx.x, p.n_items);
     if (item >= p.n_items) return;
-    // the m tiles of one n tile run side by side on an XCD: they read the same weights
-    const int tm = item % p.tiles_m, tn = item / p.tiles_m % p.tiles_n, split = item / p.tiles_m / p.tiles_n;
+    // An XCD runs a contiguous range of items, 32 or 64 at a time: bands of GM m tiles with the n tiles side by side make those a block of
+    // 8 x 4 or 8 x 8 tiles, whose operands its L2 fetches once (one n tile with every m tile instead: 384 us for 355, 7680 x 1280 x 5120)
+    constexpr int GM = 8;
+    const int split = item / (p.tiles_m * p.tiles_n), lin = item - split * p.tiles_m * p.tiles_n;
+    const int band = lin / (GM * p.tiles_n), bm = min(GM, p.tiles_m - band * GM), at_b = lin - band * GM * p.tiles_n;
+    const int tm = band * GM + at_b % bm, tn = at_b / bm;
     const int m0 = tm * BM, n0 = tn * BN;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
     const int wm = wave % NWM, wn = wave / NWM;
@@ -125,15 +134,17 @@ __global__ __launch_bounds__(NWM * NWN * 64, NWM * NWN >= 8 ? 2 : 1) void ffn_mm
     la.init(wave, lane, p.lda, p.M - m0);
     lb.init(wave, lane, p.ldb, PAIR ? p.F - n0 / 2 : p.N - n0);
     const uint32_t lds0 = lds_addr_of(conv_lds_dyn);
-    auto request = [&](int t, int buf) {
+    auto aim = [&](int t, int buf) {
         const int seg = t >= kts, kt = t - seg * kts;
         const int k0 = kt * BK;
         const uint16_t* a = LA == 0 ? p.A + (int64_t)m0 * p.lda + seg * p.K + k0 : p.A + (int64_t)k0 * p.lda + m0;
         const uint16_t* bb = PAIR || !seg ? p.B : p.B2;
         const int64_t off = LB == 0 ? (int64_t)(PAIR ? n0 / 2 : n0) * p.ldb + k0 : (int64_t)k0 * p.ldb + n0;
-        la.request(a, nullptr, p.K - k0, lds0 + buf * STAGE, wave);
-        lb.request(bb + off, PAIR ? p.B2 + off : nullptr, p.K - k0, lds0 + buf * STAGE + ABYTES, wave);
+        la.aim(a, nullptr, p.K - k0, lds0 + buf * STAGE, wave);
+        lb.aim(bb + off, PAIR ? p.B2 + off : nullptr, p.K - k0, lds0 + buf * STAGE + ABYTES, wave);
     };
+    constexpr int PA = decltype(la)::PIECES, PIECES = PA + decltype(lb)::PIECES;
+    auto piece = [&](int j) { if (j < PA) la.piece(j, wave); else lb.piece(j - PA, wave); };
     f32x16 acc[IM][IN];
 #pragma unroll
     for (int i = 0; i < IM; ++i)
@@ -143,39 +154,52 @@ __global__ __launch_bounds__(NWM * NWN * 64, NWM * NWN >= 8 ? 2 : 1) void ffn_mm
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
     // Fragments run one k-step ahead of the products, also over the edge of a tile: the workgroup meets BEFORE the last k-step's products, when
     // every wave holds its fragments of the old tile; the buffer is then free for the tile after next, whose requests have a whole tile's
-    // products to land, and the first fragments of the next tile arrive behind the last products of this one.
+    // products to land. Fragment reads and requests are issued one by one BETWEEN the products (the matrix pipe takes 32 cycles each).
     uint4 fa[2][IM], fb[2][IN];
-    auto fetch = [&](int buf, int ks, int into) {
+    auto fetch = [&](int buf, int ks, int i) {
         const unsigned char* at = conv_lds_dyn + buf * STAGE;
-#pragma unroll
-        for (int i = 0; i < IM; ++i) fa[into][i] = op_frag<LA, BM>(at, wm * WM + 32 * i, ks, lane);
-#pragma unroll
-        for (int j = 0; j < IN; ++j) fb[into][j] = op_frag<LB, BN>(at + ABYTES, wn * WN + 32 * j, ks, lane);
+        if (i < IN) fb[ks & 1][i] = op_frag<LB, BN>(at + ABYTES, wn * WN + 32 * i, ks, lane);
+        else fa[ks & 1][i - IN] = op_frag<LA, BM>(at, wm * WM + 32 * (i - IN), ks, lane);
     };
-    constexpr int KS = BK / 16;
+    constexpr int KS = BK / 16, SLOTS = IM * IN, FETCH = IM + IN;
+    static_assert(KS % 2 == 0, "k-step 0 of the next tile takes the other half of the fragment registers");
     if (t0 < t1) {
-        request(t0, 0);
+        aim(t0, 0);
+#pragma unroll
+        for (int j = 0; j < PIECES; ++j) piece(j);
         wait_all_and_meet();
-        if (t0 + 1 < t1) request(t0 + 1, 1);
-        fetch(0, 0, 0);
+        if (t0 + 1 < t1) {
+            aim(t0 + 1, 1);
+#pragma unroll
+            for (int j = 0; j < PIECES; ++j) piece(j);
+        }
+#pragma unroll
+        for (int i = 0; i < FETCH; ++i) fetch(0, 0, i);
     }
     for (int t = t0; t < t1; ++t) {
         const int buf = (t - t0) & 1;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            if (ks + 1 < KS) {
-                fetch(buf, ks + 1, (ks + 1) & 1);
-            } else if (t + 1 < t1) {
-                wait_all_and_meet();
-                if (t + 2 < t1) request(t + 2, buf);
-                fetch(buf ^ 1, 0, 0);
+            const bool edge = ks + 1 == KS, more = edge && t + 2 < t1;
+            if (edge) {
+                if (t + 1 < t1) wait_all_and_meet();
+                if (more) aim(t + 2, buf);
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < IN; ++j)
+            for (int s = 0; s < SLOTS; ++s) {
+                acc[s / IN][s % IN] = T16<F16>::mfma32(fb[ks & 1][s % IN], fa[ks & 1][s / IN], acc[s / IN][s % IN]);
 #pragma unroll
-                for (int i = 0; i < IM; ++i) acc[i][j] = T16<F16>::mfma32(fb[ks & 1][j], fa[ks & 1][i], acc[i][j]);
-            __builtin_amdgcn_sched_barrier(0);
+                for (int i = s * FETCH / SLOTS; i < (s + 1) * FETCH / SLOTS; ++i) {
+                    if (!edge) fetch(buf, ks + 1, i);
+                    else if (t + 1 < t1) fetch(buf ^ 1, 0, i);
+                }
+                if (more) {
+#pragma unroll
+                    for (int j = s * PIECES / SLOTS; j < (s + 1) * PIECES / SLOTS; ++j) piece(j);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
     }
 
