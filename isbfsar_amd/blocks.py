@@ -16,7 +16,6 @@ returned; nothing is recorded on an autograd tape and no result requires a gradi
 from __future__ import annotations
 
 import ctypes as C
-import math
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -28,17 +27,11 @@ NORMS = {None: 0, "layer": 1, "rms": 2}
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
-def _check(ok: bool, msg: str, *args) -> None:
-    if not ok:
-        raise ValueError(msg.format(*args))
+_HALF = (torch.float16, torch.bfloat16)
 
 
-def _on_gpu(name: str, t, dtype, device) -> None:
-    if not (isinstance(t, torch.Tensor) and t.is_cuda):
-        raise TypeError(f"{name} must be a torch CUDA tensor")
-    _check(t.device == device, "{} lives on {}, the first tensor on {}", name, t.device, device)
-    if t.dtype != dtype:
-        raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
+def _refuse(msg: str):
+    raise ValueError(msg)
 
 
 def _first(name: str, t, types) -> None:
@@ -48,64 +41,79 @@ def _first(name: str, t, types) -> None:
         raise TypeError(f"{name} is {t.dtype}, expected one of {sorted(str(x) for x in types)}")
 
 
-_HALF = (torch.float16, torch.bfloat16)
+def _tensor(name: str, t, dtype, device, shape) -> None:
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise TypeError(f"{name} must be a torch CUDA tensor")
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} lives on {t.device}, the first tensor on {device}")
+    if t.shape != shape:
+        raise ValueError(f"{name}: expected {tuple(shape)}, got {tuple(t.shape)}")
 
 
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t, or a contiguous copy where its last dimension is not contiguous or its rows do not lie on 16 bytes"""
-    if t.data_ptr() % 16 == 0 and t.stride(-1) == 1 and all(s % 8 == 0 for s in t.stride()[:-1]):
-        return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+def _rows16(t: torch.Tensor):
+    """(t, its leading strides), or a contiguous copy where its last dimension is not contiguous or its rows do not lie on 16 bytes"""
+    st = t.stride()
+    bits = t.data_ptr() & 15
+    for s in st[:-1]:
+        bits |= s & 7
+    if bits == 0 and st[-1] == 1:
+        return t, st[:-1]
+    t = _flat16(t)
+    st, n = [], 1
+    for d in reversed(t.shape):                  # (torch leaves the strides of dimensions of size 1 as they were)
+        st.append(n)
+        n *= d
+    return t, tuple(reversed(st))[:-1]
 
 
-def _flat16(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+def _flat16(t: torch.Tensor) -> torch.Tensor:
     """t contiguous on 16 bytes"""
-    if t is None:
-        return None
     t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return t.clone() if t.data_ptr() & 15 else t
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
-
-
-def _workspace(fn, what: str, args, *more) -> Tuple[Optional[torch.Tensor], int]:
+def _workspace(fn, what: str, args, *more) -> int:
     n = C.c_size_t()
-    _lib.check(fn(C.byref(args), *more, C.byref(n)), what)
+    rc = fn(C.byref(args), *more, C.byref(n))
+    if rc:
+        _lib.check(rc, what)
     return n.value
 
 
-def _stream(device) -> C.c_void_p:
-    return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+# the current stream's handle: the raw query costs 0.1 us of the 4 us that a launch takes, the stream object 2
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream(index: int) -> int:
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 # ------------------------------------------------------------------------------------------------ cross attention
 def _xattn_args(q, k, v, kv_len, key_mask, scale):
     _first("q", q, _HALF)
-    dev, t = q.device, q.dtype
-    _on_gpu("k", k, t, dev)
-    _on_gpu("v", v, t, dev)
-    _check(q.dim() == 4 and k.dim() == 4 and k.shape == v.shape, "expected q [B,Lq,Hq,D] and k, v [Bk,Lk,Hk,D], got {} {} {}",
-           tuple(q.shape), tuple(k.shape), tuple(v.shape))
+    t, dev = q.dtype, q.device
+    if q.dim() != 4 or not isinstance(k, torch.Tensor) or k.dim() != 4:
+        _refuse("expected q [B,Lq,Hq,D] and k, v [Bk,Lk,Hk,D]")
     B, Lq, Hq, D = q.shape
-    Bk, Lk, Hk, Dk = k.shape
-    _check(D == Dk, "head sizes {} and {} differ", D, Dk)
-    q, k, v = _rows16(q), _rows16(k), _rows16(v)
-    a = _lib.isb_xattn_args(dev.index, _TYPES[t], B, Bk, Lq, Lk, Hq, Hk, D, 1.0 / math.sqrt(max(D, 1)) if scale is None else float(scale),
-                            q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride()[:3], k.stride()[:3], v.stride()[:3])
+    Bk, Lk, Hk, _ = shape = k.shape
+    _tensor("k", k, t, dev, (Bk, Lk, Hk, D))
+    _tensor("v", v, t, dev, shape)
+    q, qs = _rows16(q)
+    k, ks = _rows16(k)
+    v, vs = _rows16(v)
+    a = _lib.isb_xattn_args(dev.index, _TYPES[t], B, Bk, Lq, Lk, Hq, Hk, D, D ** -0.5 if scale is None and D else float(scale or 0),
+                            q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs)
     keep = [q, k, v]
     if kv_len is not None:
-        _on_gpu("kv_len", kv_len, torch.int32, dev)
-        _check(tuple(kv_len.shape) == (Bk,), "kv_len: expected [{}], got {}", Bk, tuple(kv_len.shape))
+        _tensor("kv_len", kv_len, torch.int32, dev, (Bk,))
         kv_len = kv_len.contiguous()
         keep.append(kv_len)
         a.kv_len = kv_len.data_ptr()
     if key_mask is not None:
-        _on_gpu("key_mask", key_mask, torch.bool, dev)
-        _check(tuple(key_mask.shape) == (Bk, Lk), "key_mask: expected [{},{}], got {}", Bk, Lk, tuple(key_mask.shape))
-        if key_mask.stride(1) != 1:
+        _tensor("key_mask", key_mask, torch.bool, dev, (Bk, Lk))
+        if Lk > 1 and key_mask.stride(1) != 1:
             key_mask = key_mask.contiguous()
         keep.append(key_mask)
         a.key_mask, a.mask_stride = key_mask.data_ptr(), key_mask.stride(0)
@@ -121,13 +129,16 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_len: O
     support set for every window, read once for all of them. State j takes part iff j < kv_len[bk] (int32 [Bk]) and key_mask[bk, j]
     (bool [Bk,Lk]); a row without states gets zeros and lse = -inf. scale defaults to 1 / sqrt(D)."""
     a, keep = _xattn_args(q, k, v, kv_len, key_mask, scale)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=q.device)
+    B, Lq, Hq, _ = shape = q.shape
+    out = q.new_empty(shape)
+    lse = q.new_empty((B, Hq, Lq), dtype=torch.float32)
     a.out, a.lse = out.data_ptr(), lse.data_ptr()
     lib = _lib.lib()
     n = _workspace(lib.isb_xattn_workspace, "isb_xattn_workspace", a, 0)
-    ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-    _lib.check(lib.isb_xattn_forward(C.byref(a), _ptr(ws), n, _stream(q.device)), "isb_xattn_forward")
+    ws = q.new_empty(n, dtype=torch.uint8) if n else None
+    rc = lib.isb_xattn_forward(C.byref(a), ws.data_ptr() if n else None, n, _stream(a.device))
+    if rc:
+        _lib.check(rc, "isb_xattn_forward")
     return out, lse
 
 
@@ -138,47 +149,53 @@ def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     masked states get zeros."""
     a, keep = _xattn_args(q, k, v, kv_len, key_mask, scale)
     dev, t = q.device, q.dtype
-    _on_gpu("dout", dout, t, dev)
-    _on_gpu("out", out, t, dev)
-    _on_gpu("lse", lse, torch.float32, dev)
-    _check(dout.shape == q.shape and out.shape == q.shape, "dout, out: expected {}, got {} {}", tuple(q.shape), tuple(dout.shape), tuple(out.shape))
-    _check(tuple(lse.shape) == (q.shape[0], q.shape[2], q.shape[1]), "lse: expected [B,Hq,Lq], got {}", tuple(lse.shape))
-    dout, out, lse = _rows16(dout), _flat16(out), lse.contiguous()
-    dq = torch.empty(q.shape, dtype=t, device=dev)
-    dk = torch.empty(k.shape, dtype=t, device=dev)
-    dv = torch.empty(k.shape, dtype=t, device=dev)
-    a.out, a.lse, a.dout, a.dout_stride = out.data_ptr(), lse.data_ptr(), dout.data_ptr(), dout.stride()[:3]
+    _tensor("dout", dout, t, dev, q.shape)
+    _tensor("out", out, t, dev, q.shape)
+    _tensor("lse", lse, torch.float32, dev, (q.shape[0], q.shape[2], q.shape[1]))
+    dout, a.dout_stride = _rows16(dout)
+    out, lse = _flat16(out), lse.contiguous()
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), k.new_empty(k.shape)
+    a.out, a.lse, a.dout = out.data_ptr(), lse.data_ptr(), dout.data_ptr()
     a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
     lib = _lib.lib()
     n = _workspace(lib.isb_xattn_workspace, "isb_xattn_workspace", a, 1)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    _lib.check(lib.isb_xattn_backward(C.byref(a), ws.data_ptr(), n, _stream(dev)), "isb_xattn_backward")
+    ws = q.new_empty(n, dtype=torch.uint8)
+    rc = lib.isb_xattn_backward(C.byref(a), ws.data_ptr(), n, _stream(a.device))
+    if rc:
+        _lib.check(rc, "isb_xattn_backward")
     return dq, dk, dv
 
 
 # ------------------------------------------------------------------------------------------------ gated feed-forward block
 def _ffn_args(x, w_gate, w_up, w_down, activation):
     _first("x", x, _HALF)
-    dev, t = x.device, x.dtype
-    for n, w in (("w_gate", w_gate), ("w_up", w_up), ("w_down", w_down)):
-        _on_gpu(n, w, t, dev)
-    _check(x.dim() >= 1 and w_gate.dim() == 2, "expected x [..,D] and w_gate [F,D], got {} {}", tuple(x.shape), tuple(w_gate.shape))
-    F, D = w_gate.shape
-    _check(x.shape[-1] == D and tuple(w_up.shape) == (F, D) and tuple(w_down.shape) == (D, F),
-           "expected x [..,{}], w_up [{},{}], w_down [{},{}], got {} {} {}", D, F, D, D, F, tuple(x.shape), tuple(w_up.shape), tuple(w_down.shape))
-    _check(activation in ACTIVATIONS, "activation {!r} not in {}", activation, sorted(ACTIVATIONS))
-    x2 = _rows2(x)
-    w = [_flat16(w_gate), _flat16(w_up), _flat16(w_down)]
-    a = _lib.isb_ffn_args(dev.index, _TYPES[t], x2.shape[0], D, F, ACTIVATIONS[activation], x2.stride(0), 0, x2.data_ptr(),
-                          w[0].data_ptr(), w[1].data_ptr(), w[2].data_ptr())
-    return a, [x2, *w]
+    t, dev = x.dtype, x.device
+    if not isinstance(w_gate, torch.Tensor) or w_gate.dim() != 2 or x.dim() < 1:
+        _refuse("expected x [..,D] and w_gate [F,D]")
+    F, D = shape = w_gate.shape
+    if x.shape[-1] != D:
+        _refuse(f"x: expected [..,{D}], got {tuple(x.shape)}")
+    if x.numel() == 0:
+        _refuse(f"x has no rows: {tuple(x.shape)}")
+    _tensor("w_gate", w_gate, t, dev, shape)
+    _tensor("w_up", w_up, t, dev, shape)
+    _tensor("w_down", w_down, t, dev, (D, F))
+    if activation not in ACTIVATIONS:
+        _refuse(f"activation {activation!r} not in {sorted(ACTIVATIONS)}")
+    x2, xs = _rows2(x)
+    wg, wu, wd = _flat16(w_gate), _flat16(w_up), _flat16(w_down)
+    a = _lib.isb_ffn_args(dev.index, _TYPES[t], x2.shape[0], D, F, ACTIVATIONS[activation], xs, 0, x2.data_ptr(), wg.data_ptr(), wu.data_ptr(),
+                          wd.data_ptr())
+    return a, [x2, wg, wu, wd]
 
 
 def _rows2(x):
-    """x [.., D] as rows [M, D] whose starts lie on 16 bytes, a copy only where they do not; rows may be a constant stride apart, not
-    overlap"""
-    x2 = _rows16(x.reshape(-1, x.shape[-1]))
-    return x2 if x2.shape[0] == 1 or x2.stride(0) >= x2.shape[1] else x2.contiguous()
+    """x [.., D] as (rows [M, D], their stride), the rows on 16 bytes; a copy only where they are not a constant stride apart, overlap or
+    do not lie on 16 bytes"""
+    x2, (st,) = _rows16(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
+    if x2.shape[0] > 1 and st < x2.shape[1]:
+        x2, st = x2.contiguous(), x2.shape[1]
+    return x2, st
 
 
 def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, b_gate: Optional[torch.Tensor] = None,
@@ -190,26 +207,24 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     :func:`gated_ffn_backward` needs (both pre-activations in f32, the hidden rows in x's type)."""
     a, keep = _ffn_args(x, w_gate, w_up, w_down, activation)
     dev, t, M, D, F = x.device, x.dtype, a.M, a.D, a.F
-    for n, b, s in (("b_gate", b_gate, F), ("b_up", b_up, F), ("b_down", b_down, D)):
+    for n, b, size in (("b_gate", b_gate, F), ("b_up", b_up, F), ("b_down", b_down, D)):
         if b is not None:
-            _on_gpu(n, b, t, dev)
-            _check(tuple(b.shape) == (s,), "{}: expected [{}], got {}", n, s, tuple(b.shape))
+            _tensor(n, b, t, dev, (size,))
             b = _flat16(b)
             keep.append(b)
             setattr(a, n, b.data_ptr())
-    y = torch.empty(x.shape, dtype=t, device=dev)
-    if M == 0:
-        _check(False, "x has no rows")
+    y = x.new_empty(x.shape)
     a.y = y.data_ptr()
     saved = None
     if save:
-        saved = (torch.empty((M, F), dtype=torch.float32, device=dev), torch.empty((M, F), dtype=torch.float32, device=dev),
-                 torch.empty((M, F), dtype=t, device=dev))
+        saved = (x.new_empty((M, F), dtype=torch.float32), x.new_empty((M, F), dtype=torch.float32), x.new_empty((M, F)))
         a.pre_gate, a.pre_up, a.hidden = (s.data_ptr() for s in saved)
     lib = _lib.lib()
     n = _workspace(lib.isb_ffn_workspace, "isb_ffn_workspace", a, 0)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    _lib.check(lib.isb_ffn_forward(C.byref(a), _ptr(ws), n, _stream(dev)), "isb_ffn_forward")
+    ws = x.new_empty(n, dtype=torch.uint8) if n else None
+    rc = lib.isb_ffn_forward(C.byref(a), ws.data_ptr() if n else None, n, _stream(a.device))
+    if rc:
+        _lib.check(rc, "isb_ffn_forward")
     return (y, saved) if save else y
 
 
@@ -219,49 +234,55 @@ def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, 
     first weights' gradients are the halves of one [2F,D] tensor."""
     a, keep = _ffn_args(x, w_gate, w_up, w_down, activation)
     dev, t, M, D, F = x.device, x.dtype, a.M, a.D, a.F
-    _on_gpu("dy", dy, t, dev)
-    _check(dy.shape == x.shape, "dy: expected {}, got {}", tuple(x.shape), tuple(dy.shape))
-    _check(isinstance(saved, tuple) and len(saved) == 3, "saved: expected what gated_ffn(save=True) returned")
+    _tensor("dy", dy, t, dev, x.shape)
+    if not (isinstance(saved, tuple) and len(saved) == 3):
+        _refuse("saved: expected what gated_ffn(save=True) returned")
     for n, s, st in zip(("pre_gate", "pre_up", "hidden"), saved, (torch.float32, torch.float32, t)):
-        _on_gpu(n, s, st, dev)
-        _check(tuple(s.shape) == (M, F) and s.is_contiguous(), "{}: expected [{},{}], got {}", n, M, F, tuple(s.shape))
+        _tensor(n, s, st, dev, (M, F))
+        if not s.is_contiguous():
+            _refuse(f"{n} is not contiguous")
         setattr(a, n, s.data_ptr())
-    dy2 = _rows2(dy)
-    a.dy, a.dy_stride = dy2.data_ptr(), dy2.stride(0)
-    dx = torch.empty(x.shape, dtype=t, device=dev)
-    dw = torch.empty((2 * F, D), dtype=t, device=dev)
-    dwd = torch.empty((D, F), dtype=t, device=dev)
+    dy2, a.dy_stride = _rows2(dy)
+    a.dy = dy2.data_ptr()
+    dx, dw, dwd = x.new_empty(x.shape), x.new_empty((2 * F, D)), x.new_empty((D, F))
     a.dx, a.dw_gate_up, a.dw_down = dx.data_ptr(), dw.data_ptr(), dwd.data_ptr()
     r = {"dx": dx, "dw_gate": dw[:F], "dw_up": dw[F:], "dw_down": dwd}
     if bias:
-        db = torch.empty(2 * F + D, dtype=t, device=dev)
+        db = x.new_empty(2 * F + D)
         r["db_gate"], r["db_up"], r["db_down"] = db[:F], db[F:2 * F], db[2 * F:]
-        a.db_gate, a.db_up, a.db_down = (r[n].data_ptr() for n in ("db_gate", "db_up", "db_down"))
+        at = db.data_ptr()
+        a.db_gate, a.db_up, a.db_down = at, at + 2 * F, at + 4 * F
     lib = _lib.lib()
     n = _workspace(lib.isb_ffn_workspace, "isb_ffn_workspace", a, 1)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    _lib.check(lib.isb_ffn_backward(C.byref(a), ws.data_ptr(), n, _stream(dev)), "isb_ffn_backward")
+    ws = x.new_empty(n, dtype=torch.uint8)
+    rc = lib.isb_ffn_backward(C.byref(a), ws.data_ptr(), n, _stream(a.device))
+    if rc:
+        _lib.check(rc, "isb_ffn_backward")
     return r
 
 
 # ------------------------------------------------------------------------------------------------ norms around a block
 def _norm_args(x, y, gate, scale, post, post_weight, post_bias, pre, pre_weight, pre_bias, eps):
-    _first("x", x, tuple(_TYPES))
-    dev, t = x.device, x.dtype
-    _check(x.dim() == 3, "expected x [B,L,D], got {}", tuple(x.shape))
-    B, L, D = x.shape
-    _check(post in NORMS and pre in NORMS, "norms {!r}, {!r}: None, 'layer' or 'rms'", post, pre)
+    _first("x", x, _TYPES)
+    t, dev = x.dtype, x.device
+    if x.dim() != 3:
+        _refuse(f"x: expected [B,L,D], got {tuple(x.shape)}")
+    if post not in NORMS or pre not in NORMS:
+        _refuse(f"norms {post!r}, {pre!r}: None, 'layer' or 'rms'")
+    B, L, D = shape = x.shape
     x = x.contiguous()
-    keep = {"x": x}
-    for n, v, shape, dt in (("y", y, (B, L, D), t), ("gate", gate, (B, D), t), ("scale", scale, (D,), torch.float32),
-                            ("post_weight", post_weight, (D,), torch.float32), ("post_bias", post_bias, (D,), torch.float32),
-                            ("pre_weight", pre_weight, (D,), torch.float32), ("pre_bias", pre_bias, (D,), torch.float32)):
-        if v is not None:
-            _on_gpu(n, v, dt, dev)
-            _check(tuple(v.shape) == shape, "{}: expected {}, got {}", n, shape, tuple(v.shape))
-            keep[n] = v.contiguous()
-    p = [_ptr(keep.get(n)) for n in ("x", "y", "gate", "scale", "post_weight", "post_bias", "pre_weight", "pre_bias")]
-    return _lib.isb_norm_args(dev.index, _TYPES[t], B, L, D, NORMS[post], NORMS[pre], float(eps), *p), keep
+    keep, p, vec = [x], [x.data_ptr()], (D,)
+    for n, v, sh, dt in (("y", y, shape, t), ("gate", gate, (B, D), t), ("scale", scale, vec, torch.float32),
+                         ("post_weight", post_weight, vec, torch.float32), ("post_bias", post_bias, vec, torch.float32),
+                         ("pre_weight", pre_weight, vec, torch.float32), ("pre_bias", pre_bias, vec, torch.float32)):
+        if v is None:
+            p.append(None)
+        else:
+            _tensor(n, v, dt, dev, sh)
+            v = v.contiguous()
+            keep.append(v)
+            p.append(v.data_ptr())
+    return _lib.isb_norm_args(dev.index, _TYPES[t], B, L, D, NORMS[post], NORMS[pre], eps, *p), keep
 
 
 def block_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, gate: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None,
@@ -274,11 +295,19 @@ def block_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, gate: Optio
     None, "layer" or "rms" (no bias). y None: the norm before the first block, r is x itself. pre None: z is None. z is the norm of r
     before r is rounded; stats f32 [B,L,4] are for :func:`block_norm_backward`."""
     a, keep = _norm_args(x, y, gate, scale, post, post_weight, post_bias, pre, pre_weight, pre_bias, eps)
-    r = x if y is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    z = None if pre is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((*x.shape[:2], 4), dtype=torch.float32, device=x.device) if save else None
-    a.r, a.z, a.stats = None if y is None else r.data_ptr(), _ptr(z), _ptr(stats)
-    _lib.check(_lib.lib().isb_norm_forward(C.byref(a), _stream(x.device)), "isb_norm_forward")
+    r, z, stats = x, None, None
+    if y is not None:
+        r = x.new_empty(x.shape)
+        a.r = r.data_ptr()
+    if pre is not None:
+        z = x.new_empty(x.shape)
+        a.z = z.data_ptr()
+    if save:
+        stats = x.new_empty((*x.shape[:2], 4), dtype=torch.float32)
+        a.stats = stats.data_ptr()
+    rc = _lib.lib().isb_norm_forward(C.byref(a), _stream(a.device))
+    if rc:
+        _lib.check(rc, "isb_norm_forward")
     return (r, z, stats) if save else (r, z)
 
 
@@ -291,30 +320,35 @@ def block_norm_backward(dr: Optional[torch.Tensor], dz: Optional[torch.Tensor], 
     "dpre_weight"?, "dpre_bias"?}, one for each tensor given. dr (or None: zeros) and dz are the gradients of r and z."""
     a, keep = _norm_args(x, y, gate, scale, post, post_weight, post_bias, pre, pre_weight, pre_bias, eps)
     dev, t = x.device, x.dtype
-    _check((dz is not None) == (pre is not None), "dz goes with a pre norm")
-    _check(dr is not None or dz is not None, "neither dr nor dz")
+    if (dz is not None) != (pre is not None):
+        _refuse("dz goes with a pre norm")
+    if dr is None and dz is None:
+        _refuse("neither dr nor dz")
     for n, v in (("dr", dr), ("dz", dz)):
         if v is not None:
-            _on_gpu(n, v, t, dev)
-            _check(v.shape == x.shape, "{}: expected {}, got {}", n, tuple(x.shape), tuple(v.shape))
-            keep[n] = v.contiguous()
-            setattr(a, n, keep[n].data_ptr())
-    _on_gpu("stats", stats, torch.float32, dev)
-    _check(tuple(stats.shape) == (*x.shape[:2], 4) and stats.is_contiguous(), "stats: expected [B,L,4], got {}", tuple(stats.shape))
+            _tensor(n, v, t, dev, x.shape)
+            v = v.contiguous()
+            keep.append(v)
+            setattr(a, n, v.data_ptr())
+    _tensor("stats", stats, torch.float32, dev, (*x.shape[:2], 4))
+    if not stats.is_contiguous():
+        _refuse("stats are not contiguous")
     a.stats = stats.data_ptr()
-    g = {"dx": torch.empty(x.shape, dtype=t, device=dev)}
+    g = {"dx": x.new_empty(x.shape)}
     if y is not None:
-        g["dy"] = torch.empty(x.shape, dtype=t, device=dev)
+        g["dy"] = x.new_empty(x.shape)
     if gate is not None:
-        g["dgate"] = torch.empty(gate.shape, dtype=t, device=dev)
+        g["dgate"] = x.new_empty(gate.shape)
     for n, v in (("dscale", scale), ("dpost_weight", post_weight), ("dpost_bias", post_bias), ("dpre_weight", pre_weight),
                  ("dpre_bias", pre_bias)):
         if v is not None:
-            g[n] = torch.empty(v.shape, dtype=torch.float32, device=dev)
+            g[n] = v.new_empty(v.shape)
     for n, v in g.items():
         setattr(a, n, v.data_ptr())
     lib = _lib.lib()
     n = _workspace(lib.isb_norm_workspace, "isb_norm_workspace", a)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    _lib.check(lib.isb_norm_backward(C.byref(a), ws.data_ptr(), n, _stream(dev)), "isb_norm_backward")
+    ws = x.new_empty(n, dtype=torch.uint8)
+    rc = lib.isb_norm_backward(C.byref(a), ws.data_ptr(), n, _stream(a.device))
+    if rc:
+        _lib.check(rc, "isb_norm_backward")
     return g

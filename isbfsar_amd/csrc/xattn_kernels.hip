@@ -131,34 +131,20 @@ __device__ __forceinline__ void attend(const unsigned char* kt, const unsigned c
         for (int t = 0; t < 2 * NB; ++t) acc[d] = T16<F16>::mfma32(frag_cols<DT, 4, 8>(vt, 16 * t, 32 * d, lane), p[t], acc[d]);
 }
 
-// results of a row: out and lse, or (splits) its unnormalised sums with maximum and sum
+// four columns of a row's results (and, `first`, what goes with the row): out and lse, or (splits) its unnormalised sums with maximum and sum
 template <bool F16, int DT>
-__device__ __forceinline__ void store_row(const XattnArgs& a, int bk, int hk, int split, int r, const f32x16 (&acc)[DT / 32], float m, float l, int h) {
+__device__ __forceinline__ void store_piece(const XattnArgs& a, int bk, int hk, int split, int r, int c, float4 o, float m, float l, bool first) {
     if (r >= a.M) return;
     if (a.splits > 1) {
         const int64_t at = ((int64_t)split * a.Bk * a.Hk + bk * a.Hk + hk) * a.M + r;
-        float* p = a.part + at * DT;
-#pragma unroll
-        for (int d = 0; d < DT / 32; ++d)
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                *reinterpret_cast<float4*>(p + 32 * d + 8 * q + 4 * h) = make_float4(acc[d][4 * q], acc[d][4 * q + 1], acc[d][4 * q + 2], acc[d][4 * q + 3]);
-        if (h == 0) *reinterpret_cast<float2*>(a.part2 + at * 2) = make_float2(m, l);
+        *reinterpret_cast<float4*>(a.part + at * DT + c) = o;
+        if (first) *reinterpret_cast<float2*>(a.part2 + at * 2) = make_float2(m, l);
         return;
     }
     const RowAt w = row_at(a, bk, hk, r);
     const float inv = l == 0.f ? 0.f : 1.0f / l;
-    uint16_t* o = a.out + off_out(a, w);
-#pragma unroll
-    for (int d = 0; d < DT / 32; ++d)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int at = 32 * d + 8 * q + 4 * h;
-            if (at < a.D)
-                *reinterpret_cast<uint2*>(o + at) = make_uint2(T16<F16>::pack2(acc[d][4 * q] * inv, acc[d][4 * q + 1] * inv),
-                                                               T16<F16>::pack2(acc[d][4 * q + 2] * inv, acc[d][4 * q + 3] * inv));
-        }
-    if (h == 0) a.lse[off_lse(a, w)] = l == 0.f ? NEG_INF : (m + __builtin_amdgcn_logf(l)) * LN2;
+    if (c < a.D) *reinterpret_cast<uint2*>(a.out + off_out(a, w) + c) = make_uint2(T16<F16>::pack2(o.x * inv, o.y * inv), T16<F16>::pack2(o.z * inv, o.w * inv));
+    if (first) a.lse[off_lse(a, w)] = l == 0.f ? NEG_INF : (m + __builtin_amdgcn_logf(l)) * LN2;
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------------
@@ -220,24 +206,33 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XattnArgs a) {
         bits = next;
     }
     l = sum_halves(l);
-    store_row<F16, DT>(a, bk, hk, split, r, acc, m, l, h);
+#pragma unroll
+    for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            store_piece<F16, DT>(a, bk, hk, split, r, 32 * d + 8 * q + 4 * h, make_float4(acc[d][4 * q], acc[d][4 * q + 1], acc[d][4 * q + 2], acc[d][4 * q + 3]),
+                                 m, l, d == 0 && q == 0 && h == 0);
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------------
-// Forward, at most 32 rows in a group (single tokens, grouped heads): the states are the work. Every wave walks its own blocks of 32
-// states through its own LDS (no barrier in the loop, the next block always in flight), the four waves' sums meet at the end.
+// Forward, at most 32 rows in a group (single tokens, grouped heads): the states are the work. Eight waves walk their own blocks of 32 states,
+// each through its own LDS and without a barrier in the loop -- a wave waits for its block while the others use theirs --, and their sums
+// meet at the end. Up to 2048 states one workgroup does all of a group in one launch (4 heads x 1800 states x 64: 10.7 us, as long as five
+// splits and their join; four waves with two buffers each: 9.6 in two launches, 28.9 for 24.0 where 128 groups of 128 wide fill the chip).
 // ------------------------------------------------------------------------------------------------------------------------------------
+constexpr int TOKEN_WAVES = 8;
 template <bool F16, int DT>
-__global__ __launch_bounds__(256, 1) void xattn_token_kernel(XattnArgs a) {
+__global__ __launch_bounds__(TOKEN_WAVES * 64, TOKEN_WAVES / 4) void xattn_token_kernel(XattnArgs a) {
+    constexpr int NW = TOKEN_WAVES;
     T16<F16>::enter();
     const int item = xcd_item(blockIdx.x, a.n_items);
     if (item >= a.n_items) return;
     const int split = item % a.splits, grp = item / a.splits, bk = grp / a.Hk, hk = grp % a.Hk;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5, r = lane & 31;
-    constexpr int TB = 32 * DT * 2, PIECES = TB / 1024;
+    constexpr int TB = 32 * DT * 2;
 
     const int len = states_of(a, bk), k0 = split * a.chunk, k1 = min(len, k0 + a.chunk);
-    const int nt = k1 > k0 ? (k1 - k0 + 31) / 32 : 0;                        // blocks of the workgroup; wave w takes w, w + 4, ...
+    const int nt = k1 > k0 ? (k1 - k0 + 31) / 32 : 0;                        // blocks of the workgroup; wave w takes w, w + NW, ...
     uint4 qf[DT / 16];
     {
         const RowAt w = row_at(a, bk, hk, min(r, a.M - 1));
@@ -254,47 +249,44 @@ __global__ __launch_bounds__(256, 1) void xattn_token_kernel(XattnArgs a) {
 
     const uint16_t* kb = a.k + bk * a.k_sb + hk * a.k_sh + (int64_t)k0 * a.k_sl;
     const uint16_t* vb = a.v + bk * a.v_sb + hk * a.v_sh + (int64_t)k0 * a.v_sl;
-    unsigned char* own = conv_lds_dyn + wave * 4 * TB;
+    unsigned char* own = conv_lds_dyn + wave * 2 * TB;
     const uint32_t lds0 = lds_addr_of(own);
     TileLoad<DT, 32, 1> lk, lv;
     lk.init(0, lane, a.k_sl, a.D);
     lv.init(0, lane, a.v_sl, a.D);
     auto valid = [&](int t) -> uint32_t { return t < nt ? mask_byte(a, bk, k0 + 32 * t + (lane & 31), k1) : 0u; };
-    auto request = [&](int t, uint32_t bits, int buf) {
+    auto request = [&](int t, uint32_t bits) {
         const int64_t at = (int64_t)t * 32;
-        lk.request(kb + at * a.k_sl, bits, lds0 + buf * 2 * TB, 0);
-        lv.request(vb + at * a.v_sl, bits, lds0 + buf * 2 * TB + TB, 0);
+        lk.request(kb + at * a.k_sl, bits, lds0, 0);
+        lv.request(vb + at * a.v_sl, bits, lds0 + TB, 0);
     };
-    uint32_t bits = (uint32_t)__ballot(valid(wave) != 0), byte = valid(wave + 4);
-    if (wave < nt) request(wave, bits, 0);
-    for (int t = wave, buf = 0; t < nt; t += 4, buf ^= 1) {
+    uint32_t bits = (uint32_t)__ballot(valid(wave) != 0), byte = valid(wave + NW);
+    if (wave < nt) request(wave, bits);
+    for (int t = wave; t < nt; t += NW) {
         const uint32_t next = (uint32_t)__ballot(byte != 0);
-        byte = valid(t + 8);
-        // this block's 2 * PIECES requests are the oldest; everything requested behind them may stay in flight
-        if (t + 4 < nt) {
-            request(t + 4, next, buf ^ 1);
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * PIECES) : "memory");
-        } else {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        }
-        if (bits != 0) attend<F16, DT, 1>(own + buf * 2 * TB, own + buf * 2 * TB + TB, qf, acc, m, l, a.c, bits, lane);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                    // the buffer is read before it is requested again
+        byte = valid(t + 2 * NW);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (bits != 0) attend<F16, DT, 1>(own, own + TB, qf, acc, m, l, a.c, bits, lane);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                    // the block is read before its place is requested again
+        if (t + NW < nt) request(t + NW, next);
         bits = next;
     }
     l = sum_halves(l);
-    // join the waves: (m, l) of all four, then every wave scales its sums to the common maximum and they are added in wave order
+    // join the waves: (m, l) of all, then every wave scales its sums to the common maximum and each adds up its share of the columns, in wave
+    // order
     wait_all_and_meet();
     float* ml = reinterpret_cast<float*>(conv_lds_dyn);
-    float* sums = ml + 256;                                                   // [4][32][DT + 4]
+    float* sums = ml + NW * 64;                                               // [NW][32][DT + 4]
     constexpr int SW = DT + 4;
+    static_assert((NW * 64 + NW * 32 * SW) * 4 <= NW * (2 * TB + 1024), "the sums fit");
     if (h == 0) { ml[(wave * 32 + r) * 2] = m; ml[(wave * 32 + r) * 2 + 1] = l; }
     __syncthreads();
     float mm = NEG_INF, ll = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) mm = fmaxf(mm, ml[(w * 32 + r) * 2]);
+    for (int w = 0; w < NW; ++w) mm = fmaxf(mm, ml[(w * 32 + r) * 2]);
     const float mu = mm == NEG_INF ? 0.f : mm;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) ll += ml[(w * 32 + r) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * 32 + r) * 2] - mu);
+    for (int w = 0; w < NW; ++w) ll += ml[(w * 32 + r) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * 32 + r) * 2] - mu);
     const float al = __builtin_amdgcn_exp2f(m - mu);
 #pragma unroll
     for (int d = 0; d < DT / 32; ++d)
@@ -303,20 +295,20 @@ __global__ __launch_bounds__(256, 1) void xattn_token_kernel(XattnArgs a) {
             *reinterpret_cast<float4*>(sums + (wave * 32 + r) * SW + 32 * d + 8 * q + 4 * h) =
                 make_float4(acc[d][4 * q] * al, acc[d][4 * q + 1] * al, acc[d][4 * q + 2] * al, acc[d][4 * q + 3] * al);
     __syncthreads();
-    if (wave != 0) return;
+    // piece (d, q): 8 columns (4 per lane half); wave w takes pieces w, w + NW, ...
 #pragma unroll
-    for (int d = 0; d < DT / 32; ++d)
+    for (int i = 0; i < (DT / 8 + NW - 1) / NW; ++i) {
+        const int piece = wave + i * NW;
+        if (piece >= DT / 8) continue;
+        const int c = 8 * piece + 4 * h;
+        float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                const float4 u = *reinterpret_cast<const float4*>(sums + (w * 32 + r) * SW + 32 * d + 8 * q + 4 * h);
-                t.x += u.x; t.y += u.y; t.z += u.z; t.w += u.w;
-            }
-            acc[d][4 * q] = t.x; acc[d][4 * q + 1] = t.y; acc[d][4 * q + 2] = t.z; acc[d][4 * q + 3] = t.w;
+        for (int w = 0; w < NW; ++w) {
+            const float4 u = *reinterpret_cast<const float4*>(sums + (w * 32 + r) * SW + c);
+            t.x += u.x; t.y += u.y; t.z += u.z; t.w += u.w;
         }
-    store_row<F16, DT>(a, bk, hk, split, r, acc, mm, ll, h);
+        store_piece<F16, DT>(a, bk, hk, split, r, c, t, mm, ll, piece == 0 && h == 0);
+    }
 }
 
 // join the splits of a row in their order: DT / 4 lanes per row, four columns each; a lane weighs one split (or two, ...) and hands its
@@ -691,7 +683,7 @@ void choose_splits(int64_t base, int wanted, int len, int unit, int least, int& 
 // One workgroup per CU is where splitting stops to pay (us, forward / dK dV / dQ alone, 1 split .. more; 120 workgroups without a split:
 // 46.1, 42.4 (2), 50.8 (5); 30: 37.3, 22.9 (4), 24.3 (8), 31.7 (15); 416: 27.7, 46.1 (2); dK dV with 30: 153 -> 64.3 (8), 75.7 (12); with
 // 192: 78.4, 96.5 (2)): the partial results cost more than the idle half of a CU. Single tokens read instead of compute: two workgroups
-// per CU, and no split under 3 x 128 states (tick of 1800 states: 9.8 with 5, 11.7 with 15).
+// per CU, each with at least 1024 states (16 x 8 groups x 16384 x 128: 156, with one per CU 162), and no split at all up to 2048 states.
 constexpr int CUS = 256;
 int dt_of(const XattnArgs& a) { return a.D <= 64 ? 64 : 128; }
 bool few_rows(const XattnArgs& a) { return a.M <= 32; }
@@ -702,7 +694,7 @@ Plan plan_fwd(const XattnArgs& a) {
     const int64_t groups = (int64_t)a.Bk * a.Hk;
     if (few_rows(a)) {
         p.tiles = 1;
-        choose_splits(groups, 2 * CUS, a.Lk, 128, 3, p.splits, p.chunk);
+        choose_splits(groups, a.Lk > 2048 ? 2 * CUS : 1, a.Lk, 256, 4, p.splits, p.chunk);
     } else {
         p.tiles = cdiv(a.M, 128);
         choose_splits(groups * p.tiles, CUS, a.Lk, KT, 2, p.splits, p.chunk);
@@ -732,13 +724,13 @@ int items(XattnArgs& a, const Plan& p, unsigned& grid) {
     return ISB_OK;
 }
 template <auto Kernel>
-int launch(const char* name, unsigned grid, size_t lds, const XattnArgs& a, hipStream_t st) {
+int launch(const char* name, unsigned grid, unsigned threads, size_t lds, const XattnArgs& a, hipStream_t st) {
     static DevMax attr;
     if (attr.below((int)lds)) {
         ISB_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
         attr.set((int)lds);
     }
-    Kernel<<<grid, 256, lds, st>>>(a);
+    Kernel<<<grid, threads, lds, st>>>(a);
     ISB_LAUNCHED(name, st);
     return ISB_OK;
 }
@@ -751,8 +743,8 @@ int fwd(XattnArgs a, float* ws, hipStream_t st) {
     const int64_t rows = (int64_t)a.Bk * a.Hk * a.M;
     a.part = ws;
     a.part2 = ws + (int64_t)p.splits * rows * DT;
-    if (few_rows(a)) ISB_TRY((launch<xattn_token_kernel<F16, DT>>("xattn_token", grid, 4 * 4 * 32 * DT * 2, a, st)));
-    else ISB_TRY((launch<xattn_fwd_kernel<F16, DT>>("xattn_fwd", grid, 4 * KT * DT * 2, a, st)));
+    if (few_rows(a)) ISB_TRY((launch<xattn_token_kernel<F16, DT>>("xattn_token", grid, TOKEN_WAVES * 64, TOKEN_WAVES * (2 * 32 * DT * 2 + 1024), a, st)));
+    else ISB_TRY((launch<xattn_fwd_kernel<F16, DT>>("xattn_fwd", grid, 256, 4 * KT * DT * 2, a, st)));
     if (p.splits > 1) {
         constexpr int per = 1024 / DT;
         xattn_join_kernel<F16, DT><<<(unsigned)((rows + per - 1) / per), 256, 0, st>>>(a);
@@ -774,14 +766,14 @@ int bwd(XattnArgs a, float* ws, hipStream_t st) {
     ISB_TRY(items(a, p, grid));
     a.part = part;
     a.part2 = part + (int64_t)p.splits * states * DT;
-    ISB_TRY((launch<xattn_dkv_kernel<F16, DT>>("xattn_dkv", grid, 2 * (2 * 32 * DT * 2 + 256), a, st)));
+    ISB_TRY((launch<xattn_dkv_kernel<F16, DT>>("xattn_dkv", grid, 256, 2 * (2 * 32 * DT * 2 + 256), a, st)));
     if (p.splits > 1) {
         xattn_sum_kernel<F16, DT, true><<<dim3((unsigned)((states + 15) / 16), 2), 256, 0, st>>>(a, a.Lk);
         ISB_LAUNCHED("xattn_sum dk, dv", st);
     }
     p = plan_dq(a);
     ISB_TRY(items(a, p, grid));
-    ISB_TRY((launch<xattn_dq_kernel<F16, DT>>("xattn_dq", grid, 4 * KT * DT * 2, a, st)));
+    ISB_TRY((launch<xattn_dq_kernel<F16, DT>>("xattn_dq", grid, 256, 4 * KT * DT * 2, a, st)));
     if (p.splits > 1) {
         xattn_sum_kernel<F16, DT, false><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(a, a.M);
         ISB_LAUNCHED("xattn_sum dq", st);
