@@ -105,13 +105,23 @@ __device__ __forceinline__ uint4 op_frag(const unsigned char* t, int r0, int ks,
     else return frag_cols<ROWS, 8, 4>(t, 16 * ks, r0, lane);
 }
 
+// this wave's requests have landed, all but the newest N (`newest`: that many are known to be on their way), and its LDS reads are done
+template <int N>
+__device__ __forceinline__ void wait_landed(bool newest) {
+    if (newest) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+}
+__device__ __forceinline__ void meet() {
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
 // what this wave's lanes wrote to LDS is there for its other lanes (a wave's LDS accesses are done in order; this keeps the compiler to it)
 __device__ __forceinline__ void corner_done() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-template <bool F16, int BM, int BN, int NWM, int NWN, int LA, int LB, int EPI>
-__global__ __launch_bounds__(NWM * NWN * 64, NWM * NWN >= 8 ? 2 : 1) void ffn_mm_kernel(MmArgs p) {
+template <bool F16, int BM, int BN, int NWM, int NWN, int NWK, int NBUF, int LA, int LB, int EPI>
+__global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void ffn_mm_kernel(MmArgs p) {
     T16<F16>::enter();
-    constexpr int NW = NWM * NWN, WM = BM / NWM, WN = BN / NWN, IM = WM / 32, IN = WN / 32;
+    constexpr int NW = NWM * NWN * NWK, WM = BM / NWM, WN = BN / NWN, IM = WM / 32, IN = WN / 32;
     constexpr bool PAIR = EPI == EPI_GATE;
     static_assert(!PAIR || (IN % 2 == 0 && LB == 0), "a wave owns gate and up columns of the same features");
     constexpr int ABYTES = BM * BK * 2, STAGE = ABYTES + BN * BK * 2;
@@ -125,7 +135,7 @@ __global__ __launch_bounds__(NWM * NWN * 64, NWM * NWN >= 8 ? 2 : 1) void ffn_mm
     const int tm = band * GM + at_b % bm, tn = at_b / bm;
     const int m0 = tm * BM, n0 = tn * BN;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
-    const int wm = wave % NWM, wn = wave / NWM;
+    const int wm = wave % NWM, wn = wave / NWM % NWN, wk = wave / (NWM * NWN);
 
     const int kts = (p.K + BK - 1) / BK, total = kts * p.nseg;
     const int t0 = split * p.kt_per_split, t1 = min(total, t0 + p.kt_per_split);
@@ -153,8 +163,8 @@ __global__ __launch_bounds__(NWM * NWN * 64, NWM * NWN >= 8 ? 2 : 1) void ffn_mm
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
     // Fragments run one k-step ahead of the products, also over the edge of a tile: the workgroup meets BEFORE the last k-step's products, when
-    // every wave holds its fragments of the old tile; the buffer is then free for the tile after next, whose requests have a whole tile's
-    // products to land. Fragment reads and requests are issued one by one BETWEEN the products (the matrix pipe takes 32 cycles each).
+    // every wave holds its fragments of the old tile; the buffer is then free for the tile NBUF ahead, whose requests have NBUF - 1 tiles'
+    // products to land (the wait counts the requests of the tiles that may still be on their way: the loop has no other memory access). Fragment reads and requests are issued one by one BETWEEN the products (the matrix pipe takes 32 cycles each).
     uint4 fa[2][IM], fb[2][IN];
     auto fetch = [&](int buf, int ks, int i) {
         const unsigned char* at = conv_lds_dyn + buf * STAGE;
@@ -163,27 +173,69 @@ __global__ __launch_bounds__(NWM * NWN * 64, NWM * NWN >= 8 ? 2 : 1) void ffn_mm
     };
     constexpr int KS = BK / 16, SLOTS = IM * IN, FETCH = IM + IN;
     static_assert(KS % 2 == 0, "k-step 0 of the next tile takes the other half of the fragment registers");
-    if (t0 < t1) {
-        aim(t0, 0);
+    if constexpr (NWK > 1) {
+        // few rows: the waves share out the k-steps of a tile (their sums meet below), so a tile costs a wave its share of the requests, one
+        // step's fragments and its products
+        static_assert(KS % NWK == 0 && NWM == 1 && NWN == 1 && (NBUF - 1) * PIECES < 64, "whole steps per wave");
 #pragma unroll
-        for (int j = 0; j < PIECES; ++j) piece(j);
-        wait_all_and_meet();
-        if (t0 + 1 < t1) {
-            aim(t0 + 1, 1);
+        for (int n = 0; n < NBUF - 1; ++n)
+            if (t0 + n < t1) {
+                aim(t0 + n, n);
 #pragma unroll
-            for (int j = 0; j < PIECES; ++j) piece(j);
+                for (int j = 0; j < PIECES; ++j) piece(j);
+            }
+        int buf = 0, free = NBUF - 1;
+        for (int t = t0; t < t1; ++t) {
+            wait_landed<(NBUF - 2) * PIECES>(t + NBUF - 1 <= t1);
+            meet();                                                            // tile t is there, and nobody reads tile t - 1 any more
+            if (t + NBUF - 1 < t1) {
+                aim(t + NBUF - 1, free);
+#pragma unroll
+                for (int j = 0; j < PIECES; ++j) piece(j);
+            }
+#pragma unroll
+            for (int k = 0; k < KS / NWK; ++k) {
+                const unsigned char* at = conv_lds_dyn + buf * STAGE;
+                const int ks = wk * (KS / NWK) + k;
+#pragma unroll
+                for (int j = 0; j < IN; ++j) fb[0][j] = op_frag<LB, BN>(at + ABYTES, 32 * j, ks, lane);
+#pragma unroll
+                for (int i = 0; i < IM; ++i) fa[0][i] = op_frag<LA, BM>(at, 32 * i, ks, lane);
+#pragma unroll
+                for (int j = 0; j < IN; ++j)
+#pragma unroll
+                    for (int i = 0; i < IM; ++i) acc[i][j] = T16<F16>::mfma32(fb[0][j], fa[0][i], acc[i][j]);
+            }
+            free = buf;
+            buf = buf + 1 == NBUF ? 0 : buf + 1;
         }
+    } else {
+    static_assert((NBUF - 2) * PIECES < 64, "vmcnt counts to 63");
+    if (t0 < t1) {
+#pragma unroll
+        for (int n = 0; n < NBUF; ++n)
+            if (t0 + n < t1) {
+                aim(t0 + n, n);
+#pragma unroll
+                for (int j = 0; j < PIECES; ++j) piece(j);
+            }
+        wait_landed<(NBUF - 1) * PIECES>(t0 + NBUF <= t1);
+        meet();
 #pragma unroll
         for (int i = 0; i < FETCH; ++i) fetch(0, 0, i);
     }
+    int buf = 0;
     for (int t = t0; t < t1; ++t) {
-        const int buf = (t - t0) & 1;
+        const int nbuf = buf + 1 == NBUF ? 0 : buf + 1;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            const bool edge = ks + 1 == KS, more = edge && t + 2 < t1;
+            const bool edge = ks + 1 == KS, more = edge && t + NBUF < t1;
             if (edge) {
-                if (t + 1 < t1) wait_all_and_meet();
-                if (more) aim(t + 2, buf);
+                if (t + 1 < t1) {
+                    wait_landed<(NBUF - 2) * PIECES>(t + NBUF <= t1);
+                    meet();
+                }
+                if (more) aim(t + NBUF, buf);
             }
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -192,7 +244,7 @@ __global__ __launch_bounds__(NWM * NWN * 64, NWM * NWN >= 8 ? 2 : 1) void ffn_mm
 #pragma unroll
                 for (int i = s * FETCH / SLOTS; i < (s + 1) * FETCH / SLOTS; ++i) {
                     if (!edge) fetch(buf, ks + 1, i);
-                    else if (t + 1 < t1) fetch(buf ^ 1, 0, i);
+                    else if (t + 1 < t1) fetch(nbuf, 0, i);
                 }
                 if (more) {
 #pragma unroll
@@ -201,12 +253,14 @@ __global__ __launch_bounds__(NWM * NWN * 64, NWM * NWN >= 8 ? 2 : 1) void ffn_mm
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
+        buf = nbuf;
+    }
     }
 
     // The accumulators hold 32 rows m a lane column each; memory wants whole rows. Each wave turns its 32 x WN blocks round in its own corner of
     // the operand buffers (free now), so that WN / 4 lanes write one row: full lines instead of 32-byte pieces.
     constexpr int LN = WN / 4, RS = WN + 4, STEP = 64 / LN;           // lanes per row, LDS row (floats), rows per step
-    static_assert(NW * 32 * RS * 4 <= 2 * STAGE, "the corners fit");
+    static_assert(NW * 32 * RS * 4 <= NBUF * STAGE, "the corners fit");
     wait_all_and_meet();
     float* corner = reinterpret_cast<float*>(conv_lds_dyn) + wave * 32 * RS;
     const int cl = lane % LN, rl = lane / LN;
@@ -218,6 +272,25 @@ __global__ __launch_bounds__(NWM * NWN * 64, NWM * NWN >= 8 ? 2 : 1) void ffn_mm
             for (int q = 0; q < 4; ++q)
                 *reinterpret_cast<float4*>(corner + (lane & 31) * RS + 32 * j + 8 * q + 4 * h) =
                     make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+        // NWK waves hold parts of the same sums: each adds up 32 / NWK rows over the corners, in wave order, and goes on with those
+        constexpr int RN = 32 / NWK;
+        const int R0 = wk * RN;
+        float* rows = corner;
+        if constexpr (NWK > 1) {
+            __syncthreads();
+            rows = reinterpret_cast<float*>(conv_lds_dyn);
+#pragma unroll
+            for (int r = 0; r < RN; r += STEP) {
+                float* at = rows + (R0 + r + rl) * RS + 4 * cl;
+                float4 t = *reinterpret_cast<const float4*>(at);
+#pragma unroll
+                for (int w = 1; w < NWK; ++w) {
+                    const float4 v = *reinterpret_cast<const float4*>(at + w * 32 * RS);
+                    t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
+                }
+                *reinterpret_cast<float4*>(at) = t;
+            }
+        }
         corner_done();
         const int mb = m0 + wm * WM + 32 * i;
         float sg[4] = {}, su[4] = {};                                         // DH: column sums over the block's rows
@@ -238,8 +311,8 @@ __global__ __launch_bounds__(NWM * NWN * 64, NWM * NWN >= 8 ? 2 : 1) void ffn_mm
                 }
             }
 #pragma unroll
-            for (int r = 0; r < 32; r += SF) {
-                const float4 g4 = *reinterpret_cast<const float4*>(corner + (r + r2) * RS + gc), u4 = *reinterpret_cast<const float4*>(corner + (r + r2) * RS + gc + 32);
+            for (int r = R0; r < R0 + RN; r += SF) {
+                const float4 g4 = *reinterpret_cast<const float4*>(rows + (r + r2) * RS + gc), u4 = *reinterpret_cast<const float4*>(rows + (r + r2) * RS + gc + 32);
                 const int m = mb + r + r2;
                 if (m >= p.M || f >= p.F) continue;
                 const float g[4] = {g4.x + bg[0], g4.y + bg[1], g4.z + bg[2], g4.w + bg[3]}, u[4] = {u4.x + bu[0], u4.y + bu[1], u4.z + bu[2], u4.w + bu[3]};
@@ -262,8 +335,8 @@ __global__ __launch_bounds__(NWM * NWN * 64, NWM * NWN >= 8 ? 2 : 1) void ffn_mm
                     bias[0] = T16<F16>::lo(w.x); bias[1] = T16<F16>::hi(w.x); bias[2] = T16<F16>::lo(w.y); bias[3] = T16<F16>::hi(w.y);
                 }
 #pragma unroll
-            for (int r = 0; r < 32; r += STEP) {
-                const float4 o = *reinterpret_cast<const float4*>(corner + (r + rl) * RS + 4 * cl);
+            for (int r = R0; r < R0 + RN; r += STEP) {
+                const float4 o = *reinterpret_cast<const float4*>(rows + (r + rl) * RS + 4 * cl);
                 const int m = mb + r + rl;
                 if (m >= p.M || n >= p.N) continue;
                 if constexpr (EPI == EPI_DH) {
@@ -298,7 +371,22 @@ __global__ __launch_bounds__(NWM * NWN * 64, NWM * NWN >= 8 ? 2 : 1) void ffn_mm
 #pragma unroll
                     for (int o = LN; o < 64; o <<= 1) { sg[e] += __shfl_xor(sg[e], o); su[e] += __shfl_xor(su[e], o); }
                 const int n = n0 + wn * WN + 4 * cl;
-                if (rl == 0 && mb < p.M && n < p.N) {
+                if constexpr (NWK > 1) {
+                    float* part = reinterpret_cast<float*>(conv_lds_dyn) + NW * 32 * RS;       // [NWK][2][WN], behind the corners
+                    static_assert((NW * 32 * RS + NWK * 2 * WN) * 4 <= NBUF * STAGE, "the sums fit");
+                    if (rl == 0) {
+                        *reinterpret_cast<float4*>(part + wk * 2 * WN + 4 * cl) = make_float4(sg[0], sg[1], sg[2], sg[3]);
+                        *reinterpret_cast<float4*>(part + wk * 2 * WN + WN + 4 * cl) = make_float4(su[0], su[1], su[2], su[3]);
+                    }
+                    __syncthreads();
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        sg[e] = su[e] = 0.f;
+#pragma unroll
+                        for (int w = 0; w < NWK; ++w) { sg[e] += part[w * 2 * WN + 4 * cl + e]; su[e] += part[w * 2 * WN + WN + 4 * cl + e]; }
+                    }
+                }
+                if (wk == 0 && rl == 0 && mb < p.M && n < p.N) {
                     float* c = p.cs + (int64_t)(mb / 32) * 2 * p.F + n;
                     *reinterpret_cast<float4*>(c) = make_float4(sg[0], sg[1], sg[2], sg[3]);
                     *reinterpret_cast<float4*>(c + p.F) = make_float4(su[0], su[1], su[2], su[3]);
@@ -439,25 +527,27 @@ __global__ __launch_bounds__(256) void ffn_bias_kernel(const float* cs, const fl
 // ------------------------------------------------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------------------------------------------------
-// tile shapes: thin (at most 64 rows: weights are read once or twice), mid (two workgroups per CU), big (one workgroup of eight waves;
-// half the LDS and L2 bytes per product, but only where its tiles fill the 256 CUs)
+// tile shapes: thin (32 x 64, four waves on the k-steps of a tile, four tiles in flight: the weights are the work, and many small workgroups
+// read them; us forward, D = 1280, F = 5120: 32 rows 18 for mid's 30, 256 rows 36 for 41, at 600 rows it loses, 63 for 50), mid (128 x 128,
+// two workgroups per CU), big (256 x 256, one workgroup of eight waves; half the LDS and L2 bytes per product, but only where its tiles
+// fill the 256 CUs)
 enum { TILE_THIN, TILE_MID, TILE_BIG };
 int tile_of(int la, int M, int N) {
-    if (M <= 64 && la == 0) return TILE_THIN;         // (layout 1 keeps whole 128-byte rows of m in LDS: no thin form)
+    if (M <= 256 && la == 0) return TILE_THIN;         // (layout 1 keeps whole 128-byte rows of m in LDS: no thin form)
     return (int64_t)cdiv(M, 256) * cdiv(N, 256) >= 200 ? TILE_BIG : TILE_MID;
 }
 int splits_of(int la, int M, int N, int kts) {            // k splits of an OUT product whose tiles do not fill the chip
-    const int t = tile_of(la, M, N), bm = t == TILE_THIN ? 32 : t == TILE_MID ? 128 : 256, bn = t == TILE_BIG ? 256 : 128;
+    const int t = tile_of(la, M, N), bm = t == TILE_THIN ? 32 : t == TILE_MID ? 128 : 256, bn = t == TILE_BIG ? 256 : t == TILE_THIN ? 64 : 128;
     const int64_t tiles = (int64_t)cdiv(M, bm) * cdiv(N, bn);
     const int64_t want = t == TILE_BIG ? 1 : 512 / tiles;
-    int s = (int)std::min<int64_t>(want, std::max(1, kts / 4));
+    int s = (int)std::min<int64_t>(want, std::max(1, kts / (t == TILE_THIN ? 16 : 4)));
     s = std::max(1, std::min(s, 16));
     return cdiv(kts, cdiv(kts, s));
 }
 
-template <bool F16, int BM, int BN, int NWM, int NWN, int LA, int LB, int EPI>
+template <bool F16, int BM, int BN, int NWM, int NWN, int NWK, int NBUF, int LA, int LB, int EPI>
 int mm_run(MmArgs p, const char* name, hipStream_t st) {
-    constexpr size_t lds = 2 * (BM + BN) * BK * 2;
+    constexpr size_t lds = NBUF * (BM + BN) * BK * 2;
     p.tiles_m = cdiv(p.M, BM);
     p.tiles_n = cdiv(p.N, BN);
     const int64_t n = (int64_t)p.tiles_m * p.tiles_n * p.splits;
@@ -466,11 +556,11 @@ int mm_run(MmArgs p, const char* name, hipStream_t st) {
     p.kt_per_split = cdiv(cdiv(p.K, BK) * p.nseg, p.splits);
     static DevMax attr;
     if (attr.below((int)lds)) {
-        ISB_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(ffn_mm_kernel<F16, BM, BN, NWM, NWN, LA, LB, EPI>),
+        ISB_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(ffn_mm_kernel<F16, BM, BN, NWM, NWN, NWK, NBUF, LA, LB, EPI>),
                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
         attr.set((int)lds);
     }
-    ffn_mm_kernel<F16, BM, BN, NWM, NWN, LA, LB, EPI><<<(unsigned)(8 * ((n + 7) / 8)), NWM * NWN * 64, lds, st>>>(p);
+    ffn_mm_kernel<F16, BM, BN, NWM, NWN, NWK, NBUF, LA, LB, EPI><<<(unsigned)(8 * ((n + 7) / 8)), NWM * NWN * NWK * 64, lds, st>>>(p);
     ISB_LAUNCHED(name, st);
     return ISB_OK;
 }
@@ -478,9 +568,9 @@ template <bool F16, int LA, int LB, int EPI>
 int mm(const MmArgs& p, const char* name, hipStream_t st) {
     const int t = tile_of(LA, p.M, p.N);
     if constexpr (LA == 0)
-        if (t == TILE_THIN) return mm_run<F16, 32, 128, 1, 2, LA, LB, EPI>(p, name, st);
-    if (t == TILE_MID) return mm_run<F16, 128, 128, 2, 2, LA, LB, EPI>(p, name, st);
-    return mm_run<F16, 256, 256, 2, 4, LA, LB, EPI>(p, name, st);
+        if (t == TILE_THIN) return mm_run<F16, 32, 64, 1, 1, 4, 4, LA, LB, EPI>(p, name, st);
+    if (t == TILE_MID) return mm_run<F16, 128, 128, 2, 2, 1, 2, LA, LB, EPI>(p, name, st);
+    return mm_run<F16, 256, 256, 2, 4, 1, 2, LA, LB, EPI>(p, name, st);
 }
 // C = A B^T (+ bias), k split where the tiles alone leave CUs idle
 template <bool F16, int LA, int LB>
