@@ -56,42 +56,65 @@ struct TileLoad {
             voff[j] = c * 8 < D ? (uint32_t)(r * (int)sl * 2 + c * 16) : DMA_NONE;
         }
     }
-    __device__ __forceinline__ void request(const uint16_t* base, uint64_t bits, uint32_t lds, int wave) const {
+    // all: every state of the tile is valid
+    __device__ __forceinline__ void request(const uint16_t* base, bool all, uint64_t bits, uint32_t lds, int wave) const {
         const i32x4 d = dma_desc(base);
-        const bool full = bits == ~0ull;
+        if (all) {
 #pragma unroll
-        for (int j = 0; j < PIECES; ++j) {
-            const uint32_t v = full || ((bits >> row[j]) & 1) ? voff[j] : DMA_NONE;
-            dma16_desc(d, v, lds + (wave * PIECES + j) * 1024);
+            for (int j = 0; j < PIECES; ++j) dma16_desc(d, voff[j], lds + (wave * PIECES + j) * 1024);
+        } else {
+#pragma unroll
+            for (int j = 0; j < PIECES; ++j) {
+                const uint32_t none = (uint32_t)((bits >> row[j]) & 1) - 1u;         // all ones where the state is masked: past the buffer's end
+                dma16_desc(d, voff[j] | none, lds + (wave * PIECES + j) * 1024);
+            }
         }
     }
 };
 
-// masked scores become -inf; bits: validity of the 32 states of the block
-__device__ __forceinline__ void mask_scores(f32x16& s, uint32_t bits, int h) {
-    const uint32_t w = bits >> (4 * h);
+// Masked states enter as the accumulators' start: their lane of `bias` (LDS, a float per state of the tile) holds -inf, the others 0, so a
+// masked score costs the softmax no instruction (masked K rows are zeros: -inf + 0 stays).
+__device__ __forceinline__ void start_scores(f32x16& s, const float* bias, bool all, int h) {
+    if (all) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = (w >> (8 * (i / 4) + i % 4)) & 1 ? s[i] : NEG_INF;
+        for (int i = 0; i < 16; ++i) s[i] = 0.f;
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const float4 v = *reinterpret_cast<const float4*>(bias + 8 * q + 4 * h);
+            s[4 * q] = v.x; s[4 * q + 1] = v.y; s[4 * q + 2] = v.z; s[4 * q + 3] = v.w;
+        }
+    }
 }
+__device__ __forceinline__ void put_bias(float* bias, int n, uint32_t byte, bool all, int lane) {
+    if (!all && lane < n) bias[lane] = byte ? 0.f : NEG_INF;
+}
+
+// LDS reads and matrix products keep the order they are written in (vector and scalar arithmetic may move): a fragment is read several
+// products before its own, which hides the read's latency also where a SIMD has only one or two waves. Left to itself the compiler reads one
+// product ahead.
+__device__ __forceinline__ void reads_stay() { __builtin_amdgcn_sched_barrier(0x6); }
 
 // One block of NB x 32 states for 32 rows (a column of S^T each): scores, running maximum and sum, O^T += V^T P^T.
 // The maximum follows lazily: O^T is rescaled only when a row's maximum grows by more than 8 (base-2 units), so P <= 2^8.
 template <bool F16, int DT, int NB>
 __device__ __forceinline__ void attend(const unsigned char* kt, const unsigned char* vt, const uint4 (&qf)[DT / 16], f32x16 (&acc)[DT / 32],
-                                       float& m, float& l, float c, uint64_t bits, int lane) {
+                                       float& m, float& l, float c, const float* bias, bool all, int lane) {
     const int h = lane >> 5;
+    constexpr int KS = DT / 16;
     f32x16 s[NB];
+    uint4 kf[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) kf[ks] = frag_rows<DT>(kt, 0, ks, lane);
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
+        start_scores(s[b], bias + 32 * b, all, h);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[b][i] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < DT / 16; ++ks) s[b] = T16<F16>::mfma32(frag_rows<DT>(kt, 32 * b, ks, lane), qf[ks], s[b]);
-    }
-    constexpr uint64_t ALL = NB == 2 ? ~0ull : 0xffffffffull;
-    if (bits != ALL) {
-#pragma unroll
-        for (int b = 0; b < NB; ++b) mask_scores(s[b], (uint32_t)(bits >> (32 * b)), h);
+        for (int ks = 0; ks < KS; ++ks) {
+            s[b] = T16<F16>::mfma32(kf[ks], qf[ks], s[b]);
+            if (b + 1 < NB) kf[ks] = frag_rows<DT>(kt, 32 * (b + 1), ks, lane);       // the next block's fragment behind this one's product
+            reads_stay();
+        }
     }
     float mx = NEG_INF;
 #pragma unroll
@@ -109,6 +132,12 @@ __device__ __forceinline__ void attend(const unsigned char* kt, const unsigned c
             for (int i = 0; i < 16; ++i) acc[d][i] *= al;
         m = mn;
     }
+    // the first fragments of V^T travel while the weights are formed
+    constexpr int NT = 2 * NB, NV = NT * (DT / 32), AHEAD = 4;
+    uint4 vf[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) vf[i] = frag_cols<DT, 4, 8>(vt, 16 * (i % NT), 32 * (i / NT), lane);
+    reads_stay();
     const float mu = m == NEG_INF ? 0.f : m;
     uint4 p[2 * NB];
     float sum = 0.f;
@@ -126,9 +155,11 @@ __device__ __forceinline__ void attend(const unsigned char* kt, const unsigned c
         }
     l += sum;
 #pragma unroll
-    for (int d = 0; d < DT / 32; ++d)
-#pragma unroll
-        for (int t = 0; t < 2 * NB; ++t) acc[d] = T16<F16>::mfma32(frag_cols<DT, 4, 8>(vt, 16 * t, 32 * d, lane), p[t], acc[d]);
+    for (int i = 0; i < NV; ++i) {
+        acc[i / NT] = T16<F16>::mfma32(vf[i % AHEAD], p[i % NT], acc[i / NT]);
+        if (i + AHEAD < NV) vf[i % AHEAD] = frag_cols<DT, 4, 8>(vt, 16 * ((i + AHEAD) % NT), 32 * ((i + AHEAD) / NT), lane);
+        reads_stay();
+    }
 }
 
 // four columns of a row's results (and, `first`, what goes with the row): out and lse, or (splits) its unnormalised sums with maximum and sum
@@ -159,7 +190,7 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XattnArgs a) {
     const int rt = item % a.tiles, split = item / a.tiles % a.splits, grp = item / a.tiles / a.splits, bk = grp / a.Hk, hk = grp % a.Hk;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
     const int r = rt * 128 + wave * 32 + (lane & 31);
-    constexpr int TB = KT * DT * 2;
+    constexpr int TB = KT * DT * 2, STAGE = 2 * TB + KT * 4;
 
     const int len = states_of(a, bk), k0 = split * a.chunk, k1 = min(len, k0 + a.chunk);
     const int nt = k1 > k0 ? (k1 - k0 + KT - 1) / KT : 0;
@@ -186,23 +217,25 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XattnArgs a) {
     lv.init(wave, lane, a.v_sl, a.D);
     uint64_t bits = 0, next = 0;
     uint32_t byte = 0;
+    auto request = [&](int t, uint64_t valid, uint32_t at) {
+        const bool all = valid == ~0ull;
+        lk.request(kb + (int64_t)t * KT * a.k_sl, all, valid, lds0 + at, wave);
+        lv.request(vb + (int64_t)t * KT * a.v_sl, all, valid, lds0 + at + TB, wave);
+        if (wave == 0) put_bias(reinterpret_cast<float*>(conv_lds_dyn + at + 2 * TB), KT, byte, all, lane);
+        byte = mask_byte(a, bk, k0 + (t + 1) * KT + lane, k1);
+    };
     if (nt > 0) {
-        bits = __ballot(mask_byte(a, bk, k0 + lane, k1) != 0);
-        lk.request(kb, bits, lds0, wave);
-        lv.request(vb, bits, lds0 + TB, wave);
-        byte = mask_byte(a, bk, k0 + KT + lane, k1);
+        byte = mask_byte(a, bk, k0 + lane, k1);
+        bits = __ballot(byte != 0);
+        request(0, bits, 0);
     }
     for (int t = 0; t < nt; ++t) {
         next = __ballot(byte != 0);
         wait_all_and_meet();
-        const uint32_t cur = (t & 1) * 2 * TB, oth = 2 * TB - cur;
-        if (t + 1 < nt) {
-            const int64_t at = (int64_t)(t + 1) * KT;
-            lk.request(kb + at * a.k_sl, next, lds0 + oth, wave);
-            lv.request(vb + at * a.v_sl, next, lds0 + oth + TB, wave);
-            byte = mask_byte(a, bk, k0 + (t + 2) * KT + lane, k1);
-        }
-        if (bits != 0) attend<F16, DT, 2>(conv_lds_dyn + cur, conv_lds_dyn + cur + TB, qf, acc, m, l, a.c, bits, lane);
+        const uint32_t cur = (t & 1) * STAGE, oth = STAGE - cur;
+        if (t + 1 < nt) request(t + 1, next, oth);
+        const float* bias = reinterpret_cast<const float*>(conv_lds_dyn + cur + 2 * TB);
+        if (bits != 0) attend<F16, DT, 2>(conv_lds_dyn + cur, conv_lds_dyn + cur + TB, qf, acc, m, l, a.c, bias, bits == ~0ull, lane);
         bits = next;
     }
     l = sum_halves(l);
@@ -249,27 +282,29 @@ __global__ __launch_bounds__(TOKEN_WAVES * 64, TOKEN_WAVES / 4) void xattn_token
 
     const uint16_t* kb = a.k + bk * a.k_sb + hk * a.k_sh + (int64_t)k0 * a.k_sl;
     const uint16_t* vb = a.v + bk * a.v_sb + hk * a.v_sh + (int64_t)k0 * a.v_sl;
-    unsigned char* own = conv_lds_dyn + wave * 2 * TB;
+    unsigned char* own = conv_lds_dyn + wave * (2 * TB + 128);
+    float* bias = reinterpret_cast<float*>(own + 2 * TB);
     const uint32_t lds0 = lds_addr_of(own);
     TileLoad<DT, 32, 1> lk, lv;
     lk.init(0, lane, a.k_sl, a.D);
     lv.init(0, lane, a.v_sl, a.D);
+    uint32_t byte = 0, bits = 0;
     auto valid = [&](int t) -> uint32_t { return t < nt ? mask_byte(a, bk, k0 + 32 * t + (lane & 31), k1) : 0u; };
-    auto request = [&](int t, uint32_t bits) {
-        const int64_t at = (int64_t)t * 32;
-        lk.request(kb + at * a.k_sl, bits, lds0, 0);
-        lv.request(vb + at * a.v_sl, bits, lds0 + TB, 0);
+    auto request = [&](int t) {
+        bits = (uint32_t)__ballot(byte != 0);
+        const bool all = bits == ~0u;
+        lk.request(kb + (int64_t)t * 32 * a.k_sl, all, bits, lds0, 0);
+        lv.request(vb + (int64_t)t * 32 * a.v_sl, all, bits, lds0 + TB, 0);
+        put_bias(bias, 32, byte, all, lane);
+        byte = valid(t + NW);
     };
-    uint32_t bits = (uint32_t)__ballot(valid(wave) != 0), byte = valid(wave + NW);
-    if (wave < nt) request(wave, bits);
+    byte = valid(wave);
+    if (wave < nt) request(wave);
     for (int t = wave; t < nt; t += NW) {
-        const uint32_t next = (uint32_t)__ballot(byte != 0);
-        byte = valid(t + 2 * NW);
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (bits != 0) attend<F16, DT, 1>(own, own + TB, qf, acc, m, l, a.c, bits, lane);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if (bits != 0) attend<F16, DT, 1>(own, own + TB, qf, acc, m, l, a.c, bias, bits == ~0u, lane);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                    // the block is read before its place is requested again
-        if (t + NW < nt) request(t + NW, next);
-        bits = next;
+        if (t + NW < nt) request(t + NW);
     }
     l = sum_halves(l);
     // join the waves: (m, l) of all, then every wave scales its sums to the common maximum and each adds up its share of the columns, in wave
@@ -297,10 +332,8 @@ __global__ __launch_bounds__(TOKEN_WAVES * 64, TOKEN_WAVES / 4) void xattn_token
     __syncthreads();
     // piece (d, q): 8 columns (4 per lane half); wave w takes pieces w, w + NW, ...
 #pragma unroll
-    for (int i = 0; i < (DT / 8 + NW - 1) / NW; ++i) {
-        const int piece = wave + i * NW;
-        if (piece >= DT / 8) continue;
-        const int c = 8 * piece + 4 * h;
+    for (int i = 0; i < DT / 8 / NW; ++i) {
+        const int piece = wave + i * NW, c = 8 * piece + 4 * h;
         float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
@@ -485,10 +518,27 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
         f32x16 s, dp[1];
 #pragma unroll
         for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[0][i] = 0.f; }
+        {
+            constexpr int N = DT / 8, AHEAD = 4;                               // Q's fragments, then dout's
+            uint4 f[AHEAD];
 #pragma unroll
-        for (int ks = 0; ks < DT / 16; ++ks) s = T16<F16>::mfma32(frag_rows<DT>(qt, 0, ks, lane), kf[ks], s);
+            for (int i = 0; i < AHEAD; ++i) f[i] = frag_rows<DT>(qt, 0, i, lane);
 #pragma unroll
-        for (int ks = 0; ks < DT / 16; ++ks) dp[0] = T16<F16>::mfma32(frag_rows<DT>(dt, 0, ks, lane), vf[ks], dp[0]);
+            for (int i = 0; i < N; ++i) {
+                const int n = i + AHEAD;
+                if (i < N / 2) s = T16<F16>::mfma32(f[i % AHEAD], kf[i], s);
+                else dp[0] = T16<F16>::mfma32(f[i % AHEAD], vf[i - N / 2], dp[0]);
+                if (n < N) f[i % AHEAD] = n < N / 2 ? frag_rows<DT>(qt, 0, n, lane) : frag_rows<DT>(dt, 0, n - N / 2, lane);
+                reads_stay();
+            }
+        }
+        // columns of dout and Q for dV^T += dout^T P, dK^T += Q^T dS; the first ones travel while P and dS are formed
+        constexpr int NC = DT / 8, AHEAD = 4;
+        auto column = [&](int i) { return frag_cols<DT, 4, 8>(i % 2 == 0 ? dt : qt, 16 * (i / 2 % 2), 32 * (i / 4), lane); };
+        uint4 c[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) c[i] = column(i);
+        reads_stay();
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             const float4 nl = *reinterpret_cast<const float4*>(st + 8 * q + 4 * h), de = *reinterpret_cast<const float4*>(st + 32 + 8 * q + 4 * h);
@@ -510,12 +560,13 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
 #pragma unroll
         for (int u = 0; u < 2; ++u) { p[u] = pack8<F16>(s, u); ds[u] = pack8<F16>(dp[0], u); }
 #pragma unroll
-        for (int d = 0; d < DT / 32; ++d)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                dv[d] = T16<F16>::mfma32(frag_cols<DT, 4, 8>(dt, 16 * u, 32 * d, lane), p[u], dv[d]);
-                dk[d] = T16<F16>::mfma32(frag_cols<DT, 4, 8>(qt, 16 * u, 32 * d, lane), ds[u], dk[d]);
-            }
+        for (int i = 0; i < NC; ++i) {
+            const int d = i / 4, u = i / 2 % 2;
+            if (i % 2 == 0) dv[d] = T16<F16>::mfma32(c[i % AHEAD], p[u], dv[d]);
+            else dk[d] = T16<F16>::mfma32(c[i % AHEAD], ds[u], dk[d]);
+            if (i + AHEAD < NC) c[i % AHEAD] = column(i + AHEAD);
+            reads_stay();
+        }
         if (t + 1 < nt) put((t + 1) & 1);
         __syncthreads();
     }
@@ -555,7 +606,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
     const int rt = item % a.tiles, split = item / a.tiles % a.splits, grp = item / a.tiles / a.splits, bk = grp / a.Hk, hk = grp % a.Hk;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
     const int r = rt * 128 + wave * 32 + (lane & 31);
-    constexpr int TB = KT * DT * 2;
+    constexpr int TB = KT * DT * 2, STAGE = 2 * TB + KT * 4;
     const int len = states_of(a, bk), k0 = split * a.chunk, k1 = min(len, k0 + a.chunk);
     const int nt = k1 > k0 ? (k1 - k0 + KT - 1) / KT : 0;
 
@@ -585,44 +636,61 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
     lv.init(wave, lane, a.v_sl, a.D);
     uint64_t bits = 0, next = 0;
     uint32_t byte = 0;
+    auto request = [&](int t, uint64_t valid, uint32_t at) {
+        const bool all = valid == ~0ull;
+        lk.request(kb + (int64_t)t * KT * a.k_sl, all, valid, lds0 + at, wave);
+        lv.request(vb + (int64_t)t * KT * a.v_sl, all, valid, lds0 + at + TB, wave);
+        if (wave == 0) put_bias(reinterpret_cast<float*>(conv_lds_dyn + at + 2 * TB), KT, byte, all, lane);
+        byte = mask_byte(a, bk, k0 + (t + 1) * KT + lane, k1);
+    };
     if (nt > 0) {
-        bits = __ballot(mask_byte(a, bk, k0 + lane, k1) != 0);
-        lk.request(kb, bits, lds0, wave);
-        lv.request(vb, bits, lds0 + TB, wave);
-        byte = mask_byte(a, bk, k0 + KT + lane, k1);
+        byte = mask_byte(a, bk, k0 + lane, k1);
+        bits = __ballot(byte != 0);
+        request(0, bits, 0);
     }
     for (int t = 0; t < nt; ++t) {
         next = __ballot(byte != 0);
         wait_all_and_meet();
-        const uint32_t cur = (t & 1) * 2 * TB, oth = 2 * TB - cur;
-        if (t + 1 < nt) {
-            const int64_t at = (int64_t)(t + 1) * KT;
-            lk.request(kb + at * a.k_sl, next, lds0 + oth, wave);
-            lv.request(vb + at * a.v_sl, next, lds0 + oth + TB, wave);
-            byte = mask_byte(a, bk, k0 + (t + 2) * KT + lane, k1);
-        }
+        const uint32_t cur = (t & 1) * STAGE, oth = STAGE - cur;
+        if (t + 1 < nt) request(t + 1, next, oth);
+        const float* bias = reinterpret_cast<const float*>(conv_lds_dyn + cur + 2 * TB);
         const unsigned char* ktile = conv_lds_dyn + cur;
         const unsigned char* vtile = ktile + TB;
         if (bits != 0) {
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
                 f32x16 s, ds[1];
+                start_scores(s, bias + 32 * b, bits == ~0ull, h);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) { s[i] = 0.f; ds[0][i] = 0.f; }
+                for (int i = 0; i < 16; ++i) ds[0][i] = 0.f;
+                constexpr int N = DT / 8, AHEAD = 4;                           // K's and V's fragments in turn
+                auto row = [&](int i) { return frag_rows<DT>(i % 2 == 0 ? ktile : vtile, 32 * b, i / 2, lane); };
+                uint4 f[AHEAD];
 #pragma unroll
-                for (int ks = 0; ks < DT / 16; ++ks) {
-                    s = T16<F16>::mfma32(frag_rows<DT>(ktile, 32 * b, ks, lane), qf[ks], s);
-                    ds[0] = T16<F16>::mfma32(frag_rows<DT>(vtile, 32 * b, ks, lane), df[ks], ds[0]);
+                for (int i = 0; i < AHEAD; ++i) f[i] = row(i);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    if (i % 2 == 0) s = T16<F16>::mfma32(f[i % AHEAD], qf[i / 2], s);
+                    else ds[0] = T16<F16>::mfma32(f[i % AHEAD], df[i / 2], ds[0]);
+                    if (i + AHEAD < N) f[i % AHEAD] = row(i + AHEAD);
+                    reads_stay();
                 }
-                if (bits != ~0ull) mask_scores(s, (uint32_t)(bits >> (32 * b)), h);
+                constexpr int NC = DT / 16;                                    // K's columns for dQ^T += K^T dS^T
+                auto column = [&](int i) { return frag_cols<DT, 4, 8>(ktile, 32 * b + 16 * (i % 2), 32 * (i / 2), lane); };
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) f[i] = column(i);
+                reads_stay();
 #pragma unroll
                 for (int i = 0; i < 16; ++i) ds[0][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, nl)) * (ds[0][i] - de);
                 scale_ds<F16, 1, DT / 32>(ds, acc, sc);
+                uint4 g[2];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const uint4 f = pack8<F16>(ds[0], u);
+                for (int u = 0; u < 2; ++u) g[u] = pack8<F16>(ds[0], u);
 #pragma unroll
-                    for (int d = 0; d < DT / 32; ++d) acc[d] = T16<F16>::mfma32(frag_cols<DT, 4, 8>(ktile, 32 * b + 16 * u, 32 * d, lane), f, acc[d]);
+                for (int i = 0; i < NC; ++i) {
+                    acc[i / 2] = T16<F16>::mfma32(f[i % AHEAD], g[i % 2], acc[i / 2]);
+                    if (i + AHEAD < NC) f[i % AHEAD] = column(i + AHEAD);
+                    reads_stay();
                 }
             }
         }
@@ -744,7 +812,7 @@ int fwd(XattnArgs a, float* ws, hipStream_t st) {
     a.part = ws;
     a.part2 = ws + (int64_t)p.splits * rows * DT;
     if (few_rows(a)) ISB_TRY((launch<xattn_token_kernel<F16, DT>>("xattn_token", grid, TOKEN_WAVES * 64, TOKEN_WAVES * (2 * 32 * DT * 2 + 1024), a, st)));
-    else ISB_TRY((launch<xattn_fwd_kernel<F16, DT>>("xattn_fwd", grid, 256, 4 * KT * DT * 2, a, st)));
+    else ISB_TRY((launch<xattn_fwd_kernel<F16, DT>>("xattn_fwd", grid, 256, 2 * (2 * KT * DT * 2 + KT * 4), a, st)));
     if (p.splits > 1) {
         constexpr int per = 1024 / DT;
         xattn_join_kernel<F16, DT><<<(unsigned)((rows + per - 1) / per), 256, 0, st>>>(a);
@@ -773,7 +841,7 @@ int bwd(XattnArgs a, float* ws, hipStream_t st) {
     }
     p = plan_dq(a);
     ISB_TRY(items(a, p, grid));
-    ISB_TRY((launch<xattn_dq_kernel<F16, DT>>("xattn_dq", grid, 256, 4 * KT * DT * 2, a, st)));
+    ISB_TRY((launch<xattn_dq_kernel<F16, DT>>("xattn_dq", grid, 256, 2 * (2 * KT * DT * 2 + KT * 4), a, st)));
     if (p.splits > 1) {
         xattn_sum_kernel<F16, DT, false><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(a, a.M);
         ISB_LAUNCHED("xattn_sum dq", st);
