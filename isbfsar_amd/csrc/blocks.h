@@ -24,6 +24,7 @@ struct XattnArgs {
     int B, Bk, nb, Lq, Lk, Hq, Hk, G, D, M;
     int n_items;                                         // work items of the launch
     int tiles, splits, chunk;                            // row (or key) tiles per group, splits of the long axis, its keys (rows) per split
+    int walk;                                            // rows can be stepped through (RowWalk)
     float c, scale;                                      // scale * log2(e), scale
 };
 size_t xattn_workspace(const XattnArgs& a, bool backward);

@@ -56,7 +56,7 @@ int xattn_shape(const isb_xattn_args* u, XattnArgs& a) {
     const int64_t m = (int64_t)(u->B / u->Bk) * u->Lq * (u->Hq / u->Hk);
     ISB_REQUIRE(m <= (1 << 30), ISB_ERR_INVALID, "cross attention: %lld rows share one set of states: too many", (long long)m);
     const int64_t rows = m * u->Bk * u->Hk, states = (int64_t)u->Bk * u->Hk * u->Lk;
-    ISB_REQUIRE(rows < (1ll << 32) && states < (1ll << 32), ISB_ERR_INVALID, "cross attention: %lld rows, %lld states are too many", (long long)rows,
+    ISB_REQUIRE(rows < (1ll << 31) && states < (1ll << 31), ISB_ERR_INVALID, "cross attention: %lld rows, %lld states are too many", (long long)rows,
                 (long long)states);
     ISB_REQUIRE(std::isfinite(u->scale) && u->scale > 0, ISB_ERR_INVALID, "cross attention: scale %g is not positive", (double)u->scale);
     a.B = u->B; a.Bk = u->Bk; a.nb = u->B / u->Bk; a.Lq = u->Lq; a.Lk = u->Lk; a.Hq = u->Hq; a.Hk = u->Hk; a.G = u->Hq / u->Hk; a.D = u->D;

@@ -385,8 +385,8 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XattnArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------------
-// Backward. delta = rowsum(dout * out); then dK, dV (a workgroup keeps 128 states, 32 per wave, and walks the rows) and dQ (a workgroup
-// keeps 128 rows and walks the states). Every sum has a fixed order: no atomics.
+// Backward. dQ first (a workgroup keeps 128 rows, forms their delta = rowsum(dout o out) and walks the states), then dK, dV (a workgroup keeps
+// 128 states, 32 per wave, and walks the rows); one launch adds up the splits of all three. Every sum has a fixed order: no atomics.
 //
 // fp16: P is formed as 2^12 P (<= 4096), so that weights of 1 / 16384 stay normal numbers, and dS carries a power of two chosen from what
 // the wave meets: it starts so that the first tile's largest |dS| lies in [2^10, 2^11) and is lowered, with the sums so far, when a tile
@@ -394,24 +394,36 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XattnArgs a) {
 // ------------------------------------------------------------------------------------------------------------------------------------
 template <bool F16> constexpr float P_UP = F16 ? 12.0f : 0.0f;              // log2 of the factor on P
 
-template <bool F16>
-__global__ __launch_bounds__(256) void xattn_delta_kernel(XattnArgs a) {
-    const int64_t rows = (int64_t)a.Bk * a.Hk * a.M, row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (row >= rows) return;
-    const int l = threadIdx.x & 15, grp = (int)(row / a.M);
-    const RowAt w = row_at(a, grp / a.Hk, grp % a.Hk, (int)(row % a.M));
-    float s = 0.f;
-    if (8 * l < a.D) {
-        const uint4 x = *reinterpret_cast<const uint4*>(a.out + off_out(a, w) + 8 * l);
-        const uint4 y = *reinterpret_cast<const uint4*>(a.dout + off_at(w, a.d_sb, a.d_sl, a.d_sh) + 8 * l);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s += T16<F16>::lo(xs[i]) * T16<F16>::lo(ys[i]) + T16<F16>::hi(xs[i]) * T16<F16>::hi(ys[i]);
+// Where a thread's row lies, RT rows further with every step. Where G divides RT and a sample holds at least RT rows, a step stays on the same
+// head and passes at most one sample's end: two additions instead of two divisions and the products of three strides.
+template <int RT>
+struct RowWalk {
+    int64_t q, d;                  // offsets in q and dout
+    int i, r, lse;                 // position, row, index into lse
+    __device__ __forceinline__ void at(const XattnArgs& a, int bk, int hk, int row) {
+        r = row;
+        const RowAt w = row_at(a, bk, hk, min(row, a.M - 1));
+        q = off_at(w, a.q_sb, a.q_sl, a.q_sh);
+        d = off_at(w, a.d_sb, a.d_sl, a.d_sh);
+        lse = (w.b * a.Hq + w.hq) * a.Lq + w.i;
+        i = w.i;
     }
-#pragma unroll
-    for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o);
-    if (l == 0) a.delta[row] = s;
-}
+    __device__ __forceinline__ void step(const XattnArgs& a, int bk, int hk) {
+        if (!a.walk) { at(a, bk, hk, r + RT); return; }
+        const int n = RT / a.G;
+        r += RT;
+        i += n;
+        q += n * a.q_sl;
+        d += n * a.d_sl;
+        lse += n;
+        if (i >= a.Lq) {
+            i -= a.Lq;
+            q += a.q_sb - a.Lq * a.q_sl;
+            d += a.d_sb - a.Lq * a.d_sl;
+            lse += (a.Hq - 1) * a.Lq;
+        }
+    }
+};
 
 // the power of two on dS (see above); NB blocks of scores. Returns with ds scaled.
 template <bool F16, int NB, int NA>
@@ -448,6 +460,7 @@ __device__ __forceinline__ uint4 pack8(const f32x16& x, int t) {
 }
 
 // dK, dV: S = Q K^T with the rows in the accumulator's rows and a state per lane; P and dS are then operands over the rows.
+template <int DT> constexpr int DKV_ROWS = DT == 64 ? 64 : 32;      // rows per barrier: 128 wide, the registers hold the requests of 32
 template <bool F16, int DT>
 __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnArgs a) {
     T16<F16>::enter();
@@ -458,9 +471,9 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
     const int key = kt * 128 + wave * 32 + (lane & 31);
     const int len = states_of(a, bk);
     const bool ok = mask_byte(a, bk, key, len) != 0;
-    constexpr int TB = 32 * DT * 2, STAGE = 2 * TB + 256, CH = DT / 8;       // a tile of 32 rows of Q, of dout, 32 lse, 32 delta
-    constexpr int PC = 32 * CH / 256;                                         // 16-byte chunks per thread and tensor (DT 64: 1, DT 128: 2)
-    const int r0 = split * a.chunk, r1 = min(a.M, r0 + a.chunk), nt = __syncthreads_or(ok) ? (r1 - r0 + 31) / 32 : 0;
+    constexpr int RT = DKV_ROWS<DT>, TB = RT * DT * 2, STAGE = 2 * TB + RT * 8, CH = DT / 8;    // RT rows of Q, of dout, their lse, their delta
+    constexpr int PC = RT * CH / 256;                                         // 16-byte chunks per thread and tensor
+    const int r0 = split * a.chunk, r1 = min(a.M, r0 + a.chunk), nt = __syncthreads_or(ok) ? (r1 - r0 + RT - 1) / RT : 0;
 
     uint4 kf[DT / 16], vf[DT / 16];
     {
@@ -479,23 +492,26 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
 
     uint4 gq[PC], gd[PC];
     float gs = 0.f;
-    auto fetch = [&](int t) {
+    RowWalk<RT> walk[PC], stat;
+#pragma unroll
+    for (int j = 0; j < PC; ++j) walk[j].at(a, bk, hk, r0 + (tid + 256 * j) / CH);
+    if (tid < 2 * RT) stat.at(a, bk, hk, r0 + tid % RT);
+    auto fetch = [&]() {                                                       // the next tile's share of this thread
 #pragma unroll
         for (int j = 0; j < PC; ++j) {
-            const int ch = tid + 256 * j, r = r0 + t * 32 + ch / CH, c = 8 * (ch % CH);
-            const bool in = r < r1 && c < a.D;
+            const int c = 8 * ((tid + 256 * j) % CH);
             gq[j] = gd[j] = make_uint4(0, 0, 0, 0);
-            if (in) {
-                const RowAt w = row_at(a, bk, hk, r);
-                gq[j] = *reinterpret_cast<const uint4*>(a.q + off_at(w, a.q_sb, a.q_sl, a.q_sh) + c);
-                gd[j] = *reinterpret_cast<const uint4*>(a.dout + off_at(w, a.d_sb, a.d_sl, a.d_sh) + c);
+            if (walk[j].r < r1 && c < a.D) {
+                gq[j] = *reinterpret_cast<const uint4*>(a.q + walk[j].q + c);
+                gd[j] = *reinterpret_cast<const uint4*>(a.dout + walk[j].d + c);
             }
+            walk[j].step(a, bk, hk);
         }
-        if (tid < 64) {                                                        // 32 x -lse (base 2), 32 x delta; absent rows: P = exp2(-inf) = 0
-            const int r = r0 + t * 32 + (tid & 31);
-            if (r >= r1) gs = tid < 32 ? NEG_INF : 0.f;
-            else if (tid < 32) gs = P_UP<F16> - a.lse[off_lse(a, row_at(a, bk, hk, r))] * LOG2E;
-            else gs = a.delta[(int64_t)grp * a.M + r];
+        if (tid < 2 * RT) {                                                    // -lse (base 2), delta; absent rows: P = exp2(-inf) = 0
+            if (stat.r >= r1) gs = tid < RT ? NEG_INF : 0.f;
+            else if (tid < RT) gs = P_UP<F16> - a.lse[stat.lse] * LOG2E;
+            else gs = a.delta[(int64_t)grp * a.M + stat.r];
+            stat.step(a, bk, hk);
         }
     };
     auto put = [&](int buf) {
@@ -506,15 +522,17 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
             *reinterpret_cast<uint4*>(s + at) = gq[j];
             *reinterpret_cast<uint4*>(s + TB + at) = gd[j];
         }
-        if (tid < 64) reinterpret_cast<float*>(s + 2 * TB)[tid] = gs;
+        if (tid < 2 * RT) reinterpret_cast<float*>(s + 2 * TB)[tid] = gs;
     };
-    if (nt > 0) { fetch(0); put(0); }
+    if (nt > 0) { fetch(); put(0); }
     __syncthreads();
     for (int t = 0; t < nt; ++t) {
-        const unsigned char* qt = conv_lds_dyn + (t & 1) * STAGE;
+        if (t + 1 < nt) fetch();
+#pragma unroll
+        for (int rb = 0; rb < RT / 32; ++rb) {
+        const unsigned char* qt = conv_lds_dyn + (t & 1) * STAGE + rb * 32 * DT * 2;      // (a block's rows start at a multiple of 32: the same swizzle)
         const unsigned char* dt = qt + TB;
-        const float* st = reinterpret_cast<const float*>(qt + 2 * TB);
-        if (t + 1 < nt) fetch(t + 1);
+        const float* st = reinterpret_cast<const float*>(conv_lds_dyn + (t & 1) * STAGE + 2 * TB) + 32 * rb;
         f32x16 s, dp[1];
 #pragma unroll
         for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[0][i] = 0.f; }
@@ -541,7 +559,7 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
         reads_stay();
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const float4 nl = *reinterpret_cast<const float4*>(st + 8 * q + 4 * h), de = *reinterpret_cast<const float4*>(st + 32 + 8 * q + 4 * h);
+            const float4 nl = *reinterpret_cast<const float4*>(st + 8 * q + 4 * h), de = *reinterpret_cast<const float4*>(st + RT + 8 * q + 4 * h);
             const float n4[4] = {nl.x, nl.y, nl.z, nl.w}, d4[4] = {de.x, de.y, de.z, de.w};
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -566,6 +584,7 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
             else dk[d] = T16<F16>::mfma32(c[i % AHEAD], ds[u], dk[d]);
             if (i + AHEAD < NC) c[i % AHEAD] = column(i + AHEAD);
             reads_stay();
+        }
         }
         if (t + 1 < nt) put((t + 1) & 1);
         __syncthreads();
@@ -619,7 +638,18 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
 #pragma unroll
         for (int ks = 0; ks < DT / 16; ++ks) { qf[ks] = row_frag(q, ks, h, a.D, r < a.M); df[ks] = row_frag(d, ks, h, a.D, r < a.M); }
         nl = r < a.M ? P_UP<F16> - a.lse[off_lse(a, w)] * LOG2E : NEG_INF;
-        de = r < a.M ? a.delta[(int64_t)grp * a.M + r] : 0.f;
+        // delta = rowsum(dout o out): this lane's half of the row, then the other's; kept for the dK, dV kernel
+        const uint16_t* o = a.out + off_out(a, w);
+        de = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < DT / 16; ++ks) {
+            const uint4 x = row_frag(o, ks, h, a.D, r < a.M), y = df[ks];
+            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) de += T16<F16>::lo(xs[i]) * T16<F16>::lo(ys[i]) + T16<F16>::hi(xs[i]) * T16<F16>::hi(ys[i]);
+        }
+        de = sum_halves(de);
+        if (split == 0 && h == 0 && r < a.M) a.delta[(int64_t)grp * a.M + r] = de;
     }
     f32x16 acc[DT / 32];
 #pragma unroll
@@ -710,30 +740,38 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
         }
 }
 
-// sums of the splits in their order: the states' rows of [Bk, Lk, Hk, D] (KEYS: grid.y = dk, dv) or the query rows of [B, Lq, Hq, D]; 16
-// lanes per row
-template <bool F16, int DT, bool KEYS>
-__global__ __launch_bounds__(256) void xattn_sum_kernel(XattnArgs a, int n) {
+// sums of the splits in their order, 16 lanes per row: the rows of dQ, then the states of dK, then those of dV (whichever were split)
+struct SumArgs {
+    const float *pq, *pk, *pv;
+    int64_t rows, states;                          // rows of dQ, states of dK (and of dV); 0: not split
+    int sq, sk;                                    // their splits
+};
+template <bool F16, int DT>
+__global__ __launch_bounds__(256) void xattn_sum_kernel(XattnArgs a, SumArgs p) {
     T16<F16>::enter();
-    const float* part = blockIdx.y ? a.part2 : a.part;
-    uint16_t* dst = !KEYS ? a.dq : blockIdx.y ? a.dv : a.dk;
-    const int64_t rows = (int64_t)a.Bk * a.Hk * n, row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-    if (row >= rows) return;
-    const int grp = (int)(row / n), i = (int)(row % n), l = threadIdx.x & 15;
+    int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    if (row >= p.rows + 2 * p.states) return;
+    const int l = threadIdx.x & 15;
+    const bool query = row < p.rows, value = row >= p.rows + p.states;
+    if (!query) row -= value ? p.rows + p.states : p.rows;
+    const int n = query ? a.M : a.Lk, splits = query ? p.sq : p.sk, grp = (int)(row / n), i = (int)(row % n);
+    const int64_t step = (query ? p.rows : p.states) * DT;
     constexpr int E = DT / 16;
+    const float* from = (query ? p.pq : value ? p.pv : p.pk) + row * DT + l * E;
     float o[E] = {};
-    for (int s = 0; s < a.splits; ++s) {
-        const float* p = part + (s * rows + row) * DT + l * E;
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s) {
 #pragma unroll
         for (int e = 0; e < E; e += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(p + e);
+            const float4 v = *reinterpret_cast<const float4*>(from + s * step + e);
             o[e] += v.x; o[e + 1] += v.y; o[e + 2] += v.z; o[e + 3] += v.w;
         }
     }
-    const int64_t at = KEYS ? (((int64_t)(grp / a.Hk) * a.Lk + i) * a.Hk + grp % a.Hk) * a.D : off_out(a, row_at(a, grp / a.Hk, grp % a.Hk, i));
+    const int64_t at = query ? off_out(a, row_at(a, grp / a.Hk, grp % a.Hk, i)) : (((int64_t)(grp / a.Hk) * a.Lk + i) * a.Hk + grp % a.Hk) * a.D;
+    uint16_t* to = (query ? a.dq : value ? a.dv : a.dk) + at + l * E;
 #pragma unroll
     for (int e = 0; e < E; e += 4)
-        if (l * E + e < a.D) *reinterpret_cast<uint2*>(dst + at + l * E + e) = make_uint2(T16<F16>::pack2(o[e], o[e + 1]), T16<F16>::pack2(o[e + 2], o[e + 3]));
+        if (l * E + e < a.D) *reinterpret_cast<uint2*>(to + e) = make_uint2(T16<F16>::pack2(o[e], o[e + 1]), T16<F16>::pack2(o[e + 2], o[e + 3]));
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------------
@@ -823,34 +861,33 @@ int fwd(XattnArgs a, float* ws, hipStream_t st) {
 
 template <bool F16, int DT>
 int bwd(XattnArgs a, float* ws, hipStream_t st) {
-    const int64_t rows = (int64_t)a.Bk * a.Hk * a.M;
+    const int64_t rows = (int64_t)a.Bk * a.Hk * a.M, states = (int64_t)a.Bk * a.Hk * a.Lk;
+    const Plan q = plan_dq(a), k = plan_dkv(a);
+    constexpr int RT = DKV_ROWS<DT>;
+    a.walk = RT % a.G == 0 && (int64_t)a.Lq * a.G >= RT;
     a.delta = ws;
-    float* part = ws + (rows + 63) / 64 * 64;
-    xattn_delta_kernel<F16><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(a);
-    ISB_LAUNCHED("xattn_delta", st);
+    float* pq = ws + (rows + 63) / 64 * 64;
+    float* pk = pq + (q.splits > 1 ? q.splits * rows * DT : 0);
+    float* pv = pk + (int64_t)k.splits * states * DT;
     unsigned grid = 0;
-    const int64_t states = (int64_t)a.Bk * a.Hk * a.Lk;
-    Plan p = plan_dkv(a);
-    ISB_TRY(items(a, p, grid));
-    a.part = part;
-    a.part2 = part + (int64_t)p.splits * states * DT;
-    ISB_TRY((launch<xattn_dkv_kernel<F16, DT>>("xattn_dkv", grid, 256, 2 * (2 * 32 * DT * 2 + 256), a, st)));
-    if (p.splits > 1) {
-        xattn_sum_kernel<F16, DT, true><<<dim3((unsigned)((states + 15) / 16), 2), 256, 0, st>>>(a, a.Lk);
-        ISB_LAUNCHED("xattn_sum dk, dv", st);
-    }
-    p = plan_dq(a);
-    ISB_TRY(items(a, p, grid));
+    ISB_TRY(items(a, q, grid));
+    a.part = pq;
     ISB_TRY((launch<xattn_dq_kernel<F16, DT>>("xattn_dq", grid, 256, 2 * (2 * KT * DT * 2 + KT * 4), a, st)));
-    if (p.splits > 1) {
-        xattn_sum_kernel<F16, DT, false><<<(unsigned)((rows + 15) / 16), 256, 0, st>>>(a, a.M);
-        ISB_LAUNCHED("xattn_sum dq", st);
+    ISB_TRY(items(a, k, grid));
+    a.part = pk;
+    a.part2 = pv;
+    ISB_TRY((launch<xattn_dkv_kernel<F16, DT>>("xattn_dkv", grid, 256, 2 * DKV_ROWS<DT> * (2 * DT * 2 + 8), a, st)));
+    const SumArgs p{pq, pk, pv, q.splits > 1 ? rows : 0, k.splits > 1 ? states : 0, q.splits, k.splits};
+    const int64_t n = p.rows + 2 * p.states;
+    if (n > 0) {
+        xattn_sum_kernel<F16, DT><<<(unsigned)((n + 15) / 16), 256, 0, st>>>(a, p);
+        ISB_LAUNCHED("xattn_sum", st);
     }
     return ISB_OK;
 }
 }  // namespace
 
-// bytes of workspace; the partial results of dK / dV and of dQ take turns in the same place (one stream orders them)
+// bytes of workspace
 size_t xattn_workspace(const XattnArgs& a, bool backward) {
     const size_t rows = (size_t)a.Bk * a.Hk * a.M, states = (size_t)a.Bk * a.Hk * a.Lk, dt = dt_of(a);
     if (!backward) {
@@ -859,7 +896,7 @@ size_t xattn_workspace(const XattnArgs& a, bool backward) {
     }
     const Plan k = plan_dkv(a), q = plan_dq(a);
     const size_t pk = k.splits > 1 ? 2 * k.splits * states * dt : 0, pq = q.splits > 1 ? q.splits * rows * dt : 0;
-    return ((rows + 63) / 64 * 64 + std::max(pk, pq)) * 4;
+    return ((rows + 63) / 64 * 64 + pk + pq) * 4;
 }
 int launch_xattn_fwd(XattnArgs a, bool f16, float* ws, hipStream_t st) {
     if (dt_of(a) == 64) return f16 ? fwd<true, 64>(a, ws, st) : fwd<false, 64>(a, ws, st);
