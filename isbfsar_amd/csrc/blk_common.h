@@ -77,6 +77,11 @@ __device__ __forceinline__ void dma16_desc(i32x4 desc, uint32_t voff, uint32_t l
     const uint32_t la = __builtin_amdgcn_readfirstlane(lds_addr);
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(desc), "s"(la) : "memory");
 }
+// the same from an address of each lane's own
+__device__ __forceinline__ void dma16_lane(const void* src, uint32_t lds_addr) {
+    const uint32_t la = __builtin_amdgcn_readfirstlane(lds_addr);
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(la) : "memory");
+}
 __device__ __forceinline__ uint32_t lds_addr_of(const void* p) { return (uint32_t)(uintptr_t)(lds_ptr_t)(void*)p; }
 
 // every request and LDS access of this wave is done; then the workgroup meets

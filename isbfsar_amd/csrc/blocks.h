@@ -18,6 +18,7 @@ struct XattnArgs {
     float* lse;                                          // [B, Hq, Lq]
     uint16_t *dq, *dk, *dv;                              // contiguous, shapes of q, k, v
     float* delta;                                        // backward: [Bk, Hk, M] rowsum(dout * out)
+    uint16_t* zeros;                                     // 16 bytes of zeros
     float* part;                                         // partial results of the splits
     float* part2;
     FastDiv by_lqg, by_g;

@@ -460,7 +460,7 @@ __device__ __forceinline__ uint4 pack8(const f32x16& x, int t) {
 }
 
 // dK, dV: S = Q K^T with the rows in the accumulator's rows and a state per lane; P and dS are then operands over the rows.
-template <int DT> constexpr int DKV_ROWS = DT == 64 ? 64 : 32;      // rows per barrier: 128 wide, the registers hold the requests of 32
+constexpr int DKV_ROWS = 64;                                        // rows per barrier
 template <bool F16, int DT>
 __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnArgs a) {
     T16<F16>::enter();
@@ -471,7 +471,7 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
     const int key = kt * 128 + wave * 32 + (lane & 31);
     const int len = states_of(a, bk);
     const bool ok = mask_byte(a, bk, key, len) != 0;
-    constexpr int RT = DKV_ROWS<DT>, TB = RT * DT * 2, STAGE = 2 * TB + RT * 8, CH = DT / 8;    // RT rows of Q, of dout, their lse, their delta
+    constexpr int RT = DKV_ROWS, TB = RT * DT * 2, STAGE = 2 * TB + RT * 8, CH = DT / 8;    // RT rows of Q, of dout, their lse, their delta
     constexpr int PC = RT * CH / 256;                                         // 16-byte chunks per thread and tensor
     const int r0 = split * a.chunk, r1 = min(a.M, r0 + a.chunk), nt = __syncthreads_or(ok) ? (r1 - r0 + RT - 1) / RT : 0;
 
@@ -490,21 +490,22 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
         for (int i = 0; i < 16; ++i) { dk[d][i] = 0.f; dv[d][i] = 0.f; }
     float sc = F16 ? 0.f : 1.0f;
 
-    uint4 gq[PC], gd[PC];
+    // A tile's rows arrive by LDS-DMA, a 16-byte chunk per lane at a time, from wherever the row lies; absent rows and chunks past D come from a
+    // few zeros. (Through registers the 256 + 256 of a wave do not reach: the loads were waited for at once, to be put away.)
     float gs = 0.f;
     RowWalk<RT> walk[PC], stat;
 #pragma unroll
     for (int j = 0; j < PC; ++j) walk[j].at(a, bk, hk, r0 + (tid + 256 * j) / CH);
     if (tid < 2 * RT) stat.at(a, bk, hk, r0 + tid % RT);
-    auto fetch = [&]() {                                                       // the next tile's share of this thread
+    const uint32_t lds0 = lds_addr_of(conv_lds_dyn);
+    auto fetch = [&](int buf) {                                                // the next tile's share of this thread
 #pragma unroll
         for (int j = 0; j < PC; ++j) {
-            const int c = 8 * ((tid + 256 * j) % CH);
-            gq[j] = gd[j] = make_uint4(0, 0, 0, 0);
-            if (walk[j].r < r1 && c < a.D) {
-                gq[j] = *reinterpret_cast<const uint4*>(a.q + walk[j].q + c);
-                gd[j] = *reinterpret_cast<const uint4*>(a.dout + walk[j].d + c);
-            }
+            const int p = tid + 256 * j, c = 8 * ((p % CH) ^ tile_xor<DT>(p / CH));
+            const bool in = walk[j].r < r1 && c < a.D;
+            const uint32_t to = lds0 + buf * STAGE + (wave * 64 + 256 * j) * 16;
+            dma16_lane(in ? a.q + walk[j].q + c : a.zeros, to);
+            dma16_lane(in ? a.dout + walk[j].d + c : a.zeros, to + TB);
             walk[j].step(a, bk, hk);
         }
         if (tid < 2 * RT) {                                                    // -lse (base 2), delta; absent rows: P = exp2(-inf) = 0
@@ -515,79 +516,90 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
         }
     };
     auto put = [&](int buf) {
-        unsigned char* s = conv_lds_dyn + buf * STAGE;
-#pragma unroll
-        for (int j = 0; j < PC; ++j) {
-            const int ch = tid + 256 * j, at = tile_at<DT>(ch / CH, ch % CH);
-            *reinterpret_cast<uint4*>(s + at) = gq[j];
-            *reinterpret_cast<uint4*>(s + TB + at) = gd[j];
-        }
-        if (tid < 2 * RT) reinterpret_cast<float*>(s + 2 * TB)[tid] = gs;
+        if (tid < 2 * RT) reinterpret_cast<float*>(conv_lds_dyn + buf * STAGE + 2 * TB)[tid] = gs;
     };
-    if (nt > 0) { fetch(); put(0); }
-    __syncthreads();
+    if (nt > 0) { fetch(0); put(0); }
+    wait_all_and_meet();
     for (int t = 0; t < nt; ++t) {
-        if (t + 1 < nt) fetch();
-#pragma unroll
-        for (int rb = 0; rb < RT / 32; ++rb) {
-        const unsigned char* qt = conv_lds_dyn + (t & 1) * STAGE + rb * 32 * DT * 2;      // (a block's rows start at a multiple of 32: the same swizzle)
+        if (t + 1 < nt) fetch((t + 1) & 1);
+        // two blocks of 32 rows, one behind the other: while the matrix cores form the second block's S and dP, the vector ALU makes P and dS of
+        // the first; while they add the first block to dV and dK, it makes those of the second
+        const unsigned char* qt = conv_lds_dyn + (t & 1) * STAGE;
         const unsigned char* dt = qt + TB;
-        const float* st = reinterpret_cast<const float*>(conv_lds_dyn + (t & 1) * STAGE + 2 * TB) + 32 * rb;
-        f32x16 s, dp[1];
+        const float* st = reinterpret_cast<const float*>(qt + 2 * TB);
+        constexpr int N = DT / 8, AHEAD = 4, PER = 16 / N;                     // products of a block's S and dP (and of its share of dV and dK)
+        f32x16 s[2], dp[2][1];
+        uint4 f[AHEAD], w[2][2], ds[2][2];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[0][i] = 0.f; }
-        {
-            constexpr int N = DT / 8, AHEAD = 4;                               // Q's fragments, then dout's
-            uint4 f[AHEAD];
+        for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) f[i] = frag_rows<DT>(qt, 0, i, lane);
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int n = i + AHEAD;
-                if (i < N / 2) s = T16<F16>::mfma32(f[i % AHEAD], kf[i], s);
-                else dp[0] = T16<F16>::mfma32(f[i % AHEAD], vf[i - N / 2], dp[0]);
-                if (n < N) f[i % AHEAD] = n < N / 2 ? frag_rows<DT>(qt, 0, n, lane) : frag_rows<DT>(dt, 0, n - N / 2, lane);
-                reads_stay();
+            for (int i = 0; i < 16; ++i) { s[rb][i] = 0.f; dp[rb][0][i] = 0.f; }
+        auto rows = [&](int n) {                                               // fragment n of the 2 N of S and dP: Q's rows, dout's rows
+            const int rb = n / N, i = n % N;
+            return frag_rows<DT>(i < N / 2 ? qt : dt, 32 * rb, i % (N / 2), lane);
+        };
+        auto cols = [&](int n) {                                               // fragment n of the 2 N of dV and dK: dout's and Q's columns in turn
+            const int rb = n / N, i = n % N;
+            return frag_cols<DT, 4, 8>(i % 2 == 0 ? dt : qt, 32 * rb + 16 * (i / 2 % 2), 32 * (i / 4), lane);
+        };
+        auto score = [&](int n) {
+            const int rb = n / N, i = n % N;
+            if (i < N / 2) s[rb] = T16<F16>::mfma32(f[n % AHEAD], kf[i], s[rb]);
+            else dp[rb][0] = T16<F16>::mfma32(f[n % AHEAD], vf[i - N / 2], dp[rb][0]);
+            f[n % AHEAD] = n + AHEAD < 2 * N ? rows(n + AHEAD) : cols(n + AHEAD - 2 * N);
+        };
+        auto add = [&](int n) {
+            const int rb = n / N, i = n % N, d = i / 4, u = i / 2 % 2;
+            if (i % 2 == 0) dv[d] = T16<F16>::mfma32(f[n % AHEAD], w[rb][u], dv[d]);
+            else dk[d] = T16<F16>::mfma32(f[n % AHEAD], ds[rb][u], dk[d]);
+            if (n + AHEAD < 2 * N) f[n % AHEAD] = cols(n + AHEAD);
+        };
+        float4 nl, de;
+        auto weigh = [&](int rb, int i) {                                      // row i of the block: P = exp2(c S - lse), dS = P (dP - delta)
+            if (i % 4 == 0) {
+                nl = *reinterpret_cast<const float4*>(st + 32 * rb + 2 * i + 4 * h);
+                de = *reinterpret_cast<const float4*>(st + RT + 32 * rb + 2 * i + 4 * h);
             }
-        }
-        // columns of dout and Q for dV^T += dout^T P, dK^T += Q^T dS; the first ones travel while P and dS are formed
-        constexpr int NC = DT / 8, AHEAD = 4;
-        auto column = [&](int i) { return frag_cols<DT, 4, 8>(i % 2 == 0 ? dt : qt, 16 * (i / 2 % 2), 32 * (i / 4), lane); };
-        uint4 c[AHEAD];
+            const float n1 = i % 4 == 0 ? nl.x : i % 4 == 1 ? nl.y : i % 4 == 2 ? nl.z : nl.w, d1 = i % 4 == 0 ? de.x : i % 4 == 1 ? de.y : i % 4 == 2 ? de.z : de.w;
+            s[rb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][i], a.c, n1));
+            dp[rb][0][i] = s[rb][i] * (dp[rb][0][i] - d1);
+        };
+        auto round = [&](int rb) {
+            if constexpr (F16) {        // a masked state's column is not stored, but must not set the power of two either
+                if (!ok) {
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) c[i] = column(i);
-        reads_stay();
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const float4 nl = *reinterpret_cast<const float4*>(st + 8 * q + 4 * h), de = *reinterpret_cast<const float4*>(st + RT + 8 * q + 4 * h);
-            const float n4[4] = {nl.x, nl.y, nl.z, nl.w}, d4[4] = {de.x, de.y, de.z, de.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[4 * q + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * q + i], a.c, n4[i]));
-                dp[0][4 * q + i] = s[4 * q + i] * (dp[0][4 * q + i] - d4[i]);
+                    for (int i = 0; i < 16; ++i) dp[rb][0][i] = 0.f;
+                }
             }
-        }
-        if constexpr (F16) {            // a masked state's column is not stored, but must not set the power of two either
-            if (!ok) {
+            scale_ds<F16, 1, DT / 32>(dp[rb], dk, sc);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) dp[0][i] = 0.f;
-            }
-        }
-        scale_ds<F16, 1, DT / 32>(dp, dk, sc);
-        uint4 p[2], ds[2];
+            for (int u = 0; u < 2; ++u) { w[rb][u] = pack8<F16>(s[rb], u); ds[rb][u] = pack8<F16>(dp[rb][0], u); }
+        };
 #pragma unroll
-        for (int u = 0; u < 2; ++u) { p[u] = pack8<F16>(s, u); ds[u] = pack8<F16>(dp[0], u); }
+        for (int i = 0; i < AHEAD; ++i) f[i] = rows(i);
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int d = i / 4, u = i / 2 % 2;
-            if (i % 2 == 0) dv[d] = T16<F16>::mfma32(c[i % AHEAD], p[u], dv[d]);
-            else dk[d] = T16<F16>::mfma32(c[i % AHEAD], ds[u], dk[d]);
-            if (i + AHEAD < NC) c[i % AHEAD] = column(i + AHEAD);
+        for (int i = 0; i < N; ++i) { score(i); reads_stay(); }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            score(N + i);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) weigh(0, PER * i + e);
             reads_stay();
         }
+        round(0);
+        // fp16: the first block's dS carries the scale of its round; the second block may lower it only after the first is added
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            add(i);
+#pragma unroll
+            for (int e = 0; e < PER; ++e) weigh(1, PER * i + e);
+            reads_stay();
         }
+        round(1);
+#pragma unroll
+        for (int i = 0; i < N; ++i) { add(N + i); reads_stay(); }
         if (t + 1 < nt) put((t + 1) & 1);
-        __syncthreads();
+        wait_all_and_meet();
     }
     if (key >= a.Lk) return;
     const float fv = ok ? __builtin_amdgcn_exp2f(-P_UP<F16>) : 0.f;
@@ -649,6 +661,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
             for (int i = 0; i < 4; ++i) de += T16<F16>::lo(xs[i]) * T16<F16>::lo(ys[i]) + T16<F16>::hi(xs[i]) * T16<F16>::hi(ys[i]);
         }
         de = sum_halves(de);
+        if (item == 0 && threadIdx.x < 8) a.zeros[threadIdx.x] = 0;            // (the dK, dV kernel's absent rows)
         if (split == 0 && h == 0 && r < a.M) a.delta[(int64_t)grp * a.M + r] = de;
     }
     f32x16 acc[DT / 32];
@@ -863,10 +876,11 @@ template <bool F16, int DT>
 int bwd(XattnArgs a, float* ws, hipStream_t st) {
     const int64_t rows = (int64_t)a.Bk * a.Hk * a.M, states = (int64_t)a.Bk * a.Hk * a.Lk;
     const Plan q = plan_dq(a), k = plan_dkv(a);
-    constexpr int RT = DKV_ROWS<DT>;
+    constexpr int RT = DKV_ROWS;
     a.walk = RT % a.G == 0 && (int64_t)a.Lq * a.G >= RT;
-    a.delta = ws;
-    float* pq = ws + (rows + 63) / 64 * 64;
+    a.zeros = reinterpret_cast<uint16_t*>(ws);
+    a.delta = ws + 64;
+    float* pq = ws + 64 + (rows + 63) / 64 * 64;
     float* pk = pq + (q.splits > 1 ? q.splits * rows * DT : 0);
     float* pv = pk + (int64_t)k.splits * states * DT;
     unsigned grid = 0;
@@ -876,7 +890,7 @@ int bwd(XattnArgs a, float* ws, hipStream_t st) {
     ISB_TRY(items(a, k, grid));
     a.part = pk;
     a.part2 = pv;
-    ISB_TRY((launch<xattn_dkv_kernel<F16, DT>>("xattn_dkv", grid, 256, 2 * DKV_ROWS<DT> * (2 * DT * 2 + 8), a, st)));
+    ISB_TRY((launch<xattn_dkv_kernel<F16, DT>>("xattn_dkv", grid, 256, 2 * DKV_ROWS * (2 * DT * 2 + 8), a, st)));
     const SumArgs p{pq, pk, pv, q.splits > 1 ? rows : 0, k.splits > 1 ? states : 0, q.splits, k.splits};
     const int64_t n = p.rows + 2 * p.states;
     if (n > 0) {
@@ -896,7 +910,7 @@ size_t xattn_workspace(const XattnArgs& a, bool backward) {
     }
     const Plan k = plan_dkv(a), q = plan_dq(a);
     const size_t pk = k.splits > 1 ? 2 * k.splits * states * dt : 0, pq = q.splits > 1 ? q.splits * rows * dt : 0;
-    return ((rows + 63) / 64 * 64 + pk + pq) * 4;
+    return (64 + (rows + 63) / 64 * 64 + pk + pq) * 4;
 }
 int launch_xattn_fwd(XattnArgs a, bool f16, float* ws, hipStream_t st) {
     if (dt_of(a) == 64) return f16 ? fwd<true, 64>(a, ws, st) : fwd<false, 64>(a, ws, st);
