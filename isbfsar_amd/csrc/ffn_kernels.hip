@@ -18,7 +18,7 @@ namespace {
 
 enum { EPI_GATE = 0, EPI_OUT = 1, EPI_DH = 2 };
 enum { FFN_SILU = 0, FFN_GELU = 1, FFN_RELU = 2, FFN_SIGMOID = 3 };
-constexpr int BK = 64;
+constexpr int BK = 64;                   // k per tile
 
 struct MmArgs {
     const uint16_t *A, *B, *B2;          // B2: GATE: the up weights; else the operand of the second k segment
@@ -417,11 +417,12 @@ __global__ __launch_bounds__(256) void ffn_sum_kernel(const float* part, int spl
 
 // ------------------------------------------------------------------------------------------------------------------------------------
 // At most TOKENS rows: the weights are the work, each read once in whole 1-KiB rows of a wave; dot products on the vector ALU.
-// PER waves share a weight row (pair of rows); their sums are added in wave order.
+// PER waves share a weight row (pair of rows); their sums are added in wave order. Between the two launches h stays in f32 (a few KB), so
+// that y is rounded once.
 // ------------------------------------------------------------------------------------------------------------------------------------
 constexpr int TOKENS = 4;
 template <bool F16, int MT, int PER, bool GATE>
-__global__ __launch_bounds__(256) void ffn_token_kernel(MmArgs p) {
+__global__ __launch_bounds__(256) void ffn_token_kernel(MmArgs p, float* h) {
     T16<F16>::enter();
     __shared__ float sums[4][2 * MT];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -438,9 +439,20 @@ __global__ __launch_bounds__(256) void ffn_token_kernel(MmArgs p) {
             if constexpr (GATE) b = *reinterpret_cast<const uint4*>(w1 + k);
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                const uint4 x = *reinterpret_cast<const uint4*>(p.A + (int64_t)min(t, p.M - 1) * p.lda + k);
-                s[0][t] = T16<F16>::dot2(x.w, a.w, T16<F16>::dot2(x.z, a.z, T16<F16>::dot2(x.y, a.y, T16<F16>::dot2(x.x, a.x, s[0][t]))));
-                if constexpr (GATE) s[1][t] = T16<F16>::dot2(x.w, b.w, T16<F16>::dot2(x.z, b.z, T16<F16>::dot2(x.y, b.y, T16<F16>::dot2(x.x, b.x, s[1][t]))));
+                if constexpr (GATE) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(p.A + (int64_t)min(t, p.M - 1) * p.lda + k);
+                    s[0][t] = T16<F16>::dot2(x.w, a.w, T16<F16>::dot2(x.z, a.z, T16<F16>::dot2(x.y, a.y, T16<F16>::dot2(x.x, a.x, s[0][t]))));
+                    s[1][t] = T16<F16>::dot2(x.w, b.w, T16<F16>::dot2(x.z, b.z, T16<F16>::dot2(x.y, b.y, T16<F16>::dot2(x.x, b.x, s[1][t]))));
+                } else {
+                    const float4* x = reinterpret_cast<const float4*>(h + (int64_t)min(t, p.M - 1) * p.K + k);
+                    const float4 x0 = x[0], x1 = x[1];
+                    float v = s[0][t];
+                    v = __builtin_fmaf(x0.x, T16<F16>::lo(a.x), v); v = __builtin_fmaf(x0.y, T16<F16>::hi(a.x), v);
+                    v = __builtin_fmaf(x0.z, T16<F16>::lo(a.y), v); v = __builtin_fmaf(x0.w, T16<F16>::hi(a.y), v);
+                    v = __builtin_fmaf(x1.x, T16<F16>::lo(a.z), v); v = __builtin_fmaf(x1.y, T16<F16>::hi(a.z), v);
+                    v = __builtin_fmaf(x1.z, T16<F16>::lo(a.w), v); v = __builtin_fmaf(x1.w, T16<F16>::hi(a.w), v);
+                    s[0][t] = v;
+                }
             }
         }
     }
@@ -471,8 +483,9 @@ __global__ __launch_bounds__(256) void ffn_token_kernel(MmArgs p) {
             const float u = s[1][t] + (p.bias2 ? T16<F16>::to_f32(p.bias2[n]) : 0.f);
             if (p.g) { p.g[(int64_t)t * p.F + n] = o; p.u[(int64_t)t * p.F + n] = u; }
             o = act_of(p.act, o) * u;
+            h[(int64_t)t * p.F + n] = o;
         }
-        p.C[(int64_t)t * (GATE ? p.F : p.ldc) + n] = T16<F16>::from_f32(o);
+        if (!GATE || p.C) p.C[(int64_t)t * (GATE ? p.F : p.ldc) + n] = T16<F16>::from_f32(o);      // (GATE: only if h is saved)
     }
 }
 
@@ -590,10 +603,10 @@ size_t part_bytes(int la, int M, int N, int kts) {
     return s > 1 ? (size_t)s * M * N * 4 : 0;
 }
 template <bool F16, int MT, bool GATE>
-int token(const MmArgs& p, hipStream_t st) {
+int token(const MmArgs& p, float* h, hipStream_t st) {
     const int n = GATE ? p.F : p.N;
-    if (p.K > 2048) ffn_token_kernel<F16, MT, 4, GATE><<<n, 256, 0, st>>>(p);
-    else ffn_token_kernel<F16, MT, 1, GATE><<<cdiv(n, 4), 256, 0, st>>>(p);
+    if (p.K > 2048) ffn_token_kernel<F16, MT, 4, GATE><<<n, 256, 0, st>>>(p, h);
+    else ffn_token_kernel<F16, MT, 1, GATE><<<cdiv(n, 4), 256, 0, st>>>(p, h);
     ISB_LAUNCHED("ffn_token", st);
     return ISB_OK;
 }
@@ -601,7 +614,7 @@ int token(const MmArgs& p, hipStream_t st) {
 template <bool F16>
 int fwd(const FfnArgs& a, unsigned char* ws, hipStream_t st) {
     uint16_t* h = a.h;
-    if (!h) {
+    if (!h && a.M > TOKENS) {
         h = reinterpret_cast<uint16_t*>(ws);
         ws += ((size_t)a.M * a.F * 2 + 255) / 256 * 256;
     }
@@ -614,12 +627,13 @@ int fwd(const FfnArgs& a, unsigned char* ws, hipStream_t st) {
     d.M = a.M; d.N = a.D; d.K = a.F; d.nseg = 1; d.splits = 1;
     d.bias = a.bd; d.C = a.y; d.ldc = a.D;
     if (a.M <= TOKENS) {
+        float* hf = reinterpret_cast<float*>(ws);
         if (a.M == 1) {
-            ISB_TRY((token<F16, 1, true>(g, st)));
-            return token<F16, 1, false>(d, st);
+            ISB_TRY((token<F16, 1, true>(g, hf, st)));
+            return token<F16, 1, false>(d, hf, st);
         }
-        ISB_TRY((token<F16, TOKENS, true>(g, st)));
-        return token<F16, TOKENS, false>(d, st);
+        ISB_TRY((token<F16, TOKENS, true>(g, hf, st)));
+        return token<F16, TOKENS, false>(d, hf, st);
     }
     ISB_TRY((mm<F16, 0, 0, EPI_GATE>(g, "ffn gate + up", st)));
     return mm_out<F16, 0, 0>(d, reinterpret_cast<float*>(ws), "ffn down", st);
@@ -668,8 +682,9 @@ int bwd(const FfnArgs& a, unsigned char* ws, hipStream_t st) {
 size_t ffn_workspace(const FfnArgs& a, bool backward) {
     const size_t M = a.M, F = a.F;
     if (!backward) {
+        if (a.M <= TOKENS) return M * F * 4;
         const size_t h = a.h ? 0 : (M * F * 2 + 255) / 256 * 256;
-        return h + (a.M <= TOKENS ? 0 : part_bytes(0, a.M, a.D, cdiv(a.F, BK)));
+        return h + part_bytes(0, a.M, a.D, cdiv(a.F, BK));
     }
     const size_t sums = (size_t)cdiv(a.M, 32) * ((a.dbg ? 2 * F : 0) + (a.dbd ? a.D : 0)) * 4;
     const size_t part = std::max(std::max(sums, part_bytes(0, a.M, a.D, 2 * cdiv(a.F, BK))),
