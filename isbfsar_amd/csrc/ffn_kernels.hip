@@ -40,7 +40,7 @@ __device__ __forceinline__ float sigmoid_(float x) { return __builtin_amdgcn_rcp
 __device__ __forceinline__ float act_of(int act, float g) {
     if (act == FFN_SILU) return g * sigmoid_(g);
     if (act == FFN_GELU) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
-    if (act == FFN_RELU) return fmaxf(g, 0.f);
+    if (act == FFN_RELU) return g < 0.f ? 0.f : g;             // (a NaN stays one)
     return sigmoid_(g);
 }
 __device__ __forceinline__ void act_and_slope(int act, float g, float& f, float& d) {
@@ -49,7 +49,7 @@ __device__ __forceinline__ void act_and_slope(int act, float g, float& f, float&
         f = g * phi;
         d = phi + g * 0.3989422804014327f * __builtin_amdgcn_exp2f(-0.5f * LOG2E * g * g);
     } else if (act == FFN_RELU) {
-        f = fmaxf(g, 0.f);
+        f = g < 0.f ? 0.f : g;
         d = g > 0.f ? 1.f : 0.f;
     } else {
         const float s = sigmoid_(g), c = 1.0f - s;
