@@ -91,6 +91,16 @@ __device__ __forceinline__ void wait_all_and_meet() {
     asm volatile("" ::: "memory");
 }
 
+// Conversions to fp16 saturate from here on (MODE.FP16_OVFL, as T16::enter()), for kernels with matrix products: with the bit set, an fp16
+// matrix product takes a NaN operand for 0, so it is set behind the last one. Returns 1.0, and what is converted has to be a product with it:
+// that keeps the conversions behind the switch.
+template <bool F16>
+__device__ __forceinline__ float saturate_from_here() {
+    float one = 1.0f;
+    if constexpr (F16) asm volatile("s_setreg_imm32_b32 hwreg(HW_REG_MODE, 23, 1), 1\n\ts_nop 1\n\tv_mov_b32 %0, 1.0" : "=v"(one)::"memory");
+    return one;
+}
+
 // the other half's value of a pair of lanes (l, l ^ 32)
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void both_halves(float x, float& lo, float& hi) {

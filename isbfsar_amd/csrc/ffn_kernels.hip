@@ -34,7 +34,17 @@ struct MmArgs {
     float* cs;                           // DH: column sums of dG | dU over 32 rows, [ceil(M / 32)][2 F], or null
     int F, act;
     int tiles_m, tiles_n, n_items;
+    int full, tail, tail_splits, tail_per, kt_per_tail;   // OUT: the last `tail` tiles, behind `full` whole rounds of the chip, split k (0: none)
 };
+
+// Bands of GM m tiles with the n tiles side by side: the 32 or 64 items that an XCD runs at a time are a block of 8 x 4 or 8 x 8 tiles, whose
+// operands its L2 fetches once (one n tile with every m tile instead: 384 us for 355, 7680 x 1280 x 5120)
+__device__ __forceinline__ void tile_at_item(int lin, int tiles_m, int tiles_n, int& tm, int& tn) {
+    constexpr int GM = 8;
+    const int band = lin / (GM * tiles_n), bm = min(GM, tiles_m - band * GM), r = lin - band * GM * tiles_n;
+    tm = band * GM + r % bm;
+    tn = r / bm;
+}
 
 __device__ __forceinline__ float sigmoid_(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-LOG2E * x)); }
 __device__ __forceinline__ float act_of(int act, float g) {
@@ -120,25 +130,36 @@ __device__ __forceinline__ void corner_done() { asm volatile("s_waitcnt lgkmcnt(
 
 template <bool F16, int BM, int BN, int NWM, int NWN, int NWK, int NBUF, int LA, int LB, int EPI>
 __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void ffn_mm_kernel(MmArgs p) {
-    T16<F16>::enter();
     constexpr int NW = NWM * NWN * NWK, WM = BM / NWM, WN = BN / NWN, IM = WM / 32, IN = WN / 32;
     constexpr bool PAIR = EPI == EPI_GATE;
     static_assert(!PAIR || (IN % 2 == 0 && LB == 0), "a wave owns gate and up columns of the same features");
     constexpr int ABYTES = BM * BK * 2, STAGE = ABYTES + BN * BK * 2;
-    const int item = xcd_item(blockIdx.x, p.n_items);
-    if (item >= p.n_items) return;
-    // An XCD runs a contiguous range of items, 32 or 64 at a time: bands of GM m tiles with the n tiles side by side make those a block of
-    // 8 x 4 or 8 x 8 tiles, whose operands its L2 fetches once (one n tile with every m tile instead: 384 us for 355, 7680 x 1280 x 5120)
-    constexpr int GM = 8;
-    const int split = item / (p.tiles_m * p.tiles_n), lin = item - split * p.tiles_m * p.tiles_n;
-    const int band = lin / (GM * p.tiles_n), bm = min(GM, p.tiles_m - band * GM), at_b = lin - band * GM * p.tiles_n;
-    const int tm = band * GM + at_b % bm, tn = at_b / bm;
+    int item, split = 0, tm, tn;
+    bool tail = false;
+    if (EPI == EPI_OUT && p.tail > 0) {
+        // every XCD takes its eighth of the whole rounds, then its eighth of the tail's parts
+        const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3, per = p.full >> 3;
+        tail = slot >= per;
+        item = xcd * per + slot;
+        if (tail) {
+            const int t = xcd * p.tail_per + slot - per;
+            if (t >= p.tail * p.tail_splits) return;
+            item = p.full + t / p.tail_splits;
+            split = t % p.tail_splits;
+        }
+        tile_at_item(item, p.tiles_m, p.tiles_n, tm, tn);
+    } else {
+        item = xcd_item(blockIdx.x, p.n_items);
+        if (item >= p.n_items) return;
+        split = item / (p.tiles_m * p.tiles_n);
+        tile_at_item(item - split * p.tiles_m * p.tiles_n, p.tiles_m, p.tiles_n, tm, tn);
+    }
     const int m0 = tm * BM, n0 = tn * BN;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5;
     const int wm = wave % NWM, wn = wave / NWM % NWN, wk = wave / (NWM * NWN);
 
     const int kts = (p.K + BK - 1) / BK, total = kts * p.nseg;
-    const int t0 = split * p.kt_per_split, t1 = min(total, t0 + p.kt_per_split);
+    const int kt_per = tail ? p.kt_per_tail : p.kt_per_split, t0 = split * kt_per, t1 = min(total, t0 + kt_per);
     OpLoad<LA, BM, NW, false> la;
     OpLoad<LB, BN, NW, PAIR> lb;
     la.init(wave, lane, p.lda, p.M - m0);
@@ -292,6 +313,9 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
             }
         }
         corner_done();
+        // fp16 results saturate; the switch is set behind the products (saturate_from_here) and before anything read from the corner is converted
+        saturate_from_here<F16>();
+        corner_done();
         const int mb = m0 + wm * WM + 32 * i;
         float sg[4] = {}, su[4] = {};                                         // DH: column sums over the block's rows
         if constexpr (EPI == EPI_GATE) {
@@ -358,6 +382,8 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
                     *reinterpret_cast<uint2*>(c + p.F) = make_uint2(T16<F16>::pack2(du[0], du[1]), T16<F16>::pack2(du[2], du[3]));
                 } else if (p.splits > 1) {
                     *reinterpret_cast<float4*>(p.part + ((int64_t)split * p.M + m) * p.N + n) = o;
+                } else if (EPI == EPI_OUT && tail) {
+                    *reinterpret_cast<float4*>(p.part + ((int64_t)((item - p.full) * p.tail_splits + split) * BM + m - m0) * BN + n - n0) = o;
                 } else {
                     *reinterpret_cast<uint2*>(p.C + (int64_t)m * p.ldc + n) =
                         make_uint2(T16<F16>::pack2(o.x + bias[0], o.y + bias[1]), T16<F16>::pack2(o.z + bias[2], o.w + bias[3]));
@@ -413,6 +439,28 @@ __global__ __launch_bounds__(256) void ffn_sum_kernel(const float* part, int spl
         o[0] += T16<F16>::lo(w.x); o[1] += T16<F16>::hi(w.x); o[2] += T16<F16>::lo(w.y); o[3] += T16<F16>::hi(w.y);
     }
     *reinterpret_cast<uint2*>(C + i * 4) = make_uint2(T16<F16>::pack2(o[0], o[1]), T16<F16>::pack2(o[2], o[3]));
+}
+
+// the same for the tail's tiles: part [tail tile][split][BM][BN]; a workgroup takes 1024 values of a tile
+template <bool F16, int BM, int BN>
+__global__ __launch_bounds__(256) void ffn_tail_kernel(MmArgs p) {
+    T16<F16>::enter();
+    constexpr int PER = BM * BN / 1024;
+    const int t = blockIdx.x / PER, i = (blockIdx.x % PER * 256 + threadIdx.x) * 4;
+    int tm, tn;
+    tile_at_item(p.full + t, p.tiles_m, p.tiles_n, tm, tn);
+    const int m = tm * BM + i / BN, n = tn * BN + i % BN;
+    if (m >= p.M || n >= p.N) return;
+    float o[4] = {};
+    for (int s = 0; s < p.tail_splits; ++s) {
+        const float4 v = *reinterpret_cast<const float4*>(p.part + (int64_t)(t * p.tail_splits + s) * BM * BN + i);
+        o[0] += v.x; o[1] += v.y; o[2] += v.z; o[3] += v.w;
+    }
+    if (p.bias) {
+        const uint2 w = *reinterpret_cast<const uint2*>(p.bias + n);
+        o[0] += T16<F16>::lo(w.x); o[1] += T16<F16>::hi(w.x); o[2] += T16<F16>::lo(w.y); o[3] += T16<F16>::hi(w.y);
+    }
+    *reinterpret_cast<uint2*>(p.C + (int64_t)m * p.ldc + n) = make_uint2(T16<F16>::pack2(o[0], o[1]), T16<F16>::pack2(o[2], o[3]));
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------------
@@ -549,13 +597,31 @@ int tile_of(int la, int M, int N) {
     if (M <= 256 && la == 0) return TILE_THIN;         // (layout 1 keeps whole 128-byte rows of m in LDS: no thin form)
     return (int64_t)cdiv(M, 256) * cdiv(N, 256) >= 200 ? TILE_BIG : TILE_MID;
 }
-int splits_of(int la, int M, int N, int kts) {            // k splits of an OUT product whose tiles do not fill the chip
+// How an OUT product shares out k. Tiles that do not fill the chip once: every tile in `splits` parts. Tiles that leave a part round behind
+// whole ones: the tail's tiles in as many parts as fill it, if that is at most 5 / 8 full (7680 x 1280 from 5120: 600 tiles on 512 places,
+// 148 -> %s us).
+struct OutPlan { int splits = 1, full = 0, tail = 0, tail_splits = 0; size_t bytes = 0; };
+OutPlan plan_out(int la, int M, int N, int kts) {
     const int t = tile_of(la, M, N), bm = t == TILE_THIN ? 32 : t == TILE_MID ? 128 : 256, bn = t == TILE_BIG ? 256 : t == TILE_THIN ? 64 : 128;
     const int64_t tiles = (int64_t)cdiv(M, bm) * cdiv(N, bn);
-    const int64_t want = t == TILE_BIG ? 1 : 512 / tiles;
-    int s = (int)std::min<int64_t>(want, std::max(1, kts / (t == TILE_THIN ? 16 : 4)));
+    const int places = t == TILE_BIG ? 256 : 512;
+    OutPlan p;
+    int s = (int)std::min<int64_t>(t == TILE_BIG ? 1 : places / tiles, std::max(1, kts / (t == TILE_THIN ? 16 : 4)));
     s = std::max(1, std::min(s, 16));
-    return cdiv(kts, cdiv(kts, s));
+    p.splits = cdiv(kts, cdiv(kts, s));
+    if (p.splits > 1) {
+        p.bytes = (size_t)p.splits * M * N * 4;
+        return p;
+    }
+    const int tail = (int)(tiles % places);
+    if (t == TILE_THIN || tiles < places || tail == 0 || tail > places * 5 / 8) return p;
+    const int ts = std::min(std::min(places / tail, kts / 8), 8);
+    if (ts < 2) return p;
+    p.tail = tail;
+    p.full = (int)(tiles - tail);
+    p.tail_splits = cdiv(kts, cdiv(kts, ts));
+    p.bytes = (size_t)p.tail * p.tail_splits * bm * bn * 4;
+    return p;
 }
 
 template <bool F16, int BM, int BN, int NWM, int NWN, int NWK, int NBUF, int LA, int LB, int EPI>
@@ -563,10 +629,15 @@ int mm_run(MmArgs p, const char* name, hipStream_t st) {
     constexpr size_t lds = NBUF * (BM + BN) * BK * 2;
     p.tiles_m = cdiv(p.M, BM);
     p.tiles_n = cdiv(p.N, BN);
-    const int64_t n = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+    const int64_t n = p.tail > 0 ? p.full + 8 * cdiv(p.tail * p.tail_splits, 8) : (int64_t)p.tiles_m * p.tiles_n * p.splits;
     ISB_REQUIRE(n < (1ll << 30), ISB_ERR_INVALID, "gated feed-forward: %lld workgroups are more than one launch holds", (long long)n);
     p.n_items = (int)n;
-    p.kt_per_split = cdiv(cdiv(p.K, BK) * p.nseg, p.splits);
+    const int kts = cdiv(p.K, BK) * p.nseg;
+    p.kt_per_split = cdiv(kts, p.splits);
+    if (p.tail > 0) {
+        p.tail_per = cdiv(p.tail * p.tail_splits, 8);
+        p.kt_per_tail = cdiv(kts, p.tail_splits);
+    }
     static DevMax attr;
     if (attr.below((int)lds)) {
         ISB_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(ffn_mm_kernel<F16, BM, BN, NWM, NWN, NWK, NBUF, LA, LB, EPI>),
@@ -575,6 +646,12 @@ int mm_run(MmArgs p, const char* name, hipStream_t st) {
     }
     ffn_mm_kernel<F16, BM, BN, NWM, NWN, NWK, NBUF, LA, LB, EPI><<<(unsigned)(8 * ((n + 7) / 8)), NWM * NWN * NWK * 64, lds, st>>>(p);
     ISB_LAUNCHED(name, st);
+    if constexpr (EPI == EPI_OUT && BM >= 128) {
+        if (p.tail > 0) {
+            ffn_tail_kernel<F16, BM, BN><<<(unsigned)p.tail * (BM * BN / 1024), 256, 0, st>>>(p);
+            ISB_LAUNCHED("ffn_tail", st);
+        }
+    }
     return ISB_OK;
 }
 template <bool F16, int LA, int LB, int EPI>
@@ -588,7 +665,11 @@ int mm(const MmArgs& p, const char* name, hipStream_t st) {
 // C = A B^T (+ bias), k split where the tiles alone leave CUs idle
 template <bool F16, int LA, int LB>
 int mm_out(MmArgs p, float* part, const char* name, hipStream_t st) {
-    p.splits = splits_of(LA, p.M, p.N, cdiv(p.K, BK) * p.nseg);
+    const OutPlan plan = plan_out(LA, p.M, p.N, cdiv(p.K, BK) * p.nseg);
+    p.splits = plan.splits;
+    p.full = plan.full;
+    p.tail = plan.tail;
+    p.tail_splits = plan.tail_splits;
     p.part = part;
     ISB_TRY((mm<F16, LA, LB, EPI_OUT>(p, name, st)));
     if (p.splits > 1) {
@@ -598,10 +679,8 @@ int mm_out(MmArgs p, float* part, const char* name, hipStream_t st) {
     }
     return ISB_OK;
 }
-size_t part_bytes(int la, int M, int N, int kts) {
-    const int s = splits_of(la, M, N, kts);
-    return s > 1 ? (size_t)s * M * N * 4 : 0;
-}
+size_t part_bytes(int la, int M, int N, int kts) { return plan_out(la, M, N, kts).bytes; }
+
 template <bool F16, int MT, bool GATE>
 int token(const MmArgs& p, float* h, hipStream_t st) {
     const int n = GATE ? p.F : p.N;

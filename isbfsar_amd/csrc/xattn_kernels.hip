@@ -164,7 +164,7 @@ __device__ __forceinline__ void attend(const unsigned char* kt, const unsigned c
 
 // four columns of a row's results (and, `first`, what goes with the row): out and lse, or (splits) its unnormalised sums with maximum and sum
 template <bool F16, int DT>
-__device__ __forceinline__ void store_piece(const XattnArgs& a, int bk, int hk, int split, int r, int c, float4 o, float m, float l, bool first) {
+__device__ __forceinline__ void store_piece(const XattnArgs& a, int bk, int hk, int split, int r, int c, float4 o, float m, float l, bool first, float one) {
     if (r >= a.M) return;
     if (a.splits > 1) {
         const int64_t at = ((int64_t)split * a.Bk * a.Hk + bk * a.Hk + hk) * a.M + r;
@@ -173,7 +173,7 @@ __device__ __forceinline__ void store_piece(const XattnArgs& a, int bk, int hk, 
         return;
     }
     const RowAt w = row_at(a, bk, hk, r);
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const float inv = l == 0.f ? 0.f : one / l;
     if (c < a.D) *reinterpret_cast<uint2*>(a.out + off_out(a, w) + c) = make_uint2(T16<F16>::pack2(o.x * inv, o.y * inv), T16<F16>::pack2(o.z * inv, o.w * inv));
     if (first) a.lse[off_lse(a, w)] = l == 0.f ? NEG_INF : (m + __builtin_amdgcn_logf(l)) * LN2;
 }
@@ -184,7 +184,6 @@ __device__ __forceinline__ void store_piece(const XattnArgs& a, int bk, int hk, 
 // ------------------------------------------------------------------------------------------------------------------------------------
 template <bool F16, int DT>
 __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XattnArgs a) {
-    T16<F16>::enter();
     const int item = xcd_item(blockIdx.x, a.n_items);
     if (item >= a.n_items) return;
     const int rt = item % a.tiles, split = item / a.tiles % a.splits, grp = item / a.tiles / a.splits, bk = grp / a.Hk, hk = grp % a.Hk;
@@ -238,13 +237,14 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XattnArgs a) {
         if (bits != 0) attend<F16, DT, 2>(conv_lds_dyn + cur, conv_lds_dyn + cur + TB, qf, acc, m, l, a.c, bias, bits == ~0ull, lane);
         bits = next;
     }
+    const float one = saturate_from_here<F16>();
     l = sum_halves(l);
 #pragma unroll
     for (int d = 0; d < DT / 32; ++d)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
             store_piece<F16, DT>(a, bk, hk, split, r, 32 * d + 8 * q + 4 * h, make_float4(acc[d][4 * q], acc[d][4 * q + 1], acc[d][4 * q + 2], acc[d][4 * q + 3]),
-                                 m, l, d == 0 && q == 0 && h == 0);
+                                 m, l, d == 0 && q == 0 && h == 0, one);
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------------
@@ -257,7 +257,6 @@ constexpr int TOKEN_WAVES = 8;
 template <bool F16, int DT>
 __global__ __launch_bounds__(TOKEN_WAVES * 64, TOKEN_WAVES / 4) void xattn_token_kernel(XattnArgs a) {
     constexpr int NW = TOKEN_WAVES;
-    T16<F16>::enter();
     const int item = xcd_item(blockIdx.x, a.n_items);
     if (item >= a.n_items) return;
     const int split = item % a.splits, grp = item / a.splits, bk = grp / a.Hk, hk = grp % a.Hk;
@@ -306,6 +305,7 @@ __global__ __launch_bounds__(TOKEN_WAVES * 64, TOKEN_WAVES / 4) void xattn_token
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                    // the block is read before its place is requested again
         if (t + NW < nt) request(t + NW);
     }
+    const float one = saturate_from_here<F16>();
     l = sum_halves(l);
     // join the waves: (m, l) of all, then every wave scales its sums to the common maximum and each adds up its share of the columns, in wave
     // order
@@ -340,7 +340,7 @@ __global__ __launch_bounds__(TOKEN_WAVES * 64, TOKEN_WAVES / 4) void xattn_token
             const float4 u = *reinterpret_cast<const float4*>(sums + (w * 32 + r) * SW + c);
             t.x += u.x; t.y += u.y; t.z += u.z; t.w += u.w;
         }
-        store_piece<F16, DT>(a, bk, hk, split, r, c, t, mm, ll, piece == 0 && h == 0);
+        store_piece<F16, DT>(a, bk, hk, split, r, c, t, mm, ll, piece == 0 && h == 0, one);
     }
 }
 
@@ -463,7 +463,6 @@ __device__ __forceinline__ uint4 pack8(const f32x16& x, int t) {
 constexpr int DKV_ROWS = 64;                                        // rows per barrier
 template <bool F16, int DT>
 __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnArgs a) {
-    T16<F16>::enter();
     const int item = xcd_item(blockIdx.x, a.n_items);
     if (item >= a.n_items) return;
     const int kt = item % a.tiles, split = item / a.tiles % a.splits, grp = item / a.tiles / a.splits, bk = grp / a.Hk, hk = grp % a.Hk;
@@ -602,8 +601,8 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
         wait_all_and_meet();
     }
     if (key >= a.Lk) return;
-    const float fv = ok ? __builtin_amdgcn_exp2f(-P_UP<F16>) : 0.f;
-    const float fk = ok ? a.scale * fv / (sc == 0.f ? 1.0f : sc) : 0.f;
+    const float fv = saturate_from_here<F16>() * __builtin_amdgcn_exp2f(-P_UP<F16>);
+    const float fk = a.scale * fv / (sc == 0.f ? 1.0f : sc);
     const int64_t at = a.splits > 1 ? (((int64_t)split * a.Bk * a.Hk + grp) * a.Lk + key) * DT : (((int64_t)bk * a.Lk + key) * a.Hk + hk) * a.D;
 #pragma unroll
     for (int d = 0; d < DT / 32; ++d)
@@ -631,7 +630,6 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
 // dQ: as the forward kernel; dS^T has a row per lane, dQ^T += K^T dS^T reads the K tile a second time, transposed
 template <bool F16, int DT>
 __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
-    T16<F16>::enter();
     const int item = xcd_item(blockIdx.x, a.n_items);
     if (item >= a.n_items) return;
     const int rt = item % a.tiles, split = item / a.tiles % a.splits, grp = item / a.tiles / a.splits, bk = grp / a.Hk, hk = grp % a.Hk;
@@ -740,7 +738,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
         bits = next;
     }
     if (r >= a.M) return;
-    const float f = a.scale * __builtin_amdgcn_exp2f(-P_UP<F16>) / (sc == 0.f ? 1.0f : sc);
+    const float f = saturate_from_here<F16>() * a.scale * __builtin_amdgcn_exp2f(-P_UP<F16>) / (sc == 0.f ? 1.0f : sc);
     const int64_t at = a.splits > 1 ? (((int64_t)split * a.Bk * a.Hk + grp) * a.M + r) * DT : off_out(a, w);
 #pragma unroll
     for (int d = 0; d < DT / 32; ++d)

@@ -50,6 +50,11 @@ XATTN = [
     (4, 4, 100, 300, 2, 2, 64, "empty"),        # a sample without states
     (3, 3, 64, 64, 2, 2, 128, "len holes empty"),
     (1, 1, 33, 4100, 1, 1, 64, "holes"),        # few rows, a long axis: splits
+    (2, 1, 50, 140, 6, 2, 64, "len"),           # three heads to a state head
+    (1, 1, 2, 300, 40, 1, 128, "holes"),        # forty heads to a state head: more rows than a token's, two positions
+    (4, 1, 64, 200, 4, 1, 32, ""),              # samples that end with a tile of rows
+    (5, 1, 67, 129, 2, 1, 128, "len"),          # samples that end inside one
+    (40, 2, 3, 1500, 8, 2, 72, "len holes"),    # short samples, many of them on one set of states
 ]
 
 
@@ -148,6 +153,36 @@ def test_xattn_strides(Lq):
     held(o, *ref.xattn(q, odd.contiguous(), odd.contiguous())["out"], "odd rows")
 
 
+@pytest.mark.parametrize("t", HALF)
+@pytest.mark.parametrize("Lq", [2, 70])
+def test_xattn_a_nan_stays_where_it_belongs(Lq, t):
+    """a NaN in a query row makes that row NaN, one in a valid state every row of its sample and state head; nothing else"""
+    q, k, v, dout, _ = xattn_inputs((3, 3, Lq, 90, 4, 2, 64, ""), t)
+    q[0, 1, 3, 7] = math.nan
+    k[1, 44, 1, 5] = math.nan
+    v[2, 80, 0, 9] = math.nan
+    out, lse = blocks().cross_attention(q, k, v)
+    want = torch.zeros(out.shape, dtype=torch.bool, device="cuda")
+    want[0, 1, 3] = True
+    want[1, :, 2:] = True
+    want[2, :, :2, 9] = True
+    assert torch.equal(out.isnan(), want)
+    assert bool(lse[0, 3, 1].isnan()) and bool(lse[1, 2:].isnan().all()) and int(lse.isnan().sum()) == 1 + 2 * Lq
+    dq, dk, dv = blocks().cross_attention_backward(dout, q, k, v, out, lse)
+    assert bool(dq[0, 1, 3].isnan().all()) and not dq[0, :, :2].isnan().any() and not dq[1, :, :2].isnan().any()
+    assert bool(dk[0, :, 1].isnan().all()) and not dk[0, :, 0].isnan().any() and bool(dv[1, :, 1].isnan().all()) and not dv[1, :, 0].isnan().any()
+
+
+def test_xattn_results_past_the_type_s_range():
+    """fp16 results saturate: dv sums 300 rows of 6e4 into one state"""
+    q = torch.zeros(1, 300, 1, 64, dtype=FP16, device="cuda")
+    k, v = torch.zeros(1, 1, 1, 64, dtype=FP16, device="cuda"), torch.ones(1, 1, 1, 64, dtype=FP16, device="cuda")
+    dout = torch.full_like(q, 60000.0)
+    out, lse = blocks().cross_attention(q, k, v)
+    dq, dk, dv = blocks().cross_attention_backward(dout, q, k, v, out, lse)
+    assert bool((out == 1).all()) and bool((dv == 65504).all()) and not dq.any() and not dk.any()
+
+
 def test_xattn_offsets_past_32_bits():
     """k and v of more than 2^31 elements (4.3 GB each): the last states are the ones attended to"""
     Lk, Hk, D = 131200, 128, 128
@@ -218,9 +253,9 @@ def test_ffn_forward_and_gradients(shape, act, bias, t):
     assert torch.equal(y, blocks().gated_ffn(a["x"], *w, *b, activation=act))      # the same bits without saving
 
 
-@pytest.mark.parametrize("shape", [(4000, 1280, 5120), (2100, 2048, 4104)])
+@pytest.mark.parametrize("shape", [(4000, 1280, 5120), (2100, 2048, 4104), (7001, 1280, 2056)])
 def test_ffn_large_tiles(shape):
-    """enough rows and features for the largest tiles, with ragged edges"""
+    """enough rows and features for the largest tiles, with ragged edges; the last: more tiles than places, a tail of them in parts"""
     a, b, dy = ffn_inputs(*shape, BF16, True)
     w = [a["wg"], a["wu"], a["wd"]]
     y, saved = blocks().gated_ffn(a["x"], *w, *b, save=True)
@@ -262,6 +297,21 @@ def test_ffn_gradients_against_differences():
         diff = (loss(hi) - loss(lo)) / 2e-5
         along = float((d[name].double() * e).sum())
         assert abs(along - diff) <= float((want[name][1] * e.abs()).sum()) + 1e-6 * (1 + abs(diff)), (name, along, diff)
+
+
+@pytest.mark.parametrize("M", [1, 3, 40, 300])
+def test_ffn_results_past_the_type_s_range(M):
+    """fp16 results past 65504 are stored as 65504; a NaN stays one, in its row alone"""
+    t = FP16
+    x = torch.full((M, 64), 8.0, dtype=t, device="cuda")
+    w = torch.full((64, 64), 4.0, dtype=t, device="cuda")
+    y = blocks().gated_ffn(x, w, w, w, activation="relu")            # 2048 x 2048 x ...: far past the range
+    assert bool((y == 65504).all())
+    x[M // 2, 5] = math.nan
+    y = blocks().gated_ffn(x, w, w, w, activation="relu")
+    bad = torch.zeros(M, dtype=torch.bool, device="cuda")
+    bad[M // 2] = True
+    assert bool(y[bad].isnan().all()) and not y[~bad].isnan().any()
 
 
 # ------------------------------------------------------------------------------------------------ norms around a block
@@ -502,6 +552,33 @@ def test_calls_on_another_stream_and_the_same_bits_every_time():
     assert torch.equal(o2, out) and torch.equal(l2, lse) and all(torch.equal(a, b) for a, b in zip(d, d2))
 
 
+def test_two_streams_at_once():
+    """every operator on two streams that run side by side, each with its own inputs: the bits of one after the other"""
+    a = [ffn_inputs(300, 256, 1032, BF16, True, seed=s) for s in (1, 2)]
+    c = [xattn_inputs((3, 1, 40, 2500, 4, 2, 64, "holes"), BF16, seed=s) for s in (1, 2)]
+    n = [norm_inputs(4, 50, 640, BF16, ("rms", "layer"), True, seed=s) for s in (1, 2)]
+
+    def work(i):
+        (f, b, dy), (q, k, v, do, m), (x, y, dr, dz, na) = a[i], c[i], n[i]
+        w = [f["wg"], f["wu"], f["wd"]]
+        yy, saved = blocks().gated_ffn(f["x"], *w, *b, save=True)
+        o, lse = blocks().cross_attention(q, k, v, **m)
+        r, z, st = blocks().block_norm(x, y, save=True, **na)
+        return [yy, *blocks().gated_ffn_backward(dy, f["x"], *w, saved, bias=True).values(), o, lse,
+                *blocks().cross_attention_backward(do, q, k, v, o, lse, **m), r, z, *blocks().block_norm_backward(dr, dz, x, y, st, **na).values()]
+    want = [work(0), work(1)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [None, None]
+    for _ in range(3):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i] = work(i)
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert len(g) == len(w) and all(torch.equal(x, y) for x, y in zip(g, w))
+
+
 def test_nothing_is_written_past_the_results():
     """results inside larger buffers through the C ABI: what lies around them stays"""
     import ctypes as C
@@ -522,6 +599,54 @@ def test_nothing_is_written_past_the_results():
         assert bool((buf[:512] == 7).all()) and bool((buf[512 + q.numel():] == 7).all())
         assert bool((lse[:256] == 7).all()) and bool((lse[256 + 2 * Lq:] == 7).all())
         held(buf[512:512 + q.numel()].view(q.shape), *ref.xattn(q, k, v, scale=0.1)["out"], "out")
+
+
+@pytest.mark.parametrize("M,D,F", [(1, 72, 136), (3, 72, 136), (70, 72, 136), (300, 136, 264)])
+def test_ffn_and_norm_write_nothing_past_their_results(M, D, F):
+    import ctypes as C
+
+    from isbfsar_amd import _lib
+    lib = _lib.lib()
+    st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+    def around(n, t=BF16):
+        b = torch.full((n + 1024,), 7.0, dtype=t, device="cuda")
+        return b, b.data_ptr() + 512 * b.element_size(), n
+
+    def kept(b, _, n):
+        return bool((b[:512] == 7).all()) and bool((b[512 + n:] == 7).all())
+    a, b, dy = ffn_inputs(M, D, F, BF16, True)
+    o = {"y": around(M * D), "pre_gate": around(M * F, F32), "pre_up": around(M * F, F32), "hidden": around(M * F), "dx": around(M * D),
+         "dw_gate_up": around(2 * F * D), "dw_down": around(D * F), "db_gate": around(F), "db_up": around(F), "db_down": around(D)}
+    args = _lib.isb_ffn_args(0, 2, M, D, F, 0, D, D, a["x"].data_ptr(), a["wg"].data_ptr(), a["wu"].data_ptr(), a["wd"].data_ptr(),
+                             b[0].data_ptr(), b[1].data_ptr(), b[2].data_ptr())
+    args.dy = dy.data_ptr()
+    for name, v in o.items():
+        setattr(args, name, v[1])
+    for back, call in ((0, lib.isb_ffn_forward), (1, lib.isb_ffn_backward)):
+        n = C.c_size_t()
+        _lib.check(lib.isb_ffn_workspace(C.byref(args), back, C.byref(n)), "workspace")
+        ws = torch.full((n.value + 4096,), 9, dtype=torch.uint8, device="cuda")
+        _lib.check(call(C.byref(args), ws.data_ptr(), n.value, st), "call")
+        assert bool((ws[n.value:] == 9).all())
+    for name, v in o.items():
+        assert kept(*v), name
+    x, y, dr, dz, na = norm_inputs(2, M, D, BF16, ("layer", "layer"), True)
+    rows = 2 * M * D
+    o = {"r": around(rows), "z": around(rows), "stats": around(8 * M, F32), "dx": around(rows), "dy": around(rows), "dgate": around(2 * D),
+         "dscale": around(D, F32), "dpre_bias": around(D, F32)}
+    args = _lib.isb_norm_args(0, 2, 2, M, D, 1, 1, 1e-5, x.data_ptr(), y.data_ptr(), na["gate"].data_ptr(), na["scale"].data_ptr())
+    args.dr, args.dz = dr.data_ptr(), dz.data_ptr()
+    for name, v in o.items():
+        setattr(args, name, v[1])
+    n = C.c_size_t()
+    _lib.check(lib.isb_norm_workspace(C.byref(args), C.byref(n)), "workspace")
+    ws = torch.full((n.value + 4096,), 9, dtype=torch.uint8, device="cuda")
+    _lib.check(lib.isb_norm_forward(C.byref(args), st), "forward")
+    _lib.check(lib.isb_norm_backward(C.byref(args), ws.data_ptr(), n.value, st), "backward")
+    assert bool((ws[n.value:] == 9).all())
+    for name, v in o.items():
+        assert kept(*v), name
 
 
 def test_the_engine_s_embeddings_go_in():
