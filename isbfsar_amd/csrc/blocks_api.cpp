@@ -13,7 +13,9 @@ class OnDevice {
     int enter(int device) {
         ISB_HIP(hipGetDevice(&prev_));
         if (prev_ != device) {
-            ISB_HIP(hipSetDevice(device));
+            const hipError_t e = hipSetDevice(device);
+            if (e != hipSuccess) (void)hipGetLastError();          // (not left for the next launch to find)
+            ISB_REQUIRE(e == hipSuccess, ISB_ERR_HIP, "device %d: %s", device, hipGetErrorString(e));
             changed_ = true;
         }
         return ISB_OK;

@@ -599,7 +599,7 @@ int tile_of(int la, int M, int N) {
 }
 // How an OUT product shares out k. Tiles that do not fill the chip once: every tile in `splits` parts. Tiles that leave a part round behind
 // whole ones: the tail's tiles in as many parts as fill it, if that is at most 5 / 8 full (7680 x 1280 from 5120: 600 tiles on 512 places,
-// 148 -> %s us).
+// 148 -> 125 us).
 struct OutPlan { int splits = 1, full = 0, tail = 0, tail_splits = 0; size_t bytes = 0; };
 OutPlan plan_out(int la, int M, int N, int kts) {
     const int t = tile_of(la, M, N), bm = t == TILE_THIN ? 32 : t == TILE_MID ? 128 : 256, bn = t == TILE_BIG ? 256 : t == TILE_THIN ? 64 : 128;

@@ -649,6 +649,20 @@ def test_ffn_and_norm_write_nothing_past_their_results(M, D, F):
         assert kept(*v), name
 
 
+def test_a_device_that_is_not_there():
+    """the call fails with the library's error, and neither the thread's device nor the next launch notices"""
+    import ctypes as C
+
+    from isbfsar_amd import _lib
+    x, _, _, _, a = norm_inputs(1, 3, 64, F32, (None, "layer"), False)
+    z = blocks().block_norm(x, pre="layer")[1]
+    got = torch.zeros_like(x)
+    args = _lib.isb_norm_args(63, 0, 1, 3, 64, 0, 1, 1e-5, x.data_ptr())
+    args.z = got.data_ptr()
+    assert _lib.lib().isb_norm_forward(C.byref(args), None) == -3 and b"device 63" in _lib.lib().isb_last_error()
+    assert torch.cuda.current_device() == 0 and torch.equal(blocks().block_norm(x, pre="layer")[1], z) and not got.any()
+
+
 def test_the_engine_s_embeddings_go_in():
     """embeddings of query windows against the frames of the installed support set (ArEngine), shared by all windows"""
     from isbfsar_amd import synth, weights
