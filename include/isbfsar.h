@@ -464,6 +464,8 @@ int isb_dist_all_gather(isb_dist* d, const void* d_send, void* d_recv, size_t by
  *   (NULL: all). What masked states hold is never used (NaN and infinities included).
  *   out [B,Lq,Hq,D] = softmax(scale q k^T) v, lse [B,Hq,Lq] f32 = log sum exp(scale q k^T) (natural logarithm). A row with no
  *   state gets out = 0, lse = -inf and passes no gradient. scale > 0.
+ *   At most 2^23 tiles of 128 rows (B / Bk * Lq * Hq / Hk rows read the states of one Bk and Hk) or 128 states; k and v: at most
+ *   2^22 elements from one state to the next.
  * Backward: dout [B,Lq,Hq,D], out and lse of the forward call -> dq, dk, dv (contiguous, shapes of q, k, v; gradients of
  * shared heads and shared states are summed in 32 bits; masked states get zeros). */
 typedef struct isb_xattn_args {
@@ -487,7 +489,7 @@ int isb_xattn_backward(const isb_xattn_args* a, void* d_workspace, size_t bytes,
 
 /* Gated feed-forward block: y = (act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd, 16-bit, torch Linear weights.
  *   x [M,D] (row stride x_stride), w_gate, w_up [F,D], w_down [D,F], b_gate, b_up [F], b_down [D] or NULL, y [M,D].
- *   D, F multiples of 8; M >= 1.
+ *   D, F multiples of 8, at most 2^20; M 1 .. 2^22; row strides D .. 2^22 elements.
  *   For the backward pass forward also fills pre_gate, pre_up [M,F] f32 (both or neither) and hidden [M,F] (needed with them,
  *   else NULL: it lives in the workspace).
  * Backward: dy [M,D] (row stride dy_stride) and those three -> dx [M,D], dw_gate_up [2F,D] (the gate's rows first), dw_down [D,F],

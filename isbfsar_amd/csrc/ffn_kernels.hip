@@ -185,7 +185,8 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
     // Fragments run one k-step ahead of the products, also over the edge of a tile: the workgroup meets BEFORE the last k-step's products, when
     // every wave holds its fragments of the old tile; the buffer is then free for the tile NBUF ahead, whose requests have NBUF - 1 tiles'
-    // products to land (the wait counts the requests of the tiles that may still be on their way: the loop has no other memory access). Fragment reads and requests are issued one by one BETWEEN the products (the matrix pipe takes 32 cycles each).
+    // products to land (the wait counts the requests of the tiles that may still be on their way: the loop has no other memory access).
+    // Fragment reads and requests are issued one by one BETWEEN the products (the matrix pipe takes 32 cycles each).
     uint4 fa[2][IM], fb[2][IN];
     auto fetch = [&](int buf, int ks, int i) {
         const unsigned char* at = conv_lds_dyn + buf * STAGE;
@@ -630,7 +631,7 @@ int mm_run(MmArgs p, const char* name, hipStream_t st) {
     p.tiles_m = cdiv(p.M, BM);
     p.tiles_n = cdiv(p.N, BN);
     const int64_t n = p.tail > 0 ? p.full + 8 * cdiv(p.tail * p.tail_splits, 8) : (int64_t)p.tiles_m * p.tiles_n * p.splits;
-    ISB_REQUIRE(n < (1ll << 30), ISB_ERR_INVALID, "gated feed-forward: %lld workgroups are more than one launch holds", (long long)n);
+    ISB_REQUIRE((n + 7) * (NWM * NWN * NWK * 64) < (1ll << 32), ISB_ERR_INVALID, "gated feed-forward: %lld workgroups are more than one launch holds", (long long)n);
     p.n_items = (int)n;
     const int kts = cdiv(p.K, BK) * p.nseg;
     p.kt_per_split = cdiv(kts, p.splits);

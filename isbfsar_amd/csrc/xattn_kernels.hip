@@ -830,15 +830,12 @@ Plan plan_dq(const XattnArgs& a) {
     choose_splits((int64_t)a.Bk * a.Hk * p.tiles, CUS, a.Lk, KT, 2, p.splits, p.chunk);
     return p;
 }
-int items(XattnArgs& a, const Plan& p, unsigned& grid) {
-    const int64_t n = (int64_t)a.Bk * a.Hk * p.tiles * p.splits;
-    ISB_REQUIRE(n < (1ll << 30), ISB_ERR_INVALID, "cross attention: %lld workgroups are more than one launch holds", (long long)n);
+unsigned items(XattnArgs& a, const Plan& p) {
     a.tiles = p.tiles;
     a.splits = p.splits;
     a.chunk = p.chunk;
-    a.n_items = (int)n;
-    grid = (unsigned)(8 * ((n + 7) / 8));
-    return ISB_OK;
+    a.n_items = a.Bk * a.Hk * p.tiles * p.splits;                // (below 2^23: blocks_api.cpp)
+    return 8u * ((a.n_items + 7) / 8);
 }
 template <auto Kernel>
 int launch(const char* name, unsigned grid, unsigned threads, size_t lds, const XattnArgs& a, hipStream_t st) {
@@ -855,8 +852,7 @@ int launch(const char* name, unsigned grid, unsigned threads, size_t lds, const 
 template <bool F16, int DT>
 int fwd(XattnArgs a, float* ws, hipStream_t st) {
     const Plan p = plan_fwd(a);
-    unsigned grid = 0;
-    ISB_TRY(items(a, p, grid));
+    const unsigned grid = items(a, p);
     const int64_t rows = (int64_t)a.Bk * a.Hk * a.M;
     a.part = ws;
     a.part2 = ws + (int64_t)p.splits * rows * DT;
@@ -881,11 +877,10 @@ int bwd(XattnArgs a, float* ws, hipStream_t st) {
     float* pq = ws + 64 + (rows + 63) / 64 * 64;
     float* pk = pq + (q.splits > 1 ? q.splits * rows * DT : 0);
     float* pv = pk + (int64_t)k.splits * states * DT;
-    unsigned grid = 0;
-    ISB_TRY(items(a, q, grid));
+    unsigned grid = items(a, q);
     a.part = pq;
     ISB_TRY((launch<xattn_dq_kernel<F16, DT>>("xattn_dq", grid, 256, 2 * (2 * KT * DT * 2 + KT * 4), a, st)));
-    ISB_TRY(items(a, k, grid));
+    grid = items(a, k);
     a.part = pk;
     a.part2 = pv;
     ISB_TRY((launch<xattn_dkv_kernel<F16, DT>>("xattn_dkv", grid, 256, 2 * DKV_ROWS * (2 * DT * 2 + 8), a, st)));

@@ -58,6 +58,17 @@ def test_xattn_backward_arguments(lib, bad):
     assert lib.isb_xattn_backward(C.byref(xattn(**bad)), OK16, 1 << 40, None) == -1
 
 
+def test_xattn_more_workgroups_than_a_launch_holds(lib):
+    n = C.c_size_t()
+    for big in (dict(B=1 << 21, Bk=1 << 21, Lq=1, Hq=4, Hk=4), dict(B=1, Bk=1, Lq=1 << 27, Hq=8, Hk=8), dict(B=1, Bk=1, Hq=8, Hk=8, Lk=1 << 27)):
+        assert lib.isb_xattn_workspace(C.byref(xattn(**big)), 0, C.byref(n)) == -1, big
+        assert lib.isb_xattn_backward(C.byref(xattn(**big)), OK16, 1 << 50, None) == -1
+        for f in ("Bk", "Lq", "Lk"):
+            if big.get(f, 0) >= 1 << 21:
+                less = {**big, f: big[f] // 2, **({"B": big["B"] // 2} if f == "Bk" else {})}
+                assert lib.isb_xattn_workspace(C.byref(xattn(**less)), 1, C.byref(n)) == 0, less
+
+
 def test_null_and_workspace(lib):
     n = C.c_size_t()
     assert lib.isb_xattn_forward(None, None, 0, None) == -1 and lib.isb_ffn_forward(None, None, 0, None) == -1
