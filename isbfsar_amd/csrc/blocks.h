@@ -1,8 +1,24 @@
 // Argument blocks + host launchers of the stand-alone layer operators, shared by their translation units and blocks_api.cpp.
 #pragma once
+#include <atomic>
+
 #include "blk_common.h"
 
 namespace isb {
+
+// Kernel may use `bytes` (always the same) of dynamic LDS on the current device: asked of the runtime once per device. The operators have no
+// handle, so threads that drive different devices meet here.
+template <auto Kernel>
+int allow_lds(size_t bytes) {
+    static std::atomic<uint64_t> done{0};                // a bit per device
+    int dev = 0;
+    ISB_HIP(hipGetDevice(&dev));
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_acquire) & bit) return ISB_OK;
+    ISB_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    done.fetch_or(bit, std::memory_order_release);
+    return ISB_OK;
+}
 
 // ---------------------------------------------------------------- xattn_kernels.hip
 // Rows: every query row that reads the same states (bk, hk) -- the nb = B / Bk samples that share them, Lq positions, G = Hq / Hk heads --

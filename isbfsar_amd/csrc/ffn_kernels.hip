@@ -639,12 +639,7 @@ int mm_run(MmArgs p, const char* name, hipStream_t st) {
         p.tail_per = cdiv(p.tail * p.tail_splits, 8);
         p.kt_per_tail = cdiv(kts, p.tail_splits);
     }
-    static DevMax attr;
-    if (attr.below((int)lds)) {
-        ISB_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(ffn_mm_kernel<F16, BM, BN, NWM, NWN, NWK, NBUF, LA, LB, EPI>),
-                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        attr.set((int)lds);
-    }
+    ISB_TRY((allow_lds<ffn_mm_kernel<F16, BM, BN, NWM, NWN, NWK, NBUF, LA, LB, EPI>>(lds)));
     ffn_mm_kernel<F16, BM, BN, NWM, NWN, NWK, NBUF, LA, LB, EPI><<<(unsigned)(8 * ((n + 7) / 8)), NWM * NWN * NWK * 64, lds, st>>>(p);
     ISB_LAUNCHED(name, st);
     if constexpr (EPI == EPI_OUT && BM >= 128) {

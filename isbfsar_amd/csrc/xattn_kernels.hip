@@ -839,11 +839,7 @@ unsigned items(XattnArgs& a, const Plan& p) {
 }
 template <auto Kernel>
 int launch(const char* name, unsigned grid, unsigned threads, size_t lds, const XattnArgs& a, hipStream_t st) {
-    static DevMax attr;
-    if (attr.below((int)lds)) {
-        ISB_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        attr.set((int)lds);
-    }
+    ISB_TRY(allow_lds<Kernel>(lds));
     Kernel<<<grid, threads, lds, st>>>(a);
     ISB_LAUNCHED(name, st);
     return ISB_OK;

@@ -579,6 +579,38 @@ def test_two_streams_at_once():
         assert len(g) == len(w) and all(torch.equal(x, y) for x, y in zip(g, w))
 
 
+def test_threads_that_call_at_once():
+    """four host threads, a stream each, the same calls: the bits of a call alone"""
+    import threading
+
+    q, k, v, dout, m = xattn_inputs((2, 1, 40, 300, 4, 2, 72, "holes"), FP16)
+    a, b, dy = ffn_inputs(70, 136, 264, FP16, True)
+    w = [a["wg"], a["wu"], a["wd"]]
+
+    def work():
+        o, lse = blocks().cross_attention(q, k, v, **m)
+        y, saved = blocks().gated_ffn(a["x"], *w, *b, save=True)
+        return [o, lse, *blocks().cross_attention_backward(dout, q, k, v, o, lse, **m), y,
+                *blocks().gated_ffn_backward(dy, a["x"], *w, saved, bias=True).values()]
+    want = work()
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def run(i):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            for _ in range(5):
+                got[i] = work()
+        st.synchronize()
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for g in got:
+        assert g is not None and all(torch.equal(x, y) for x, y in zip(g, want))
+
+
 def test_nothing_is_written_past_the_results():
     """results inside larger buffers through the C ABI: what lies around them stays"""
     import ctypes as C
