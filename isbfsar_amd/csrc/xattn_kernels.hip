@@ -388,9 +388,9 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XattnArgs a) {
 // Backward. dQ first (a workgroup keeps 128 rows, forms their delta = rowsum(dout o out) and walks the states), then dK, dV (a workgroup keeps
 // 128 states, 32 per wave, and walks the rows); one launch adds up the splits of all three. Every sum has a fixed order: no atomics.
 //
-// fp16: P is formed as 2^12 P (<= 4096), so that weights of 1 / 16384 stay normal numbers, and dS carries a power of two chosen from what
-// the wave meets: it starts so that the first tile's largest |dS| lies in [2^10, 2^11) and is lowered, with the sums so far, when a tile
-// passes 2^14. bf16 has f32's range and needs neither.
+// fp16: P is formed as 2^12 P (<= 4096), so that weights of 1 / 16384 stay normal numbers, and each column of dS carries a power of two chosen
+// from what it meets: it starts so that the first block's largest |dS| lies in [2^10, 2^11) and is lowered, with the sums so far, when a block
+// passes 2^15. bf16 has f32's range and needs neither.
 // ------------------------------------------------------------------------------------------------------------------------------------
 template <bool F16> constexpr float P_UP = F16 ? 12.0f : 0.0f;              // log2 of the factor on P
 
@@ -425,32 +425,30 @@ struct RowWalk {
     }
 };
 
-// the power of two on dS (see above); NB blocks of scores. Returns with ds scaled.
-template <bool F16, int NB, int NA>
-__device__ __forceinline__ void scale_ds(f32x16 (&ds)[NB], f32x16 (&acc)[NA], float& sc) {
+// The power of two on dS (see above). A lane and its other half hold one column of dS -- a row of dQ, a state of dK -- and of what it is added
+// to, so each column has a factor of its own: an infinity or a large row leaves its neighbours alone. Returns with ds scaled.
+template <bool F16, int NA>
+__device__ __forceinline__ void scale_ds(f32x16& ds, f32x16 (&acc)[NA], float& sc) {
     if constexpr (F16) {
         float mx = 0.f;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fabsf(ds[i]));
+        if (__any(mx * sc > 32768.0f || (sc == 0.f && mx > 0.f))) {
+            mx = max_halves(mx);
+            if (mx * sc > 32768.0f || (sc == 0.f && mx > 0.f)) {
+                const int e = min(max(11 - (int)__builtin_amdgcn_frexp_expf(mx), -100), 100);      // mx = f 2^x, f in [1/2, 1): mx 2^e in [2^10, 2^11)
+                const float ns = __builtin_ldexpf(1.0f, e);
+                const float f = sc == 0.f ? 1.0f : ns / sc;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, fabsf(ds[b][i]));
-        if (__any(mx * sc > 16384.0f || (sc == 0.f && mx > 0.f))) {
+                for (int d = 0; d < NA; ++d)
 #pragma unroll
-            for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-            const int e = min(max(10 - (int)__builtin_amdgcn_frexp_expf(mx) + 1, -100), 100);      // mx = f 2^x, f in [1/2, 1): mx 2^e in [2^10, 2^11)
-            const float ns = __builtin_ldexpf(1.0f, e);
-            const float f = sc == 0.f ? 1.0f : ns / sc;
-#pragma unroll
-            for (int d = 0; d < NA; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[d][i] *= f;
-            sc = ns;
+                    for (int i = 0; i < 16; ++i) acc[d][i] *= f;
+                sc = ns;
+            }
         }
         const float by = sc == 0.f ? 1.0f : sc;
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) ds[b][i] *= by;
+        for (int i = 0; i < 16; ++i) ds[i] *= by;
     }
 }
 template <bool F16>
@@ -527,12 +525,12 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
         const unsigned char* dt = qt + TB;
         const float* st = reinterpret_cast<const float*>(qt + 2 * TB);
         constexpr int N = DT / 8, AHEAD = 4, PER = 16 / N;                     // products of a block's S and dP (and of its share of dV and dK)
-        f32x16 s[2], dp[2][1];
+        f32x16 s[2], dp[2];
         uint4 f[AHEAD], w[2][2], ds[2][2];
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) { s[rb][i] = 0.f; dp[rb][0][i] = 0.f; }
+            for (int i = 0; i < 16; ++i) { s[rb][i] = 0.f; dp[rb][i] = 0.f; }
         auto rows = [&](int n) {                                               // fragment n of the 2 N of S and dP: Q's rows, dout's rows
             const int rb = n / N, i = n % N;
             return frag_rows<DT>(i < N / 2 ? qt : dt, 32 * rb, i % (N / 2), lane);
@@ -544,7 +542,7 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
         auto score = [&](int n) {
             const int rb = n / N, i = n % N;
             if (i < N / 2) s[rb] = T16<F16>::mfma32(f[n % AHEAD], kf[i], s[rb]);
-            else dp[rb][0] = T16<F16>::mfma32(f[n % AHEAD], vf[i - N / 2], dp[rb][0]);
+            else dp[rb] = T16<F16>::mfma32(f[n % AHEAD], vf[i - N / 2], dp[rb]);
             f[n % AHEAD] = n + AHEAD < 2 * N ? rows(n + AHEAD) : cols(n + AHEAD - 2 * N);
         };
         auto add = [&](int n) {
@@ -561,18 +559,12 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
             }
             const float n1 = i % 4 == 0 ? nl.x : i % 4 == 1 ? nl.y : i % 4 == 2 ? nl.z : nl.w, d1 = i % 4 == 0 ? de.x : i % 4 == 1 ? de.y : i % 4 == 2 ? de.z : de.w;
             s[rb][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rb][i], a.c, n1));
-            dp[rb][0][i] = s[rb][i] * (dp[rb][0][i] - d1);
+            dp[rb][i] = s[rb][i] * (dp[rb][i] - d1);
         };
         auto round = [&](int rb) {
-            if constexpr (F16) {        // a masked state's column is not stored, but must not set the power of two either
-                if (!ok) {
+            scale_ds<F16, DT / 32>(dp[rb], dk, sc);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) dp[rb][0][i] = 0.f;
-                }
-            }
-            scale_ds<F16, 1, DT / 32>(dp[rb], dk, sc);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) { w[rb][u] = pack8<F16>(s[rb], u); ds[rb][u] = pack8<F16>(dp[rb][0], u); }
+            for (int u = 0; u < 2; ++u) { w[rb][u] = pack8<F16>(s[rb], u); ds[rb][u] = pack8<F16>(dp[rb], u); }
         };
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) f[i] = rows(i);
@@ -700,10 +692,10 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
         if (bits != 0) {
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-                f32x16 s, ds[1];
+                f32x16 s, ds;
                 start_scores(s, bias + 32 * b, bits == ~0ull, h);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) ds[0][i] = 0.f;
+                for (int i = 0; i < 16; ++i) ds[i] = 0.f;
                 constexpr int N = DT / 8, AHEAD = 4;                           // K's and V's fragments in turn
                 auto row = [&](int i) { return frag_rows<DT>(i % 2 == 0 ? ktile : vtile, 32 * b, i / 2, lane); };
                 uint4 f[AHEAD];
@@ -712,7 +704,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     if (i % 2 == 0) s = T16<F16>::mfma32(f[i % AHEAD], qf[i / 2], s);
-                    else ds[0] = T16<F16>::mfma32(f[i % AHEAD], df[i / 2], ds[0]);
+                    else ds = T16<F16>::mfma32(f[i % AHEAD], df[i / 2], ds);
                     if (i + AHEAD < N) f[i % AHEAD] = row(i + AHEAD);
                     reads_stay();
                 }
@@ -722,11 +714,11 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
                 for (int i = 0; i < AHEAD; ++i) f[i] = column(i);
                 reads_stay();
 #pragma unroll
-                for (int i = 0; i < 16; ++i) ds[0][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, nl)) * (ds[0][i] - de);
-                scale_ds<F16, 1, DT / 32>(ds, acc, sc);
+                for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, nl)) * (ds[i] - de);
+                scale_ds<F16, DT / 32>(ds, acc, sc);
                 uint4 g[2];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) g[u] = pack8<F16>(ds[0], u);
+                for (int u = 0; u < 2; ++u) g[u] = pack8<F16>(ds, u);
 #pragma unroll
                 for (int i = 0; i < NC; ++i) {
                     acc[i / 2] = T16<F16>::mfma32(f[i % AHEAD], g[i % 2], acc[i / 2]);

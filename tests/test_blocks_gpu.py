@@ -173,6 +173,22 @@ def test_xattn_a_nan_stays_where_it_belongs(Lq, t):
     assert bool(dk[0, :, 1].isnan().all()) and not dk[0, :, 0].isnan().any() and bool(dv[1, :, 1].isnan().all()) and not dv[1, :, 0].isnan().any()
 
 
+@pytest.mark.parametrize("t", HALF)
+def test_xattn_an_infinite_gradient_stays_in_its_row(t):
+    """dout holds an infinity (a loss scaled too far): dq of the other rows, dk and dv of the other head are what they are without it"""
+    q, k, v, dout, _ = xattn_inputs((1, 1, 64, 300, 2, 2, 64, ""), t, std=8.0)
+    out, lse = blocks().cross_attention(q, k, v)
+    without, bad = dout.clone(), dout.clone()
+    without[0, 3, 0], bad[0, 3, 0, 7] = 0, math.inf
+    want = ref.xattn(q, k, v, dout=without)
+    dq, dk, dv = blocks().cross_attention_backward(bad, q, k, v, out, lse)
+    assert not dq[0, 3, 0].isfinite().any()
+    dq[0, 3, 0] = 0
+    held(dq, *want["dq"], "dq")
+    for name, got in (("dk", dk), ("dv", dv)):
+        held(got[:, :, 1], want[name][0][:, :, 1], want[name][1][:, :, 1], name)
+
+
 def test_xattn_results_past_the_type_s_range():
     """fp16 results saturate: dv sums 300 rows of 6e4 into one state"""
     q = torch.zeros(1, 300, 1, 64, dtype=FP16, device="cuda")
@@ -282,6 +298,23 @@ def test_ffn_strides_and_leading_dimensions():
     assert torch.equal(blocks().gated_ffn(odd[:, 1:], *w, *b), y)
 
 
+def test_ffn_offsets_past_32_bits():
+    """pre-activations of more than 2^31 elements: rows of zeros (which leave no trace in any gradient), the last ones filled"""
+    M, D, F, n = (1 << 20) + 37, 64, 2056, 77
+    a, _, dy = ffn_inputs(n, D, F, BF16, False)
+    w = [a["wg"], a["wu"], a["wd"]]
+    x, d = torch.zeros(M, D, dtype=BF16, device="cuda"), torch.zeros(M, D, dtype=BF16, device="cuda")
+    x[-n:], d[-n:] = a["x"], dy
+    y, saved = blocks().gated_ffn(x, *w, save=True)
+    g = blocks().gated_ffn_backward(d, x, *w, saved)
+    want = ref.ffn(a["x"], *w, dy=dy)
+    for name, got in (("y", y), ("dx", g["dx"])):
+        held(got[-n:], *want[name], name)
+        assert not got[:-n].any(), name
+    for name in ("dw_gate", "dw_up", "dw_down"):
+        held(g[name], *want[name], name)
+
+
 def test_ffn_gradients_against_differences():
     a, b, dy = ffn_inputs(7, 24, 40, FP16, True)
     x = [a["x"], a["wg"], a["wu"], a["wd"], *b]
@@ -381,6 +414,24 @@ def test_norm_unaligned_tensors():
     r, z = blocks().block_norm(odd, y, **a)
     r0, z0 = blocks().block_norm(x, y, **a)
     assert torch.equal(r, r0) and torch.equal(z, z0)
+
+
+def test_norm_offsets_past_32_bits():
+    """more than 2^31 elements: rows of zeros, the last ones filled"""
+    L, D, n = (1 << 20) + 11, 2056, 60
+    x, y, dr, dz, a = norm_inputs(1, n, D, BF16, ("rms", "rms"), False)
+    big = []
+    for v in (x, y, dr, dz):
+        big.append(torch.zeros(1, L, D, dtype=BF16, device="cuda"))
+        big[-1][:, -n:] = v
+    r, z, stats = blocks().block_norm(big[0], big[1], save=True, **a)
+    d = blocks().block_norm_backward(big[2], big[3], big[0], big[1], stats, **a)
+    want = ref.norm(x, y, dr=dr, dz=dz, **a)
+    for name, got in (("r", r), ("z", z), ("dx", d["dx"]), ("dy", d["dy"])):
+        held(got[:, -n:], *want[name], name)
+        assert not got[:, :-n].any(), name
+    for name in ("dscale", "dpost_weight", "dpre_weight"):
+        held(d[name], *want[name], name)
 
 
 def test_norm_gradients_against_differences():
