@@ -368,12 +368,20 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XattnArgs a) {
             wl = w * ml.y;
         }
         const int n = min(L, a.splits - s0);
-#pragma unroll 4
-        for (int s = 0; s < n; ++s) {
-            const float4 p = *reinterpret_cast<const float4*>(a.part + ((s0 + s) * rows + row) * DT + 4 * lane);
-            const float ws = __shfl(w, s, L);
-            l += __shfl(wl, s, L);
-            o.x = __builtin_fmaf(ws, p.x, o.x); o.y = __builtin_fmaf(ws, p.y, o.y); o.z = __builtin_fmaf(ws, p.z, o.z); o.w = __builtin_fmaf(ws, p.w, o.w);
+        const float* from = a.part + (s0 * rows + row) * DT + 4 * lane;
+        for (int s = 0; s < n; s += 4) {                     // four partial sums on their way at once (past the last: the last again, not added)
+            float4 p[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[i] = *reinterpret_cast<const float4*>(from + min(s + i, n - 1) * rows * DT);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float ws = __shfl(w, s + i, L);
+                if (s + i < n) {
+                    l += __shfl(wl, s + i, L);
+                    o.x = __builtin_fmaf(ws, p[i].x, o.x); o.y = __builtin_fmaf(ws, p[i].y, o.y);
+                    o.z = __builtin_fmaf(ws, p[i].z, o.z); o.w = __builtin_fmaf(ws, p[i].w, o.w);
+                }
+            }
         }
     }
     const int grp = (int)(row / a.M);
