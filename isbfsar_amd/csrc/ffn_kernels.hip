@@ -592,11 +592,21 @@ __global__ __launch_bounds__(256) void ffn_bias_kernel(const float* cs, const fl
 // tile shapes: thin (32 x 64, four waves on the k-steps of a tile, four tiles in flight: the weights are the work, and many small workgroups
 // read them; us forward, D = 1280, F = 5120: 32 rows 18 for mid's 30, 256 rows 36 for 41, at 600 rows it loses, 63 for 50), mid (128 x 128,
 // two workgroups per CU), big (256 x 256, one workgroup of eight waves; half the LDS and L2 bytes per product, but only where its tiles
-// fill the 256 CUs)
-enum { TILE_THIN, TILE_MID, TILE_BIG };
+// fill the 256 CUs), tall (fused_tile)
+enum { TILE_THIN, TILE_MID, TILE_BIG, TILE_TALL };
 int tile_of(int la, int M, int N) {
     if (M <= 256 && la == 0) return TILE_THIN;         // (layout 1 keeps whole 128-byte rows of m in LDS: no thin form)
     return (int64_t)cdiv(M, 256) * cdiv(N, 256) >= 200 ? TILE_BIG : TILE_MID;
+}
+// GATE and DH finish a tile in their epilogue: k cannot be split, and a last round of the chip that is part full costs a whole one. They take
+// the tile whose rounds together are shortest -- rounds x a CU's work per round, with mid's products a quarter dearer than big's; tall (192 x
+// 256) is there for what leaves big a nearly empty round (us, forward with saving + backward, before and with this rule: 4111 rows, 640 x 2560:
+// 254 and 241; 2000, 1280 x 5120: 366 and 335; 12000, 256 x 1024: 182 and 175; 8192, 512 x 2048, where big fits: 300 and 295).
+int fused_tile(int M, int N) {
+    if (M <= 256) return TILE_THIN;
+    const auto rounds = [&](int bm, int bn, int places) { return ((int64_t)cdiv(M, bm) * cdiv(N, bn) + places - 1) / places; };
+    const int64_t mid = rounds(128, 128, 512) * 10, big = rounds(256, 256, 256) * 16, tall = rounds(192, 256, 256) * 12;
+    return mid < big && mid < tall ? TILE_MID : tall < big ? TILE_TALL : TILE_BIG;
 }
 // How an OUT product shares out k. Tiles that do not fill the chip once: every tile in `splits` parts. Tiles that leave a part round behind
 // whole ones: the tail's tiles in as many parts as fill it, if that is at most 5 / 8 full (7680 x 1280 from 5120: 600 tiles on 512 places,
@@ -652,7 +662,9 @@ int mm_run(MmArgs p, const char* name, hipStream_t st) {
 }
 template <bool F16, int LA, int LB, int EPI>
 int mm(const MmArgs& p, const char* name, hipStream_t st) {
-    const int t = tile_of(LA, p.M, p.N);
+    const int t = EPI == EPI_OUT ? tile_of(LA, p.M, p.N) : fused_tile(p.M, p.N);
+    if constexpr (EPI != EPI_OUT)
+        if (t == TILE_TALL) return mm_run<F16, 192, 256, 2, 4, 1, 2, LA, LB, EPI>(p, name, st);
     if constexpr (LA == 0)
         if (t == TILE_THIN) return mm_run<F16, 32, 64, 1, 1, 4, 4, LA, LB, EPI>(p, name, st);
     if (t == TILE_MID) return mm_run<F16, 128, 128, 2, 2, 1, 2, LA, LB, EPI>(p, name, st);

@@ -282,6 +282,19 @@ def test_ffn_large_tiles(shape):
         held(got, *want[n], n)
 
 
+@pytest.mark.parametrize("act", ["gelu", "relu"])
+def test_ffn_tall_tiles(act):
+    """rows and features that leave the largest tiles a nearly empty round, both with ragged edges"""
+    a, b, dy = ffn_inputs(2101, 264, 4104, FP16, True)
+    w = [a["wg"], a["wu"], a["wd"]]
+    y, saved = blocks().gated_ffn(a["x"], *w, *b, activation=act, save=True)
+    d = blocks().gated_ffn_backward(dy, a["x"], *w, saved, bias=True, activation=act)
+    want = ref.ffn(a["x"], *w, *b, activation=act, dy=dy)
+    held(y, *want["y"], "y")
+    for n, got in d.items():
+        held(got, *want[n], n)
+
+
 def test_ffn_strides_and_leading_dimensions():
     a, b, dy = ffn_inputs(60, 128, 264, BF16, True)
     w = [a["wg"], a["wu"], a["wd"]]
