@@ -467,7 +467,7 @@ __global__ __launch_bounds__(256) void ffn_tail_kernel(MmArgs p) {
 // ------------------------------------------------------------------------------------------------------------------------------------
 // At most TOKENS rows: the weights are the work, each read once in whole 1-KiB rows of a wave; dot products on the vector ALU.
 // PER waves share a weight row (pair of rows); their sums are added in wave order. Between the two launches h stays in f32 (a few KB), so
-// that y is rounded once.
+// that y is rounded once. One row, 1280 x 5120: 6.1 us for 26 MB, 4.5 us for 13 MB (the weights partly in the last-level cache), two launches.
 // ------------------------------------------------------------------------------------------------------------------------------------
 constexpr int TOKENS = 4;
 template <bool F16, int MT, int PER, bool GATE>
