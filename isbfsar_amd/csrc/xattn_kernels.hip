@@ -250,9 +250,9 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XattnArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------------------------
-// Forward, at most 32 rows in a group (single tokens, grouped heads): the states are the work. Eight waves walk their own blocks of 32 states,
-// each through its own LDS and without a barrier in the loop -- a wave waits for its block while the others use theirs --, and their sums
-// meet at the end. Up to 2048 states one workgroup does all of a group in one launch (4 heads x 1800 states x 64: 10.0 us, as long as five
+// Forward, tiles of 32 rows (single tokens, grouped heads; a few windows): the states are the work. Eight waves walk their own blocks of 32
+// states, each through its own LDS and without a barrier in the loop -- a wave waits for its block while the others use theirs --, and their
+// sums meet at the end (few_rows says when). Up to 2048 states one workgroup does all of a group in one launch (4 heads x 1800 states x 64: 10.0 us, as long as five
 // splits and their join; four waves with two buffers each: 9.6 in two launches, 28.9 for 24.0 where 128 groups of 128 wide fill the chip).
 // ------------------------------------------------------------------------------------------------------------------------------------
 constexpr int TOKEN_WAVES = 8;
@@ -261,18 +261,18 @@ __global__ __launch_bounds__(TOKEN_WAVES * 64, TOKEN_WAVES / 4) void xattn_token
     constexpr int NW = TOKEN_WAVES;
     const int item = xcd_item(blockIdx.x, a.n_items);
     if (item >= a.n_items) return;
-    const int split = item % a.splits, grp = item / a.splits, bk = grp / a.Hk, hk = grp % a.Hk;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5, r = lane & 31;
+    const int rt = item % a.tiles, split = item / a.tiles % a.splits, grp = item / a.tiles / a.splits, bk = grp / a.Hk, hk = grp % a.Hk;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5, r = lane & 31, row = rt * 32 + r;
     constexpr int TB = 32 * DT * 2;
 
     const int len = states_of(a, bk), k0 = split * a.chunk, k1 = min(len, k0 + a.chunk);
     const int nt = k1 > k0 ? (k1 - k0 + 31) / 32 : 0;                        // blocks of the workgroup; wave w takes w, w + NW, ...
     uint4 qf[DT / 16];
     {
-        const RowAt w = row_at(a, bk, hk, min(r, a.M - 1));
+        const RowAt w = row_at(a, bk, hk, min(row, a.M - 1));
         const uint16_t* q = a.q + off_at(w, a.q_sb, a.q_sl, a.q_sh);
 #pragma unroll
-        for (int ks = 0; ks < DT / 16; ++ks) qf[ks] = row_frag(q, ks, h, a.D, r < a.M);
+        for (int ks = 0; ks < DT / 16; ++ks) qf[ks] = row_frag(q, ks, h, a.D, row < a.M);
     }
     f32x16 acc[DT / 32];
 #pragma unroll
@@ -342,7 +342,7 @@ __global__ __launch_bounds__(TOKEN_WAVES * 64, TOKEN_WAVES / 4) void xattn_token
             const float4 u = *reinterpret_cast<const float4*>(sums + (w * 32 + r) * SW + c);
             t.x += u.x; t.y += u.y; t.z += u.z; t.w += u.w;
         }
-        store_piece<F16, DT>(a, bk, hk, split, r, c, t, mm, ll, piece == 0 && h == 0, one);
+        store_piece<F16, DT>(a, bk, hk, split, row, c, t, mm, ll, piece == 0 && h == 0, one);
     }
 }
 
@@ -808,15 +808,25 @@ void choose_splits(int64_t base, int wanted, int len, int unit, int least, int& 
 // per CU, each with at least 1024 states (16 x 8 groups x 16384 x 128: 156, with one per CU 162), and no split at all up to 2048 states.
 constexpr int CUS = 256;
 int dt_of(const XattnArgs& a) { return a.D <= 64 ? 64 : 128; }
-bool few_rows(const XattnArgs& a) { return a.M <= 32; }
+// Tiles of 32 rows, their states shared out over the waves of a workgroup, instead of tiles of 128 rows whose states are shared out over
+// workgroups and joined by another launch: for at most 32 rows, and where the 128-row tiles would leave most CUs idle, between 64 states (two
+// blocks: the other waves had none) and 2048. us, 128-row tiles and these (tiles of 32 x states x width):
+//   120 x 1800 x 128: 23.2, 16.5    240 x 1800 x 128: 27.6, 18.7    480 x 1800 x 128: 36.9, 33.3    768 x 300 x 128: 13.5, 22.8
+//   256 x 300 x 64: 11.4, 6.2       512 x 300 x 64: 13.6, 9.1       768 x 300 x 64: 9.2, 11.9       128 x 4000 x 64: 18.2, 19.4
+//   128 x 64 x 128: 6.8, 7.2        128 x 65 x 128: 8.1, 7.4        8 x 1800 x 128: 13.8, 15.0      8 x 1800 x 64: 10.7, 10.7
+bool few_rows(const XattnArgs& a) {
+    if (a.M <= 32) return true;
+    const int64_t tiles = (int64_t)a.Bk * a.Hk * cdiv(a.M, 32);
+    return a.Lk > 64 && a.Lk <= 2048 && tiles <= 2 * CUS && (tiles >= 32 || a.Lk * dt_of(a) <= 2048 * 64);
+}
 
 struct Plan { int tiles, splits, chunk; };
 Plan plan_fwd(const XattnArgs& a) {
     Plan p{};
     const int64_t groups = (int64_t)a.Bk * a.Hk;
     if (few_rows(a)) {
-        p.tiles = 1;
-        choose_splits(groups, a.Lk > 2048 ? 2 * CUS : 1, a.Lk, 256, 4, p.splits, p.chunk);
+        p.tiles = cdiv(a.M, 32);
+        choose_splits(groups * p.tiles, a.Lk > 2048 ? 2 * CUS : 1, a.Lk, 256, 4, p.splits, p.chunk);
     } else {
         p.tiles = cdiv(a.M, 128);
         choose_splits(groups * p.tiles, CUS, a.Lk, KT, 2, p.splits, p.chunk);

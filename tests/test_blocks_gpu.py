@@ -97,6 +97,28 @@ def test_xattn_forward_and_gradients(case, t):
 
 
 @pytest.mark.parametrize("t", HALF)
+@pytest.mark.parametrize("case", [
+    (1, 1, 257, 2100, 2, 1, 128, "holes"),         # a long axis in splits of 128-row tiles
+    (3, 3, 70, 2055, 2, 2, 72, "len holes empty"),
+    (600, 600, 33, 65, 1, 1, 40, "len holes empty"),       # more tiles than one round of the chip
+    (140, 70, 67, 70, 4, 2, 64, "len"),
+    (260, 2, 30, 333, 4, 2, 128, "holes"),
+    (2, 2, 100, 64, 2, 2, 128, "holes"),           # two blocks of states
+    (32, 32, 32, 2048, 2, 2, 64, "len"),           # tiles of 32 rows at their most states
+    (1, 1, 33, 2048, 2, 1, 128, ""),
+    (16, 1, 31, 1800, 1, 1, 128, "holes"),
+])
+def test_xattn_forms(case, t):
+    """the forms that test_xattn_forward_and_gradients' sizes do not reach"""
+    q, k, v, dout, m = xattn_inputs(case, t)
+    out, lse = blocks().cross_attention(q, k, v, **m)
+    d = blocks().cross_attention_backward(dout, q, k, v, out, lse, **m)
+    want = ref.xattn(q, k, v, dout=dout, **m)
+    for name, got in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *d)):
+        held(got, *want[name], name)
+
+
+@pytest.mark.parametrize("t", HALF)
 def test_xattn_small_gradients_keep_their_digits(t):
     """dout of 2^-12: dS lies far below fp16's normal range and must not lose digits there"""
     case = (2, 1, 40, 700, 2, 2, 64, "")
