@@ -631,6 +631,70 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
         }
 }
 
+// What a row of dQ (a lane and its other half) holds while it walks the states: Q, dout, P_UP - lse (base 2) and delta = rowsum(dout o out)
+template <bool F16, int DT>
+struct GradRow {
+    uint4 q[DT / 16], d[DT / 16];
+    float nl, de;
+    __device__ __forceinline__ void load(const XattnArgs& a, const RowAt& w, int h, bool in) {
+        const uint16_t* qp = a.q + off_at(w, a.q_sb, a.q_sl, a.q_sh);
+        const uint16_t* dp = a.dout + off_at(w, a.d_sb, a.d_sl, a.d_sh);
+#pragma unroll
+        for (int ks = 0; ks < DT / 16; ++ks) { q[ks] = row_frag(qp, ks, h, a.D, in); d[ks] = row_frag(dp, ks, h, a.D, in); }
+        nl = in ? P_UP<F16> - a.lse[off_lse(a, w)] * LOG2E : NEG_INF;
+        // this lane's half of the row, then the other's
+        const uint16_t* o = a.out + off_out(a, w);
+        de = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < DT / 16; ++ks) {
+            const uint4 x = row_frag(o, ks, h, a.D, in), y = d[ks];
+            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) de += T16<F16>::lo(xs[i]) * T16<F16>::lo(ys[i]) + T16<F16>::hi(xs[i]) * T16<F16>::hi(ys[i]);
+        }
+        de = sum_halves(de);
+    }
+};
+// dQ^T += K^T dS^T of 32 states (tiles in LDS)
+template <bool F16, int DT>
+__device__ __forceinline__ void add_dq(const unsigned char* ktile, const unsigned char* vtile, const GradRow<F16, DT>& g, f32x16 (&acc)[DT / 32],
+                                       float& sc, float c, const float* bias, bool all, int lane) {
+    const int h = lane >> 5;
+    f32x16 s, ds;
+    start_scores(s, bias, all, h);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) ds[i] = 0.f;
+    constexpr int N = DT / 8, AHEAD = 4;                           // K's and V's fragments in turn
+    auto row = [&](int i) { return frag_rows<DT>(i % 2 == 0 ? ktile : vtile, 0, i / 2, lane); };
+    uint4 f[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) f[i] = row(i);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (i % 2 == 0) s = T16<F16>::mfma32(f[i % AHEAD], g.q[i / 2], s);
+        else ds = T16<F16>::mfma32(f[i % AHEAD], g.d[i / 2], ds);
+        if (i + AHEAD < N) f[i % AHEAD] = row(i + AHEAD);
+        reads_stay();
+    }
+    constexpr int NC = DT / 16;                                    // K's columns for dQ^T += K^T dS^T
+    auto column = [&](int i) { return frag_cols<DT, 4, 8>(ktile, 16 * (i % 2), 32 * (i / 2), lane); };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) f[i] = column(i);
+    reads_stay();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, g.nl)) * (ds[i] - g.de);
+    scale_ds<F16, DT / 32>(ds, acc, sc);
+    uint4 p[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) p[u] = pack8<F16>(ds, u);
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        acc[i / 2] = T16<F16>::mfma32(f[i % AHEAD], p[i % 2], acc[i / 2]);
+        if (i + AHEAD < NC) f[i % AHEAD] = column(i + AHEAD);
+        reads_stay();
+    }
+}
+
 // dQ: as the forward kernel; dS^T has a row per lane, dQ^T += K^T dS^T reads the K tile a second time, transposed. 2 x 16 heads, 4096 rows and
 // states: 386 us 128 wide (1068 TFLOP/s), 259 us 64 wide (797).
 template <bool F16, int DT>
@@ -644,29 +708,11 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
     const int len = states_of(a, bk), k0 = split * a.chunk, k1 = min(len, k0 + a.chunk);
     const int nt = k1 > k0 ? (k1 - k0 + KT - 1) / KT : 0;
 
-    uint4 qf[DT / 16], df[DT / 16];
     const RowAt w = row_at(a, bk, hk, min(r, a.M - 1));
-    float nl, de;
-    {
-        const uint16_t* q = a.q + off_at(w, a.q_sb, a.q_sl, a.q_sh);
-        const uint16_t* d = a.dout + off_at(w, a.d_sb, a.d_sl, a.d_sh);
-#pragma unroll
-        for (int ks = 0; ks < DT / 16; ++ks) { qf[ks] = row_frag(q, ks, h, a.D, r < a.M); df[ks] = row_frag(d, ks, h, a.D, r < a.M); }
-        nl = r < a.M ? P_UP<F16> - a.lse[off_lse(a, w)] * LOG2E : NEG_INF;
-        // delta = rowsum(dout o out): this lane's half of the row, then the other's; kept for the dK, dV kernel
-        const uint16_t* o = a.out + off_out(a, w);
-        de = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < DT / 16; ++ks) {
-            const uint4 x = row_frag(o, ks, h, a.D, r < a.M), y = df[ks];
-            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) de += T16<F16>::lo(xs[i]) * T16<F16>::lo(ys[i]) + T16<F16>::hi(xs[i]) * T16<F16>::hi(ys[i]);
-        }
-        de = sum_halves(de);
-        if (item == 0 && threadIdx.x < 8) a.zeros[threadIdx.x] = 0;            // (the dK, dV kernel's absent rows)
-        if (split == 0 && h == 0 && r < a.M) a.delta[(int64_t)grp * a.M + r] = de;
-    }
+    GradRow<F16, DT> g;
+    g.load(a, w, h, r < a.M);
+    if (item == 0 && threadIdx.x < 8) a.zeros[threadIdx.x] = 0;            // (the dK, dV kernel's absent rows)
+    if (split == 0 && h == 0 && r < a.M) a.delta[(int64_t)grp * a.M + r] = g.de;
     f32x16 acc[DT / 32];
 #pragma unroll
     for (int d = 0; d < DT / 32; ++d)
@@ -704,41 +750,8 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
         const unsigned char* vtile = ktile + TB;
         if (bits != 0) {
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                f32x16 s, ds;
-                start_scores(s, bias + 32 * b, bits == ~0ull, h);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) ds[i] = 0.f;
-                constexpr int N = DT / 8, AHEAD = 4;                           // K's and V's fragments in turn
-                auto row = [&](int i) { return frag_rows<DT>(i % 2 == 0 ? ktile : vtile, 32 * b, i / 2, lane); };
-                uint4 f[AHEAD];
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i) f[i] = row(i);
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    if (i % 2 == 0) s = T16<F16>::mfma32(f[i % AHEAD], qf[i / 2], s);
-                    else ds = T16<F16>::mfma32(f[i % AHEAD], df[i / 2], ds);
-                    if (i + AHEAD < N) f[i % AHEAD] = row(i + AHEAD);
-                    reads_stay();
-                }
-                constexpr int NC = DT / 16;                                    // K's columns for dQ^T += K^T dS^T
-                auto column = [&](int i) { return frag_cols<DT, 4, 8>(ktile, 32 * b + 16 * (i % 2), 32 * (i / 2), lane); };
-#pragma unroll
-                for (int i = 0; i < AHEAD; ++i) f[i] = column(i);
-                reads_stay();
-#pragma unroll
-                for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, nl)) * (ds[i] - de);
-                scale_ds<F16, DT / 32>(ds, acc, sc);
-                uint4 g[2];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) g[u] = pack8<F16>(ds, u);
-#pragma unroll
-                for (int i = 0; i < NC; ++i) {
-                    acc[i / 2] = T16<F16>::mfma32(f[i % AHEAD], g[i % 2], acc[i / 2]);
-                    if (i + AHEAD < NC) f[i % AHEAD] = column(i + AHEAD);
-                    reads_stay();
-                }
-            }
+            for (int b = 0; b < 2; ++b)
+                add_dq<F16, DT>(ktile + 32 * b * DT * 2, vtile + 32 * b * DT * 2, g, acc, sc, a.c, bias + 32 * b, bits == ~0ull, lane);
         }
         bits = next;
     }
@@ -754,6 +767,81 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
             if (a.splits > 1) *reinterpret_cast<float4*>(a.part + at + e) = x;
             else if (e < a.D) *reinterpret_cast<uint2*>(a.dq + at + e) = make_uint2(T16<F16>::pack2(x.x, x.y), T16<F16>::pack2(x.z, x.w));
         }
+}
+
+// dQ in tiles of 32 rows, as the token kernel: eight waves walk their own blocks of 32 states, their sums meet in LDS and are added in wave order
+template <bool F16, int DT>
+__global__ __launch_bounds__(TOKEN_WAVES * 64, TOKEN_WAVES / 4) void xattn_dq_few_kernel(XattnArgs a) {
+    constexpr int NW = TOKEN_WAVES;
+    const int item = xcd_item(blockIdx.x, a.n_items);
+    if (item >= a.n_items) return;
+    const int rt = item % a.tiles, grp = item / a.tiles, bk = grp / a.Hk, hk = grp % a.Hk;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, h = lane >> 5, r = lane & 31, row = rt * 32 + r;
+    constexpr int TB = 32 * DT * 2;
+
+    const int len = states_of(a, bk), nt = (len + 31) / 32;
+    GradRow<F16, DT> g;
+    g.load(a, row_at(a, bk, hk, min(row, a.M - 1)), h, row < a.M);
+    if (item == 0 && threadIdx.x < 8) a.zeros[threadIdx.x] = 0;            // (the dK, dV kernel's absent rows)
+    if (wave == 0 && h == 0 && row < a.M) a.delta[(int64_t)grp * a.M + row] = g.de;
+    f32x16 acc[DT / 32];
+#pragma unroll
+    for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+    float sc = F16 ? 0.f : 1.0f;
+
+    const uint16_t* kb = a.k + bk * a.k_sb + hk * a.k_sh;
+    const uint16_t* vb = a.v + bk * a.v_sb + hk * a.v_sh;
+    unsigned char* own = conv_lds_dyn + wave * (2 * TB + 128);
+    float* bias = reinterpret_cast<float*>(own + 2 * TB);
+    const uint32_t lds0 = lds_addr_of(own);
+    TileLoad<DT, 32, 1> lk, lv;
+    lk.init(0, lane, a.k_sl, a.D);
+    lv.init(0, lane, a.v_sl, a.D);
+    uint32_t byte = 0, bits = 0;
+    auto valid = [&](int t) -> uint32_t { return t < nt ? mask_byte(a, bk, 32 * t + (lane & 31), len) : 0u; };
+    auto request = [&](int t) {
+        bits = (uint32_t)__ballot(byte != 0);
+        const bool all = bits == ~0u;
+        lk.request(kb + (int64_t)t * 32 * a.k_sl, all, bits, lds0, 0);
+        lv.request(vb + (int64_t)t * 32 * a.v_sl, all, bits, lds0 + TB, 0);
+        put_bias(bias, 32, byte, all, lane);
+        byte = valid(t + NW);
+    };
+    byte = valid(wave);
+    if (wave < nt) request(wave);
+    for (int t = wave; t < nt; t += NW) {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if (bits != 0) add_dq<F16, DT>(own, own + TB, g, acc, sc, a.c, bias, bits == ~0u, lane);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                    // the block is read before its place is requested again
+        if (t + NW < nt) request(t + NW);
+    }
+    const float f = saturate_from_here<F16>() * a.scale * __builtin_amdgcn_exp2f(-P_UP<F16>) / (sc == 0.f ? 1.0f : sc);
+    wait_all_and_meet();
+    float* sums = reinterpret_cast<float*>(conv_lds_dyn);                     // [NW][32][DT + 4]
+    constexpr int SW = DT + 4;
+    static_assert(NW * 32 * SW * 4 <= NW * (2 * TB + 1024), "the sums fit");
+#pragma unroll
+    for (int d = 0; d < DT / 32; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<float4*>(sums + (wave * 32 + r) * SW + 32 * d + 8 * q + 4 * h) =
+                make_float4(acc[d][4 * q] * f, acc[d][4 * q + 1] * f, acc[d][4 * q + 2] * f, acc[d][4 * q + 3] * f);
+    __syncthreads();
+    if (row >= a.M) return;
+    const RowAt w = row_at(a, bk, hk, row);
+#pragma unroll
+    for (int i = 0; i < DT / 8 / NW; ++i) {
+        const int c = 8 * (wave + i * NW) + 4 * h;
+        float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int u = 0; u < NW; ++u) {
+            const float4 x = *reinterpret_cast<const float4*>(sums + (u * 32 + r) * SW + c);
+            t.x += x.x; t.y += x.y; t.z += x.z; t.w += x.w;
+        }
+        if (c < a.D) *reinterpret_cast<uint2*>(a.dq + off_out(a, w) + c) = make_uint2(T16<F16>::pack2(t.x, t.y), T16<F16>::pack2(t.z, t.w));
+    }
 }
 
 // sums of the splits in their order, 16 lanes per row: the rows of dQ, then the states of dK, then those of dV (whichever were split)
@@ -817,7 +905,15 @@ int dt_of(const XattnArgs& a) { return a.D <= 64 ? 64 : 128; }
 bool few_rows(const XattnArgs& a) {
     if (a.M <= 32) return true;
     const int64_t tiles = (int64_t)a.Bk * a.Hk * cdiv(a.M, 32);
-    return a.Lk > 64 && a.Lk <= 2048 && tiles <= 2 * CUS && (tiles >= 32 || a.Lk * dt_of(a) <= 2048 * 64);
+    return a.Lk > 64 && a.Lk <= 2048 && tiles <= 2 * CUS && (tiles >= 32 || (int64_t)a.Lk * dt_of(a) <= 2048 * 64);
+}
+
+// The same for dQ, whose splits share their join with those of dK and dV: from 64 tiles of 32 rows (below, splits spread better) to one per CU
+// (a workgroup each). us of the whole backward pass, 128-row tiles and these: 256 x 300 x 64: 22.1, 17.1; 128 x 300 x 128: 31.1, 26.8; 384 x 300
+// x 128: 48.7, 50.3; 240 x 1800 x 64: 49.4, 43.4; 32 x 1800 x 64: 25.7, 28.8; 128 x 1000 x 128: 42.7, 37.0; 120 x 1800 x 128: 54.9, 58.3
+bool few_dq(const XattnArgs& a) {
+    const int64_t tiles = (int64_t)a.Bk * a.Hk * cdiv(a.M, 32);
+    return a.Lk > 64 && (int64_t)a.Lk * dt_of(a) <= 2048 * 64 && tiles >= 64 && tiles <= CUS;
 }
 
 struct Plan { int tiles, splits, chunk; };
@@ -841,6 +937,7 @@ Plan plan_dkv(const XattnArgs& a) {
 }
 Plan plan_dq(const XattnArgs& a) {
     Plan p{};
+    if (few_dq(a)) return {cdiv(a.M, 32), 1, a.Lk};
     p.tiles = cdiv(a.M, 128);
     choose_splits((int64_t)a.Bk * a.Hk * p.tiles, CUS, a.Lk, KT, 2, p.splits, p.chunk);
     return p;
@@ -890,7 +987,8 @@ int bwd(XattnArgs a, float* ws, hipStream_t st) {
     float* pv = pk + (int64_t)k.splits * states * DT;
     unsigned grid = items(a, q);
     a.part = pq;
-    ISB_TRY((launch<xattn_dq_kernel<F16, DT>>("xattn_dq", grid, 256, 2 * (2 * KT * DT * 2 + KT * 4), a, st)));
+    if (few_dq(a)) ISB_TRY((launch<xattn_dq_few_kernel<F16, DT>>("xattn_dq_few", grid, TOKEN_WAVES * 64, TOKEN_WAVES * (2 * 32 * DT * 2 + 1024), a, st)));
+    else ISB_TRY((launch<xattn_dq_kernel<F16, DT>>("xattn_dq", grid, 256, 2 * (2 * KT * DT * 2 + KT * 4), a, st)));
     grid = items(a, k);
     a.part = pk;
     a.part2 = pv;

@@ -107,6 +107,10 @@ def test_xattn_forward_and_gradients(case, t):
     (32, 32, 32, 2048, 2, 2, 64, "len"),           # tiles of 32 rows at their most states
     (1, 1, 33, 2048, 2, 1, 128, ""),
     (16, 1, 31, 1800, 1, 1, 128, "holes"),
+    (8, 8, 100, 300, 4, 4, 64, "len holes empty"), # tiles of 32 rows backward too
+    (16, 16, 70, 130, 2, 2, 72, "len holes"),
+    (6, 3, 60, 1000, 16, 2, 128, "holes"),
+    (100, 100, 3, 66, 1, 1, 8, "len"),
 ])
 def test_xattn_forms(case, t):
     """the forms that test_xattn_forward_and_gradients' sizes do not reach"""
@@ -196,9 +200,10 @@ def test_xattn_a_nan_stays_where_it_belongs(Lq, t):
 
 
 @pytest.mark.parametrize("t", HALF)
-def test_xattn_an_infinite_gradient_stays_in_its_row(t):
+@pytest.mark.parametrize("Lq", [64, 1200])
+def test_xattn_an_infinite_gradient_stays_in_its_row(t, Lq):
     """dout holds an infinity (a loss scaled too far): dq of the other rows, dk and dv of the other head are what they are without it"""
-    q, k, v, dout, _ = xattn_inputs((1, 1, 64, 300, 2, 2, 64, ""), t, std=8.0)
+    q, k, v, dout, _ = xattn_inputs((1, 1, Lq, 300, 2, 2, 64, ""), t, std=8.0)
     out, lse = blocks().cross_attention(q, k, v)
     without, bad = dout.clone(), dout.clone()
     without[0, 3, 0], bad[0, 3, 0, 7] = 0, math.inf
