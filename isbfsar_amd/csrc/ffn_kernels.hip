@@ -424,22 +424,30 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
     }
 }
 
-// sums of the splits of k in their order, + bias; four values per thread
+// sums of the splits of k in their order, + bias; four values per thread. The three products of a backward pass share one launch (us of the
+// pass, a launch each and this: 600 rows, 512 x 2048: 74, 63; 1030, 640 x 2560: 91, 84; 4111 and more: the same within 1 %).
+struct Sums {
+    struct One { const float* part; const uint16_t* bias; uint16_t* C; int64_t n4; int N, splits, blocks; } of[3];
+    int blocks() const { return of[0].blocks + of[1].blocks + of[2].blocks; }
+};
 template <bool F16>
-__global__ __launch_bounds__(256) void ffn_sum_kernel(const float* part, int splits, int64_t n4, int N, const uint16_t* bias, uint16_t* C) {
+__global__ __launch_bounds__(256) void ffn_sum_kernel(Sums all) {
     T16<F16>::enter();
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n4) return;
+    int b = blockIdx.x, k = 0;
+    while (b >= all.of[k].blocks) b -= all.of[k++].blocks;
+    const Sums::One p = all.of[k];
+    const int64_t i = (int64_t)b * 256 + threadIdx.x;
+    if (i >= p.n4) return;
     float o[4] = {};
-    for (int s = 0; s < splits; ++s) {
-        const float4 v = *reinterpret_cast<const float4*>(part + (s * n4 + i) * 4);
+    for (int s = 0; s < p.splits; ++s) {
+        const float4 v = *reinterpret_cast<const float4*>(p.part + (s * p.n4 + i) * 4);
         o[0] += v.x; o[1] += v.y; o[2] += v.z; o[3] += v.w;
     }
-    if (bias) {
-        const uint2 w = *reinterpret_cast<const uint2*>(bias + i * 4 % N);
+    if (p.bias) {
+        const uint2 w = *reinterpret_cast<const uint2*>(p.bias + i * 4 % p.N);
         o[0] += T16<F16>::lo(w.x); o[1] += T16<F16>::hi(w.x); o[2] += T16<F16>::lo(w.y); o[3] += T16<F16>::hi(w.y);
     }
-    *reinterpret_cast<uint2*>(C + i * 4) = make_uint2(T16<F16>::pack2(o[0], o[1]), T16<F16>::pack2(o[2], o[3]));
+    *reinterpret_cast<uint2*>(p.C + i * 4) = make_uint2(T16<F16>::pack2(o[0], o[1]), T16<F16>::pack2(o[2], o[3]));
 }
 
 // the same for the tail's tiles: part [tail tile][split][BM][BN]; a workgroup takes 1024 values of a tile
@@ -670,24 +678,28 @@ int mm(const MmArgs& p, const char* name, hipStream_t st) {
     if (t == TILE_MID) return mm_run<F16, 128, 128, 2, 2, 1, 2, LA, LB, EPI>(p, name, st);
     return mm_run<F16, 256, 256, 2, 4, 1, 2, LA, LB, EPI>(p, name, st);
 }
-// C = A B^T (+ bias), k split where the tiles alone leave CUs idle
+// C = A B^T (+ bias), k split where the tiles alone leave CUs idle: into `part`, to be added up as `sum` says
 template <bool F16, int LA, int LB>
-int mm_out(MmArgs p, float* part, const char* name, hipStream_t st) {
+int mm_out(MmArgs p, unsigned char* part, Sums::One& sum, const char* name, hipStream_t st) {
     const OutPlan plan = plan_out(LA, p.M, p.N, cdiv(p.K, BK) * p.nseg);
     p.splits = plan.splits;
     p.full = plan.full;
     p.tail = plan.tail;
     p.tail_splits = plan.tail_splits;
-    p.part = part;
+    p.part = reinterpret_cast<float*>(part);
     ISB_TRY((mm<F16, LA, LB, EPI_OUT>(p, name, st)));
-    if (p.splits > 1) {
-        const int64_t n4 = (int64_t)p.M * p.N / 4;
-        ffn_sum_kernel<F16><<<(unsigned)((n4 + 255) / 256), 256, 0, st>>>(part, p.splits, n4, p.N, p.bias, p.C);
-        ISB_LAUNCHED("ffn_sum", st);
-    }
+    const int64_t n4 = (int64_t)p.M * p.N / 4;
+    sum = {p.part, p.bias, p.C, n4, p.N, p.splits, p.splits > 1 ? (int)((n4 + 255) / 256) : 0};
     return ISB_OK;
 }
-size_t part_bytes(int la, int M, int N, int kts) { return plan_out(la, M, N, kts).bytes; }
+template <bool F16>
+int add_up(const Sums& s, hipStream_t st) {
+    if (s.blocks() == 0) return ISB_OK;
+    ffn_sum_kernel<F16><<<(unsigned)s.blocks(), 256, 0, st>>>(s);
+    ISB_LAUNCHED("ffn_sum", st);
+    return ISB_OK;
+}
+size_t part_bytes(int la, int M, int N, int kts) { return (plan_out(la, M, N, kts).bytes + 255) / 256 * 256; }
 
 template <bool F16, int MT, bool GATE>
 int token(const MmArgs& p, float* h, hipStream_t st) {
@@ -723,13 +735,16 @@ int fwd(const FfnArgs& a, unsigned char* ws, hipStream_t st) {
         return token<F16, TOKENS, false>(d, hf, st);
     }
     ISB_TRY((mm<F16, 0, 0, EPI_GATE>(g, "ffn gate + up", st)));
-    return mm_out<F16, 0, 0>(d, reinterpret_cast<float*>(ws), "ffn down", st);
+    Sums s{};
+    ISB_TRY((mm_out<F16, 0, 0>(d, ws, s.of[0], "ffn down", st)));
+    return add_up<F16>(s, st);
 }
 
 template <bool F16>
 int bwd(const FfnArgs& a, unsigned char* ws, hipStream_t st) {
     uint16_t* dgu = reinterpret_cast<uint16_t*>(ws);
-    float* part = reinterpret_cast<float*>(ws + ((size_t)a.M * 2 * a.F * 2 + 255) / 256 * 256);
+    unsigned char* rest = ws + ((size_t)a.M * 2 * a.F * 2 + 255) / 256 * 256;
+    float* part = reinterpret_cast<float*>(rest);
     MmArgs p{};
     // dG, dU from dh = dy Wd
     p.A = a.dy; p.B = a.wd; p.lda = a.dy_s; p.ldb = a.F; p.M = a.M; p.N = a.F; p.K = a.D; p.nseg = 1; p.splits = 1;
@@ -752,17 +767,21 @@ int bwd(const FfnArgs& a, unsigned char* ws, hipStream_t st) {
     p = MmArgs{};
     p.A = dgu; p.B = a.wg; p.B2 = a.wu; p.lda = 2 * (int64_t)a.F; p.ldb = a.D; p.M = a.M; p.N = a.D; p.K = a.F; p.nseg = 2;
     p.C = a.dx; p.ldc = a.D;
-    ISB_TRY((mm_out<F16, 0, 1>(p, part, "ffn dx", st)));
+    Sums s{};
+    ISB_TRY((mm_out<F16, 0, 1>(p, rest, s.of[0], "ffn dx", st)));
+    rest += part_bytes(0, a.M, a.D, 2 * cdiv(a.F, BK));
     // [dWg; dWu] = [dG | dU]^T x
     p = MmArgs{};
     p.A = dgu; p.B = a.x; p.lda = 2 * (int64_t)a.F; p.ldb = a.x_s; p.M = 2 * a.F; p.N = a.D; p.K = a.M; p.nseg = 1;
     p.C = a.dwgu; p.ldc = a.D;
-    ISB_TRY((mm_out<F16, 1, 1>(p, part, "ffn dW gate, up", st)));
+    ISB_TRY((mm_out<F16, 1, 1>(p, rest, s.of[1], "ffn dW gate, up", st)));
+    rest += part_bytes(1, 2 * a.F, a.D, cdiv(a.M, BK));
     // dWd = dy^T h
     p = MmArgs{};
     p.A = a.dy; p.B = a.h; p.lda = a.dy_s; p.ldb = a.F; p.M = a.D; p.N = a.F; p.K = a.M; p.nseg = 1;
     p.C = a.dwd; p.ldc = a.F;
-    return mm_out<F16, 1, 1>(p, part, "ffn dW down", st);
+    ISB_TRY((mm_out<F16, 1, 1>(p, rest, s.of[2], "ffn dW down", st)));
+    return add_up<F16>(s, st);
 }
 }  // namespace
 
@@ -774,8 +793,8 @@ size_t ffn_workspace(const FfnArgs& a, bool backward) {
         return h + part_bytes(0, a.M, a.D, cdiv(a.F, BK));
     }
     const size_t sums = (size_t)cdiv(a.M, 32) * ((a.dbg ? 2 * F : 0) + (a.dbd ? a.D : 0)) * 4;
-    const size_t part = std::max(std::max(sums, part_bytes(0, a.M, a.D, 2 * cdiv(a.F, BK))),
-                                 std::max(part_bytes(1, 2 * a.F, a.D, cdiv(a.M, BK)), part_bytes(1, a.D, a.F, cdiv(a.M, BK))));
+    const size_t part = std::max(sums, part_bytes(0, a.M, a.D, 2 * cdiv(a.F, BK)) + part_bytes(1, 2 * a.F, a.D, cdiv(a.M, BK)) +
+                                           part_bytes(1, a.D, a.F, cdiv(a.M, BK)));
     return (M * 2 * F * 2 + 255) / 256 * 256 + part;
 }
 int launch_ffn_fwd(const FfnArgs& a, bool f16, unsigned char* ws, hipStream_t st) { return f16 ? fwd<true>(a, ws, st) : fwd<false>(a, ws, st); }
