@@ -424,8 +424,7 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
     }
 }
 
-// sums of the splits of k in their order, + bias; four values per thread. The three products of a backward pass share one launch (us of the
-// pass, a launch each and this: 600 rows, 512 x 2048: 74, 63; 1030, 640 x 2560: 91, 84; 4111 and more: the same within 1 %).
+// sums of the splits of k in their order, + bias; four values per thread. The three products of a backward pass may share one launch (BwdParts)
 struct Sums {
     struct One { const float* part; const uint16_t* bias; uint16_t* C; int64_t n4; int N, splits, blocks; } of[3];
     int blocks() const { return of[0].blocks + of[1].blocks + of[2].blocks; }
@@ -693,10 +692,11 @@ int mm_out(MmArgs p, unsigned char* part, Sums::One& sum, const char* name, hipS
     return ISB_OK;
 }
 template <bool F16>
-int add_up(const Sums& s, hipStream_t st) {
+int add_up(Sums& s, hipStream_t st) {
     if (s.blocks() == 0) return ISB_OK;
     ffn_sum_kernel<F16><<<(unsigned)s.blocks(), 256, 0, st>>>(s);
     ISB_LAUNCHED("ffn_sum", st);
+    s = Sums{};
     return ISB_OK;
 }
 size_t part_bytes(int la, int M, int N, int kts) { return (plan_out(la, M, N, kts).bytes + 255) / 256 * 256; }
@@ -709,6 +709,20 @@ int token(const MmArgs& p, float* h, hipStream_t st) {
     ISB_LAUNCHED("ffn_token", st);
     return ISB_OK;
 }
+
+// Where the partial sums of the backward pass's three products lie. Together, one launch adds them all up (us of the pass, a launch each and
+// together: 600 rows, 512 x 2048: 74, 63; 1030, 640 x 2560: 91, 84) -- as long as they and what else passes between the launches (14 bytes for
+// each value of h) stay well inside the 256 MB last-level cache: at 4111 rows, 237 MB, dh takes 52 for 44 us and the shared launch gains 3.
+struct BwdParts {
+    size_t at[3] = {}, bytes = 0;
+    bool together = false;
+    explicit BwdParts(const FfnArgs& a) {
+        const size_t n[3] = {part_bytes(0, a.M, a.D, 2 * cdiv(a.F, BK)), part_bytes(1, 2 * a.F, a.D, cdiv(a.M, BK)), part_bytes(1, a.D, a.F, cdiv(a.M, BK))};
+        together = 14 * (size_t)a.M * a.F + n[0] + n[1] + n[2] <= (160u << 20);
+        if (together) { at[1] = n[0]; at[2] = n[0] + n[1]; }
+        for (int i = 0; i < 3; ++i) bytes = std::max(bytes, at[i] + n[i]);
+    }
+};
 
 template <bool F16>
 int fwd(const FfnArgs& a, unsigned char* ws, hipStream_t st) {
@@ -767,20 +781,21 @@ int bwd(const FfnArgs& a, unsigned char* ws, hipStream_t st) {
     p = MmArgs{};
     p.A = dgu; p.B = a.wg; p.B2 = a.wu; p.lda = 2 * (int64_t)a.F; p.ldb = a.D; p.M = a.M; p.N = a.D; p.K = a.F; p.nseg = 2;
     p.C = a.dx; p.ldc = a.D;
+    const BwdParts parts_at(a);
     Sums s{};
-    ISB_TRY((mm_out<F16, 0, 1>(p, rest, s.of[0], "ffn dx", st)));
-    rest += part_bytes(0, a.M, a.D, 2 * cdiv(a.F, BK));
+    ISB_TRY((mm_out<F16, 0, 1>(p, rest + parts_at.at[0], s.of[0], "ffn dx", st)));
+    if (!parts_at.together) ISB_TRY(add_up<F16>(s, st));
     // [dWg; dWu] = [dG | dU]^T x
     p = MmArgs{};
     p.A = dgu; p.B = a.x; p.lda = 2 * (int64_t)a.F; p.ldb = a.x_s; p.M = 2 * a.F; p.N = a.D; p.K = a.M; p.nseg = 1;
     p.C = a.dwgu; p.ldc = a.D;
-    ISB_TRY((mm_out<F16, 1, 1>(p, rest, s.of[1], "ffn dW gate, up", st)));
-    rest += part_bytes(1, 2 * a.F, a.D, cdiv(a.M, BK));
+    ISB_TRY((mm_out<F16, 1, 1>(p, rest + parts_at.at[1], s.of[1], "ffn dW gate, up", st)));
+    if (!parts_at.together) ISB_TRY(add_up<F16>(s, st));
     // dWd = dy^T h
     p = MmArgs{};
     p.A = a.dy; p.B = a.h; p.lda = a.dy_s; p.ldb = a.F; p.M = a.D; p.N = a.F; p.K = a.M; p.nseg = 1;
     p.C = a.dwd; p.ldc = a.F;
-    ISB_TRY((mm_out<F16, 1, 1>(p, rest, s.of[2], "ffn dW down", st)));
+    ISB_TRY((mm_out<F16, 1, 1>(p, rest + parts_at.at[2], s.of[2], "ffn dW down", st)));
     return add_up<F16>(s, st);
 }
 }  // namespace
@@ -793,8 +808,7 @@ size_t ffn_workspace(const FfnArgs& a, bool backward) {
         return h + part_bytes(0, a.M, a.D, cdiv(a.F, BK));
     }
     const size_t sums = (size_t)cdiv(a.M, 32) * ((a.dbg ? 2 * F : 0) + (a.dbd ? a.D : 0)) * 4;
-    const size_t part = std::max(sums, part_bytes(0, a.M, a.D, 2 * cdiv(a.F, BK)) + part_bytes(1, 2 * a.F, a.D, cdiv(a.M, BK)) +
-                                           part_bytes(1, a.D, a.F, cdiv(a.M, BK)));
+    const size_t part = std::max(sums, BwdParts(a).bytes);
     return (M * 2 * F * 2 + 255) / 256 * 256 + part;
 }
 int launch_ffn_fwd(const FfnArgs& a, bool f16, unsigned char* ws, hipStream_t st) { return f16 ? fwd<true>(a, ws, st) : fwd<false>(a, ws, st); }
