@@ -491,7 +491,8 @@ int isb_xattn_backward(const isb_xattn_args* a, void* d_workspace, size_t bytes,
  *   x [M,D] (row stride x_stride), w_gate, w_up [F,D], w_down [D,F], b_gate, b_up [F], b_down [D] or NULL, y [M,D].
  *   D, F multiples of 8, at most 2^20; M 1 .. 2^22; row strides D .. 2^22 elements.
  *   For the backward pass forward also fills pre_gate, pre_up [M,F] f32 (both or neither) and hidden [M,F] (needed with them,
- *   else NULL: it lives in the workspace).
+ *   else NULL: it lives in the workspace). fp16: hidden is the library's own -- groups of its values carry a power of two where they
+ *   would leave the type's range (a hidden value past 65504 does no harm to a y inside), and backward may write such groups anew.
  * Backward: dy [M,D] (row stride dy_stride) and those three -> dx [M,D], dw_gate_up [2F,D] (the gate's rows first), dw_down [D,F],
  * db_gate, db_up (both or neither) [F], db_down [D] or NULL. */
 #define ISB_ACT_SILU 0

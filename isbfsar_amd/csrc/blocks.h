@@ -61,7 +61,7 @@ struct FfnArgs {
     uint16_t *dx, *dwgu, *dwd, *dbg, *dbu, *dbd;         // dwgu [2 F, D]
     int M, D, F, act;
 };
-size_t ffn_workspace(const FfnArgs& a, bool backward);
+size_t ffn_workspace(const FfnArgs& a, bool f16, bool backward);
 int launch_ffn_fwd(const FfnArgs& a, bool f16, unsigned char* ws, hipStream_t st);
 int launch_ffn_bwd(const FfnArgs& a, bool f16, unsigned char* ws, hipStream_t st);
 

@@ -163,7 +163,7 @@ int ffn_args(const isb_ffn_args* u, bool backward, FfnArgs& a) {
 int ffn_run(const isb_ffn_args* u, bool backward, void* ws, size_t bytes, void* stream) {
     FfnArgs a{};
     ISB_TRY(ffn_args(u, backward, a));
-    ISB_TRY(room("gated feed-forward", ws, bytes, ffn_workspace(a, backward)));
+    ISB_TRY(room("gated feed-forward", ws, bytes, ffn_workspace(a, u->dtype == ISB_T_F16, backward)));
     OnDevice dev;
     ISB_TRY(dev.enter(u->device));
     const bool f16 = u->dtype == ISB_T_F16;
@@ -219,7 +219,7 @@ extern "C" int isb_ffn_workspace(const isb_ffn_args* u, int32_t backward, size_t
         ISB_REQUIRE(bytes, ISB_ERR_INVALID, "null argument");
         isb::FfnArgs a{};
         ISB_TRY(ffn_shape(u, a));
-        *bytes = isb::ffn_workspace(a, backward != 0);
+        *bytes = isb::ffn_workspace(a, u->dtype == ISB_T_F16, backward != 0);
         return ISB_OK;
     });
 }

@@ -18,7 +18,7 @@ namespace {
 
 enum { EPI_GATE = 0, EPI_OUT = 1, EPI_DH = 2 };
 enum { FFN_SILU = 0, FFN_GELU = 1, FFN_RELU = 2, FFN_SIGMOID = 3 };
-constexpr int BK = 64;                   // k per tile
+constexpr int BK = 64, KS = BK / 16;     // k per tile, its steps
 
 struct MmArgs {
     const uint16_t *A, *B, *B2;          // B2: GATE: the up weights; else the operand of the second k segment
@@ -32,6 +32,10 @@ struct MmArgs {
     float *g, *u;                        // GATE: saved (or null); DH: read
     float* part;                         // OUT with splits > 1: [split][M][N]
     float* cs;                           // DH: column sums of dG | dU over 32 rows, [ceil(M / 32)][2 F], or null
+    int8_t* ex;                          // fp16 (Powers): GATE: exponents of h
+    uint16_t* h;                         // fp16, DH: the saved h, for dWd, and its exponents
+    int8_t* ex_h;
+    const int8_t *xa, *xb;               // fp16, OUT: exponents of A's, B's values, or null
     int F, act;
     int tiles_m, tiles_n, n_items;
     int full, tail, tail_splits, tail_per, kt_per_tail;   // OUT: the last `tail` tiles, behind `full` whole rounds of the chip, split k (0: none)
@@ -105,6 +109,133 @@ struct OpLoad {
         const uint32_t v = kk[j] < k_left ? voff[j] : DMA_NONE;
         const bool up = PAIR && (((wave * PIECES + j) >> 2) & 1);          // a piece is 8 rows: 4 pieces per 32-row group (wave-uniform)
         dma16_desc(up ? d2 : d, v, to + j * 1024);
+    }
+};
+
+// ---- fp16 between two products. h = act(g) o u may lie past 65504, or far below fp16's normal numbers, where y does not. So a group of 8 rows x 32
+// features carries a power of two of its own: what is stored is value 2^-e, e = 0 while the group's largest magnitude lies in [2^-10, 65504] -- as
+// good as always --, above just enough to bring it below 2^15, below in steps of 16. Exponents: a byte per group, [ceil(F / 32)][4 ceil(rows / 32)];
+// EXP_NONE: nothing but zeros, infinities and NaN.
+constexpr int EXP_NONE = -128;
+// Whether groups that a wave has stored as they are should have carried a power of two: the common case has no branch, so that the steps of an
+// epilogue stay side by side (with one in every step: GATE 56 -> 65 us, DH 48 -> 59 at 4111 rows, 640 x 2560). MARGIN: a little sooner.
+template <bool MARGIN>
+struct GroupCheck {
+    static constexpr float LOW = MARGIN ? 0x1.01p-10f : 0x1p-10f, HIGH = MARGIN ? 65248.f : 65504.f;
+    float hi = 0.f;
+    uint64_t seen = 0;
+    bool tiny = false;
+    // a step's values; `fresh`: of new groups. Then, groups complete: which lanes hold each, and which of them are part of the matrix (uniform)
+    __device__ __forceinline__ void add(const float (&v)[4], bool fresh) {
+        const float mx = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+        hi = fmaxf(hi, mx);
+        const uint64_t b = __ballot(mx >= LOW);
+        seen = fresh ? b : seen | b;
+    }
+    __device__ __forceinline__ void close(uint64_t lanes, bool live) { tiny |= live && (seen & lanes) == 0; }
+    // (of the whole wave: not behind a branch that some of its lanes take)
+    __device__ __forceinline__ bool zero() const { return __ballot(hi > 0.f) == 0; }                      // (or NaN)
+    __device__ __forceinline__ bool odd() const { return (tiny && !zero()) || __ballot(hi > HIGH) != 0; }
+};
+constexpr uint64_t ALL_LANES = ~0ull, LOW_COLUMNS = 0x00ff00ff00ff00ffull;         // the wave; of every 16 lanes the first 8
+__device__ __forceinline__ float finite_max(const float (&v)[4], float mx = 0.f) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mx = fabsf(v[i]) < __builtin_inff() ? fmaxf(mx, fabsf(v[i])) : mx;
+    return mx;
+}
+__device__ __forceinline__ int exp_of(float mx) {
+    const int x = __builtin_amdgcn_frexp_expf(mx);                        // mx = f 2^x, f in [1/2, 1)
+    return mx == 0.f ? EXP_NONE : mx > 65504.f ? x - 15 : mx >= 0x1p-10f ? 0 : -16 * min((-10 - x) / 16 + 1, 7);
+}
+// over the lanes that hold 32 features: 8 of every 16
+__device__ __forceinline__ float half_max(float mx) {
+#pragma unroll
+    for (int k : {1, 2, 4, 16, 32}) mx = fmaxf(mx, __shfl_xor(mx, k));
+    return mx;
+}
+// N groups' bytes at once: all of them e
+template <int N>
+__device__ __forceinline__ void store_exps(int8_t* to, int e) {
+    const uint32_t w = 0x01010101u * (uint8_t)e;
+    if constexpr (N == 1) *to = (int8_t)w;
+    else if constexpr (N == 2) *reinterpret_cast<uint16_t*>(to) = (uint16_t)w;
+    else if constexpr (N == 4) *reinterpret_cast<uint32_t*>(to) = w;
+    else *reinterpret_cast<uint2*>(to) = make_uint2(w, w);
+}
+__device__ __forceinline__ float stored_by(int e) { return e == 0 || e == EXP_NONE ? 1.0f : __builtin_ldexpf(1.0f, -e); }
+
+// What a wave of the product that reads such values knows of their exponents. BY_ROW (layout 0): lane l holds rows row0 + 32 i + (l & 31) of the
+// matrix, and k runs over its columns; else (layout 1) lane l holds columns, k runs over the rows. A wave looks its part of the table over
+// while its first tiles travel; nothing but zeros (the rule) costs no more than that. Else every lane's fragments are brought to the largest of the
+// exponents that it will meet (2^(e - largest): exact down to subnormal numbers), whose power the sums get at the end.
+template <int N, bool BY_ROW>
+struct Powers {
+    static constexpr int RG = 8, CG = 32, PER = 32 / RG;
+    const int8_t* at;
+    int stride, groups, blocks, first, half, width;                       // bytes per column block, those in use; column blocks; the wave's first row (column)
+    int e[N];
+    bool any, uneven;
+    // rows x cols: the matrix. half_: columns of its first half (dG | dU), whose column blocks are counted apart, or cols
+    __device__ __forceinline__ void init(const int8_t* table, int rows, int cols, int first_, int half_) {
+        at = table;
+        any = uneven = false;
+        if (!at) return;
+        stride = (rows + 31) / 32 * PER;
+        groups = (rows + RG - 1) / RG;
+        first = first_;
+        half = half_;
+        width = cols;
+        blocks = (half + CG - 1) / CG * (cols > half ? 2 : 1);
+    }
+    __device__ __forceinline__ int block_of(int c) const {
+        c = min(c, width - 1);
+        return c < half ? c / CG : (half + CG - 1) / CG + (c - half) / CG;
+    }
+    __device__ __forceinline__ int exp_at(int block, int group) const { return block < blocks && group < groups ? at[(int64_t)block * stride + group] : EXP_NONE; }
+    // BY_ROW: the column block of k-step ks of tile t (a half's last tile may be part full: zeros, whatever their exponent)
+    __device__ __forceinline__ int block_of_k(int t, int ks) const {
+        const int kts = (half + BK - 1) / BK, seg = t >= kts, b = 2 * (t - seg * kts) + (ks >> 1), per = (half + CG - 1) / CG;
+        return seg * per + min(b, per - 1);
+    }
+    // tiles t0 .. t1 of 64 k
+    __device__ __forceinline__ void look(int t0, int t1, int lane) {
+        if (!at) return;
+        uint32_t bits = 0;
+        const int c0 = BY_ROW ? block_of_k(t0, 0) : block_of(first), c9 = 1 + (BY_ROW ? block_of_k(t1 - 1, KS - 1) : block_of(first + 32 * N - 1));
+        const int r0 = BY_ROW ? first / 32 : t0 * 2, r9 = min(stride / PER, BY_ROW ? first / 32 + N : t1 * 2);
+        const auto take = [&](int c, int r) { bits |= *reinterpret_cast<const uint32_t*>(at + (int64_t)c * stride + r * PER); };
+        if constexpr (BY_ROW) {
+            for (int c = c0 + lane; c < c9; c += 64)
+                for (int r = r0; r < r9; ++r) take(c, r);
+        } else {
+            for (int c = c0; c < c9; ++c)
+                for (int r = r0 + lane; r < r9; r += 64) take(c, r);
+        }
+        any = __any((bits & 0x7f7f7f7fu) != 0);
+        if (!any) return;
+        bool differ = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int mine = first + 32 * i + (lane & 31);
+            const int n0 = BY_ROW ? c0 : r0 * PER, n9 = BY_ROW ? c9 : r9 * PER;
+            int hi = EXP_NONE, lo = 127;
+            for (int n = n0; n < n9; ++n) {
+                const int x = BY_ROW ? exp_at(n, mine / RG) : exp_at(block_of(mine), n);
+                if (x != EXP_NONE) { hi = max(hi, x); lo = min(lo, x); }
+            }
+            e[i] = hi == EXP_NONE ? 0 : hi;
+            differ |= hi != EXP_NONE && lo < hi;
+        }
+        uneven = __any(differ);
+    }
+    static __device__ __forceinline__ uint32_t times(uint32_t w, uint32_t f) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, w) * __builtin_bit_cast(f16x2_t, f)); }
+    // fragment i of k-step ks of tile t, brought to the lane's common exponent (8 rows or 16 features of one group)
+    __device__ __forceinline__ uint4 level(uint4 f, int i, int t, int ks, int lane) const {
+        const int mine = first + 32 * i + (lane & 31);
+        const int x = BY_ROW ? exp_at(block_of_k(t, ks), mine / RG) : exp_at(block_of(mine), t * (BK / RG) + 2 * ks + (lane >> 5));
+        const int d = max(x - e[i], -24);                                 // (fp16's smallest power of two: an infinity stays one)
+        const uint32_t h = d >= -14 ? (uint32_t)(15 + d) << 10 : 1u << (24 + d), hh = h | h << 16;
+        return make_uint4(times(f.x, hh), times(f.y, hh), times(f.z, hh), times(f.w, hh));
     }
 };
 
@@ -193,7 +324,37 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
         if (i < IN) fb[ks & 1][i] = op_frag<LB, BN>(at + ABYTES, wn * WN + 32 * i, ks, lane);
         else fa[ks & 1][i - IN] = op_frag<LA, BM>(at, wm * WM + 32 * (i - IN), ks, lane);
     };
-    constexpr int KS = BK / 16, SLOTS = IM * IN, FETCH = IM + IN;
+    // fp16 operands with powers of two: A's rows (down, dx), A's columns (dW gate, up) or B's (dW down)
+    constexpr bool POWERS = F16 && EPI == EPI_OUT;
+    Powers<IM, LA == 0> pa;
+    Powers<IN, false> pb;
+    if constexpr (POWERS) {
+        if constexpr (LA == 0) pa.init(p.xa, p.M, p.K * p.nseg, m0 + wm * WM, p.K);
+        else pa.init(p.xa, p.K, p.M, m0 + wm * WM, p.F);
+        pb.init(LA == 1 ? p.xb : nullptr, p.K, p.N, n0 + wn * WN, p.N);
+    }
+    auto look = [&] {
+        if constexpr (POWERS) {
+            pa.look(t0, t1, lane);
+            if constexpr (LA == 1) pb.look(t0, t1, lane);
+        }
+    };
+    auto uneven = [&] { return pa.uneven || (LA == 1 && pb.uneven); };
+    // (the loop over the tiles exists twice, with and without this: its waits and meetings are the same, so a wave chooses for itself)
+    auto level = [&](auto on, uint4 (&a)[IM], uint4 (&b)[IN], int t, int ks) {
+        if constexpr (decltype(on)::value) {
+            if (pa.uneven) {
+#pragma unroll
+                for (int i = 0; i < IM; ++i) a[i] = pa.level(a[i], i, t, ks, lane);
+            }
+            if constexpr (LA == 1)
+                if (pb.uneven) {
+#pragma unroll
+                    for (int j = 0; j < IN; ++j) b[j] = pb.level(b[j], j, t, ks, lane);
+                }
+        }
+    };
+    constexpr int SLOTS = IM * IN, FETCH = IM + IN;
     static_assert(KS % 2 == 0, "k-step 0 of the next tile takes the other half of the fragment registers");
     if constexpr (NWK > 1) {
         // few rows: the waves share out the k-steps of a tile (their sums meet below), so a tile costs a wave its share of the requests, one
@@ -206,6 +367,8 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
 #pragma unroll
                 for (int j = 0; j < PIECES; ++j) piece(j);
             }
+        look();
+        const auto walk = [&](auto leveled) {
         int buf = 0, free = NBUF - 1;
         for (int t = t0; t < t1; ++t) {
             wait_landed<(NBUF - 2) * PIECES>(t + NBUF - 1 <= t1);
@@ -223,6 +386,7 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
                 for (int j = 0; j < IN; ++j) fb[0][j] = op_frag<LB, BN>(at + ABYTES, 32 * j, ks, lane);
 #pragma unroll
                 for (int i = 0; i < IM; ++i) fa[0][i] = op_frag<LA, BM>(at, 32 * i, ks, lane);
+                level(leveled, fa[0], fb[0], t, ks);
 #pragma unroll
                 for (int j = 0; j < IN; ++j)
 #pragma unroll
@@ -231,6 +395,9 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
             free = buf;
             buf = buf + 1 == NBUF ? 0 : buf + 1;
         }
+        };
+        if (POWERS && uneven()) walk(std::bool_constant<POWERS>());
+        else walk(std::false_type());
     } else {
     static_assert((NBUF - 2) * PIECES < 64, "vmcnt counts to 63");
     if (t0 < t1) {
@@ -241,11 +408,13 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
 #pragma unroll
                 for (int j = 0; j < PIECES; ++j) piece(j);
             }
+        look();
         wait_landed<(NBUF - 1) * PIECES>(t0 + NBUF <= t1);
         meet();
 #pragma unroll
         for (int i = 0; i < FETCH; ++i) fetch(0, 0, i);
     }
+    const auto walk = [&](auto leveled) {
     int buf = 0;
     for (int t = t0; t < t1; ++t) {
         const int nbuf = buf + 1 == NBUF ? 0 : buf + 1;
@@ -259,6 +428,7 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
                 }
                 if (more) aim(t + NBUF, buf);
             }
+            level(leveled, fa[ks & 1], fb[ks & 1], t, ks);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int s = 0; s < SLOTS; ++s) {
@@ -277,6 +447,22 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
         }
         buf = nbuf;
     }
+    };
+    if (POWERS && uneven()) walk(std::bool_constant<POWERS>());
+    else walk(std::false_type());
+    }
+
+    if constexpr (POWERS) {
+        if (pa.any || (LA == 1 && pb.any)) {
+#pragma unroll
+            for (int i = 0; i < IM; ++i)
+#pragma unroll
+                for (int j = 0; j < IN; ++j) {                            // (32 columns of B are one column block: e[j] is the wave's)
+                    const float f = __builtin_ldexpf(1.0f, (pa.any ? pa.e[i] : 0) + (LA == 1 && pb.any ? pb.e[j] : 0));
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) acc[i][j][k] *= f;
+                }
+        }
     }
 
     // The accumulators hold 32 rows m a lane column each; memory wants whole rows. Each wave turns its 32 x WN blocks round in its own corner of
@@ -286,14 +472,19 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
     wait_all_and_meet();
     float* corner = reinterpret_cast<float*>(conv_lds_dyn) + wave * 32 * RS;
     const int cl = lane % LN, rl = lane / LN;
-#pragma unroll
+    // (one copy of what follows: unrolled over the blocks it does not fit the instruction cache)
+#pragma unroll 1
     for (int i = 0; i < IM; ++i) {
 #pragma unroll
-        for (int j = 0; j < IN; ++j)
+        for (int k = 0; k < IM; ++k) {
+            if (k != i) continue;
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                *reinterpret_cast<float4*>(corner + (lane & 31) * RS + 32 * j + 8 * q + 4 * h) =
-                    make_float4(acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]);
+            for (int j = 0; j < IN; ++j)
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *reinterpret_cast<float4*>(corner + (lane & 31) * RS + 32 * j + 8 * q + 4 * h) =
+                        make_float4(acc[k][j][4 * q], acc[k][j][4 * q + 1], acc[k][j][4 * q + 2], acc[k][j][4 * q + 3]);
+        }
         // NWK waves hold parts of the same sums: each adds up 32 / NWK rows over the corners, in wave order, and goes on with those
         constexpr int RN = 32 / NWK;
         const int R0 = wk * RN;
@@ -335,21 +526,57 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
                     bu[0] = T16<F16>::lo(w.x); bu[1] = T16<F16>::hi(w.x); bu[2] = T16<F16>::lo(w.y); bu[3] = T16<F16>::hi(w.y);
                 }
             }
+            // fp16: a wave's step is a group of 8 rows x 32 features
+            static_assert(!F16 || (SF == 8 && WN == 64), "8 rows x 32 features");
+            GroupCheck<false> check;
+            const bool live = (n0 + wn * WN) / 2 < p.F;
+            const auto hidden = [&](int r, float (&g)[4], float (&u)[4], float (&o)[4]) {
+                const float4 g4 = *reinterpret_cast<const float4*>(rows + (r + r2) * RS + gc), u4 = *reinterpret_cast<const float4*>(rows + (r + r2) * RS + gc + 32);
+                const bool in = mb + r + r2 < p.M && f < p.F;
+                g[0] = g4.x + bg[0]; g[1] = g4.y + bg[1]; g[2] = g4.z + bg[2]; g[3] = g4.w + bg[3];
+                u[0] = u4.x + bu[0]; u[1] = u4.y + bu[1]; u[2] = u4.z + bu[2]; u[3] = u4.w + bu[3];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = F16 && !in ? 0.f : act_of(p.act, g[e]) * u[e];
+                return in;
+            };
+            const auto put = [&](int r, const float (&o)[4], float by) {
+                *reinterpret_cast<uint2*>(p.C + (int64_t)(mb + r + r2) * p.F + f) = make_uint2(T16<F16>::pack2(o[0] * by, o[1] * by), T16<F16>::pack2(o[2] * by, o[3] * by));
+            };
 #pragma unroll
             for (int r = R0; r < R0 + RN; r += SF) {
-                const float4 g4 = *reinterpret_cast<const float4*>(rows + (r + r2) * RS + gc), u4 = *reinterpret_cast<const float4*>(rows + (r + r2) * RS + gc + 32);
-                const int m = mb + r + r2;
-                if (m >= p.M || f >= p.F) continue;
-                const float g[4] = {g4.x + bg[0], g4.y + bg[1], g4.z + bg[2], g4.w + bg[3]}, u[4] = {u4.x + bu[0], u4.y + bu[1], u4.z + bu[2], u4.w + bu[3]};
-                const int64_t at = (int64_t)m * p.F + f;
+                float g[4], u[4], o[4];
+                const bool in = hidden(r, g, u, o);
+                if constexpr (F16) {
+                    check.add(o, true);
+                    check.close(ALL_LANES, live && mb + r < p.M);
+                }
+                if (!in) continue;
                 if (p.g) {
+                    const int64_t at = (int64_t)(mb + r + r2) * p.F + f;
                     *reinterpret_cast<float4*>(p.g + at) = make_float4(g[0], g[1], g[2], g[3]);
                     *reinterpret_cast<float4*>(p.u + at) = make_float4(u[0], u[1], u[2], u[3]);
                 }
-                float o[4];
+                put(r, o, 1.0f);
+            }
+            if constexpr (F16) {
+                int8_t* ex = p.ex + (int64_t)(f / 32) * ((p.M + 31) / 32 * 4) + (mb + R0) / 8;
+                const bool first = lane == 0 && live && mb < p.M;
+                const int plain = check.zero() ? EXP_NONE : 0;
+                if (!check.odd()) {
+                    if (first) store_exps<RN / SF>(ex, plain);
+                } else {
+#pragma unroll 1
+                    for (int r = R0; r < R0 + RN; r += SF) {
+                        float g[4], u[4], o[4];
+                        const bool in = hidden(r, g, u, o);
+                        float mx = finite_max(o);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[e] = act_of(p.act, g[e]) * u[e];
-                *reinterpret_cast<uint2*>(p.C + at) = make_uint2(T16<F16>::pack2(o[0], o[1]), T16<F16>::pack2(o[2], o[3]));
+                        for (int k = 1; k < 64; k <<= 1) mx = fmaxf(mx, __shfl_xor(mx, k));
+                        const int x = exp_of(mx);
+                        if (in) put(r, o, stored_by(x));
+                        if (first) ex[(r - R0) / SF] = (int8_t)x;
+                    }
+                }
             }
         } else {
             const int n = n0 + wn * WN + 4 * cl;
@@ -359,35 +586,87 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
                     const uint2 w = *reinterpret_cast<const uint2*>(p.bias + n);
                     bias[0] = T16<F16>::lo(w.x); bias[1] = T16<F16>::hi(w.x); bias[2] = T16<F16>::lo(w.y); bias[3] = T16<F16>::hi(w.y);
                 }
+            // DH, fp16: two steps of a wave are two groups of 8 rows x 32 features, side by side
+            static_assert(!(F16 && EPI == EPI_DH) || (STEP == 4 && WN == 64 && RN % 8 == 0), "8 rows x 64 features");
+            GroupCheck<true> ch;                                              // (h: what GATE has scaled has to be found again)
+            const bool live = n0 + wn * WN < p.N, live2 = n0 + wn * WN + 32 < p.N;
+            const auto in_range = [&](int r) { return mb + r + rl < p.M && n < p.N; };
+            const auto grads = [&](int r, float (&dg)[4], float (&du)[4], float (&hh)[4]) {         // (outside: all 0)
+                const float4 o = *reinterpret_cast<const float4*>(rows + (r + rl) * RS + 4 * cl);
+                const int64_t at = (int64_t)(mb + r + rl) * p.F + n;
+                float4 g4 = make_float4(0.f, 0.f, 0.f, 0.f), u4 = g4;
+                if (in_range(r)) {
+                    g4 = *reinterpret_cast<const float4*>(p.g + at);
+                    u4 = *reinterpret_cast<const float4*>(p.u + at);
+                }
+                const float g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w}, d[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float f, s;
+                    act_and_slope(p.act, g[e], f, s);
+                    dg[e] = d[e] * u[e] * s;
+                    du[e] = d[e] * f;
+                    hh[e] = f * u[e];
+                }
+            };
+            const auto put_h = [&](int r, const float (&hh)[4], float by) {
+                *reinterpret_cast<uint2*>(p.h + (int64_t)(mb + r + rl) * p.F + n) =
+                    make_uint2(T16<F16>::pack2(hh[0] * by, hh[1] * by), T16<F16>::pack2(hh[2] * by, hh[3] * by));
+            };
 #pragma unroll
             for (int r = R0; r < R0 + RN; r += STEP) {
-                const float4 o = *reinterpret_cast<const float4*>(rows + (r + rl) * RS + 4 * cl);
                 const int m = mb + r + rl;
-                if (m >= p.M || n >= p.N) continue;
                 if constexpr (EPI == EPI_DH) {
-                    const int64_t at = (int64_t)m * p.F + n;
-                    const float4 g4 = *reinterpret_cast<const float4*>(p.g + at), u4 = *reinterpret_cast<const float4*>(p.u + at);
-                    const float g[4] = {g4.x, g4.y, g4.z, g4.w}, u[4] = {u4.x, u4.y, u4.z, u4.w}, d[4] = {o.x, o.y, o.z, o.w};
-                    float dg[4], du[4];
+                    if (!F16 && !in_range(r)) continue;
+                    float dg[4], du[4], hh[4];
+                    grads(r, dg, du, hh);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float f, s;
-                        act_and_slope(p.act, g[e], f, s);
-                        dg[e] = d[e] * u[e] * s;
-                        du[e] = d[e] * f;
                         sg[e] += dg[e];
                         su[e] += du[e];
+                    }
+                    if constexpr (F16) {
+                        ch.add(hh, (r - R0) % 8 == 0);
+                        if ((r - R0) % 8 != 0) {
+                            ch.close(LOW_COLUMNS, live && mb + r - 4 < p.M);
+                            ch.close(~LOW_COLUMNS, live2 && mb + r - 4 < p.M);
+                        }
+                        if (!in_range(r)) continue;
                     }
                     uint16_t* c = p.C + (int64_t)m * p.ldc + n;
                     *reinterpret_cast<uint2*>(c) = make_uint2(T16<F16>::pack2(dg[0], dg[1]), T16<F16>::pack2(dg[2], dg[3]));
                     *reinterpret_cast<uint2*>(c + p.F) = make_uint2(T16<F16>::pack2(du[0], du[1]), T16<F16>::pack2(du[2], du[3]));
-                } else if (p.splits > 1) {
-                    *reinterpret_cast<float4*>(p.part + ((int64_t)split * p.M + m) * p.N + n) = o;
-                } else if (EPI == EPI_OUT && tail) {
-                    *reinterpret_cast<float4*>(p.part + ((int64_t)((item - p.full) * p.tail_splits + split) * BM + m - m0) * BN + n - n0) = o;
                 } else {
-                    *reinterpret_cast<uint2*>(p.C + (int64_t)m * p.ldc + n) =
-                        make_uint2(T16<F16>::pack2(o.x + bias[0], o.y + bias[1]), T16<F16>::pack2(o.z + bias[2], o.w + bias[3]));
+                    if (!in_range(r)) continue;
+                    const float4 o = *reinterpret_cast<const float4*>(rows + (r + rl) * RS + 4 * cl);
+                    if (p.splits > 1) {
+                        *reinterpret_cast<float4*>(p.part + ((int64_t)split * p.M + m) * p.N + n) = o;
+                    } else if (EPI == EPI_OUT && tail) {
+                        *reinterpret_cast<float4*>(p.part + ((int64_t)((item - p.full) * p.tail_splits + split) * BM + m - m0) * BN + n - n0) = o;
+                    } else {
+                        *reinterpret_cast<uint2*>(p.C + (int64_t)m * p.ldc + n) =
+                            make_uint2(T16<F16>::pack2(o.x + bias[0], o.y + bias[1]), T16<F16>::pack2(o.z + bias[2], o.w + bias[3]));
+                    }
+                }
+            }
+            if constexpr (F16 && EPI == EPI_DH) {
+                const int64_t ex = (int64_t)(n / 32) * ((p.M + 31) / 32 * 4) + (mb + R0) / 8;
+                const bool first = (lane & ~8) == 0 && n < p.N && mb < p.M;
+                const int plain = ch.zero() ? EXP_NONE : 0;
+                if (!ch.odd()) {
+                    if (first) store_exps<RN / 8>(p.ex_h + ex, plain);
+                } else {
+#pragma unroll 1
+                    for (int r = R0; r < R0 + RN; r += 8) {
+                        float dg[4], du[4], hh[2][4];
+                        grads(r, dg, du, hh[0]);
+                        grads(r + 4, dg, du, hh[1]);
+                        const int x = exp_of(half_max(finite_max(hh[1], finite_max(hh[0]))));
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            if (in_range(r + 4 * k)) put_h(r + 4 * k, hh[k], stored_by(x));
+                        if (first) p.ex_h[ex + (r - R0) / 8] = (int8_t)x;
+                    }
                 }
             }
         }
@@ -713,6 +992,10 @@ int token(const MmArgs& p, float* h, hipStream_t st) {
 // Where the partial sums of the backward pass's three products lie. Together, one launch adds them all up (us of the pass, a launch each and
 // together: 600 rows, 512 x 2048: 74, 63; 1030, 640 x 2560: 91, 84) -- as long as they and what else passes between the launches (14 bytes for
 // each value of h) stay well inside the 256 MB last-level cache: at 4111 rows, 237 MB, dh takes 52 for 44 us and the shared launch gains 3.
+// bytes of the exponents of [rows, cols] values (Powers)
+size_t exp_bytes(int rows, int cols) { return ((size_t)cdiv(cols, 32) * cdiv(rows, 32) * 4 + 255) / 256 * 256; }
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+
 struct BwdParts {
     size_t at[3] = {}, bytes = 0;
     bool together = false;
@@ -729,16 +1012,21 @@ int fwd(const FfnArgs& a, unsigned char* ws, hipStream_t st) {
     uint16_t* h = a.h;
     if (!h && a.M > TOKENS) {
         h = reinterpret_cast<uint16_t*>(ws);
-        ws += ((size_t)a.M * a.F * 2 + 255) / 256 * 256;
+        ws += up256((size_t)a.M * a.F * 2);
+    }
+    int8_t* ex = nullptr;
+    if (F16 && a.M > TOKENS) {
+        ex = reinterpret_cast<int8_t*>(ws);
+        ws += exp_bytes(a.M, a.F);
     }
     MmArgs g{};
     g.A = a.x; g.B = a.wg; g.B2 = a.wu; g.lda = a.x_s; g.ldb = a.D;
     g.M = a.M; g.N = 64 * cdiv(a.F, 32); g.K = a.D; g.F = a.F; g.nseg = 1; g.splits = 1;
-    g.bias = a.bg; g.bias2 = a.bu; g.C = h; g.g = a.g; g.u = a.u; g.act = a.act;
+    g.bias = a.bg; g.bias2 = a.bu; g.C = h; g.g = a.g; g.u = a.u; g.act = a.act; g.ex = ex;
     MmArgs d{};
     d.A = h; d.B = a.wd; d.lda = a.F; d.ldb = a.F;
     d.M = a.M; d.N = a.D; d.K = a.F; d.nseg = 1; d.splits = 1;
-    d.bias = a.bd; d.C = a.y; d.ldc = a.D;
+    d.bias = a.bd; d.C = a.y; d.ldc = a.D; d.xa = ex;
     if (a.M <= TOKENS) {
         float* hf = reinterpret_cast<float*>(ws);
         if (a.M == 1) {
@@ -757,12 +1045,20 @@ int fwd(const FfnArgs& a, unsigned char* ws, hipStream_t st) {
 template <bool F16>
 int bwd(const FfnArgs& a, unsigned char* ws, hipStream_t st) {
     uint16_t* dgu = reinterpret_cast<uint16_t*>(ws);
-    unsigned char* rest = ws + ((size_t)a.M * 2 * a.F * 2 + 255) / 256 * 256;
+    unsigned char* rest = ws + up256((size_t)a.M * 2 * a.F * 2);
+    // fp16: DH finds the groups of the saved h that carry powers of two, or were cut off at 65504 (one to four rows), from the pre-activations -- with
+    // a margin for its own rounding, so none is missed --, and puts its own value in their place. The table is not saved: the next call finds the same.
+    int8_t* ex_h = nullptr;
+    if (F16) {
+        ex_h = reinterpret_cast<int8_t*>(rest);
+        rest += exp_bytes(a.M, a.F);
+    }
     float* part = reinterpret_cast<float*>(rest);
     MmArgs p{};
     // dG, dU from dh = dy Wd
     p.A = a.dy; p.B = a.wd; p.lda = a.dy_s; p.ldb = a.F; p.M = a.M; p.N = a.F; p.K = a.D; p.nseg = 1; p.splits = 1;
     p.g = a.g; p.u = a.u; p.F = a.F; p.act = a.act; p.C = dgu; p.ldc = 2 * (int64_t)a.F;
+    p.h = a.h; p.ex_h = ex_h;
     // (the bias gradients' partial sums use the place of the products' partial results before those need it)
     const int parts = cdiv(a.M, 32);
     float* down = part + (a.dbg ? (int64_t)parts * 2 * a.F : 0);
@@ -793,23 +1089,23 @@ int bwd(const FfnArgs& a, unsigned char* ws, hipStream_t st) {
     if (!parts_at.together) ISB_TRY(add_up<F16>(s, st));
     // dWd = dy^T h
     p = MmArgs{};
-    p.A = a.dy; p.B = a.h; p.lda = a.dy_s; p.ldb = a.F; p.M = a.D; p.N = a.F; p.K = a.M; p.nseg = 1;
+    p.A = a.dy; p.B = a.h; p.xb = ex_h; p.lda = a.dy_s; p.ldb = a.F; p.M = a.D; p.N = a.F; p.K = a.M; p.nseg = 1;
     p.C = a.dwd; p.ldc = a.F;
     ISB_TRY((mm_out<F16, 1, 1>(p, rest + parts_at.at[2], s.of[2], "ffn dW down", st)));
     return add_up<F16>(s, st);
 }
 }  // namespace
 
-size_t ffn_workspace(const FfnArgs& a, bool backward) {
+size_t ffn_workspace(const FfnArgs& a, bool f16, bool backward) {
     const size_t M = a.M, F = a.F;
     if (!backward) {
         if (a.M <= TOKENS) return M * F * 4;
-        const size_t h = a.h ? 0 : (M * F * 2 + 255) / 256 * 256;
-        return h + part_bytes(0, a.M, a.D, cdiv(a.F, BK));
+        const size_t h = a.h ? 0 : up256(M * F * 2);
+        return h + (f16 ? exp_bytes(a.M, a.F) : 0) + part_bytes(0, a.M, a.D, cdiv(a.F, BK));
     }
     const size_t sums = (size_t)cdiv(a.M, 32) * ((a.dbg ? 2 * F : 0) + (a.dbd ? a.D : 0)) * 4;
     const size_t part = std::max(sums, BwdParts(a).bytes);
-    return (M * 2 * F * 2 + 255) / 256 * 256 + part;
+    return up256(M * 2 * F * 2) + (f16 ? exp_bytes(a.M, a.F) : 0) + part;
 }
 int launch_ffn_fwd(const FfnArgs& a, bool f16, unsigned char* ws, hipStream_t st) { return f16 ? fwd<true>(a, ws, st) : fwd<false>(a, ws, st); }
 int launch_ffn_bwd(const FfnArgs& a, bool f16, unsigned char* ws, hipStream_t st) { return f16 ? bwd<true>(a, ws, st) : bwd<false>(a, ws, st); }

@@ -1,0 +1,121 @@
+"""GPU tests of the layer operators (isbfsar_amd/blocks.py) where a value's size is what matters: intermediates past fp16's range or below
+its normal numbers while the results lie inside, activations far out on their tails, weights far below a row's largest.
+
+Bounds, beside those of blocks_ref: u is half a step of the type, e = 2^-24. What the feed-forward block keeps in fp16 between its products (h,
+dG, dU) carries a power of two per group of rows and features, chosen from the group's largest magnitude m: none while 2^-10 <= m <= 65504, up
+by 2^16, 2^32, ... below, down by just enough above. A value is then off by u of itself or by half an fp16 step of 2^-24 times the power, and a
+product brings the groups that it adds up to the largest of their powers. With m the largest magnitude of what is added up that half step is at
+most 2^-25 (m in between), 2^-25 2^10 m (below) or 2^-25 2^-14 m (above); it is counted twice, for the store and for the common power."""
+import math
+
+import pytest
+import torch
+
+import blocks_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16, F32 = torch.bfloat16, torch.float16, torch.float32
+E = 2.0 ** -24
+
+
+def blocks():
+    from isbfsar_amd import blocks as b
+    return b
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def normal(g, *shape, type=F32, std=1.0):
+    return torch.empty(shape, device="cuda", dtype=F32).normal_(0, std, generator=g).to(type)
+
+
+def held(got, want, bound, name):
+    assert got.shape == want.shape, (name, got.shape, want.shape)
+    off = (got.double() - want).abs() - bound
+    assert not off.isnan().any() and bool((off <= 0).all()), (name, float(off.nan_to_num(math.inf).max()), float((got.double() - want).abs().max()),
+                                                              float(((got.double() - want).abs() / bound).max()))
+
+
+# ------------------------------------------------------------------------------------------------ gated feed-forward block, fp16
+def step16(m):
+    """twice half a step of fp16 values whose power of two follows the magnitude m (see above)"""
+    return 2 * torch.where(m < 2.0 ** -10, 2.0 ** -15 * m, torch.where(m <= 65504, 2.0 ** -25, 2.0 ** -39 * m))
+
+
+def groups(x, rows, cols):
+    """the largest magnitude of each group of `rows` x `cols` (0: all of them), for every element"""
+    M, N = x.shape
+    r, c = rows or M, cols or N
+    pad = torch.nn.functional.pad(x.abs(), (0, -N % c, 0, -M % r))
+    m = pad.view(pad.shape[0] // r, r, pad.shape[1] // c, c).amax((1, 3))
+    return m.repeat_interleave(r, 0).repeat_interleave(c, 1)[:M, :N]
+
+
+def ffn16(x, wg, wu, wd, act, dy=None):
+    """{name: (value, bound)} in fp16 with f32 sums: blocks_ref.ffn with the half steps of step16"""
+    u = 2.0 ** -11
+    M, D = x.shape
+    F = wg.shape[0]
+    X, G, U, W = (a.double() for a in (x, wg, wu, wd))
+    g, v = X @ G.T, X @ U.T
+    eg, ev = ((X.abs() @ w.abs().T) * (D + 4) * E for w in (G, U))
+    a, da = ref.act(act, g)
+    ea, eda = 1.2 * eg + 16 * E * (1 + g.abs()), eg + 16 * E * (1 + g.abs())
+    if act == "relu":
+        eda = torch.where(g.abs() <= eg, 1.0, 0.0)
+    h = a * v
+    eh = h.abs() * (u + 2 * E) + (ea * v.abs() + (a.abs() + ea) * ev) * (1 + u)
+    e_row = eh + (step16(groups(h, 8, 0)) if M > 4 else 0)                        # one to four rows keep h in f32
+    y = h @ W.T
+    out = lambda val, err: (val, u * val.abs() + err * (1 + u) + 2.0 ** -25)      # noqa: E731
+    r = {"y": out(y, e_row @ W.abs().T + (F + 8) * E * (h.abs() @ W.abs().T))}
+    if dy is None:
+        return r
+    Y = dy.double()
+    dh, edh = Y @ W, (Y.abs() @ W.abs()) * (D + 4) * E
+    dg, dv = dh * v * da, dh * a
+    edg = dg.abs() * (u + 4 * E) + (edh * v.abs() * da.abs() + dh.abs() * (ev * da.abs() + (v.abs() + ev) * eda)) * (1 + u)
+    edv = dv.abs() * (u + 4 * E) + (edh * a.abs() + (dh.abs() + edh) * ea) * (1 + u)
+    both = step16(torch.maximum(groups(dg, 4, 0), groups(dv, 4, 0)))
+    n = M + 8
+    r["dx"] = out(dg @ G + dv @ U, (edg + both) @ G.abs() + (edv + both) @ U.abs() + (2 * F + 8) * E * (dg.abs() @ G.abs() + dv.abs() @ U.abs()))
+    for name, d, ed in (("dw_gate", dg, edg), ("dw_up", dv, edv)):
+        r[name] = out(d.T @ X, (ed + step16(groups(d, 0, 64))).T @ X.abs() + n * E * (d.abs().T @ X.abs()))
+    r["dw_down"] = out(Y.T @ h, Y.abs().T @ (eh + step16(groups(h, 0, 64))) + n * E * (Y.abs().T @ h.abs()))
+    return r
+
+
+def check_ffn16(x, wg, wu, wd, act, dy, names=("y", "dx", "dw_gate", "dw_up", "dw_down")):
+    y, saved = blocks().gated_ffn(x, wg, wu, wd, activation=act, save=True)
+    d = {"y": y, **blocks().gated_ffn_backward(dy, x, wg, wu, wd, saved, activation=act)}
+    want = ffn16(x, wg, wu, wd, act, dy)
+    for name in names:
+        assert bool((want[name][0].abs() < 65504).all()), name
+        held(d[name], *want[name], name)
+
+
+@pytest.mark.parametrize("M", [1, 4, 5, 40, 300])
+def test_ffn_hidden_values_past_the_type_s_range(M):
+    """h = 320 x 320 = 102400 does not fit fp16, y = 64 h / 256 = 25600 and dw_down = M h / 1024 = 100 M do, exactly"""
+    x = torch.full((M, 64), 8.0, dtype=FP16, device="cuda")
+    w = torch.full((64, 64), 0.625, dtype=FP16, device="cuda")
+    wd = torch.full((64, 64), 2.0 ** -8, dtype=FP16, device="cuda")
+    y, saved = blocks().gated_ffn(x, w, w, wd, activation="relu", save=True)
+    assert bool((y == 25600).all())
+    d = blocks().gated_ffn_backward(torch.full_like(x, 2.0 ** -10), x, w, w, wd, saved, activation="relu")
+    assert bool((d["dw_down"] == 100 * M).all())
+    assert bool((blocks().gated_ffn(x, w, w, wd, activation="relu") == 25600).all())
+
+
+@pytest.mark.parametrize("M,D,F", [(5, 64, 136), (37, 128, 520), (300, 136, 1032), (1500, 264, 2056)])
+@pytest.mark.parametrize("act", ["relu", "silu", "sigmoid"])
+def test_ffn_rows_of_very_different_size(M, D, F, act):
+    """rows of x from 2^-8 to 2^8: h spans more than fp16, and a row of large hidden values leaves the digits of the rows behind its group alone"""
+    g = gen(M + F)
+    x = (normal(g, M, D) * 2.0 ** torch.randint(-8, 9, ((M + 15) // 16, 1), generator=g, device="cuda").repeat_interleave(16, 0)[:M]).to(FP16)
+    w = [normal(g, F, D, type=FP16, std=4 * D ** -0.5) for _ in range(2)]
+    wd = normal(g, D, F, type=FP16, std=2.0 ** -8 * F ** -0.5)
+    check_ffn16(x, *w, wd, act, normal(g, M, D, type=FP16, std=2.0 ** -10), ("y", "dw_down"))
