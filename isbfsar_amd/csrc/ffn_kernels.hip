@@ -32,7 +32,7 @@ struct MmArgs {
     float *g, *u;                        // GATE: saved (or null); DH: read
     float* part;                         // OUT with splits > 1: [split][M][N]
     float* cs;                           // DH: column sums of dG | dU over 32 rows, [ceil(M / 32)][2 F], or null
-    int8_t* ex;                          // fp16 (Powers): GATE: exponents of h
+    int8_t* ex;                          // fp16 (Powers): exponents of h (GATE), of dG | dU (DH)
     uint16_t* h;                         // fp16, DH: the saved h, for dWd, and its exponents
     int8_t* ex_h;
     const int8_t *xa, *xb;               // fp16, OUT: exponents of A's, B's values, or null
@@ -112,8 +112,8 @@ struct OpLoad {
     }
 };
 
-// ---- fp16 between two products. h = act(g) o u may lie past 65504, or far below fp16's normal numbers, where y does not. So a group of 8 rows x 32
-// features carries a power of two of its own: what is stored is value 2^-e, e = 0 while the group's largest magnitude lies in [2^-10, 65504] -- as
+// ---- fp16 between two products. h = act(g) o u, dG and dU may lie past 65504, or far below fp16's normal numbers, where y, dx and the weights'
+// gradients do not. So a group of 8 rows x 32 features carries a power of two of its own: what is stored is value 2^-e, e = 0 while the group's largest magnitude lies in [2^-10, 65504] -- as
 // good as always --, above just enough to bring it below 2^15, below in steps of 16. Exponents: a byte per group, [ceil(F / 32)][4 ceil(rows / 32)];
 // EXP_NONE: nothing but zeros, infinities and NaN.
 constexpr int EXP_NONE = -128;
@@ -173,7 +173,7 @@ struct Powers {
     static constexpr int RG = 8, CG = 32, PER = 32 / RG;
     const int8_t* at;
     int stride, groups, blocks, first, half, width;                       // bytes per column block, those in use; column blocks; the wave's first row (column)
-    int e[N];
+    int e[N], lane_;
     bool any, uneven;
     // rows x cols: the matrix. half_: columns of its first half (dG | dU), whose column blocks are counted apart, or cols
     __device__ __forceinline__ void init(const int8_t* table, int rows, int cols, int first_, int half_) {
@@ -200,6 +200,7 @@ struct Powers {
     // tiles t0 .. t1 of 64 k
     __device__ __forceinline__ void look(int t0, int t1, int lane) {
         if (!at) return;
+        lane_ = lane;
         uint32_t bits = 0;
         const int c0 = BY_ROW ? block_of_k(t0, 0) : block_of(first), c9 = 1 + (BY_ROW ? block_of_k(t1 - 1, KS - 1) : block_of(first + 32 * N - 1));
         const int r0 = BY_ROW ? first / 32 : t0 * 2, r9 = min(stride / PER, BY_ROW ? first / 32 + N : t1 * 2);
@@ -213,29 +214,74 @@ struct Powers {
         }
         any = __any((bits & 0x7f7f7f7fu) != 0);
         if (!any) return;
+        // the largest and smallest exponent per lane: every lane takes its share of the words, byte k of which (BY_ROW: of row group k) it keeps apart
         bool differ = false;
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < N; ++i) {
-            const int mine = first + 32 * i + (lane & 31);
-            const int n0 = BY_ROW ? c0 : r0 * PER, n9 = BY_ROW ? c9 : r9 * PER;
-            int hi = EXP_NONE, lo = 127;
-            for (int n = n0; n < n9; ++n) {
-                const int x = BY_ROW ? exp_at(n, mine / RG) : exp_at(block_of(mine), n);
-                if (x != EXP_NONE) { hi = max(hi, x); lo = min(lo, x); }
+            const int mine = first + 32 * i + (lane & 31), b0 = BY_ROW ? 0 : block_of(first + 32 * i), b1 = BY_ROW ? 0 : block_of(first + 32 * i + 31);
+            int top = 0;
+#pragma unroll 1
+            for (int b = b0; b <= b1; ++b) {                              // (32 columns lie in at most two blocks)
+                int hi[4], lo[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) { hi[k] = EXP_NONE; lo[k] = 127; }
+                const int r = first / 32 + i;
+                if (!BY_ROW || r < stride / PER) {
+                    for (int n = (BY_ROW ? c0 : r0) + lane; n < (BY_ROW ? c9 : r9); n += 64) {
+                        const uint32_t w = *reinterpret_cast<const uint32_t*>(at + (int64_t)(BY_ROW ? n : b) * stride + (BY_ROW ? r : n) * PER);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int x = (int8_t)(w >> (8 * k));
+                            if (x != EXP_NONE && (BY_ROW ? r : n) * PER + k < groups) { hi[k] = max(hi[k], x); lo[k] = min(lo[k], x); }
+                        }
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+#pragma unroll
+                    for (int o = 1; o < 64; o <<= 1) { hi[k] = max(hi[k], __shfl_xor(hi[k], o)); lo[k] = min(lo[k], __shfl_xor(lo[k], o)); }
+                int h = hi[0], l = lo[0];
+#pragma unroll
+                for (int k = 1; k < 4; ++k) {
+                    if (!BY_ROW) { h = max(h, hi[k]); l = min(l, lo[k]); }
+                    else if ((mine / RG) % PER == k) { h = hi[k]; l = lo[k]; }
+                }
+                if (BY_ROW || block_of(mine) == b) {
+                    top = h == EXP_NONE ? 0 : h;
+                    differ |= h != EXP_NONE && l < h;
+                }
             }
-            e[i] = hi == EXP_NONE ? 0 : hi;
-            differ |= hi != EXP_NONE && lo < hi;
+#pragma unroll
+            for (int k = 0; k < N; ++k) e[k] = k == i ? top : e[k];
         }
         uneven = __any(differ);
     }
+    // the exponents of tile t for a lane's fragment i: a byte per k-step (BY_ROW), or per half a k-step
+    __device__ __forceinline__ uint2 of_tile(int i, int t) const {
+        const int mine = first + 32 * i + (lane_ & 31);
+        if constexpr (BY_ROW) {
+            const int a = exp_at(block_of_k(t, 0), mine / RG) & 0xff, b = exp_at(block_of_k(t, 2), mine / RG) & 0xff;
+            return make_uint2(a * 0x101u | b * 0x1010000u, 0u);
+        } else {
+            const int g = t * (BK / RG);                                  // (past the last row: zeros, whatever their exponent)
+            const uint32_t* w = reinterpret_cast<const uint32_t*>(at + (int64_t)block_of(mine) * stride + g);
+            return make_uint2(g < stride ? w[0] : 0u, g + 4 < stride ? w[1] : 0u);
+        }
+    }
+    // 2^d in both halves of a word, -24 <= d <= 0
+    static __device__ __forceinline__ uint32_t half_power(int d) {
+        const uint32_t h = d >= -14 ? (uint32_t)(15 + d) << 10 : 1u << (24 + d);
+        return h | h << 16;
+    }
     static __device__ __forceinline__ uint32_t times(uint32_t w, uint32_t f) { return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, w) * __builtin_bit_cast(f16x2_t, f)); }
-    // fragment i of k-step ks of tile t, brought to the lane's common exponent (8 rows or 16 features of one group)
-    __device__ __forceinline__ uint4 level(uint4 f, int i, int t, int ks, int lane) const {
-        const int mine = first + 32 * i + (lane & 31);
-        const int x = BY_ROW ? exp_at(block_of_k(t, ks), mine / RG) : exp_at(block_of(mine), t * (BK / RG) + 2 * ks + (lane >> 5));
-        const int d = max(x - e[i], -24);                                 // (fp16's smallest power of two: an infinity stays one)
-        const uint32_t h = d >= -14 ? (uint32_t)(15 + d) << 10 : 1u << (24 + d), hh = h | h << 16;
-        return make_uint4(times(f.x, hh), times(f.y, hh), times(f.z, hh), times(f.w, hh));
+    // fragment i of k-step ks, brought to the lane's common exponent (8 rows or 16 features of one group); x: of_tile
+    __device__ __forceinline__ uint4 level(uint4 f, int i, uint2 x, int ks) const {
+        const uint32_t w = BY_ROW || ks < 2 ? x.x : x.y;
+        const int at_byte = BY_ROW ? ks : 2 * (ks & 1) + (lane_ >> 5);
+        // in two factors: 2^d reaches below fp16's smallest number where the value does not. -48 leaves nothing of a finite one; an infinity stays one
+        const int d = min(max((int)(int8_t)(w >> (8 * at_byte)) - e[i], -48), 0), d0 = d >> 1;
+        const uint32_t h0 = half_power(d0), h1 = half_power(d - d0);
+        return make_uint4(times(times(f.x, h0), h1), times(times(f.y, h0), h1), times(times(f.z, h0), h1), times(times(f.w, h0), h1));
     }
 };
 
@@ -341,16 +387,38 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
     };
     auto uneven = [&] { return pa.uneven || (LA == 1 && pb.uneven); };
     // (the loop over the tiles exists twice, with and without this: its waits and meetings are the same, so a wave chooses for itself)
-    auto level = [&](auto on, uint4 (&a)[IM], uint4 (&b)[IN], int t, int ks) {
+    uint2 xa[IM], xb[IN], xa_next[IM], xb_next[IN];                       // exponents of this tile and of the next one
+    auto exps = [&](auto on, int t, uint2 (&a)[IM], uint2 (&b)[IN]) {
         if constexpr (decltype(on)::value) {
             if (pa.uneven) {
 #pragma unroll
-                for (int i = 0; i < IM; ++i) a[i] = pa.level(a[i], i, t, ks, lane);
+                for (int i = 0; i < IM; ++i) a[i] = pa.of_tile(i, t);
             }
             if constexpr (LA == 1)
                 if (pb.uneven) {
 #pragma unroll
-                    for (int j = 0; j < IN; ++j) b[j] = pb.level(b[j], j, t, ks, lane);
+                    for (int j = 0; j < IN; ++j) b[j] = pb.of_tile(j, t);
+                }
+        }
+    };
+    auto turn = [&](auto on) {
+        if constexpr (decltype(on)::value) {
+#pragma unroll
+            for (int i = 0; i < IM; ++i) xa[i] = xa_next[i];
+#pragma unroll
+            for (int j = 0; j < IN; ++j) xb[j] = xb_next[j];
+        }
+    };
+    auto level = [&](auto on, uint4 (&a)[IM], uint4 (&b)[IN], int ks) {
+        if constexpr (decltype(on)::value) {
+            if (pa.uneven) {
+#pragma unroll
+                for (int i = 0; i < IM; ++i) a[i] = pa.level(a[i], i, xa[i], ks);
+            }
+            if constexpr (LA == 1)
+                if (pb.uneven) {
+#pragma unroll
+                    for (int j = 0; j < IN; ++j) b[j] = pb.level(b[j], j, xb[j], ks);
                 }
         }
     };
@@ -370,7 +438,10 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
         look();
         const auto walk = [&](auto leveled) {
         int buf = 0, free = NBUF - 1;
+        if (t0 < t1) exps(leveled, t0, xa_next, xb_next);
         for (int t = t0; t < t1; ++t) {
+            turn(leveled);
+            if (t + 1 < t1) exps(leveled, t + 1, xa_next, xb_next);
             wait_landed<(NBUF - 2) * PIECES>(t + NBUF - 1 <= t1);
             meet();                                                            // tile t is there, and nobody reads tile t - 1 any more
             if (t + NBUF - 1 < t1) {
@@ -386,7 +457,7 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
                 for (int j = 0; j < IN; ++j) fb[0][j] = op_frag<LB, BN>(at + ABYTES, 32 * j, ks, lane);
 #pragma unroll
                 for (int i = 0; i < IM; ++i) fa[0][i] = op_frag<LA, BM>(at, 32 * i, ks, lane);
-                level(leveled, fa[0], fb[0], t, ks);
+                level(leveled, fa[0], fb[0], ks);
 #pragma unroll
                 for (int j = 0; j < IN; ++j)
 #pragma unroll
@@ -416,8 +487,11 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
     }
     const auto walk = [&](auto leveled) {
     int buf = 0;
+    if (t0 < t1) exps(leveled, t0, xa_next, xb_next);
     for (int t = t0; t < t1; ++t) {
         const int nbuf = buf + 1 == NBUF ? 0 : buf + 1;
+        turn(leveled);
+        if (t + 1 < t1) exps(leveled, t + 1, xa_next, xb_next);
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const bool edge = ks + 1 == KS, more = edge && t + NBUF < t1;
@@ -428,7 +502,7 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
                 }
                 if (more) aim(t + NBUF, buf);
             }
-            level(leveled, fa[ks & 1], fb[ks & 1], t, ks);
+            level(leveled, fa[ks & 1], fb[ks & 1], ks);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int s = 0; s < SLOTS; ++s) {
@@ -473,6 +547,7 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
     float* corner = reinterpret_cast<float*>(conv_lds_dyn) + wave * 32 * RS;
     const int cl = lane % LN, rl = lane / LN;
     // (one copy of what follows: unrolled over the blocks it does not fit the instruction cache)
+    int guess_g = 0, guess_u = 0;                                          // DH, fp16: the exponents that the next block's dG and dU are stored with first
 #pragma unroll 1
     for (int i = 0; i < IM; ++i) {
 #pragma unroll
@@ -588,6 +663,10 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
                 }
             // DH, fp16: two steps of a wave are two groups of 8 rows x 32 features, side by side
             static_assert(!(F16 && EPI == EPI_DH) || (STEP == 4 && WN == 64 && RN % 8 == 0), "8 rows x 64 features");
+            // dG and dU are tried with the exponent (0 or below) of the last group that needed one: small gradients are small all over, and a block is
+            // stored anew only where that changes
+            const float by_g = stored_by(guess_g), by_u = stored_by(guess_u);
+            GroupCheck<false> cg, cu;
             GroupCheck<true> ch;                                              // (h: what GATE has scaled has to be found again)
             const bool live = n0 + wn * WN < p.N, live2 = n0 + wn * WN + 32 < p.N;
             const auto in_range = [&](int r) { return mb + r + rl < p.M && n < p.N; };
@@ -609,12 +688,17 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
                     hh[e] = f * u[e];
                 }
             };
+            const auto put_d = [&](uint16_t* c, int r, const float (&d)[4], float by) {
+                *reinterpret_cast<uint2*>(c + (int64_t)(mb + r + rl) * p.ldc + n) = make_uint2(T16<F16>::pack2(d[0] * by, d[1] * by), T16<F16>::pack2(d[2] * by, d[3] * by));
+            };
             const auto put_h = [&](int r, const float (&hh)[4], float by) {
                 *reinterpret_cast<uint2*>(p.h + (int64_t)(mb + r + rl) * p.F + n) =
                     make_uint2(T16<F16>::pack2(hh[0] * by, hh[1] * by), T16<F16>::pack2(hh[2] * by, hh[3] * by));
             };
+#pragma unroll 1
+            for (int r8 = R0; r8 < R0 + RN; r8 += 8)
 #pragma unroll
-            for (int r = R0; r < R0 + RN; r += STEP) {
+            for (int r = r8; r < r8 + 8; r += STEP) {
                 const int m = mb + r + rl;
                 if constexpr (EPI == EPI_DH) {
                     if (!F16 && !in_range(r)) continue;
@@ -626,16 +710,27 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
                         su[e] += du[e];
                     }
                     if constexpr (F16) {
-                        ch.add(hh, (r - R0) % 8 == 0);
-                        if ((r - R0) % 8 != 0) {
-                            ch.close(LOW_COLUMNS, live && mb + r - 4 < p.M);
-                            ch.close(~LOW_COLUMNS, live2 && mb + r - 4 < p.M);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            dg[e] *= by_g;
+                            du[e] *= by_u;
                         }
+                        cg.add(dg, r == r8);
+                        cu.add(du, r == r8);
+                        ch.add(hh, r == r8);
+                        if (r != r8)
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                const uint64_t lanes = k == 0 ? LOW_COLUMNS : ~LOW_COLUMNS;
+                                const bool in = (k == 0 ? live : live2) && mb + r - 4 < p.M;
+                                cg.close(lanes, in);
+                                cu.close(lanes, in);
+                                ch.close(lanes, in);
+                            }
                         if (!in_range(r)) continue;
                     }
-                    uint16_t* c = p.C + (int64_t)m * p.ldc + n;
-                    *reinterpret_cast<uint2*>(c) = make_uint2(T16<F16>::pack2(dg[0], dg[1]), T16<F16>::pack2(dg[2], dg[3]));
-                    *reinterpret_cast<uint2*>(c + p.F) = make_uint2(T16<F16>::pack2(du[0], du[1]), T16<F16>::pack2(du[2], du[3]));
+                    put_d(p.C, r, dg, 1.0f);
+                    put_d(p.C + p.F, r, du, 1.0f);
                 } else {
                     if (!in_range(r)) continue;
                     const float4 o = *reinterpret_cast<const float4*>(rows + (r + rl) * RS + 4 * cl);
@@ -652,22 +747,39 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
             if constexpr (F16 && EPI == EPI_DH) {
                 const int64_t ex = (int64_t)(n / 32) * ((p.M + 31) / 32 * 4) + (mb + R0) / 8;
                 const bool first = (lane & ~8) == 0 && n < p.N && mb < p.M;
-                const int plain = ch.zero() ? EXP_NONE : 0;
-                if (!ch.odd()) {
-                    if (first) store_exps<RN / 8>(p.ex_h + ex, plain);
-                } else {
+                const int64_t up = (int64_t)((p.F + 31) / 32) * ((p.M + 31) / 32 * 4);         // dU's column blocks follow dG's
+                const bool og = cg.odd(), ou = cu.odd(), oh = ch.odd();
+                const int zg = cg.zero() ? EXP_NONE : guess_g, zu = cu.zero() ? EXP_NONE : guess_u, zh = ch.zero() ? EXP_NONE : 0;
+                if (first) {
+                    if (!og) store_exps<RN / 8>(p.ex + ex, zg);
+                    if (!ou) store_exps<RN / 8>(p.ex + up + ex, zu);
+                    if (!oh) store_exps<RN / 8>(p.ex_h + ex, zh);
+                }
+                // (one of the three at a time: a wave's registers are taken)
+                const auto anew = [&](int8_t* to, auto pick, auto put) {
+                    int last = 0;
 #pragma unroll 1
                     for (int r = R0; r < R0 + RN; r += 8) {
-                        float dg[4], du[4], hh[2][4];
-                        grads(r, dg, du, hh[0]);
-                        grads(r + 4, dg, du, hh[1]);
-                        const int x = exp_of(half_max(finite_max(hh[1], finite_max(hh[0]))));
+                        float v[2][4];
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            float dg[4], du[4], hh[4];
+                            grads(r + 4 * k, dg, du, hh);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[k][e] = pick(dg[e], du[e], hh[e]);
+                        }
+                        const int x = exp_of(half_max(finite_max(v[1], finite_max(v[0]))));
 #pragma unroll
                         for (int k = 0; k < 2; ++k)
-                            if (in_range(r + 4 * k)) put_h(r + 4 * k, hh[k], stored_by(x));
-                        if (first) p.ex_h[ex + (r - R0) / 8] = (int8_t)x;
+                            if (in_range(r + 4 * k)) put(r + 4 * k, v[k], stored_by(x));
+                        if (first) to[ex + (r - R0) / 8] = (int8_t)x;
+                        last = x == EXP_NONE ? last : min(x, 0);
                     }
-                }
+                    return __builtin_amdgcn_readfirstlane(last);
+                };
+                if (og) guess_g = anew(p.ex, [](float a, float, float) { return a; }, [&](int r, const float (&v)[4], float by) { put_d(p.C, r, v, by); });
+                if (ou) guess_u = anew(p.ex + up, [](float, float a, float) { return a; }, [&](int r, const float (&v)[4], float by) { put_d(p.C + p.F, r, v, by); });
+                if (oh) anew(p.ex_h, [](float, float, float a) { return a; }, put_h);
             }
         }
         if constexpr (EPI == EPI_DH) {
@@ -1048,17 +1160,19 @@ int bwd(const FfnArgs& a, unsigned char* ws, hipStream_t st) {
     unsigned char* rest = ws + up256((size_t)a.M * 2 * a.F * 2);
     // fp16: DH finds the groups of the saved h that carry powers of two, or were cut off at 65504 (one to four rows), from the pre-activations -- with
     // a margin for its own rounding, so none is missed --, and puts its own value in their place. The table is not saved: the next call finds the same.
-    int8_t* ex_h = nullptr;
+    int8_t *ex_h = nullptr, *ex_d = nullptr;
     if (F16) {
         ex_h = reinterpret_cast<int8_t*>(rest);
         rest += exp_bytes(a.M, a.F);
+        ex_d = reinterpret_cast<int8_t*>(rest);
+        rest += 2 * exp_bytes(a.M, a.F);
     }
     float* part = reinterpret_cast<float*>(rest);
     MmArgs p{};
     // dG, dU from dh = dy Wd
     p.A = a.dy; p.B = a.wd; p.lda = a.dy_s; p.ldb = a.F; p.M = a.M; p.N = a.F; p.K = a.D; p.nseg = 1; p.splits = 1;
     p.g = a.g; p.u = a.u; p.F = a.F; p.act = a.act; p.C = dgu; p.ldc = 2 * (int64_t)a.F;
-    p.h = a.h; p.ex_h = ex_h;
+    p.h = a.h; p.ex_h = ex_h; p.ex = ex_d;
     // (the bias gradients' partial sums use the place of the products' partial results before those need it)
     const int parts = cdiv(a.M, 32);
     float* down = part + (a.dbg ? (int64_t)parts * 2 * a.F : 0);
@@ -1076,7 +1190,7 @@ int bwd(const FfnArgs& a, unsigned char* ws, hipStream_t st) {
     // dx = dG Wg + dU Wu
     p = MmArgs{};
     p.A = dgu; p.B = a.wg; p.B2 = a.wu; p.lda = 2 * (int64_t)a.F; p.ldb = a.D; p.M = a.M; p.N = a.D; p.K = a.F; p.nseg = 2;
-    p.C = a.dx; p.ldc = a.D;
+    p.C = a.dx; p.ldc = a.D; p.xa = ex_d;
     const BwdParts parts_at(a);
     Sums s{};
     ISB_TRY((mm_out<F16, 0, 1>(p, rest + parts_at.at[0], s.of[0], "ffn dx", st)));
@@ -1084,7 +1198,7 @@ int bwd(const FfnArgs& a, unsigned char* ws, hipStream_t st) {
     // [dWg; dWu] = [dG | dU]^T x
     p = MmArgs{};
     p.A = dgu; p.B = a.x; p.lda = 2 * (int64_t)a.F; p.ldb = a.x_s; p.M = 2 * a.F; p.N = a.D; p.K = a.M; p.nseg = 1;
-    p.C = a.dwgu; p.ldc = a.D;
+    p.C = a.dwgu; p.ldc = a.D; p.xa = ex_d; p.F = a.F;
     ISB_TRY((mm_out<F16, 1, 1>(p, rest + parts_at.at[1], s.of[1], "ffn dW gate, up", st)));
     if (!parts_at.together) ISB_TRY(add_up<F16>(s, st));
     // dWd = dy^T h
@@ -1105,7 +1219,7 @@ size_t ffn_workspace(const FfnArgs& a, bool f16, bool backward) {
     }
     const size_t sums = (size_t)cdiv(a.M, 32) * ((a.dbg ? 2 * F : 0) + (a.dbd ? a.D : 0)) * 4;
     const size_t part = std::max(sums, BwdParts(a).bytes);
-    return up256(M * 2 * F * 2) + (f16 ? exp_bytes(a.M, a.F) : 0) + part;
+    return up256(M * 2 * F * 2) + (f16 ? 3 * exp_bytes(a.M, a.F) : 0) + part;
 }
 int launch_ffn_fwd(const FfnArgs& a, bool f16, unsigned char* ws, hipStream_t st) { return f16 ? fwd<true>(a, ws, st) : fwd<false>(a, ws, st); }
 int launch_ffn_bwd(const FfnArgs& a, bool f16, unsigned char* ws, hipStream_t st) { return f16 ? bwd<true>(a, ws, st) : bwd<false>(a, ws, st); }

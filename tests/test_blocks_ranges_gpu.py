@@ -2,7 +2,7 @@
 its normal numbers while the results lie inside, activations far out on their tails, weights far below a row's largest.
 
 Bounds, beside those of blocks_ref: u is half a step of the type, e = 2^-24. What the feed-forward block keeps in fp16 between its products (h,
-dG, dU) carries a power of two per group of rows and features, chosen from the group's largest magnitude m: none while 2^-10 <= m <= 65504, up
+dG, dU) carries a power of two per group of 8 rows x 32 features, chosen from the group's largest magnitude m: none while 2^-10 <= m <= 65504, up
 by 2^16, 2^32, ... below, down by just enough above. A value is then off by u of itself or by half an fp16 step of 2^-24 times the power, and a
 product brings the groups that it adds up to the largest of their powers. With m the largest magnitude of what is added up that half step is at
 most 2^-25 (m in between), 2^-25 2^10 m (below) or 2^-25 2^-14 m (above); it is counted twice, for the store and for the common power."""
@@ -79,12 +79,12 @@ def ffn16(x, wg, wu, wd, act, dy=None):
     dg, dv = dh * v * da, dh * a
     edg = dg.abs() * (u + 4 * E) + (edh * v.abs() * da.abs() + dh.abs() * (ev * da.abs() + (v.abs() + ev) * eda)) * (1 + u)
     edv = dv.abs() * (u + 4 * E) + (edh * a.abs() + (dh.abs() + edh) * ea) * (1 + u)
-    both = step16(torch.maximum(groups(dg, 4, 0), groups(dv, 4, 0)))
+    both = step16(torch.maximum(groups(dg, 8, 0), groups(dv, 8, 0)))
     n = M + 8
     r["dx"] = out(dg @ G + dv @ U, (edg + both) @ G.abs() + (edv + both) @ U.abs() + (2 * F + 8) * E * (dg.abs() @ G.abs() + dv.abs() @ U.abs()))
     for name, d, ed in (("dw_gate", dg, edg), ("dw_up", dv, edv)):
-        r[name] = out(d.T @ X, (ed + step16(groups(d, 0, 64))).T @ X.abs() + n * E * (d.abs().T @ X.abs()))
-    r["dw_down"] = out(Y.T @ h, Y.abs().T @ (eh + step16(groups(h, 0, 64))) + n * E * (Y.abs().T @ h.abs()))
+        r[name] = out(d.T @ X, (ed + step16(groups(d, 0, 32))).T @ X.abs() + n * E * (d.abs().T @ X.abs()))
+    r["dw_down"] = out(Y.T @ h, Y.abs().T @ (eh + step16(groups(h, 0, 32))) + n * E * (Y.abs().T @ h.abs()))
     return r
 
 
@@ -119,3 +119,63 @@ def test_ffn_rows_of_very_different_size(M, D, F, act):
     w = [normal(g, F, D, type=FP16, std=4 * D ** -0.5) for _ in range(2)]
     wd = normal(g, D, F, type=FP16, std=2.0 ** -8 * F ** -0.5)
     check_ffn16(x, *w, wd, act, normal(g, M, D, type=FP16, std=2.0 ** -10), ("y", "dw_down"))
+
+
+@pytest.mark.parametrize("std", [2.0 ** -8, 2.0 ** -12, 2.0 ** -18, 2.0 ** -22])
+@pytest.mark.parametrize("M,D,F", [(3, 64, 136), (33, 136, 520), (300, 72, 1032), (2101, 264, 1160)])
+def test_ffn_small_gradients_keep_their_digits(M, D, F, std):
+    """dy far below fp16's normal numbers' middle: dG and dU must not lose what dx and the weights' gradients can hold"""
+    g = gen(M)
+    x, dy = normal(g, M, D, type=FP16), normal(g, M, D, std=std).to(FP16)
+    w = [normal(g, F, D, type=FP16, std=D ** -0.5) for _ in range(2)]
+    check_ffn16(x, *w, normal(g, D, F, type=FP16, std=F ** -0.5), "silu", dy)
+
+
+@pytest.mark.parametrize("M,D,F", [(12, 64, 136), (300, 72, 1032), (1030, 264, 520), (2101, 264, 2056)])
+def test_ffn_gradients_of_very_different_size(M, D, F):
+    """rows of dy from 2^-20 to 2^6 in blocks that end inside tiles, features of the up projection from 2^-12 to 2^2: every group of dG and dU has
+    its own power of two"""
+    g = gen(M + 1)
+    x = normal(g, M, D, type=FP16)
+    dy = (normal(g, M, D) * 2.0 ** torch.randint(-20, 7, ((M + 11) // 12, 1), generator=g, device="cuda").repeat_interleave(12, 0)[:M]).to(FP16)
+    dy[:3] = 0
+    wu = normal(g, F, D) * 2.0 ** torch.randint(-12, 3, ((F + 39) // 40, 1), generator=g, device="cuda").repeat_interleave(40, 0)[:F]
+    check_ffn16(x, normal(g, F, D, type=FP16, std=D ** -0.5), (wu * D ** -0.5).to(FP16), normal(g, D, F, type=FP16, std=F ** -0.5), "gelu", dy)
+
+
+@pytest.mark.parametrize("M,D,F", [(3, 64, 136), (40, 64, 264), (300, 136, 520)])
+def test_ffn_gradients_past_the_type_s_range(M, D, F):
+    """dG past 65504, the weights' gradients inside"""
+    g = gen(M + 2)
+    x = normal(g, M, D, type=FP16, std=2.0 ** -9)
+    dy = normal(g, M, D, type=FP16, std=2.0 ** 8)
+    wg, wu = normal(g, F, D, type=FP16, std=2.0 ** -10), normal(g, F, D, type=FP16, std=2.0 ** 8)
+    wd = normal(g, D, F, type=FP16, std=2.0 ** 6)
+    v, dh = x.double() @ wu.double().T, dy.double() @ wd.double()
+    assert float((dh * v / 4).abs().max()) > 65504
+    check_ffn16(x, wg, wu, wd, "sigmoid", dy, ("dw_gate", "dw_up"))
+
+
+@pytest.mark.parametrize("M", [12, 300])
+def test_ffn_an_infinite_gradient_row_leaves_the_others_alone(M):
+    """a row of dy with an infinity: dx of the other rows is what it is without it, within its bound"""
+    g = gen(M + 3)
+    x, dy = normal(g, M, 64, type=FP16), normal(g, M, 64, std=2.0 ** -14).to(FP16)
+    w = [normal(g, 136, 64, type=FP16, std=0.125) for _ in range(2)] + [normal(g, 64, 136, type=FP16, std=0.1)]
+    y, saved = blocks().gated_ffn(x, *w, save=True)
+    want = ffn16(x, *w, "silu", dy)["dx"]
+    bad = dy.clone()
+    bad[5, 7] = math.inf
+    d = blocks().gated_ffn_backward(bad, x, *w, saved)["dx"]
+    assert not d[5].isfinite().any()
+    d[5] = want[0][5].to(FP16)
+    held(d, *want, "dx")
+
+
+@pytest.mark.parametrize("M", [1, 4, 5])
+def test_ffn_weights_below_the_normal_numbers(M):
+    """weights of 2^-20 (fp16 holds them as subnormal numbers): g = 64 x 2^-20 = 2^-14, u = 1, y = 64 x 2^-14 x 4096 = 16, exactly"""
+    x = torch.ones(M, 64, dtype=FP16, device="cuda")
+    wg, wu, wd = (torch.full((64, 64), v, dtype=FP16, device="cuda") for v in (2.0 ** -20, 2.0 ** -6, 4096.0))
+    assert bool((blocks().gated_ffn(x, wg, wu, wd, activation="relu") == 16).all())
+    assert bool((blocks().gated_ffn(x * 2.0 ** -18, wg * 2.0 ** 20, wu * 2.0 ** 18, wd, activation="relu") == 64 * 2.0 ** -12 * 4096 * 1).all())
