@@ -66,7 +66,8 @@ __device__ __forceinline__ void act_and_slope(int act, float g, float& f, float&
         f = g < 0.f ? 0.f : g;
         d = g > 0.f ? 1.f : 0.f;
     } else {
-        const float s = sigmoid_(g), c = 1.0f - s;
+        const float t = __builtin_amdgcn_exp2f(-LOG2E * g), s = __builtin_amdgcn_rcpf(1.0f + t);
+        const float c = g < 0.f ? 1.0f - s : t * s;            // 1 - s: by subtraction only where s is the smaller one
         f = act == FFN_SILU ? g * s : s;
         d = act == FFN_SILU ? s * __builtin_fmaf(g, c, 1.0f) : s * c;
     }

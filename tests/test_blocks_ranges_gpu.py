@@ -179,3 +179,40 @@ def test_ffn_weights_below_the_normal_numbers(M):
     wg, wu, wd = (torch.full((64, 64), v, dtype=FP16, device="cuda") for v in (2.0 ** -20, 2.0 ** -6, 4096.0))
     assert bool((blocks().gated_ffn(x, wg, wu, wd, activation="relu") == 16).all())
     assert bool((blocks().gated_ffn(x * 2.0 ** -18, wg * 2.0 ** 20, wu * 2.0 ** 18, wd, activation="relu") == 64 * 2.0 ** -12 * 4096 * 1).all())
+
+
+# ------------------------------------------------------------------------------------------------ activations' tails
+def tail(act, M):
+    """a feed-forward block that hands its activation through: g = the bias, u = 1, w_down = 1 -> y = act(g), db_gate = M act'(g)"""
+    n = 64
+    bg = torch.linspace(-20, 20, n, device="cuda").to(BF16)
+    one, nul = torch.ones(n, dtype=BF16, device="cuda"), torch.zeros(n, n, dtype=BF16, device="cuda")
+    x, eye = torch.zeros(M, n, dtype=BF16, device="cuda"), torch.eye(n, device="cuda").to(BF16)
+    y, saved = blocks().gated_ffn(x, nul, nul, eye, bg, one, torch.zeros_like(one), activation=act, save=True)
+    d = blocks().gated_ffn_backward(torch.ones_like(x), x, nul, nul, eye, saved, bias=True, activation=act)
+    g = bg.double()
+    if act == "gelu":
+        phi = 0.5 * torch.erfc(-g / math.sqrt(2))
+        return y, d["db_gate"], g * phi, phi + g * torch.exp(-g * g / 2) / math.sqrt(2 * math.pi)
+    s, c = 1 / (1 + torch.exp(-g)), 1 / (1 + torch.exp(g))
+    return (y, d["db_gate"], s, s * c) if act == "sigmoid" else (y, d["db_gate"], g * s, s * (1 + g * c))
+
+
+@pytest.mark.parametrize("act", ["sigmoid", "silu"])
+@pytest.mark.parametrize("M", [1, 5])
+def test_ffn_activations_keep_their_digits_on_the_tails(act, M):
+    """values relative to themselves: h and y are rounded once each (half a step of bf16, 2^-8), the functions are good to 2^-14 of what they
+    return: e^-x to x 2^-23 relative (x <= 20; 200 for GELU's e^-xx/2), a handful of f32 steps. The slopes of SiLU and GELU pass through
+    zero: to 2^-14 of their two terms' magnitudes. db_gate is rounded once. bf16 and f32 end at 2^-126 alike: what lies below (GELU from -13 on) may
+    come out as anything up to that."""
+    y, db, want, slope = tail(act, M)
+    half = 2.0 ** -8
+    held(y, want.expand(M, -1), (want.abs() * (2 * half + half * half + 2.0 ** -14) + 2.0 ** -126).expand(M, -1), "y")
+    terms = slope.abs()
+    if act == "silu":
+        g = torch.linspace(-20, 20, 64, device="cuda").to(BF16).double()
+        terms = 1 / (1 + torch.exp(-g)) * (1 + g.abs() / (1 + torch.exp(g)))
+    if act == "gelu":
+        g = torch.linspace(-20, 20, 64, device="cuda").to(BF16).double()
+        terms = 0.5 * torch.erfc(-g / math.sqrt(2)) + g.abs() * torch.exp(-g * g / 2) / math.sqrt(2 * math.pi)
+    held(db, M * slope, M * (slope.abs() * half + terms * 2.0 ** -14 * (1 + half)) + M * 2.0 ** -126, "db_gate")
