@@ -51,17 +51,35 @@ __device__ __forceinline__ void tile_at_item(int lin, int tiles_m, int tiles_n, 
 }
 
 __device__ __forceinline__ float sigmoid_(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-LOG2E * x)); }
+// The normal distribution's integral, e = exp(-g g / 2) on the side. Below 0 as e R(|g|): 1 + erf would lose its digits there (from -6 on all of
+// them). R(x) = exp(x x / 2) Phi(-x) runs from 1/2 to 1 / (x sqrt(2 pi)) and is a polynomial in t = 1 / (1 + 0.3 x), t the factor of all terms: the
+// least largest relative deviation over 0 .. 14.5 (a fit in 64 bits) is 1.7e-7.
+__device__ __forceinline__ float normal_(float g, float& e) {
+    e = __builtin_amdgcn_exp2f(-0.5f * LOG2E * g * g);
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3f, fabsf(g), 1.0f));
+    constexpr float C[8] = {0.11963200649944483f, 0.12071214884664003f, 0.10017585937116391f, 0.1276920947382172f,
+                            -0.052034684618224844f, 0.20455757001720992f, -0.15615893604636474f, 0.0354238594837955f};
+    float r = C[7];
+#pragma unroll
+    for (int i = 6; i >= 0; --i) r = __builtin_fmaf(r, t, C[i]);
+    r *= t * e;
+    return g < 0.f ? r : 1.0f - r;
+}
 __device__ __forceinline__ float act_of(int act, float g) {
     if (act == FFN_SILU) return g * sigmoid_(g);
-    if (act == FFN_GELU) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
+    if (act == FFN_GELU) {
+        float e;
+        return g * normal_(g, e);
+    }
     if (act == FFN_RELU) return g < 0.f ? 0.f : g;             // (a NaN stays one)
     return sigmoid_(g);
 }
 __device__ __forceinline__ void act_and_slope(int act, float g, float& f, float& d) {
     if (act == FFN_GELU) {
-        const float phi = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
+        float e;
+        const float phi = normal_(g, e);
         f = g * phi;
-        d = phi + g * 0.3989422804014327f * __builtin_amdgcn_exp2f(-0.5f * LOG2E * g * g);
+        d = __builtin_fmaf(g * 0.3989422804014327f, e, phi);
     } else if (act == FFN_RELU) {
         f = g < 0.f ? 0.f : g;
         d = g > 0.f ? 1.f : 0.f;

@@ -198,7 +198,7 @@ def tail(act, M):
     return (y, d["db_gate"], s, s * c) if act == "sigmoid" else (y, d["db_gate"], g * s, s * (1 + g * c))
 
 
-@pytest.mark.parametrize("act", ["sigmoid", "silu"])
+@pytest.mark.parametrize("act", ["sigmoid", "silu", "gelu"])
 @pytest.mark.parametrize("M", [1, 5])
 def test_ffn_activations_keep_their_digits_on_the_tails(act, M):
     """values relative to themselves: h and y are rounded once each (half a step of bf16, 2^-8), the functions are good to 2^-14 of what they
