@@ -95,8 +95,13 @@ __device__ __forceinline__ void put_bias(float* bias, int n, uint32_t byte, bool
 // product ahead.
 __device__ __forceinline__ void reads_stay() { __builtin_amdgcn_sched_barrier(0x6); }
 
-// One block of NB x 32 states for 32 rows (a column of S^T each): scores, running maximum and sum, O^T += V^T P^T.
-// The maximum follows lazily: O^T is rescaled only when a row's maximum grows by more than 8 (base-2 units), so P <= 2^8.
+// fp16: P is formed as 2^12 P, so that weights down to 2^-26 of a row's largest stay normal numbers (many small ones can make up the result, next to
+// a large one with a small value: rounded to steps of 2^-24, 20000 weights of 2^-24.5 came out 44 % too large). bf16 has f32's range.
+template <bool F16> constexpr float P_UP = F16 ? 12.0f : 0.0f;              // log2 of the factor on P
+template <bool F16> constexpr float P_LAG = F16 ? 3.0f : 8.0f;
+
+// One block of NB x 32 states for 32 rows (a column of S^T each): scores, running maximum (m: less P_UP) and sum, O^T += V^T P^T.
+// The maximum follows lazily: O^T is rescaled only when a row's maximum grows by more than P_LAG (base-2 units), so P <= 2^15 (fp16), 2^8.
 template <bool F16, int DT, int NB>
 __device__ __forceinline__ void attend(const unsigned char* kt, const unsigned char* vt, const uint4 (&qf)[DT / 16], f32x16 (&acc)[DT / 32],
                                        float& m, float& l, float c, const float* bias, bool all, int lane) {
@@ -122,8 +127,8 @@ __device__ __forceinline__ void attend(const unsigned char* kt, const unsigned c
 #pragma unroll
         for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[b][i]);
     mx = max_halves(mx) * c;
-    if (__any(mx > m + 8.0f)) {
-        const float mn = fmaxf(m, mx);
+    if (__any(mx > m + (P_UP<F16> + P_LAG<F16>))) {
+        const float mn = fmaxf(m, mx - P_UP<F16>);
         const float al = __builtin_amdgcn_exp2f(m - (mn == NEG_INF ? 0.f : mn));
         l *= al;
 #pragma unroll
@@ -398,11 +403,9 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XattnArgs a) {
 // Backward. dQ first (a workgroup keeps 128 rows, forms their delta = rowsum(dout o out) and walks the states), then dK, dV (a workgroup keeps
 // 128 states, 32 per wave, and walks the rows); one launch adds up the splits of all three. Every sum has a fixed order: no atomics.
 //
-// fp16: P is formed as 2^12 P (<= 4096), so that weights of 1 / 16384 stay normal numbers, and each column of dS carries a power of two chosen
-// from what it meets: it starts so that the first block's largest |dS| lies in [2^10, 2^11) and is lowered, with the sums so far, when a block
-// passes 2^15. bf16 has f32's range and needs neither.
+// fp16: P is formed as 2^12 P (P_UP), and each column of dS carries a power of two chosen from what it meets: it starts so that the first block's
+// largest |dS| lies in [2^10, 2^11) and is lowered, with the sums so far, when a block passes 2^15. bf16 has f32's range and needs neither.
 // ------------------------------------------------------------------------------------------------------------------------------------
-template <bool F16> constexpr float P_UP = F16 ? 12.0f : 0.0f;              // log2 of the factor on P
 
 // Where a thread's row lies, RT rows further with every step. Where G divides RT and a sample holds at least RT rows, a step stays on the same
 // head and passes at most one sample's end: two additions instead of two divisions and the products of three strides.

@@ -216,3 +216,20 @@ def test_ffn_activations_keep_their_digits_on_the_tails(act, M):
         g = torch.linspace(-20, 20, 64, device="cuda").to(BF16).double()
         terms = 0.5 * torch.erfc(-g / math.sqrt(2)) + g.abs() * torch.exp(-g * g / 2) / math.sqrt(2 * math.pi)
     held(db, M * slope, M * (slope.abs() * half + terms * 2.0 ** -14 * (1 + half)) + M * 2.0 ** -126, "db_gate")
+
+
+# ------------------------------------------------------------------------------------------------ cross attention, fp16
+@pytest.mark.parametrize("Lq,Lk", [(1, 2000), (1, 20000), (40, 2000), (40, 20000), (700, 2000)])
+def test_xattn_weights_far_below_a_row_s_largest(Lq, Lk):
+    """one state of weight 1 and value 0, all others of weight e^-17 = 2^-24.5 and value 1: together they make the result, and their weights must
+    not be rounded to steps of 2^-24. A weight is rounded to half a step u = 2^-11 (normal numbers), the result once more; f32's part is Lk e at most"""
+    q = torch.zeros(1, Lq, 1, 64, dtype=FP16, device="cuda")
+    k, v = torch.zeros(1, Lk, 1, 64, dtype=FP16, device="cuda"), torch.ones(1, Lk, 1, 64, dtype=FP16, device="cuda")
+    q[..., 0] = 1
+    k[:, 1:, :, 0] = -17
+    v[:, 0] = 0
+    out, lse = blocks().cross_attention(q, k, v, scale=1.0)
+    w = (Lk - 1) * math.exp(-17)
+    want = torch.full(out.shape, w / (1 + w), dtype=torch.float64, device="cuda")
+    held(out, want, want * (2 * 2.0 ** -11 + 2 ** -22 + (Lk + 64) * E) + 2.0 ** -25, "out")
+    held(lse, torch.full(lse.shape, math.log1p(w), dtype=torch.float64, device="cuda"), torch.full(lse.shape, (Lk + 64) * E * 2, dtype=torch.float64, device="cuda"), "lse")
