@@ -8,7 +8,9 @@
 // within a sample:
 //   dgate_b = scale o sum t,  dscale = sum_b gate_b o sum t,  t = w o (dR o y^) + bias o dR;   dw_post = sum_b f_b o sum (dR o y^),
 //   dbias_post = sum_b f_b o sum dR  (f_b = scale o gate_b);   dw_pre = sum dz o r^,  dbias_pre = sum dz.
-// The partial sums of the workgroups are added in their order: the results do not depend on the schedule.
+// The partial sums of the workgroups are added in their order: the results do not depend on the schedule. With many short samples
+// (MANY, `plan`) a workgroup walks several whole ones, writes their dgate itself and adds sum dR and sum dR o y^ up with each sample's gate: the partial sums
+// are then as many as the workgroups, not the samples, and the gate is done with (65535 samples of one row of 8192: 136 MB for 17 GB).
 #include <algorithm>
 
 #include "blocks.h"
@@ -202,35 +204,45 @@ __global__ __launch_bounds__(MOST, MOST <= 256 ? 5 : 4) void norm_fwd_kernel(Nor
     }
 }
 
-template <int DT, bool VEC, int MOST>
+template <int DT, bool VEC, int MOST, bool MANY>
 __global__ __launch_bounds__(MOST, MOST <= 256 ? 3 : 4) void norm_bwd_kernel(NormArgs a) {
     if constexpr (DT == 1) T16<true>::enter();
     __shared__ __attribute__((aligned(16))) float buf[64];
     const int tid = threadIdx.x, c = tid * 8, D = a.D;
     const bool in = c < D;
     Meet meet{buf, (int)blockDim.x >> 6, tid >> 6, tid & 63, 0};
-    const int b = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
-    const int l0 = chunk * a.rows_per_chunk, l1 = min(a.L, l0 + a.rows_per_chunk);
-    float qw[8], qb[8], pw[8], f[8], g[8];
+    // a chunk of one sample's rows, or (MANY: rows_per_chunk counts samples) the rows of several whole samples
+    const int chunk = blockIdx.x % a.chunks, b0 = MANY ? chunk * a.rows_per_chunk : blockIdx.x / a.chunks;
+    const int l0 = MANY ? 0 : chunk * a.rows_per_chunk, l1 = MANY ? (min(a.B, b0 + a.rows_per_chunk) - b0) * a.L : min(a.L, l0 + a.rows_per_chunk);
+    int b = b0, end = a.L;                                    // MANY: the sample, the row behind its last
+    float qw[8], qb[8], pw[8], f[8];
     param8(a.post_w, c, D, 1.f, qw);
     param8(a.post_b, c, D, 0.f, qb);
     param8(a.pre_w, c, D, 1.f, pw);
     param8(a.scale, c, D, 1.f, f);
+    Row8<DT, VEC> gate, ng;                                   // this sample's, the next one's (MANY)
     if (a.gate && in) {
-        Row8<DT, VEC> t;
-        t.load(a.gate, b, c, D);
-        t.get(g);
+        float g[8];
+        gate.load(a.gate, b, c, D);
+        gate.get(g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] *= g[i];
     }
     const float rD = 1.0f / (float)D;
     float s0[8] = {}, s1[8] = {}, s2[8] = {}, s3[8] = {};
+    // MANY: s0 and s1 with the gates, over the samples; every lane its own (registers are taken)
+    __shared__ float all[MANY ? 16 * MOST : 1];
+    if (MANY) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) all[i * MOST + tid] = 0.f;
+    }
     Row8<DT, VEC> nx, ny, ndr, ndz;
     float4 nst = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto request = [&](int l) {
+    auto request = [&](int l, bool next_sample) {
         if (l >= l1) return;
-        const int64_t row = (int64_t)b * a.L + l;
+        const int64_t row = (int64_t)b0 * a.L + l;
         if (in) {
+            if (MANY && next_sample) ng.load(a.gate, b + 1, c, D);
             nx.load(a.x, row, c, D);
             if (a.y) ny.load(a.y, row, c, D);
             if (a.dr) ndr.load(a.dr, row, c, D);
@@ -238,16 +250,17 @@ __global__ __launch_bounds__(MOST, MOST <= 256 ? 3 : 4) void norm_bwd_kernel(Nor
         }
         nst = *reinterpret_cast<const float4*>(a.stats + 4 * row);
     };
-    request(l0);
+    request(l0, false);
     for (int l = l0; l < l1; ++l) {
-        const int64_t row = (int64_t)b * a.L + l;
+        const int64_t row = (int64_t)b0 * a.L + l;
         float x[8], y[8], dr[8], dz[8];
         nx.get(x);
         ny.get(y);
         ndr.get(dr);
         ndz.get(dz);
         const float4 st = nst;
-        request(l + 1);
+        const bool ends = MANY && l + 1 == end;
+        request(l + 1, ends);
         if (a.y) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -290,6 +303,32 @@ __global__ __launch_bounds__(MOST, MOST <= 256 ? 3 : 4) void norm_bwd_kernel(Nor
             }
             if (in) store8<DT, VEC>(a.dy, row, c, D, dr);
         }
+        if (MANY && ends) {
+            float sc[8], g[8];
+            gate.get(g);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                all[i * MOST + tid] += g[i] * s0[i];
+                all[(8 + i) * MOST + tid] += g[i] * s1[i];
+            }
+            param8(a.scale, c, D, 1.f, sc);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                g[i] = sc[i] * (qw[i] * s1[i] + qb[i] * s0[i]);
+                s0[i] = s1[i] = 0.f;
+            }
+            if (in && a.dgate) store8<DT, VEC>(a.dgate, b, c, D, g);
+            gate = ng;
+            gate.get(g);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = sc[i] * g[i];
+            end += a.L;
+            ++b;
+        }
+    }
+    if (MANY) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { s0[i] = all[i * MOST + tid]; s1[i] = all[(8 + i) * MOST + tid]; }
     }
     float* p = a.part + (int64_t)blockIdx.x * 4 * D;
 #pragma unroll
@@ -298,14 +337,16 @@ __global__ __launch_bounds__(MOST, MOST <= 256 ? 3 : 4) void norm_bwd_kernel(Nor
 }
 
 // sums over the chunks of a sample: part [B, chunks, 4, D] -> joint [B, 4, D], and the sample's dgate. 64 columns x 4 chunk lanes.
+// (`total` chunks in all: after MANY they stand in groups of JOIN, the last of which may be part full)
+constexpr int JOIN = 64;
 template <int DT>
-__global__ __launch_bounds__(256) void norm_join_kernel(NormArgs a, float* joint) {
+__global__ __launch_bounds__(256) void norm_join_kernel(NormArgs a, float* joint, int total) {
     if constexpr (DT == 1) T16<true>::enter();
     __shared__ float red[4][4][64];
     const int cl = threadIdx.x & 63, kl = threadIdx.x >> 6, b = blockIdx.y, c = blockIdx.x * 64 + cl, D = a.D;
     float s[4] = {};
     if (c < D)
-        for (int k = kl; k < a.chunks; k += 4) {
+        for (int k = kl; k < min(a.chunks, total - b * a.chunks); k += 4) {
             const float* p = a.part + ((int64_t)b * a.chunks + k) * 4 * D + c;
 #pragma unroll
             for (int j = 0; j < 4; ++j) s[j] += p[j * D];
@@ -314,7 +355,7 @@ __global__ __launch_bounds__(256) void norm_join_kernel(NormArgs a, float* joint
     for (int j = 0; j < 4; ++j) red[kl][j][cl] = s[j];
     __syncthreads();
     if (c >= D) return;
-    joint[((int64_t)b * 4 + kl) * D + c] = red[0][kl][cl] + red[1][kl][cl] + red[2][kl][cl] + red[3][kl][cl];
+    if (joint != a.part) joint[((int64_t)b * 4 + kl) * D + c] = red[0][kl][cl] + red[1][kl][cl] + red[2][kl][cl] + red[3][kl][cl];
     if (kl == 0 && a.dgate) {
         float t[2];
 #pragma unroll
@@ -369,12 +410,19 @@ bool vec_ok(const NormArgs& a) {
     for (const void* p : {a.x, a.y, a.gate, a.dr, a.dz, (const void*)a.r, (const void*)a.z, (const void*)a.dx, (const void*)a.dy}) m |= (uintptr_t)p;
     return a.D % 8 == 0 && m % 16 == 0;
 }
-// chunks of rows per sample; without a gate all rows are one sample
-void plan(NormArgs& a) {
+// Chunks of rows per sample; without a gate all rows are one sample. More short samples than workgroups: chunks of whole samples (the kernel's MANY),
+// up to 16 rows to a sample, 2 where a row takes more than four waves (their registers do not hold MANY's sums beside a row's). us, forward and
+// backward, a chunk per sample and MANY: samples x rows x D, bf16: 20000 x 1 x 256 528, 92; 9000 x 1 x 512 298, 107; 7000 x 16 x 512 481, 369; 7000 x
+// 60 x 256 754, 922; 6000 x 1 x 4096 1049, 397; 600 x 2 x 4096 140, 130; 600 x 8 x 4096 254, 290; f32: 7000 x 4 x 512 321, 228; 600 x 8 x 4096 354, 447.
+// One chunk per sample needs no copy for the sums over the samples (600 x 16 x 8192 bf16 872, 752 without).
+bool plan(NormArgs& a) {
     if (!a.gate) { a.L *= a.B; a.B = 1; }
-    const int want = std::max(1, walkers(64 * cdiv(a.D, 512), 3) / a.B);
-    a.rows_per_chunk = cdiv(a.L, std::min(want, a.L));
-    a.chunks = cdiv(a.L, a.rows_per_chunk);
+    const int wgs = walkers(64 * cdiv(a.D, 512), 3);
+    const bool many = a.B > 2 * wgs && a.L <= (a.D <= 2048 ? 16 : 2);
+    const int n = many ? a.B : a.L, want = many ? 4 * wgs : std::max(1, wgs / a.B);
+    a.rows_per_chunk = cdiv(n, std::min(want, n));
+    a.chunks = cdiv(n, a.rows_per_chunk);
+    return many;
 }
 template <int DT>
 int fwd(const NormArgs& a, hipStream_t st) {
@@ -389,21 +437,36 @@ int fwd(const NormArgs& a, hipStream_t st) {
     ISB_LAUNCHED("norm_fwd", st);
     return ISB_OK;
 }
-template <int DT>
-int bwd(NormArgs a, float* ws, hipStream_t st) {
-    plan(a);
-    a.part = ws;
-    float* joint = ws + (int64_t)a.B * a.chunks * 4 * a.D;
+template <int DT, bool MANY>
+void bwd_rows(const NormArgs& a, unsigned grid, hipStream_t st) {
     const int threads = 64 * cdiv(a.D, 512);
     if (vec_ok(a)) {
-        if (threads <= 256) norm_bwd_kernel<DT, true, 256><<<a.B * a.chunks, threads, 0, st>>>(a);
-        else norm_bwd_kernel<DT, true, 1024><<<a.B * a.chunks, threads, 0, st>>>(a);
+        if (threads <= 256) norm_bwd_kernel<DT, true, 256, MANY><<<grid, threads, 0, st>>>(a);
+        else norm_bwd_kernel<DT, true, 1024, MANY><<<grid, threads, 0, st>>>(a);
     } else {
-        norm_bwd_kernel<DT, false, 1024><<<a.B * a.chunks, threads, 0, st>>>(a);
+        norm_bwd_kernel<DT, false, 1024, MANY><<<grid, threads, 0, st>>>(a);
+    }
+}
+template <int DT>
+int bwd(NormArgs a, float* ws, hipStream_t st) {
+    const bool many = plan(a);
+    const int total = many ? a.chunks : a.B * a.chunks;
+    a.part = ws;
+    if (many) {
+        bwd_rows<DT, true>(a, (unsigned)total, st);
+        a.B = cdiv(total, JOIN);                             // what is left to add up knows no gate
+        a.chunks = JOIN;
+        a.gate = nullptr;
+        a.dgate = nullptr;
+    } else {
+        bwd_rows<DT, false>(a, (unsigned)total, st);
     }
     ISB_LAUNCHED("norm_bwd", st);
-    norm_join_kernel<DT><<<dim3(cdiv(a.D, 64), a.B), 256, 0, st>>>(a, joint);
-    ISB_LAUNCHED("norm_join", st);
+    float* joint = a.chunks == 1 ? ws : ws + (int64_t)total * 4 * a.D;
+    if (joint != ws || a.dgate) {
+        norm_join_kernel<DT><<<dim3(cdiv(a.D, 64), a.B), 256, 0, st>>>(a, joint, total);
+        ISB_LAUNCHED("norm_join", st);
+    }
     norm_params_kernel<DT><<<cdiv(a.D, 32), 1024, 0, st>>>(a, joint);
     ISB_LAUNCHED("norm_params", st);
     return ISB_OK;
@@ -412,8 +475,8 @@ int bwd(NormArgs a, float* ws, hipStream_t st) {
 
 size_t norm_workspace(const NormArgs& a0) {
     NormArgs a = a0;
-    plan(a);
-    return ((size_t)a.B * a.chunks + a.B) * 4 * a.D * sizeof(float);
+    if (plan(a)) return ((size_t)a.chunks + cdiv(a.chunks, JOIN)) * 4 * a.D * sizeof(float);
+    return ((size_t)a.B * a.chunks + (a.chunks == 1 ? 0 : a.B)) * 4 * a.D * sizeof(float);
 }
 int launch_norm_fwd(const NormArgs& a, int dtype, hipStream_t st) { return dtype == 0 ? fwd<0>(a, st) : dtype == 1 ? fwd<1>(a, st) : fwd<2>(a, st); }
 int launch_norm_bwd(NormArgs a, int dtype, float* ws, hipStream_t st) { return dtype == 0 ? bwd<0>(a, ws, st) : dtype == 1 ? bwd<1>(a, ws, st) : bwd<2>(a, ws, st); }
