@@ -52,13 +52,17 @@ def _tensor(name: str, t, dtype, device, shape) -> None:
         raise ValueError(f"{name}: expected {tuple(shape)}, got {tuple(t.shape)}")
 
 
-def _rows16(t: torch.Tensor):
-    """(t, its leading strides), or a contiguous copy where its last dimension is not contiguous or its rows do not lie on 16 bytes"""
+_FAR = 1 << 22         # elements between the rows that a kernel steps through, at most (include/isbfsar.h)
+
+
+def _rows16(t: torch.Tensor, walked: Optional[int] = None):
+    """(t, its leading strides), or a contiguous copy where its last dimension is not contiguous, its rows do not lie on 16 bytes or those along
+    dimension `walked` lie too far apart"""
     st = t.stride()
     bits = t.data_ptr() & 15
     for s in st[:-1]:
         bits |= s & 7
-    if bits == 0 and st[-1] == 1:
+    if bits == 0 and st[-1] == 1 and (walked is None or st[walked] <= _FAR):
         return t, st[:-1]
     t = _flat16(t)
     st, n = [], 1
@@ -101,8 +105,8 @@ def _xattn_args(q, k, v, kv_len, key_mask, scale):
     _tensor("k", k, t, dev, (Bk, Lk, Hk, D))
     _tensor("v", v, t, dev, shape)
     q, qs = _rows16(q)
-    k, ks = _rows16(k)
-    v, vs = _rows16(v)
+    k, ks = _rows16(k, 1)
+    v, vs = _rows16(v, 1)
     a = _lib.isb_xattn_args(dev.index, _TYPES[t], B, Bk, Lq, Lk, Hq, Hk, D, D ** -0.5 if scale is None and D else float(scale or 0),
                             q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs)
     keep = [q, k, v]
@@ -124,9 +128,9 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_len: O
                     key_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """softmax(scale q k^T) v over an encoder's states of another length; (out [B,Lq,Hq,D], lse f32 [B,Hq,Lq]).
 
-    q [B,Lq,Hq,D], k and v [Bk,Lk,Hk,D], fp16 or bf16, any strides (copied where rows do not lie on 16 bytes); D a multiple of 8 up to
-    128. Hq is a multiple of Hk (grouped heads). B is a multiple of Bk: sample b reads the states of b // (B // Bk), so Bk = 1 is ONE
-    support set for every window, read once for all of them. State j takes part iff j < kv_len[bk] (int32 [Bk]) and key_mask[bk, j]
+    q [B,Lq,Hq,D], k and v [Bk,Lk,Hk,D], fp16 or bf16, any strides (copied where rows do not lie on 16 bytes, or k's and v's
+    states too far apart); D a multiple of 8 up to 128. Hq is a multiple of Hk (grouped heads). B is a multiple of Bk: sample b reads the states
+    of b // (B // Bk), so Bk = 1 is ONE support set for every window, read once for all of them. State j takes part iff j < kv_len[bk] (int32 [Bk]) and key_mask[bk, j]
     (bool [Bk,Lk]); a row without states gets zeros and lse = -inf. scale defaults to 1 / sqrt(D)."""
     a, keep = _xattn_args(q, k, v, kv_len, key_mask, scale)
     B, Lq, Hq, _ = shape = q.shape
@@ -190,9 +194,9 @@ def _ffn_args(x, w_gate, w_up, w_down, activation):
 
 
 def _rows2(x):
-    """x [.., D] as (rows [M, D], their stride), the rows on 16 bytes; a copy only where they are not a constant stride apart, overlap or
-    do not lie on 16 bytes"""
-    x2, (st,) = _rows16(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]))
+    """x [.., D] as (rows [M, D], their stride), the rows on 16 bytes; a copy only where they are not a constant stride apart, overlap, lie too far
+    apart or not on 16 bytes"""
+    x2, (st,) = _rows16(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]), 0)
     if x2.shape[0] > 1 and st < x2.shape[1]:
         x2, st = x2.contiguous(), x2.shape[1]
     return x2, st
