@@ -464,7 +464,7 @@ int isb_dist_all_gather(isb_dist* d, const void* d_send, void* d_recv, size_t by
  *   (NULL: all). What masked states hold is never used (NaN and infinities included).
  *   out [B,Lq,Hq,D] = softmax(scale q k^T) v, lse [B,Hq,Lq] f32 = log sum exp(scale q k^T) (natural logarithm). A row with no
  *   state gets out = 0, lse = -inf and passes no gradient. scale > 0.
- *   At most 2^23 tiles of 128 rows (B / Bk * Lq * Hq / Hk rows read the states of one Bk and Hk) or 128 states; k and v: at most
+ *   Fewer than 2^23 - 7 tiles of 128 rows (B / Bk * Lq * Hq / Hk rows read the states of one Bk and Hk) or 128 states; k and v: at most
  *   2^22 elements from one state to the next.
  * Backward: dout [B,Lq,Hq,D], out and lse of the forward call -> dq, dk, dv (contiguous, shapes of q, k, v; gradients of
  * shared heads and shared states are summed in 32 bits; masked states get zeros). */

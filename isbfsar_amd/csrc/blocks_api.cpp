@@ -61,9 +61,10 @@ int xattn_shape(const isb_xattn_args* u, XattnArgs& a) {
     const int64_t rows = m * u->Bk * u->Hk, states = (int64_t)u->Bk * u->Hk * u->Lk;
     ISB_REQUIRE(rows < (1ll << 31) && states < (1ll << 31), ISB_ERR_INVALID, "cross attention: %lld rows, %lld states are too many", (long long)rows,
                 (long long)states);
-    // (a launch holds fewer than 2^32 threads: 2^23 workgroups of at most 512; splits come only where there are less than 2^10)
+    // (a launch holds fewer than 2^32 threads: not quite 2^23 workgroups of at most 512, their number rounded up to the 8 XCDs; splits come only
+    // where there are less than 2^10)
     const int64_t groups = (int64_t)u->Bk * u->Hk, tiles = groups * std::max((m + 127) / 128, ((int64_t)u->Lk + 127) / 128);
-    ISB_REQUIRE(tiles < (1 << 23), ISB_ERR_INVALID, "cross attention: %lld tiles of 128 rows or states are more than one launch holds", (long long)tiles);
+    ISB_REQUIRE(tiles <= (1 << 23) - 8, ISB_ERR_INVALID, "cross attention: %lld tiles of 128 rows or states are more than one launch holds", (long long)tiles);
     ISB_REQUIRE(std::isfinite(u->scale) && u->scale > 0, ISB_ERR_INVALID, "cross attention: scale %g is not positive", (double)u->scale);
     a.B = u->B; a.Bk = u->Bk; a.nb = u->B / u->Bk; a.Lq = u->Lq; a.Lk = u->Lk; a.Hq = u->Hq; a.Hk = u->Hk; a.G = u->Hq / u->Hk; a.D = u->D;
     a.M = (int)m;
