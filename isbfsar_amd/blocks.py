@@ -16,6 +16,7 @@ returned; nothing is recorded on an autograd tape and no result requires a gradi
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import Dict, Optional, Tuple
 
 import torch
@@ -86,6 +87,11 @@ def _workspace(fn, what: str, args, *more) -> int:
     return n.value
 
 
+def _address(t: torch.Tensor) -> int:
+    """t's address; of an empty tensor one that is not null (nothing is read there)"""
+    return t.data_ptr() or 16
+
+
 # the current stream's handle: the raw query costs 0.1 us of the 4 us that a launch takes, the stream object 2
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
@@ -124,6 +130,17 @@ def _xattn_args(q, k, v, kv_len, key_mask, scale):
     return a, keep
 
 
+def _xattn_empty(a) -> bool:
+    """there is nothing to attend, or to attend to: no launch. What can be wrong with the arguments all the same is refused."""
+    if a.B and a.Bk and a.Lq and a.Lk:
+        return False
+    if a.B and not a.Bk:
+        _refuse(f"{a.B} samples share no set of states")
+    one = _lib.isb_xattn_args(a.device, a.dtype, a.B or a.Bk or 1, a.Bk or 1, a.Lq or 1, a.Lk or 1, a.Hq, a.Hk, a.D, a.scale)
+    _workspace(_lib.lib().isb_xattn_workspace, "isb_xattn_workspace", one, 0)
+    return True
+
+
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_len: Optional[torch.Tensor] = None,
                     key_mask: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """softmax(scale q k^T) v over an encoder's states of another length; (out [B,Lq,Hq,D], lse f32 [B,Hq,Lq]).
@@ -131,8 +148,10 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_len: O
     q [B,Lq,Hq,D], k and v [Bk,Lk,Hk,D], fp16 or bf16, any strides (copied where rows do not lie on 16 bytes, or k's and v's
     states too far apart); D a multiple of 8 up to 128. Hq is a multiple of Hk (grouped heads). B is a multiple of Bk: sample b reads the states
     of b // (B // Bk), so Bk = 1 is ONE support set for every window, read once for all of them. State j takes part iff j < kv_len[bk] (int32 [Bk]) and key_mask[bk, j]
-    (bool [Bk,Lk]); a row without states gets zeros and lse = -inf. scale defaults to 1 / sqrt(D)."""
+    (bool [Bk,Lk]); a row without states (Lk may be 0) gets zeros and lse = -inf. scale defaults to 1 / sqrt(D)."""
     a, keep = _xattn_args(q, k, v, kv_len, key_mask, scale)
+    if _xattn_empty(a):
+        return q.new_zeros(q.shape), q.new_full((a.B, a.Hq, a.Lq), -math.inf, dtype=torch.float32)
     B, Lq, Hq, _ = shape = q.shape
     out = q.new_empty(shape)
     lse = q.new_empty((B, Hq, Lq), dtype=torch.float32)
@@ -156,6 +175,8 @@ def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     _tensor("dout", dout, t, dev, q.shape)
     _tensor("out", out, t, dev, q.shape)
     _tensor("lse", lse, torch.float32, dev, (q.shape[0], q.shape[2], q.shape[1]))
+    if _xattn_empty(a):
+        return q.new_zeros(q.shape), k.new_zeros(k.shape), v.new_zeros(v.shape)
     dout, a.dout_stride = _rows16(dout)
     out, lse = _flat16(out), lse.contiguous()
     dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), k.new_empty(k.shape)
@@ -179,8 +200,6 @@ def _ffn_args(x, w_gate, w_up, w_down, activation):
     F, D = shape = w_gate.shape
     if x.shape[-1] != D:
         _refuse(f"x: expected [..,{D}], got {tuple(x.shape)}")
-    if x.numel() == 0:
-        _refuse(f"x has no rows: {tuple(x.shape)}")
     _tensor("w_gate", w_gate, t, dev, shape)
     _tensor("w_up", w_up, t, dev, shape)
     _tensor("w_down", w_down, t, dev, (D, F))
@@ -188,6 +207,9 @@ def _ffn_args(x, w_gate, w_up, w_down, activation):
         _refuse(f"activation {activation!r} not in {sorted(ACTIVATIONS)}")
     x2, xs = _rows2(x)
     wg, wu, wd = _flat16(w_gate), _flat16(w_up), _flat16(w_down)
+    if x2.shape[0] == 0:                                     # no launch; what can be wrong with the arguments all the same is refused
+        one = _lib.isb_ffn_args(dev.index, _TYPES[t], 1, D, F, ACTIVATIONS[activation])
+        _workspace(_lib.lib().isb_ffn_workspace, "isb_ffn_workspace", one, 0)
     a = _lib.isb_ffn_args(dev.index, _TYPES[t], x2.shape[0], D, F, ACTIVATIONS[activation], xs, 0, x2.data_ptr(), wg.data_ptr(), wu.data_ptr(),
                           wd.data_ptr())
     return a, [x2, wg, wu, wd]
@@ -196,7 +218,7 @@ def _ffn_args(x, w_gate, w_up, w_down, activation):
 def _rows2(x):
     """x [.., D] as (rows [M, D], their stride), the rows on 16 bytes; a copy only where they are not a constant stride apart, overlap, lie too far
     apart or not on 16 bytes"""
-    x2, (st,) = _rows16(x if x.dim() == 2 else x.reshape(-1, x.shape[-1]), 0)
+    x2, (st,) = _rows16(x if x.dim() == 2 else x.reshape(x.numel() // max(x.shape[-1], 1), x.shape[-1]), 0)
     if x2.shape[0] > 1 and st < x2.shape[1]:
         x2, st = x2.contiguous(), x2.shape[1]
     return x2, st
@@ -223,6 +245,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     if save:
         saved = (x.new_empty((M, F), dtype=torch.float32), x.new_empty((M, F), dtype=torch.float32), x.new_empty((M, F)))
         a.pre_gate, a.pre_up, a.hidden = (s.data_ptr() for s in saved)
+    if M == 0:
+        return (y, saved) if save else y
     lib = _lib.lib()
     n = _workspace(lib.isb_ffn_workspace, "isb_ffn_workspace", a, 0)
     ws = x.new_empty(n, dtype=torch.uint8) if n else None
@@ -256,6 +280,10 @@ def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, 
         r["db_gate"], r["db_up"], r["db_down"] = db[:F], db[F:2 * F], db[2 * F:]
         at = db.data_ptr()
         a.db_gate, a.db_up, a.db_down = at, at + 2 * F, at + 4 * F
+    if M == 0:
+        for v in r.values():
+            v.zero_()
+        return r
     lib = _lib.lib()
     n = _workspace(lib.isb_ffn_workspace, "isb_ffn_workspace", a, 1)
     ws = x.new_empty(n, dtype=torch.uint8)
@@ -275,7 +303,7 @@ def _norm_args(x, y, gate, scale, post, post_weight, post_bias, pre, pre_weight,
         _refuse(f"norms {post!r}, {pre!r}: None, 'layer' or 'rms'")
     B, L, D = shape = x.shape
     x = x.contiguous()
-    keep, p, vec = [x], [x.data_ptr()], (D,)
+    keep, p, vec = [x], [_address(x)], (D,)
     for n, v, sh, dt in (("y", y, shape, t), ("gate", gate, (B, D), t), ("scale", scale, vec, torch.float32),
                          ("post_weight", post_weight, vec, torch.float32), ("post_bias", post_bias, vec, torch.float32),
                          ("pre_weight", pre_weight, vec, torch.float32), ("pre_bias", pre_bias, vec, torch.float32)):
@@ -285,8 +313,12 @@ def _norm_args(x, y, gate, scale, post, post_weight, post_bias, pre, pre_weight,
             _tensor(n, v, dt, dev, sh)
             v = v.contiguous()
             keep.append(v)
-            p.append(v.data_ptr())
-    return _lib.isb_norm_args(dev.index, _TYPES[t], B, L, D, NORMS[post], NORMS[pre], eps, *p), keep
+            p.append(_address(v))
+    a = _lib.isb_norm_args(dev.index, _TYPES[t], B, L, D, NORMS[post], NORMS[pre], eps, *p)
+    if B == 0 or L == 0:                                     # no launch; what can be wrong with the arguments all the same is refused
+        one = _lib.isb_norm_args(dev.index, _TYPES[t], 1, 1, D, NORMS[post], NORMS[pre], eps, *p)
+        _workspace(_lib.lib().isb_norm_workspace, "isb_norm_workspace", one)
+    return a, keep
 
 
 def block_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, gate: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None,
@@ -309,7 +341,7 @@ def block_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, gate: Optio
     if save:
         stats = x.new_empty((*x.shape[:2], 4), dtype=torch.float32)
         a.stats = stats.data_ptr()
-    rc = _lib.lib().isb_norm_forward(C.byref(a), _stream(a.device))
+    rc = _lib.lib().isb_norm_forward(C.byref(a), _stream(a.device)) if a.B * a.L else 0
     if rc:
         _lib.check(rc, "isb_norm_forward")
     return (r, z, stats) if save else (r, z)
@@ -347,6 +379,10 @@ def block_norm_backward(dr: Optional[torch.Tensor], dz: Optional[torch.Tensor], 
                  ("dpre_bias", pre_bias)):
         if v is not None:
             g[n] = v.new_empty(v.shape)
+    if a.B * a.L == 0:
+        for v in g.values():
+            v.zero_()
+        return g
     for n, v in g.items():
         setattr(a, n, v.data_ptr())
     lib = _lib.lib()

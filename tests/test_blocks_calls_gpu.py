@@ -44,3 +44,63 @@ def test_ffn_rows_far_apart(M):
     grads = blocks().gated_ffn_backward(dy, a["x"], *w, saved)
     for n, g in blocks().gated_ffn_backward(far(dy), far(a["x"]), *w, saved).items():
         assert torch.equal(g, grads[n]), n
+
+
+@pytest.mark.parametrize("t", [BF16, FP16])
+@pytest.mark.parametrize("B,Bk,Lq,Lk", [(2, 1, 3, 0), (0, 1, 3, 5), (2, 2, 0, 5), (0, 0, 3, 5), (0, 2, 0, 0)])
+def test_xattn_of_nothing(t, B, Bk, Lq, Lk):
+    """no states: zeros, lse -inf, no gradient; no rows: empty results, the states' gradients zero"""
+    q, dout = (torch.ones(B, Lq, 4, 64, dtype=t, device="cuda") for _ in range(2))
+    k, v = (torch.ones(Bk, Lk, 2, 64, dtype=t, device="cuda") for _ in range(2))
+    m = {"kv_len": torch.full((Bk,), Lk, dtype=torch.int32, device="cuda"), "key_mask": torch.ones(Bk, Lk, dtype=torch.bool, device="cuda")}
+    for mask in ({}, m):
+        out, lse = blocks().cross_attention(q, k, v, **mask)
+        assert out.shape == q.shape and out.dtype == t and not out.any()
+        assert lse.shape == (B, 4, Lq) and lse.dtype == F32 and bool((lse == -math.inf).all())
+        for g, like in zip(blocks().cross_attention_backward(dout, q, k, v, out, lse, **mask), (q, k, v)):
+            assert g.shape == like.shape and g.dtype == t and not g.any()
+
+
+def test_xattn_of_nothing_is_checked_all_the_same():
+    q, k = torch.ones(0, 3, 4, 64, dtype=BF16, device="cuda"), torch.ones(1, 5, 2, 64, dtype=BF16, device="cuda")
+    for bad in ((q, k, k[:, :, :, :32]), (q, k, k.half()), (q[..., :60], k[..., :60], k[..., :60]), (q[:, :, :3], k, k), (q[:, :, :0], k, k),
+                (torch.ones(2, 3, 4, 64, dtype=BF16, device="cuda"), k[:0], k[:0])):
+        with pytest.raises((ValueError, TypeError, RuntimeError)):
+            blocks().cross_attention(*bad)
+    with pytest.raises((ValueError, RuntimeError)):
+        blocks().cross_attention(q, k, k, scale=-1.0)
+
+
+@pytest.mark.parametrize("shape", [(0, 64), (3, 0, 64)])
+def test_ffn_of_nothing(shape):
+    a, b, _ = ffn_inputs(1, 64, 136, FP16, True)
+    w = [a["wg"], a["wu"], a["wd"]]
+    x = torch.ones(*shape, dtype=FP16, device="cuda")
+    assert blocks().gated_ffn(x, *w, *b).shape == shape
+    y, saved = blocks().gated_ffn(x, *w, *b, save=True)
+    assert y.shape == shape and y.dtype == FP16
+    d = blocks().gated_ffn_backward(y, x, *w, saved, bias=True)
+    for n, like in zip(("dx", "dw_gate", "dw_up", "dw_down", "db_gate", "db_up", "db_down"), (x, *w, *b)):
+        assert d[n].shape == like.shape and d[n].dtype == FP16 and not d[n].any(), n
+    for bad in ((x, w[0], w[1][:, :32], w[2]), (x[..., :60], *(v[:, :60] for v in w[:2]), w[2][:60])):
+        with pytest.raises((ValueError, RuntimeError)):
+            blocks().gated_ffn(*bad)
+
+
+@pytest.mark.parametrize("B,L", [(0, 3), (2, 0)])
+def test_norm_of_nothing(B, L):
+    x, y, dr, dz, a = norm_inputs(1, 1, 72, BF16, ("layer", "rms"), True)
+    x, y, dr, dz = (v[:, :0].expand(B, 0, 72) if L == 0 else v[:0].expand(0, L, 72) for v in (x, y, dr, dz))
+    a["gate"] = a["gate"].expand(B, 72) if B else a["gate"][:0]
+    r, z, stats = blocks().block_norm(x, y, save=True, **a)
+    assert r.shape == z.shape == (B, L, 72) and stats.shape == (B, L, 4)
+    d = blocks().block_norm_backward(dr, dz, x, y, stats, **a)
+    for n, like in {"dx": x, "dy": y, "dgate": a["gate"], "dscale": a["scale"], "dpost_weight": a["post_weight"], "dpost_bias": a["post_bias"],
+                    "dpre_weight": a["pre_weight"]}.items():
+        assert d[n].shape == like.shape and d[n].dtype == like.dtype and not d[n].any(), n
+    r, z = blocks().block_norm(x, pre="layer")
+    assert r is x and z.shape == x.shape
+    with pytest.raises((ValueError, RuntimeError)):
+        blocks().block_norm(x, y, pre="rms", pre_bias=a["scale"])
+    with pytest.raises((ValueError, RuntimeError)):
+        blocks().block_norm(torch.ones(2, 3, 0, device="cuda"), pre="layer")
