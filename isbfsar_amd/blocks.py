@@ -11,7 +11,9 @@ what it hands out: the embeddings of query windows ([B, L, 256], ``infer(want_em
 
 torch owns the device memory and the stream (the tensors' current stream); every call is asynchronous on it, allocates its results and
 its workspace with torch and may be captured into a graph. Backward passes are calls of their own and take what the forward call
-returned; nothing is recorded on an autograd tape and no result requires a gradient.
+returned; nothing is recorded on an autograd tape. A tensor that requires a gradient is therefore refused while gradients are recorded (the
+result would not carry it): call under torch.no_grad(), or detach; parameters then take the gradients that the backward calls return. Forward-mode
+tangents are refused likewise.
 """
 from __future__ import annotations
 
@@ -20,6 +22,7 @@ import math
 from typing import Dict, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 
@@ -35,11 +38,24 @@ def _refuse(msg: str):
     raise ValueError(msg)
 
 
+def _on_tape(name: str):
+    _refuse(f"{name} requires a gradient, which no result would carry: call under torch.no_grad() or detach it (gradients: the backward calls)")
+
+
+def _tangents(*tensors) -> None:
+    """called inside forward_ad.dual_level only"""
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
+            _refuse("a tensor has a forward-mode tangent, which no result would carry")
+
+
 def _first(name: str, t, types) -> None:
     if not (isinstance(t, torch.Tensor) and t.is_cuda):
         raise TypeError(f"{name} must be a torch CUDA tensor")
     if t.dtype not in types:
         raise TypeError(f"{name} is {t.dtype}, expected one of {sorted(str(x) for x in types)}")
+    if t.requires_grad and torch.is_grad_enabled():
+        _on_tape(name)
 
 
 def _tensor(name: str, t, dtype, device, shape) -> None:
@@ -51,6 +67,8 @@ def _tensor(name: str, t, dtype, device, shape) -> None:
         raise ValueError(f"{name} lives on {t.device}, the first tensor on {device}")
     if t.shape != shape:
         raise ValueError(f"{name}: expected {tuple(shape)}, got {tuple(t.shape)}")
+    if t.requires_grad and torch.is_grad_enabled():
+        _on_tape(name)
 
 
 _FAR = 1 << 22         # elements between the rows that a kernel steps through, at most (include/isbfsar.h)
@@ -149,6 +167,8 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_len: O
     states too far apart); D a multiple of 8 up to 128. Hq is a multiple of Hk (grouped heads). B is a multiple of Bk: sample b reads the states
     of b // (B // Bk), so Bk = 1 is ONE support set for every window, read once for all of them. State j takes part iff j < kv_len[bk] (int32 [Bk]) and key_mask[bk, j]
     (bool [Bk,Lk]); a row without states (Lk may be 0) gets zeros and lse = -inf. scale defaults to 1 / sqrt(D)."""
+    if _forward_ad._current_level >= 0:
+        _tangents(q, k, v)
     a, keep = _xattn_args(q, k, v, kv_len, key_mask, scale)
     if _xattn_empty(a):
         return q.new_zeros(q.shape), q.new_full((a.B, a.Hq, a.Lq), -math.inf, dtype=torch.float32)
@@ -170,6 +190,8 @@ def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tenso
                              scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(dq, dk, dv) of :func:`cross_attention`, given its arguments and results. Gradients of shared heads and shared states are summed;
     masked states get zeros."""
+    if _forward_ad._current_level >= 0:
+        _tangents(dout, q, k, v, out, lse)
     a, keep = _xattn_args(q, k, v, kv_len, key_mask, scale)
     dev, t = q.device, q.dtype
     _tensor("dout", dout, t, dev, q.shape)
@@ -231,6 +253,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     x [..,D] (rows a constant stride apart), w_gate and w_up [F,D], w_down [D,F] (torch Linear layout), biases or None; D and F multiples
     of 8; activation "silu", "gelu" (exact), "relu" or "sigmoid". Returns y, or (y, saved) with save=True: what
     :func:`gated_ffn_backward` needs (both pre-activations in f32, the hidden rows in x's type)."""
+    if _forward_ad._current_level >= 0:
+        _tangents(x, w_gate, w_up, w_down, b_gate, b_up, b_down)
     a, keep = _ffn_args(x, w_gate, w_up, w_down, activation)
     dev, t, M, D, F = x.device, x.dtype, a.M, a.D, a.F
     for n, b, size in (("b_gate", b_gate, F), ("b_up", b_up, F), ("b_down", b_down, D)):
@@ -260,6 +284,8 @@ def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, 
                        bias: bool = False, activation: str = "silu") -> Dict[str, torch.Tensor]:
     """Gradients of :func:`gated_ffn`: {"dx", "dw_gate", "dw_up", "dw_down"} and, with bias=True, {"db_gate", "db_up", "db_down"}. The two
     first weights' gradients are the halves of one [2F,D] tensor."""
+    if _forward_ad._current_level >= 0:
+        _tangents(dy, x, w_gate, w_up, w_down)
     a, keep = _ffn_args(x, w_gate, w_up, w_down, activation)
     dev, t, M, D, F = x.device, x.dtype, a.M, a.D, a.F
     _tensor("dy", dy, t, dev, x.shape)
@@ -330,6 +356,8 @@ def block_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, gate: Optio
     x, y [B,L,D] f32, fp16 or bf16, D up to 8192 (any); gate [B,D] of x's type, scale, weights and biases f32 [D], or None; post / pre:
     None, "layer" or "rms" (no bias). y None: the norm before the first block, r is x itself. pre None: z is None. z is the norm of r
     before r is rounded; stats f32 [B,L,4] are for :func:`block_norm_backward`."""
+    if _forward_ad._current_level >= 0:
+        _tangents(x, y, gate, scale, post_weight, post_bias, pre_weight, pre_bias)
     a, keep = _norm_args(x, y, gate, scale, post, post_weight, post_bias, pre, pre_weight, pre_bias, eps)
     r, z, stats = x, None, None
     if y is not None:
@@ -354,6 +382,8 @@ def block_norm_backward(dr: Optional[torch.Tensor], dz: Optional[torch.Tensor], 
                         eps: float = 1e-5) -> Dict[str, torch.Tensor]:
     """Gradients of :func:`block_norm` (same arguments, its stats): {"dx", "dy"?, "dgate"?, "dscale"?, "dpost_weight"?, "dpost_bias"?,
     "dpre_weight"?, "dpre_bias"?}, one for each tensor given. dr (or None: zeros) and dz are the gradients of r and z."""
+    if _forward_ad._current_level >= 0:
+        _tangents(dr, dz, x, y, stats, gate, scale, post_weight, post_bias, pre_weight, pre_bias)
     a, keep = _norm_args(x, y, gate, scale, post, post_weight, post_bias, pre, pre_weight, pre_bias, eps)
     dev, t = x.device, x.dtype
     if (dz is not None) != (pre is not None):

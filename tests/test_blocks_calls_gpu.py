@@ -104,3 +104,57 @@ def test_norm_of_nothing(B, L):
         blocks().block_norm(x, y, pre="rms", pre_bias=a["scale"])
     with pytest.raises((ValueError, RuntimeError)):
         blocks().block_norm(torch.ones(2, 3, 0, device="cuda"), pre="layer")
+
+
+# ------------------------------------------------------------------------------------------------ autograd
+def calls():
+    q, k, v, dout, _ = xattn_inputs((2, 1, 3, 40, 2, 2, 64, ""), BF16)
+    out, lse = blocks().cross_attention(q, k, v)
+    a, b, dy = ffn_inputs(6, 64, 136, BF16, True)
+    f = [a["x"], a["wg"], a["wu"], a["wd"]]
+    y, saved = blocks().gated_ffn(*f, *b, save=True)
+    nx, ny, dr, dz, na = norm_inputs(2, 3, 64, BF16, ("layer", "rms"), True)
+    _, _, st = blocks().block_norm(nx, ny, save=True, **na)
+    names = [n for n, t in na.items() if torch.is_tensor(t)]
+
+    def norm(x, y, *p):
+        return blocks().block_norm(x, y, **{**na, **dict(zip(names, p))})
+
+    def norm_backward(dr, dz, x, y, *p):
+        return list(blocks().block_norm_backward(dr, dz, x, y, st, **{**na, **dict(zip(names, p))}).values())
+    return {"xattn": (blocks().cross_attention, [q, k, v]), "xattn backward": (blocks().cross_attention_backward, [dout, q, k, v, out]),
+            "ffn": (lambda *t: [blocks().gated_ffn(*t)], [*f, *b]), "ffn backward": (lambda *t: list(blocks().gated_ffn_backward(*t, saved).values()), [dy, *f]),
+            "norm": (norm, [nx, ny, *(na[n] for n in names)]), "norm backward": (norm_backward, [dr, dz, nx, ny, *(na[n] for n in names)])}, lse
+
+
+@pytest.mark.parametrize("name", ["xattn", "xattn backward", "ffn", "ffn backward", "norm", "norm backward"])
+def test_tensors_on_the_tape_are_refused(name):
+    """no result would carry their gradient: an error, not silence. Under no_grad they are tensors like others."""
+    (f, args), lse = calls()[0][name], calls()[1]
+    more = [lse] if name == "xattn backward" else []
+    want = f(*args, *more)
+    for i in range(len(args)):
+        on = list(args)
+        on[i] = args[i].clone().requires_grad_(True)
+        with pytest.raises(ValueError, match="no_grad"):
+            f(*on, *more)
+        with torch.no_grad():
+            got = f(*on, *more)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_forward_mode_tangents_and_transforms_are_refused():
+    import torch.autograd.forward_ad as fw
+    q, k, v, _, _ = xattn_inputs((2, 1, 3, 40, 2, 2, 64, ""), BF16)
+    with fw.dual_level():
+        with pytest.raises(ValueError, match="tangent"):
+            blocks().cross_attention(fw.make_dual(q, torch.ones_like(q)), k, v)
+        blocks().cross_attention(q, k, v)
+        for f, args in (c for n, c in calls()[0].items() if n != "xattn backward"):
+            for i in range(len(args)):
+                with pytest.raises(ValueError, match="tangent"):
+                    f(*args[:i], fw.make_dual(args[i], torch.ones_like(args[i])), *args[i + 1:])
+    with pytest.raises((ValueError, TypeError, RuntimeError)):
+        torch.func.grad(lambda x: blocks().cross_attention(x, k, v)[0].float().sum())(q)
+    with pytest.raises((ValueError, TypeError, RuntimeError)):
+        torch.func.vmap(lambda x: blocks().cross_attention(x[None], k, v)[0])(q)
