@@ -901,14 +901,18 @@ constexpr int CUS = 256;
 int dt_of(const XattnArgs& a) { return a.D <= 64 ? 64 : 128; }
 // Tiles of 32 rows, their states shared out over the waves of a workgroup, instead of tiles of 128 rows whose states are shared out over
 // workgroups and joined by another launch: for at most 32 rows, and where the 128-row tiles would leave most CUs idle, between 64 states (two
-// blocks: the other waves had none) and 2048. us, 128-row tiles and these (tiles of 32 x states x width):
+// blocks: the other waves had none; where the CUs take these tiles in two rounds, 192, up to which the 128-row form splits nothing) and 2048. us,
+// 128-row tiles and these (tiles of 32 x states x width):
 //   120 x 1800 x 128: 23.2, 16.5    240 x 1800 x 128: 27.6, 18.7    480 x 1800 x 128: 36.9, 33.3    768 x 300 x 128: 13.5, 22.8
 //   256 x 300 x 64: 11.4, 6.2       512 x 300 x 64: 13.6, 9.1       768 x 300 x 64: 9.2, 11.9       128 x 4000 x 64: 18.2, 19.4
 //   128 x 64 x 128: 6.8, 7.2        128 x 65 x 128: 8.1, 7.4        8 x 1800 x 128: 13.8, 15.0      8 x 1800 x 64: 10.7, 10.7
+//   256 x 192 x 128: 9.3, 7.9       320 x 100 x 128: 8.3, 12.8      320 x 192 x 128: 9.4, 13.8      320 x 224 x 128: 17.4, 14.0
+//   512 x 192 x 128: 9.6, 14.1      512 x 300 x 128: 21.7, 15.4     512 x 1000 x 128: 28.5, 22.4    320 x 192 x 64: 6.8, 7.4
+//   320 x 224 x 64: 12.1, 7.5       512 x 600 x 64: 17.0, 10.0      512 x 1800 x 64: 24.6, 16.8     400 x 600 x 128: 22.7, 17.9
 bool few_rows(const XattnArgs& a) {
     if (a.M <= 32) return true;
     const int64_t tiles = (int64_t)a.Bk * a.Hk * cdiv(a.M, 32);
-    return a.Lk > 64 && a.Lk <= 2048 && tiles <= 2 * CUS && (tiles >= 32 || (int64_t)a.Lk * dt_of(a) <= 2048 * 64);
+    return a.Lk > (tiles > CUS ? 3 * KT : KT) && a.Lk <= 2048 && tiles <= 2 * CUS && (tiles >= 32 || (int64_t)a.Lk * dt_of(a) <= 2048 * 64);
 }
 
 // The same for dQ, whose splits share their join with those of dK and dV: from 64 tiles of 32 rows (below, splits spread better) to one per CU

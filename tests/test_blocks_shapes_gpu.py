@@ -4,9 +4,25 @@ import pytest
 import torch
 
 import blocks_ref as ref
-from test_blocks_gpu import BF16, F32, FP16, blocks, held, norm_inputs
+from test_blocks_gpu import BF16, F32, FP16, blocks, held, norm_inputs, xattn_inputs
 
 pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------------ cross attention
+@pytest.mark.parametrize("t", [BF16, FP16])
+@pytest.mark.parametrize("case", [
+    # B, Bk, Lq, Lk, Hq, Hk, D, masks: tiles of 32 rows in one round of the CUs and in two, around the lengths where the form changes
+    (16, 16, 512, 100, 1, 1, 128, "len holes"), (17, 17, 512, 100, 1, 1, 128, "len holes"), (20, 5, 128, 192, 16, 4, 64, "holes"),
+    (20, 5, 128, 193, 16, 4, 64, "holes"), (32, 32, 511, 65, 1, 1, 72, "len empty"), (33, 33, 512, 250, 1, 1, 128, "len"),
+])
+def test_xattn_short_states_many_tiles(case, t):
+    q, k, v, dout, m = xattn_inputs(case, t)
+    out, lse = blocks().cross_attention(q, k, v, **m)
+    d = blocks().cross_attention_backward(dout, q, k, v, out, lse, **m)
+    want = ref.xattn(q, k, v, dout=dout, **m)
+    for name, got in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *d)):
+        held(got, *want[name], name)
 
 
 # ------------------------------------------------------------------------------------------------ norms around a block
