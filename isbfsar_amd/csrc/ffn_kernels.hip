@@ -690,10 +690,10 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
             const bool live = n0 + wn * WN < p.N, live2 = n0 + wn * WN + 32 < p.N;
             const auto in_range = [&](int r) { return mb + r + rl < p.M && n < p.N; };
             const auto grads = [&](int r, float (&dg)[4], float (&du)[4], float (&hh)[4]) {         // (outside: all 0)
-                const float4 o = *reinterpret_cast<const float4*>(rows + (r + rl) * RS + 4 * cl);
                 const int64_t at = (int64_t)(mb + r + rl) * p.F + n;
-                float4 g4 = make_float4(0.f, 0.f, 0.f, 0.f), u4 = g4;
+                float4 g4 = make_float4(0.f, 0.f, 0.f, 0.f), u4 = g4, o = g4;          // (a zero row's product with an infinite weight is none)
                 if (in_range(r)) {
+                    o = *reinterpret_cast<const float4*>(rows + (r + rl) * RS + 4 * cl);
                     g4 = *reinterpret_cast<const float4*>(p.g + at);
                     u4 = *reinterpret_cast<const float4*>(p.u + at);
                 }

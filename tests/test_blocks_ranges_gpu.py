@@ -172,6 +172,19 @@ def test_ffn_an_infinite_gradient_row_leaves_the_others_alone(M):
     held(d, *want, "dx")
 
 
+@pytest.mark.parametrize("t", [BF16, FP16])
+@pytest.mark.parametrize("M", [3, 5, 260])
+def test_ffn_an_infinite_weight_reaches_the_bias_gradients_as_it_is(M, t):
+    """dh = inf in one feature of every row: db_up there is inf -- the rows that fill a tile up behind the last one must not make a NaN of it"""
+    a = [torch.ones(M, 64, dtype=t, device="cuda"), *(torch.full((136, 64), 2.0 ** -6, dtype=t, device="cuda") for _ in range(2))]
+    wd = torch.full((64, 136), 2.0 ** -6, dtype=t, device="cuda")
+    wd[5, 77] = math.inf
+    y, saved = blocks().gated_ffn(*a, wd, activation="sigmoid", save=True)
+    d = blocks().gated_ffn_backward(torch.ones_like(a[0]), *a, wd, saved, bias=True, activation="sigmoid")
+    for n in ("db_gate", "db_up"):
+        assert float(d[n][77]) == math.inf and bool(d[n][:77].isfinite().all()) and bool(d[n][78:].isfinite().all()), n
+
+
 @pytest.mark.parametrize("M", [1, 4, 5])
 def test_ffn_weights_below_the_normal_numbers(M):
     """weights of 2^-20 (fp16 holds them as subnormal numbers): g = 64 x 2^-20 = 2^-14, u = 1, y = 64 x 2^-14 x 4096 = 16, exactly"""
