@@ -565,9 +565,10 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
     wait_all_and_meet();
     float* corner = reinterpret_cast<float*>(conv_lds_dyn) + wave * 32 * RS;
     const int cl = lane % LN, rl = lane / LN;
-    // (one copy of what follows: unrolled over the blocks it does not fit the instruction cache)
+    // (GATE, DH: one copy of what follows: unrolled over the blocks the activations do not fit the instruction cache)
     int guess_g = 0, guess_u = 0;                                          // DH, fp16: the exponents that the next block's dG and dU are stored with first
-#pragma unroll 1
+    constexpr int BLOCKS_AT_ONCE = EPI == EPI_OUT ? IM : 1, STEPS_AT_ONCE = EPI == EPI_OUT ? 4 : 1;
+#pragma unroll BLOCKS_AT_ONCE
     for (int i = 0; i < IM; ++i) {
 #pragma unroll
         for (int k = 0; k < IM; ++k) {
@@ -624,9 +625,9 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
             static_assert(!F16 || (SF == 8 && WN == 64), "8 rows x 32 features");
             GroupCheck<false> check;
             const bool live = (n0 + wn * WN) / 2 < p.F;
-            const auto hidden = [&](int r, float (&g)[4], float (&u)[4], float (&o)[4]) {
+            const auto hidden = [&](auto whole, int r, float (&g)[4], float (&u)[4], float (&o)[4]) {
                 const float4 g4 = *reinterpret_cast<const float4*>(rows + (r + r2) * RS + gc), u4 = *reinterpret_cast<const float4*>(rows + (r + r2) * RS + gc + 32);
-                const bool in = mb + r + r2 < p.M && f < p.F;
+                const bool in = decltype(whole)::value || (mb + r + r2 < p.M && f < p.F);
                 g[0] = g4.x + bg[0]; g[1] = g4.y + bg[1]; g[2] = g4.z + bg[2]; g[3] = g4.w + bg[3];
                 u[0] = u4.x + bu[0]; u[1] = u4.y + bu[1]; u[2] = u4.z + bu[2]; u[3] = u4.w + bu[3];
 #pragma unroll
@@ -636,13 +637,15 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
             const auto put = [&](int r, const float (&o)[4], float by) {
                 *reinterpret_cast<uint2*>(p.C + (int64_t)(mb + r + r2) * p.F + f) = make_uint2(T16<F16>::pack2(o[0] * by, o[1] * by), T16<F16>::pack2(o[2] * by, o[3] * by));
             };
+            // (a block that lies in the matrix as a whole has no masks between its steps)
+            const auto store = [&](auto whole) {
 #pragma unroll
             for (int r = R0; r < R0 + RN; r += SF) {
                 float g[4], u[4], o[4];
-                const bool in = hidden(r, g, u, o);
+                const bool in = hidden(whole, r, g, u, o);
                 if constexpr (F16) {
                     check.add(o, true);
-                    check.close(ALL_LANES, live && mb + r < p.M);
+                    check.close(ALL_LANES, decltype(whole)::value || (live && mb + r < p.M));
                 }
                 if (!in) continue;
                 if (p.g) {
@@ -652,6 +655,9 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
                 }
                 put(r, o, 1.0f);
             }
+            };
+            if (mb + 32 <= p.M && (n0 + wn * WN) / 2 + 32 <= p.F) store(std::true_type());
+            else store(std::false_type());
             if constexpr (F16) {
                 int8_t* ex = p.ex + (int64_t)(f / 32) * ((p.M + 31) / 32 * 4) + (mb + R0) / 8;
                 const bool first = lane == 0 && live && mb < p.M;
@@ -662,7 +668,7 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
 #pragma unroll 1
                     for (int r = R0; r < R0 + RN; r += SF) {
                         float g[4], u[4], o[4];
-                        const bool in = hidden(r, g, u, o);
+                        const bool in = hidden(std::false_type(), r, g, u, o);
                         float mx = finite_max(o);
 #pragma unroll
                         for (int k = 1; k < 64; k <<= 1) mx = fmaxf(mx, __shfl_xor(mx, k));
@@ -689,10 +695,10 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
             GroupCheck<true> ch;                                              // (h: what GATE has scaled has to be found again)
             const bool live = n0 + wn * WN < p.N, live2 = n0 + wn * WN + 32 < p.N;
             const auto in_range = [&](int r) { return mb + r + rl < p.M && n < p.N; };
-            const auto grads = [&](int r, float (&dg)[4], float (&du)[4], float (&hh)[4]) {         // (outside: all 0)
+            const auto grads = [&](auto whole, int r, float (&dg)[4], float (&du)[4], float (&hh)[4]) {         // (outside: all 0)
                 const int64_t at = (int64_t)(mb + r + rl) * p.F + n;
                 float4 g4 = make_float4(0.f, 0.f, 0.f, 0.f), u4 = g4, o = g4;          // (a zero row's product with an infinite weight is none)
-                if (in_range(r)) {
+                if (decltype(whole)::value || in_range(r)) {
                     o = *reinterpret_cast<const float4*>(rows + (r + rl) * RS + 4 * cl);
                     g4 = *reinterpret_cast<const float4*>(p.g + at);
                     u4 = *reinterpret_cast<const float4*>(p.u + at);
@@ -714,15 +720,17 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
                 *reinterpret_cast<uint2*>(p.h + (int64_t)(mb + r + rl) * p.F + n) =
                     make_uint2(T16<F16>::pack2(hh[0] * by, hh[1] * by), T16<F16>::pack2(hh[2] * by, hh[3] * by));
             };
-#pragma unroll 1
+            const auto store = [&](auto whole_) {
+            constexpr bool whole = decltype(whole_)::value;
+#pragma unroll STEPS_AT_ONCE
             for (int r8 = R0; r8 < R0 + RN; r8 += 8)
 #pragma unroll
             for (int r = r8; r < r8 + 8; r += STEP) {
                 const int m = mb + r + rl;
                 if constexpr (EPI == EPI_DH) {
-                    if (!F16 && !in_range(r)) continue;
+                    if (!F16 && !whole && !in_range(r)) continue;
                     float dg[4], du[4], hh[4];
-                    grads(r, dg, du, hh);
+                    grads(whole_, r, dg, du, hh);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         sg[e] += dg[e];
@@ -741,17 +749,17 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
 #pragma unroll
                             for (int k = 0; k < 2; ++k) {
                                 const uint64_t lanes = k == 0 ? LOW_COLUMNS : ~LOW_COLUMNS;
-                                const bool in = (k == 0 ? live : live2) && mb + r - 4 < p.M;
+                                const bool in = whole || ((k == 0 ? live : live2) && mb + r - 4 < p.M);
                                 cg.close(lanes, in);
                                 cu.close(lanes, in);
                                 ch.close(lanes, in);
                             }
-                        if (!in_range(r)) continue;
+                        if (!whole && !in_range(r)) continue;
                     }
                     put_d(p.C, r, dg, 1.0f);
                     put_d(p.C + p.F, r, du, 1.0f);
                 } else {
-                    if (!in_range(r)) continue;
+                    if (!whole && !in_range(r)) continue;
                     const float4 o = *reinterpret_cast<const float4*>(rows + (r + rl) * RS + 4 * cl);
                     if (p.splits > 1) {
                         *reinterpret_cast<float4*>(p.part + ((int64_t)split * p.M + m) * p.N + n) = o;
@@ -763,6 +771,9 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
                     }
                 }
             }
+            };
+            if (mb + 32 <= p.M && n0 + wn * WN + WN <= p.N) store(std::true_type());
+            else store(std::false_type());
             if constexpr (F16 && EPI == EPI_DH) {
                 const int64_t ex = (int64_t)(n / 32) * ((p.M + 31) / 32 * 4) + (mb + R0) / 8;
                 const bool first = (lane & ~8) == 0 && n < p.N && mb < p.M;
@@ -783,7 +794,7 @@ __global__ __launch_bounds__(NWM * NWN * NWK * 64, NWM * NWN >= 8 ? 2 : 1) void 
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             float dg[4], du[4], hh[4];
-                            grads(r + 4 * k, dg, du, hh);
+                            grads(std::false_type(), r + 4 * k, dg, du, hh);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) v[k][e] = pick(dg[e], du[e], hh[e]);
                         }
