@@ -15,6 +15,7 @@ namespace isb {
 namespace {
 
 constexpr int KT = 64;                    // states per tile
+constexpr int FEW_STATES = KT;            // up to these many P and dS enter products with their rests (rest8)
 constexpr float NEG_INF = -__builtin_inff();
 
 // element offset of row r of group (bk, hk) in a [B, Lq, Hq, .] tensor with strides sb, sl, sh
@@ -100,9 +101,30 @@ __device__ __forceinline__ void reads_stay() { __builtin_amdgcn_sched_barrier(0x
 template <bool F16> constexpr float P_UP = F16 ? 12.0f : 0.0f;              // log2 of the factor on P
 template <bool F16> constexpr float P_LAG = F16 ? 3.0f : 8.0f;
 
+template <bool F16>
+__device__ __forceinline__ uint4 pack8(const f32x16& x, int t) {
+    return t == 0 ? make_uint4(T16<F16>::pack2(x[0], x[1]), T16<F16>::pack2(x[2], x[3]), T16<F16>::pack2(x[4], x[5]), T16<F16>::pack2(x[6], x[7]))
+                  : make_uint4(T16<F16>::pack2(x[8], x[9]), T16<F16>::pack2(x[10], x[11]), T16<F16>::pack2(x[12], x[13]), T16<F16>::pack2(x[14], x[15]));
+}
+// What that rounds off, as a second operand. Where a sum has few terms (up to FEW_STATES states, up to 64 rows) the roundings of P and dS do not average
+// out: they scale whole rows of V, K, dout or Q, and the results are as far off as with roundings of their own, or further. There both operands
+// enter (hi + lo: 2^-16 or better), which costs a few products of a launch that waits for its loads.
+template <bool F16>
+__device__ __forceinline__ uint4 rest8(const f32x16& x, int t, const uint4& hi) {
+    const uint32_t w[4] = {hi.x, hi.y, hi.z, hi.w};
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float a = t == 0 ? x[2 * i] : x[8 + 2 * i], b = t == 0 ? x[2 * i + 1] : x[9 + 2 * i];
+        r[i] = T16<F16>::pack2(a - T16<F16>::lo(w[i]), b - T16<F16>::hi(w[i]));
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
 // One block of NB x 32 states for 32 rows (a column of S^T each): scores, running maximum (m: less P_UP) and sum, O^T += V^T P^T.
 // The maximum follows lazily: O^T is rescaled only when a row's maximum grows by more than P_LAG (base-2 units), so P <= 2^15 (fp16), 2^8.
-template <bool F16, int DT, int NB>
+// FEW: with the rest of P (rest8).
+template <bool F16, int DT, int NB, bool FEW = false>
 __device__ __forceinline__ void attend(const unsigned char* kt, const unsigned char* vt, const uint4 (&qf)[DT / 16], f32x16 (&acc)[DT / 32],
                                        float& m, float& l, float c, const float* bias, bool all, int lane) {
     const int h = lane >> 5;
@@ -150,18 +172,18 @@ __device__ __forceinline__ void attend(const unsigned char* kt, const unsigned c
     for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-            float e[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][8 * t + i], c, -mu));
-                sum += e[i];
+                s[b][8 * t + i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][8 * t + i], c, -mu));
+                sum += s[b][8 * t + i];
             }
-            p[2 * b + t] = make_uint4(T16<F16>::pack2(e[0], e[1]), T16<F16>::pack2(e[2], e[3]), T16<F16>::pack2(e[4], e[5]), T16<F16>::pack2(e[6], e[7]));
+            p[2 * b + t] = pack8<F16>(s[b], t);
         }
     l += sum;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         acc[i / NT] = T16<F16>::mfma32(vf[i % AHEAD], p[i % NT], acc[i / NT]);
+        if constexpr (FEW) acc[i / NT] = T16<F16>::mfma32(vf[i % AHEAD], rest8<F16>(s[i % NT / 2], i % 2, p[i % NT]), acc[i / NT]);
         if (i + AHEAD < NV) vf[i % AHEAD] = frag_cols<DT, 4, 8>(vt, 16 * ((i + AHEAD) % NT), 32 * ((i + AHEAD) / NT), lane);
         reads_stay();
     }
@@ -199,7 +221,7 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XattnArgs a) {
     constexpr int TB = KT * DT * 2, STAGE = 2 * TB + KT * 4;
 
     const int len = states_of(a, bk), k0 = split * a.chunk, k1 = min(len, k0 + a.chunk);
-    const int nt = k1 > k0 ? (k1 - k0 + KT - 1) / KT : 0;
+    int nt = k1 > k0 ? (k1 - k0 + KT - 1) / KT : 0;
 
     uint4 qf[DT / 16];
     {
@@ -234,6 +256,14 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XattnArgs a) {
         byte = mask_byte(a, bk, k0 + lane, k1);
         bits = __ballot(byte != 0);
         request(0, bits, 0);
+    }
+    if (nt == 1 && len <= FEW_STATES) {
+        wait_all_and_meet();
+        for (int b = 0; b < 2; ++b)
+            if (bits >> (32 * b) & 0xffffffffu)
+                attend<F16, DT, 1, true>(conv_lds_dyn + 32 * b * DT * 2, conv_lds_dyn + TB + 32 * b * DT * 2, qf, acc, m, l, a.c,
+                                         reinterpret_cast<const float*>(conv_lds_dyn + 2 * TB) + 32 * b, bits == ~0ull, lane);
+        nt = 0;
     }
     for (int t = 0; t < nt; ++t) {
         next = __ballot(byte != 0);
@@ -306,7 +336,13 @@ __global__ __launch_bounds__(TOKEN_WAVES * 64, TOKEN_WAVES / 4) void xattn_token
     };
     byte = valid(wave);
     if (wave < nt) request(wave);
-    for (int t = wave; t < nt; t += NW) {
+    int t = wave;
+    if (len <= FEW_STATES && t < nt) {                                        // (at most one block per wave)
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if (bits != 0) attend<F16, DT, 1, true>(own, own + TB, qf, acc, m, l, a.c, bias, bits == ~0u, lane);
+        t = nt;
+    }
+    for (; t < nt; t += NW) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         if (bits != 0) attend<F16, DT, 1>(own, own + TB, qf, acc, m, l, a.c, bias, bits == ~0u, lane);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                    // the block is read before its place is requested again
@@ -464,12 +500,6 @@ __device__ __forceinline__ void scale_ds(f32x16& ds, f32x16 (&acc)[NA], float& s
         for (int i = 0; i < 16; ++i) ds[i] *= by;
     }
 }
-template <bool F16>
-__device__ __forceinline__ uint4 pack8(const f32x16& x, int t) {
-    return t == 0 ? make_uint4(T16<F16>::pack2(x[0], x[1]), T16<F16>::pack2(x[2], x[3]), T16<F16>::pack2(x[4], x[5]), T16<F16>::pack2(x[6], x[7]))
-                  : make_uint4(T16<F16>::pack2(x[8], x[9]), T16<F16>::pack2(x[10], x[11]), T16<F16>::pack2(x[12], x[13]), T16<F16>::pack2(x[14], x[15]));
-}
-
 // dK, dV: S = Q K^T with the rows in the accumulator's rows and a state per lane; P and dS are then operands over the rows. 2 x 16 heads, 4096 rows
 // and states: 856 us 128 wide (642 TFLOP/s: dK, dV, K and V of a wave's 32 states need more than 256 registers, so a SIMD has one wave, and
 // its products wait for LDS), 334 us 64 wide (823, two waves).
@@ -485,7 +515,8 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
     const bool ok = mask_byte(a, bk, key, len) != 0;
     constexpr int RT = DKV_ROWS, TB = RT * DT * 2, STAGE = 2 * TB + RT * 8, CH = DT / 8;    // RT rows of Q, of dout, their lse, their delta
     constexpr int PC = RT * CH / 256;                                         // 16-byte chunks per thread and tensor
-    const int r0 = split * a.chunk, r1 = min(a.M, r0 + a.chunk), nt = __syncthreads_or(ok) ? (r1 - r0 + RT - 1) / RT : 0;
+    const int r0 = split * a.chunk, r1 = min(a.M, r0 + a.chunk);
+    int nt = __syncthreads_or(ok) ? (r1 - r0 + RT - 1) / RT : 0;
 
     uint4 kf[DT / 16], vf[DT / 16];
     {
@@ -532,6 +563,40 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
     };
     if (nt > 0) { fetch(0); put(0); }
     wait_all_and_meet();
+    if (a.M <= RT && nt > 0) {                                                 // few rows: one tile, P and dS with their rests (rest8)
+#pragma unroll 1
+        for (int rb = 0; rb < 2; ++rb) {
+            const float* st = reinterpret_cast<const float*>(conv_lds_dyn + 2 * TB) + 32 * rb;
+            f32x16 s, dp;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = 0.f; }
+#pragma unroll
+            for (int ks = 0; ks < DT / 16; ++ks) {
+                s = T16<F16>::mfma32(frag_rows<DT>(conv_lds_dyn, 32 * rb, ks, lane), kf[ks], s);
+                dp = T16<F16>::mfma32(frag_rows<DT>(conv_lds_dyn + TB, 32 * rb, ks, lane), vf[ks], dp);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int row = 8 * (i / 4) + 4 * h + i % 4;
+                s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.c, st[row]));
+                dp[i] = s[i] * (dp[i] - st[RT + row]);
+            }
+            scale_ds<F16, DT / 32>(dp, dk, sc);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint4 w = pack8<F16>(s, u), x = pack8<F16>(dp, u), wr = rest8<F16>(s, u, w), xr = rest8<F16>(dp, u, x);
+#pragma unroll
+                for (int d = 0; d < DT / 32; ++d) {
+                    const uint4 o = frag_cols<DT, 4, 8>(conv_lds_dyn + TB, 32 * rb + 16 * u, 32 * d, lane), q = frag_cols<DT, 4, 8>(conv_lds_dyn, 32 * rb + 16 * u, 32 * d, lane);
+                    dv[d] = T16<F16>::mfma32(o, w, dv[d]);
+                    dv[d] = T16<F16>::mfma32(o, wr, dv[d]);
+                    dk[d] = T16<F16>::mfma32(q, x, dk[d]);
+                    dk[d] = T16<F16>::mfma32(q, xr, dk[d]);
+                }
+            }
+        }
+        nt = 0;
+    }
     for (int t = 0; t < nt; ++t) {
         if (t + 1 < nt) fetch((t + 1) & 1);
         // two blocks of 32 rows, one behind the other: while the matrix cores form the second block's S and dP, the vector ALU makes P and dS of
@@ -634,7 +699,9 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
         }
 }
 
-// What a row of dQ (a lane and its other half) holds while it walks the states: Q, dout, P_UP - lse (base 2) and delta = rowsum(dout o out)
+// What a row of dQ (a lane and its other half) holds while it walks the states: Q, dout, P_UP - lse (base 2) and delta = rowsum(dout o out), with out
+// as it was rounded. That rounding meets dP = dout v directly and weighs 1 / sqrt(n) of dS's own with n states: up to 32 of them delta is formed
+// anew from P and dP.
 template <bool F16, int DT>
 struct GradRow {
     uint4 q[DT / 16], d[DT / 16];
@@ -658,9 +725,10 @@ struct GradRow {
         de = sum_halves(de);
     }
 };
-// dQ^T += K^T dS^T of 32 states (tiles in LDS)
-template <bool F16, int DT>
-__device__ __forceinline__ void add_dq(const unsigned char* ktile, const unsigned char* vtile, const GradRow<F16, DT>& g, f32x16 (&acc)[DT / 32],
+// dQ^T += K^T dS^T of 32 states (tiles in LDS). REST: with the rest of dS (rest8); WHOLE: they are all that the row has, delta = sum P dP
+enum { MANY, REST, WHOLE };
+template <bool F16, int DT, int FEW = MANY>
+__device__ __forceinline__ void add_dq(const unsigned char* ktile, const unsigned char* vtile, GradRow<F16, DT>& g, f32x16 (&acc)[DT / 32],
                                        float& sc, float c, const float* bias, bool all, int lane) {
     const int h = lane >> 5;
     f32x16 s, ds;
@@ -685,7 +753,15 @@ __device__ __forceinline__ void add_dq(const unsigned char* ktile, const unsigne
     for (int i = 0; i < AHEAD; ++i) f[i] = column(i);
     reads_stay();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) ds[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, g.nl)) * (ds[i] - g.de);
+    for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], c, g.nl));
+    if constexpr (FEW == WHOLE) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t = __builtin_fmaf(s[i], ds[i], t);
+        g.de = sum_halves(t) * __builtin_amdgcn_exp2f(-P_UP<F16>);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) ds[i] = s[i] * (ds[i] - g.de);
     scale_ds<F16, DT / 32>(ds, acc, sc);
     uint4 p[2];
 #pragma unroll
@@ -693,6 +769,7 @@ __device__ __forceinline__ void add_dq(const unsigned char* ktile, const unsigne
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
         acc[i / 2] = T16<F16>::mfma32(f[i % AHEAD], p[i % 2], acc[i / 2]);
+        if constexpr (FEW != MANY) acc[i / 2] = T16<F16>::mfma32(f[i % AHEAD], rest8<F16>(ds, i % 2, p[i % 2]), acc[i / 2]);
         if (i + AHEAD < NC) f[i % AHEAD] = column(i + AHEAD);
         reads_stay();
     }
@@ -709,7 +786,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
     const int r = rt * 128 + wave * 32 + (lane & 31);
     constexpr int TB = KT * DT * 2, STAGE = 2 * TB + KT * 4;
     const int len = states_of(a, bk), k0 = split * a.chunk, k1 = min(len, k0 + a.chunk);
-    const int nt = k1 > k0 ? (k1 - k0 + KT - 1) / KT : 0;
+    int nt = k1 > k0 ? (k1 - k0 + KT - 1) / KT : 0;
 
     const RowAt w = row_at(a, bk, hk, min(r, a.M - 1));
     GradRow<F16, DT> g;
@@ -742,6 +819,19 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
         byte = mask_byte(a, bk, k0 + lane, k1);
         bits = __ballot(byte != 0);
         request(0, bits, 0);
+    }
+    if (nt == 1 && len <= FEW_STATES) {
+        wait_all_and_meet();
+        const float* bias = reinterpret_cast<const float*>(conv_lds_dyn + 2 * TB);
+        if (len <= 32) {
+            if (bits != 0) add_dq<F16, DT, WHOLE>(conv_lds_dyn, conv_lds_dyn + TB, g, acc, sc, a.c, bias, false, lane);
+            if (h == 0 && r < a.M) a.delta[(int64_t)grp * a.M + r] = g.de;
+        } else {
+#pragma unroll 1
+            for (int b = 0; b < 2; ++b)
+                add_dq<F16, DT, REST>(conv_lds_dyn + 32 * b * DT * 2, conv_lds_dyn + TB + 32 * b * DT * 2, g, acc, sc, a.c, bias + 32 * b, bits == ~0ull, lane);
+        }
+        nt = 0;
     }
     for (int t = 0; t < nt; ++t) {
         next = __ballot(byte != 0);
@@ -814,7 +904,18 @@ __global__ __launch_bounds__(TOKEN_WAVES * 64, TOKEN_WAVES / 4) void xattn_dq_fe
     };
     byte = valid(wave);
     if (wave < nt) request(wave);
-    for (int t = wave; t < nt; t += NW) {
+    int t = wave;
+    if (len <= FEW_STATES && t < nt) {                                        // (at most one block per wave)
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if (nt == 1) {
+            if (bits != 0) add_dq<F16, DT, WHOLE>(own, own + TB, g, acc, sc, a.c, bias, bits == ~0u, lane);
+            if (h == 0 && row < a.M) a.delta[(int64_t)grp * a.M + row] = g.de;
+        } else {
+            add_dq<F16, DT, REST>(own, own + TB, g, acc, sc, a.c, bias, bits == ~0u, lane);
+        }
+        t = nt;
+    }
+    for (; t < nt; t += NW) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         if (bits != 0) add_dq<F16, DT>(own, own + TB, g, acc, sc, a.c, bias, bits == ~0u, lane);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                    // the block is read before its place is requested again

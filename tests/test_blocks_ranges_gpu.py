@@ -246,3 +246,53 @@ def test_xattn_weights_far_below_a_row_s_largest(Lq, Lk):
     want = torch.full(out.shape, w / (1 + w), dtype=torch.float64, device="cuda")
     held(out, want, want * (2 * 2.0 ** -11 + 2 ** -22 + (Lk + 64) * E) + 2.0 ** -25, "out")
     held(lse, torch.full(lse.shape, math.log1p(w), dtype=torch.float64, device="cuda"), torch.full(lse.shape, (Lk + 64) * E * 2, dtype=torch.float64, device="cuda"), "lse")
+
+
+@pytest.mark.parametrize("t", [BF16, FP16])
+@pytest.mark.parametrize("B,Bk,Lq,Lk,Hq,Hk,D,lens", [
+    (1, 1, 1, 2, 1, 1, 64, None), (4, 4, 1, 5, 4, 4, 96, None), (11, 1, 4, 5, 4, 1, 64, None), (2, 2, 1, 54, 1, 1, 128, [54, 27]), (3, 3, 3, 32, 2, 2, 72, [32, 1, 9]),
+    (2, 2, 40, 64, 2, 2, 128, [64, 33]), (3, 3, 200, 30, 2, 1, 64, [30, 2, 4]), (4, 4, 1, 300, 2, 2, 64, [2, 3, 60, 31]), (2, 2, 70, 2500, 1, 1, 128, [4, 40]),
+    (3, 3, 130, 700, 1, 1, 128, [5, 33, 64])])
+def test_xattn_few_states_or_rows(B, Bk, Lq, Lk, Hq, Hk, D, lens, t):
+    """up to 64 states enter P and dS whole (two operands: u^2 of a rounding is left, and fp16's steps of 2^-24 behind 2^12 P and a dS of 2^10), up to
+    64 rows the same for dk and dv; up to 32 states delta is sum P dP in f32 (before, out's rounding stood in it). What is left: one rounding u
+    of each result and f32's part -- ep as in blocks_ref, D + 16 terms in dP, Lk + 16 in delta."""
+    g = gen(D + Lk)
+    q, dout = normal(g, B, Lq, Hq, D, type=t), normal(g, B, Lq, Hq, D, type=t)
+    k, v = normal(g, Bk, Lk, Hk, D, type=t), normal(g, Bk, Lk, Hk, D, type=t)
+    kv_len = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out, lse = blocks().cross_attention(q, k, v, kv_len=kv_len)
+    dq, dk, dv = blocks().cross_attention_backward(dout, q, k, v, out, lse, kv_len=kv_len)
+    u, G, nb, scale = ref.half_step(t), Hq // Hk, B // Bk, 1 / math.sqrt(D)
+    rest = u * u + 2 * E
+    for b in range(Bk):
+        n = Lk if lens is None else lens[b]
+        for h in range(Hk):
+            bs, hs = slice(b * nb, (b + 1) * nb), slice(h * G, (h + 1) * G)
+            Q, dO = (x[bs, :, hs].double().reshape(-1, D) for x in (q, dout))
+            K, V = k[b, :n, h].double(), v[b, :n, h].double()
+            s = Q @ K.T * scale
+            P = torch.softmax(s, -1)
+            es = ((Q.abs() @ K.abs().T) * scale * (D + 4) * E + s.abs() * 4 * E).amax(-1, keepdim=True)
+            ep = 2 * es + 8 * E + (n + 64) * E
+            o = P @ V
+            held(out[bs, :, hs].reshape(-1, D), o, u * o.abs() + (P @ V.abs()) * (ep + rest) * (1 + u) + 2.0 ** -25 + (2.0 ** -36 if t == FP16 else 0) * V.abs().sum(0), "out")
+            dP = dO @ V.T
+            abs_dP = dO.abs() @ V.abs().T
+            delta = (P * dP).sum(-1, keepdim=True)
+            dS = P * (dP - delta)
+            edelta = (P * abs_dP).sum(-1, keepdim=True) * (ep + (D + n + 32) * E)
+            if n > 32:                                                      # rowsum(dout o out) with out as it was rounded
+                edelta = edelta + (dO.abs() * (u * o.abs() + 2.0 ** -25)).sum(-1, keepdim=True)
+            edS = dS.abs() * (ep + rest) + P * (edelta + (D + 16) * E * abs_dP) * (1 + u)
+            tiny = 2.0 ** -34 if t == FP16 else 0.0
+            want = dS @ K * scale
+            held(dq[bs, :, hs].reshape(-1, D), want, u * want.abs() + scale * ((edS + tiny * dS.abs().amax(-1, keepdim=True)) @ K.abs()) * (1 + u) + 2.0 ** -25, "dq")
+            M = Q.shape[0]
+            if M > 64:
+                continue
+            want = dS.T @ Q * scale
+            held(dk[b, :n, h], want, u * want.abs() + scale * ((edS + tiny * dS.abs().amax(0)).T @ Q.abs() + (M + 16) * E * (dS.abs().T @ Q.abs())) * (1 + u) + 2.0 ** -25, "dk")
+            want = P.T @ dO
+            held(dv[b, :n, h], want, u * want.abs() + ((P * (ep + rest)).T @ dO.abs() + (M + 16) * E * (P.T @ dO.abs())) * (1 + u) + 2.0 ** -25
+                 + (2.0 ** -36 if t == FP16 else 0) * dO.abs().sum(0), "dv")
