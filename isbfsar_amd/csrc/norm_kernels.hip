@@ -336,17 +336,20 @@ __global__ __launch_bounds__(MOST, MOST <= 256 ? 3 : 4) void norm_bwd_kernel(Nor
         if (c + i < D) { p[c + i] = s0[i]; p[D + c + i] = s1[i]; p[2 * D + c + i] = s2[i]; p[3 * D + c + i] = s3[i]; }
 }
 
-// sums over the chunks of a sample: part [B, chunks, 4, D] -> joint [B, 4, D], and the sample's dgate. 64 columns x 4 chunk lanes.
-// (`total` chunks in all: after MANY they stand in groups of JOIN, the last of which may be part full)
+// sums over the chunks of a sample: part [B, chunks, 4, D] -> joint [B, 4, D], and the sample's dgate. COLS columns x 256 / COLS chunk lanes: 64 x 4, or
+// 16 x 16 for long lists of chunks (4 samples of 768 chunks of 512: 75 us with 64 x 4).
+// (`total` chunks in all: those of no sample in particular -- no gate, MANY -- stand in groups of JOIN, the last of which may be part full: in one
+// group 1022 chunks of 1280 took 82 us)
 constexpr int JOIN = 64;
-template <int DT>
+template <int DT, int COLS>
 __global__ __launch_bounds__(256) void norm_join_kernel(NormArgs a, float* joint, int total) {
     if constexpr (DT == 1) T16<true>::enter();
-    __shared__ float red[4][4][64];
-    const int cl = threadIdx.x & 63, kl = threadIdx.x >> 6, b = blockIdx.y, c = blockIdx.x * 64 + cl, D = a.D;
+    constexpr int LANES = 256 / COLS;
+    __shared__ float red[LANES][4][COLS];
+    const int cl = threadIdx.x % COLS, kl = threadIdx.x / COLS, b = blockIdx.y, c = blockIdx.x * COLS + cl, D = a.D;
     float s[4] = {};
     if (c < D)
-        for (int k = kl; k < min(a.chunks, total - b * a.chunks); k += 4) {
+        for (int k = kl; k < min(a.chunks, total - b * a.chunks); k += LANES) {
             const float* p = a.part + ((int64_t)b * a.chunks + k) * 4 * D + c;
 #pragma unroll
             for (int j = 0; j < 4; ++j) s[j] += p[j * D];
@@ -354,14 +357,17 @@ __global__ __launch_bounds__(256) void norm_join_kernel(NormArgs a, float* joint
 #pragma unroll
     for (int j = 0; j < 4; ++j) red[kl][j][cl] = s[j];
     __syncthreads();
-    if (c >= D) return;
-    if (joint != a.part) joint[((int64_t)b * 4 + kl) * D + c] = red[0][kl][cl] + red[1][kl][cl] + red[2][kl][cl] + red[3][kl][cl];
-    if (kl == 0 && a.dgate) {
-        float t[2];
+    if (c >= D || kl >= 4) return;
+    const auto sum = [&](int j) {
+        float t = red[0][j][cl];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) t[j] = red[0][j][cl] + red[1][j][cl] + red[2][j][cl] + red[3][j][cl];
+        for (int k = 1; k < LANES; ++k) t += red[k][j][cl];
+        return t;
+    };
+    if (joint != a.part) joint[((int64_t)b * 4 + kl) * D + c] = sum(kl);
+    if (kl == 0 && a.dgate) {
         const float w = a.post_w ? a.post_w[c] : 1.f, q = a.post_b ? a.post_b[c] : 0.f;
-        const float v = (a.scale ? a.scale[c] : 1.f) * (w * t[1] + q * t[0]);
+        const float v = (a.scale ? a.scale[c] : 1.f) * (w * sum(1) + q * sum(0));
         if constexpr (DT == 0) static_cast<float*>(a.dgate)[(int64_t)b * D + c] = v;
         else static_cast<uint16_t*>(a.dgate)[(int64_t)b * D + c] = T16<DT == 1>::from_f32(v);
     }
@@ -424,6 +430,7 @@ bool plan(NormArgs& a) {
     a.chunks = cdiv(n, a.rows_per_chunk);
     return many;
 }
+bool grouped(const NormArgs& a) { return !a.gate && a.chunks > JOIN; }
 template <int DT>
 int fwd(const NormArgs& a, hipStream_t st) {
     const int rows = a.B * a.L, threads = 64 * cdiv(a.D, 512);
@@ -452,19 +459,19 @@ int bwd(NormArgs a, float* ws, hipStream_t st) {
     const bool many = plan(a);
     const int total = many ? a.chunks : a.B * a.chunks;
     a.part = ws;
-    if (many) {
-        bwd_rows<DT, true>(a, (unsigned)total, st);
-        a.B = cdiv(total, JOIN);                             // what is left to add up knows no gate
+    if (many) bwd_rows<DT, true>(a, (unsigned)total, st);
+    else bwd_rows<DT, false>(a, (unsigned)total, st);
+    if (many || grouped(a)) {                                // what is left to add up knows no gate
+        a.B = cdiv(total, JOIN);
         a.chunks = JOIN;
         a.gate = nullptr;
         a.dgate = nullptr;
-    } else {
-        bwd_rows<DT, false>(a, (unsigned)total, st);
     }
     ISB_LAUNCHED("norm_bwd", st);
     float* joint = a.chunks == 1 ? ws : ws + (int64_t)total * 4 * a.D;
     if (joint != ws || a.dgate) {
-        norm_join_kernel<DT><<<dim3(cdiv(a.D, 64), a.B), 256, 0, st>>>(a, joint, total);
+        if (a.chunks > JOIN) norm_join_kernel<DT, 16><<<dim3(cdiv(a.D, 16), a.B), 256, 0, st>>>(a, joint, total);
+        else norm_join_kernel<DT, 64><<<dim3(cdiv(a.D, 64), a.B), 256, 0, st>>>(a, joint, total);
         ISB_LAUNCHED("norm_join", st);
     }
     norm_params_kernel<DT><<<cdiv(a.D, 32), 1024, 0, st>>>(a, joint);
@@ -475,7 +482,7 @@ int bwd(NormArgs a, float* ws, hipStream_t st) {
 
 size_t norm_workspace(const NormArgs& a0) {
     NormArgs a = a0;
-    if (plan(a)) return ((size_t)a.chunks + cdiv(a.chunks, JOIN)) * 4 * a.D * sizeof(float);
+    if (plan(a) || grouped(a)) return ((size_t)a.chunks + cdiv(a.chunks, JOIN)) * 4 * a.D * sizeof(float);
     return ((size_t)a.B * a.chunks + (a.chunks == 1 ? 0 : a.B)) * 4 * a.D * sizeof(float);
 }
 int launch_norm_fwd(const NormArgs& a, int dtype, hipStream_t st) { return dtype == 0 ? fwd<0>(a, st) : dtype == 1 ? fwd<1>(a, st) : fwd<2>(a, st); }
