@@ -58,13 +58,13 @@ def _first(name: str, t, types) -> None:
         _on_tape(name)
 
 
-def _tensor(name: str, t, dtype, device, shape) -> None:
-    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+def _tensor(name: str, t, dtype, dev: int, shape) -> None:
+    if not (isinstance(t, torch.Tensor) and (t.get_device() == dev or t.is_cuda)):
         raise TypeError(f"{name} must be a torch CUDA tensor")
     if t.dtype is not dtype:
         raise TypeError(f"{name} is {t.dtype}, expected {dtype}")
-    if t.device != device:
-        raise ValueError(f"{name} lives on {t.device}, the first tensor on {device}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name} lives on {t.device}, the first tensor on cuda:{dev}")
     if t.shape != shape:
         raise ValueError(f"{name}: expected {tuple(shape)}, got {tuple(t.shape)}")
     if t.requires_grad and torch.is_grad_enabled():
@@ -105,11 +105,6 @@ def _workspace(fn, what: str, args, *more) -> int:
     return n.value
 
 
-def _address(t: torch.Tensor) -> int:
-    """t's address; of an empty tensor one that is not null (nothing is read there)"""
-    return t.data_ptr() or 16
-
-
 # the current stream's handle: the raw query costs 0.1 us of the 4 us that a launch takes, the stream object 2
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
@@ -121,7 +116,7 @@ def _stream(index: int) -> int:
 # ------------------------------------------------------------------------------------------------ cross attention
 def _xattn_args(q, k, v, kv_len, key_mask, scale):
     _first("q", q, _HALF)
-    t, dev = q.dtype, q.device
+    t, dev = q.dtype, q.get_device()
     if q.dim() != 4 or not isinstance(k, torch.Tensor) or k.dim() != 4:
         _refuse("expected q [B,Lq,Hq,D] and k, v [Bk,Lk,Hk,D]")
     B, Lq, Hq, D = q.shape
@@ -131,7 +126,7 @@ def _xattn_args(q, k, v, kv_len, key_mask, scale):
     q, qs = _rows16(q)
     k, ks = _rows16(k, 1)
     v, vs = _rows16(v, 1)
-    a = _lib.isb_xattn_args(dev.index, _TYPES[t], B, Bk, Lq, Lk, Hq, Hk, D, D ** -0.5 if scale is None and D else float(scale or 0),
+    a = _lib.isb_xattn_args(dev, _TYPES[t], B, Bk, Lq, Lk, Hq, Hk, D, D ** -0.5 if scale is None and D else float(scale or 0),
                             q.data_ptr(), k.data_ptr(), v.data_ptr(), qs, ks, vs)
     keep = [q, k, v]
     if kv_len is not None:
@@ -170,7 +165,7 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_len: O
     if _forward_ad._current_level >= 0:
         _tangents(q, k, v)
     a, keep = _xattn_args(q, k, v, kv_len, key_mask, scale)
-    if _xattn_empty(a):
+    if not (q.numel() and k.numel()) and _xattn_empty(a):
         return q.new_zeros(q.shape), q.new_full((a.B, a.Hq, a.Lq), -math.inf, dtype=torch.float32)
     B, Lq, Hq, _ = shape = q.shape
     out = q.new_empty(shape)
@@ -193,11 +188,11 @@ def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tenso
     if _forward_ad._current_level >= 0:
         _tangents(dout, q, k, v, out, lse)
     a, keep = _xattn_args(q, k, v, kv_len, key_mask, scale)
-    dev, t = q.device, q.dtype
+    dev, t = q.get_device(), q.dtype
     _tensor("dout", dout, t, dev, q.shape)
     _tensor("out", out, t, dev, q.shape)
     _tensor("lse", lse, torch.float32, dev, (q.shape[0], q.shape[2], q.shape[1]))
-    if _xattn_empty(a):
+    if not (q.numel() and k.numel()) and _xattn_empty(a):
         return q.new_zeros(q.shape), k.new_zeros(k.shape), v.new_zeros(v.shape)
     dout, a.dout_stride = _rows16(dout)
     out, lse = _flat16(out), lse.contiguous()
@@ -216,7 +211,7 @@ def cross_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tenso
 # ------------------------------------------------------------------------------------------------ gated feed-forward block
 def _ffn_args(x, w_gate, w_up, w_down, activation):
     _first("x", x, _HALF)
-    t, dev = x.dtype, x.device
+    t, dev = x.dtype, x.get_device()
     if not isinstance(w_gate, torch.Tensor) or w_gate.dim() != 2 or x.dim() < 1:
         _refuse("expected x [..,D] and w_gate [F,D]")
     F, D = shape = w_gate.shape
@@ -230,9 +225,9 @@ def _ffn_args(x, w_gate, w_up, w_down, activation):
     x2, xs = _rows2(x)
     wg, wu, wd = _flat16(w_gate), _flat16(w_up), _flat16(w_down)
     if x2.shape[0] == 0:                                     # no launch; what can be wrong with the arguments all the same is refused
-        one = _lib.isb_ffn_args(dev.index, _TYPES[t], 1, D, F, ACTIVATIONS[activation])
+        one = _lib.isb_ffn_args(dev, _TYPES[t], 1, D, F, ACTIVATIONS[activation])
         _workspace(_lib.lib().isb_ffn_workspace, "isb_ffn_workspace", one, 0)
-    a = _lib.isb_ffn_args(dev.index, _TYPES[t], x2.shape[0], D, F, ACTIVATIONS[activation], xs, 0, x2.data_ptr(), wg.data_ptr(), wu.data_ptr(),
+    a = _lib.isb_ffn_args(dev, _TYPES[t], x2.shape[0], D, F, ACTIVATIONS[activation], xs, 0, x2.data_ptr(), wg.data_ptr(), wu.data_ptr(),
                           wd.data_ptr())
     return a, [x2, wg, wu, wd]
 
@@ -256,7 +251,7 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     if _forward_ad._current_level >= 0:
         _tangents(x, w_gate, w_up, w_down, b_gate, b_up, b_down)
     a, keep = _ffn_args(x, w_gate, w_up, w_down, activation)
-    dev, t, M, D, F = x.device, x.dtype, a.M, a.D, a.F
+    dev, t, M, D, F = x.get_device(), x.dtype, a.M, a.D, a.F
     for n, b, size in (("b_gate", b_gate, F), ("b_up", b_up, F), ("b_down", b_down, D)):
         if b is not None:
             _tensor(n, b, t, dev, (size,))
@@ -287,7 +282,7 @@ def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, 
     if _forward_ad._current_level >= 0:
         _tangents(dy, x, w_gate, w_up, w_down)
     a, keep = _ffn_args(x, w_gate, w_up, w_down, activation)
-    dev, t, M, D, F = x.device, x.dtype, a.M, a.D, a.F
+    dev, t, M, D, F = x.get_device(), x.dtype, a.M, a.D, a.F
     _tensor("dy", dy, t, dev, x.shape)
     if not (isinstance(saved, tuple) and len(saved) == 3):
         _refuse("saved: expected what gated_ffn(save=True) returned")
@@ -322,14 +317,14 @@ def gated_ffn_backward(dy: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, 
 # ------------------------------------------------------------------------------------------------ norms around a block
 def _norm_args(x, y, gate, scale, post, post_weight, post_bias, pre, pre_weight, pre_bias, eps):
     _first("x", x, _TYPES)
-    t, dev = x.dtype, x.device
+    t, dev = x.dtype, x.get_device()
     if x.dim() != 3:
         _refuse(f"x: expected [B,L,D], got {tuple(x.shape)}")
     if post not in NORMS or pre not in NORMS:
         _refuse(f"norms {post!r}, {pre!r}: None, 'layer' or 'rms'")
     B, L, D = shape = x.shape
     x = x.contiguous()
-    keep, p, vec = [x], [_address(x)], (D,)
+    keep, p, vec = [x], [x.data_ptr()], (D,)
     for n, v, sh, dt in (("y", y, shape, t), ("gate", gate, (B, D), t), ("scale", scale, vec, torch.float32),
                          ("post_weight", post_weight, vec, torch.float32), ("post_bias", post_bias, vec, torch.float32),
                          ("pre_weight", pre_weight, vec, torch.float32), ("pre_bias", pre_bias, vec, torch.float32)):
@@ -339,10 +334,11 @@ def _norm_args(x, y, gate, scale, post, post_weight, post_bias, pre, pre_weight,
             _tensor(n, v, dt, dev, sh)
             v = v.contiguous()
             keep.append(v)
-            p.append(_address(v))
-    a = _lib.isb_norm_args(dev.index, _TYPES[t], B, L, D, NORMS[post], NORMS[pre], eps, *p)
+            p.append(v.data_ptr())
+    a = _lib.isb_norm_args(dev, _TYPES[t], B, L, D, NORMS[post], NORMS[pre], eps, *p)
     if B == 0 or L == 0:                                     # no launch; what can be wrong with the arguments all the same is refused
-        one = _lib.isb_norm_args(dev.index, _TYPES[t], 1, 1, D, NORMS[post], NORMS[pre], eps, *p)
+        p = [None if v is None else 16 for v in (x, y, gate, scale, post_weight, post_bias, pre_weight, pre_bias)]      # (never read)
+        one = _lib.isb_norm_args(dev, _TYPES[t], 1, 1, D, NORMS[post], NORMS[pre], eps, *p)
         _workspace(_lib.lib().isb_norm_workspace, "isb_norm_workspace", one)
     return a, keep
 
@@ -369,9 +365,10 @@ def block_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, gate: Optio
     if save:
         stats = x.new_empty((*x.shape[:2], 4), dtype=torch.float32)
         a.stats = stats.data_ptr()
-    rc = _lib.lib().isb_norm_forward(C.byref(a), _stream(a.device)) if a.B * a.L else 0
-    if rc:
-        _lib.check(rc, "isb_norm_forward")
+    if x.numel() or not x.shape[2]:
+        rc = _lib.lib().isb_norm_forward(C.byref(a), _stream(a.device))
+        if rc:
+            _lib.check(rc, "isb_norm_forward")
     return (r, z, stats) if save else (r, z)
 
 
@@ -385,7 +382,7 @@ def block_norm_backward(dr: Optional[torch.Tensor], dz: Optional[torch.Tensor], 
     if _forward_ad._current_level >= 0:
         _tangents(dr, dz, x, y, stats, gate, scale, post_weight, post_bias, pre_weight, pre_bias)
     a, keep = _norm_args(x, y, gate, scale, post, post_weight, post_bias, pre, pre_weight, pre_bias, eps)
-    dev, t = x.device, x.dtype
+    dev, t = x.get_device(), x.dtype
     if (dz is not None) != (pre is not None):
         _refuse("dz goes with a pre norm")
     if dr is None and dz is None:
@@ -409,7 +406,7 @@ def block_norm_backward(dr: Optional[torch.Tensor], dz: Optional[torch.Tensor], 
                  ("dpre_bias", pre_bias)):
         if v is not None:
             g[n] = v.new_empty(v.shape)
-    if a.B * a.L == 0:
+    if x.numel() == 0 and x.shape[2]:
         for v in g.values():
             v.zero_()
         return g
