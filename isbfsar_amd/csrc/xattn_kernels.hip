@@ -108,7 +108,8 @@ __device__ __forceinline__ uint4 pack8(const f32x16& x, int t) {
 }
 // What that rounds off, as a second operand. Where a sum has few terms (up to FEW_STATES states, up to 64 rows) the roundings of P and dS do not average
 // out: they scale whole rows of V, K, dout or Q, and the results are as far off as with roundings of their own, or further. There both operands
-// enter (hi + lo: 2^-16 or better), which costs a few products of a launch that waits for its loads.
+// enter (hi + lo: 2^-16 or better), which costs a few products of a launch that waits for its loads. An infinity of V or dout times a rest of 0 would be
+// a NaN: where one comes out (any_nan) the wave adds up once more without the rests.
 template <bool F16>
 __device__ __forceinline__ uint4 rest8(const f32x16& x, int t, const uint4& hi) {
     const uint32_t w[4] = {hi.x, hi.y, hi.z, hi.w};
@@ -119,6 +120,23 @@ __device__ __forceinline__ uint4 rest8(const f32x16& x, int t, const uint4& hi) 
         r[i] = T16<F16>::pack2(a - T16<F16>::lo(w[i]), b - T16<F16>::hi(w[i]));
     }
     return make_uint4(r[0], r[1], r[2], r[3]);
+}
+
+template <int NA>
+__device__ __forceinline__ bool any_nan(const f32x16 (&acc)[NA]) {
+    bool n = false;
+#pragma unroll
+    for (int d = 0; d < NA; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) n |= acc[d][i] != acc[d][i];
+    return __any(n);
+}
+template <int NA>
+__device__ __forceinline__ void clear(f32x16 (&acc)[NA]) {
+#pragma unroll
+    for (int d = 0; d < NA; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
 }
 
 // One block of NB x 32 states for 32 rows (a column of S^T each): scores, running maximum (m: less P_UP) and sum, O^T += V^T P^T.
@@ -259,10 +277,19 @@ __global__ __launch_bounds__(256, 2) void xattn_fwd_kernel(XattnArgs a) {
     }
     if (nt == 1 && len <= FEW_STATES) {
         wait_all_and_meet();
-        for (int b = 0; b < 2; ++b)
-            if (bits >> (32 * b) & 0xffffffffu)
-                attend<F16, DT, 1, true>(conv_lds_dyn + 32 * b * DT * 2, conv_lds_dyn + TB + 32 * b * DT * 2, qf, acc, m, l, a.c,
-                                         reinterpret_cast<const float*>(conv_lds_dyn + 2 * TB) + 32 * b, bits == ~0ull, lane);
+        const auto few = [&](auto rests) {
+            for (int b = 0; b < 2; ++b)
+                if (bits >> (32 * b) & 0xffffffffu)
+                    attend<F16, DT, 1, decltype(rests)::value>(conv_lds_dyn + 32 * b * DT * 2, conv_lds_dyn + TB + 32 * b * DT * 2, qf, acc, m, l, a.c,
+                                                               reinterpret_cast<const float*>(conv_lds_dyn + 2 * TB) + 32 * b, bits == ~0ull, lane);
+        };
+        few(std::true_type());
+        if (any_nan(acc)) {
+            clear(acc);
+            m = NEG_INF;
+            l = 0.f;
+            few(std::false_type());
+        }
         nt = 0;
     }
     for (int t = 0; t < nt; ++t) {
@@ -340,6 +367,12 @@ __global__ __launch_bounds__(TOKEN_WAVES * 64, TOKEN_WAVES / 4) void xattn_token
     if (len <= FEW_STATES && t < nt) {                                        // (at most one block per wave)
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         if (bits != 0) attend<F16, DT, 1, true>(own, own + TB, qf, acc, m, l, a.c, bias, bits == ~0u, lane);
+        if (any_nan(acc)) {
+            clear(acc);
+            m = NEG_INF;
+            l = 0.f;
+            attend<F16, DT, 1>(own, own + TB, qf, acc, m, l, a.c, bias, bits == ~0u, lane);
+        }
         t = nt;
     }
     for (; t < nt; t += NW) {
@@ -564,6 +597,7 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
     if (nt > 0) { fetch(0); put(0); }
     wait_all_and_meet();
     if (a.M <= RT && nt > 0) {                                                 // few rows: one tile, P and dS with their rests (rest8)
+        bool rests = true;
 #pragma unroll 1
         for (int rb = 0; rb < 2; ++rb) {
             const float* st = reinterpret_cast<const float*>(conv_lds_dyn + 2 * TB) + 32 * rb;
@@ -589,10 +623,19 @@ __global__ __launch_bounds__(256, DT == 64 ? 2 : 1) void xattn_dkv_kernel(XattnA
                 for (int d = 0; d < DT / 32; ++d) {
                     const uint4 o = frag_cols<DT, 4, 8>(conv_lds_dyn + TB, 32 * rb + 16 * u, 32 * d, lane), q = frag_cols<DT, 4, 8>(conv_lds_dyn, 32 * rb + 16 * u, 32 * d, lane);
                     dv[d] = T16<F16>::mfma32(o, w, dv[d]);
-                    dv[d] = T16<F16>::mfma32(o, wr, dv[d]);
                     dk[d] = T16<F16>::mfma32(q, x, dk[d]);
-                    dk[d] = T16<F16>::mfma32(q, xr, dk[d]);
+                    if (rests) {
+                        dv[d] = T16<F16>::mfma32(o, wr, dv[d]);
+                        dk[d] = T16<F16>::mfma32(q, xr, dk[d]);
+                    }
                 }
+            }
+            if (rb == 1 && rests && any_nan(dv)) {                             // both blocks again
+                clear(dv);
+                clear(dk);
+                sc = F16 ? 0.f : 1.0f;
+                rests = false;
+                rb = -1;
             }
         }
         nt = 0;

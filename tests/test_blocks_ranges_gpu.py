@@ -296,3 +296,18 @@ def test_xattn_few_states_or_rows(B, Bk, Lq, Lk, Hq, Hk, D, lens, t):
             want = P.T @ dO
             held(dv[b, :n, h], want, u * want.abs() + ((P * (ep + rest)).T @ dO.abs() + (M + 16) * E * (P.T @ dO.abs())) * (1 + u) + 2.0 ** -25
                  + (2.0 ** -36 if t == FP16 else 0) * dO.abs().sum(0), "dv")
+
+
+@pytest.mark.parametrize("t", [BF16, FP16])
+@pytest.mark.parametrize("Lq,Lk", [(1, 5), (3, 40), (40, 60), (130, 20), (70, 300)])
+def test_xattn_an_infinity_stays_one(Lq, Lk, t):
+    """an infinite value of a valid state makes that column of every row's result infinite (not NaN), an infinite gradient that column of dv"""
+    q, k, v, dout = (normal(gen(9 + i), 1, n, 1, 64, type=t) for i, n in enumerate((Lq, Lk, Lk, Lq)))
+    inf = v.clone()
+    inf[0, Lk // 2, 0, 3], inf[0, Lk - 1, 0, 9] = math.inf, -math.inf
+    out, _ = blocks().cross_attention(q, k, inf)
+    assert bool((out[..., 3] == math.inf).all()) and bool((out[..., 9] == -math.inf).all()) and int((~out.isfinite()).sum()) == 2 * Lq
+    out, lse = blocks().cross_attention(q, k, v)
+    dout[0, Lq // 2, 0, 7] = math.inf
+    dv = blocks().cross_attention_backward(dout, q, k, v, out, lse)[2]
+    assert bool((dv[..., 7] == math.inf).all()) and int((~dv.isfinite()).sum()) == Lk
