@@ -517,7 +517,7 @@ int isb_ffn_backward(const isb_ffn_args* a, void* d_workspace, size_t bytes, voi
 /* The norms around a block with its gate and residual scale: r = x + scale * gate * N_post(y), z = N_pre(r).
  *   x, y, r, z [B,L,D] contiguous, f32, fp16 or bf16; gate [B,D] of the same type or NULL (1); scale [D] f32 or NULL (1).
  *   post, pre: ISB_NORM_*; weights and biases [D] f32 or NULL (1 and 0; a bias or weight needs its norm, an RMS norm takes no bias).
- *   y NULL: r is x (not written), only z = N_pre(x). pre NONE: z is not written. D at most 8192.
+ *   y NULL: r is x (not written), only z = N_pre(x). pre NONE: z is not written. D at most 8192; B at most 65535 with a gate.
  *   z is the norm of r before r is rounded. stats [B,L,4] f32 or NULL: what the backward pass needs of the row's statistics.
  * Backward: dr (NULL: zeros) and dz (with a pre norm), x, y, stats -> dx, dy (unless y is NULL), dgate (gate's type, if gate),
  * dscale, dpost_weight, dpost_bias, dpre_weight, dpre_bias f32 (each may be NULL). */

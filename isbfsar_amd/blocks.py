@@ -2,7 +2,7 @@
 
 They stand beside the tuple attention, the MLPs and the LayerNorm that live inside :class:`isbfsar_amd.engine.ArEngine` and work on
 what it hands out: the embeddings of query windows ([B, L, 256], ``infer(want_embed=True)``) and the frames of a support set
-(``support_features()``)::
+(``support_features()``), both f32: :func:`cross_attention` and :func:`gated_ffn` take them as fp16 or bf16 (``.half()``)::
 
     n = block_norm(x, pre="layer", pre_weight=w, pre_bias=b)                      # norm before the block
     out, lse = cross_attention(q, k, v, kv_len=lengths)                           # windows against the support set's frames
@@ -247,7 +247,8 @@ def gated_ffn(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
 
     x [..,D] (rows a constant stride apart), w_gate and w_up [F,D], w_down [D,F] (torch Linear layout), biases or None; D and F multiples
     of 8; activation "silu", "gelu" (exact), "relu" or "sigmoid". Returns y, or (y, saved) with save=True: what
-    :func:`gated_ffn_backward` needs (both pre-activations in f32, the hidden rows in x's type)."""
+    :func:`gated_ffn_backward` needs (both pre-activations in f32, the hidden rows in x's type; fp16: in a form of the library's own, which the backward
+    call may write anew)."""
     if _forward_ad._current_level >= 0:
         _tangents(x, w_gate, w_up, w_down, b_gate, b_up, b_down)
     a, keep = _ffn_args(x, w_gate, w_up, w_down, activation)
@@ -349,7 +350,7 @@ def block_norm(x: torch.Tensor, y: Optional[torch.Tensor] = None, *, gate: Optio
                eps: float = 1e-5, save: bool = False):
     """r = x + scale * gate * N_post(y) and z = N_pre(r) in one pass; (r, z), or (r, z, stats) with save=True.
 
-    x, y [B,L,D] f32, fp16 or bf16, D up to 8192 (any); gate [B,D] of x's type, scale, weights and biases f32 [D], or None; post / pre:
+    x, y [B,L,D] f32, fp16 or bf16, D up to 8192 (any); gate [B,D] of x's type (B up to 65535), scale, weights and biases f32 [D], or None; post / pre:
     None, "layer" or "rms" (no bias). y None: the norm before the first block, r is x itself. pre None: z is None. z is the norm of r
     before r is rounded; stats f32 [B,L,4] are for :func:`block_norm_backward`."""
     if _forward_ad._current_level >= 0:

@@ -176,10 +176,9 @@ __device__ __forceinline__ float half_max(float mx) {
 template <int N>
 __device__ __forceinline__ void store_exps(int8_t* to, int e) {
     const uint32_t w = 0x01010101u * (uint8_t)e;
+    static_assert(N == 1 || N == 4, "a wave's rows of a block: 8 or 32");
     if constexpr (N == 1) *to = (int8_t)w;
-    else if constexpr (N == 2) *reinterpret_cast<uint16_t*>(to) = (uint16_t)w;
-    else if constexpr (N == 4) *reinterpret_cast<uint32_t*>(to) = w;
-    else *reinterpret_cast<uint2*>(to) = make_uint2(w, w);
+    else *reinterpret_cast<uint32_t*>(to) = w;
 }
 __device__ __forceinline__ float stored_by(int e) { return e == 0 || e == EXP_NONE ? 1.0f : __builtin_ldexpf(1.0f, -e); }
 
@@ -1120,7 +1119,10 @@ int add_up(Sums& s, hipStream_t st) {
     s = Sums{};
     return ISB_OK;
 }
-size_t part_bytes(int la, int M, int N, int kts) { return (plan_out(la, M, N, kts).bytes + 255) / 256 * 256; }
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+size_t part_bytes(int la, int M, int N, int kts) { return up256(plan_out(la, M, N, kts).bytes); }
+// the exponents of [rows, cols] values (Powers)
+size_t exp_bytes(int rows, int cols) { return up256((size_t)cdiv(cols, 32) * cdiv(rows, 32) * 4); }
 
 template <bool F16, int MT, bool GATE>
 int token(const MmArgs& p, float* h, hipStream_t st) {
@@ -1134,10 +1136,6 @@ int token(const MmArgs& p, float* h, hipStream_t st) {
 // Where the partial sums of the backward pass's three products lie. Together, one launch adds them all up (us of the pass, a launch each and
 // together: 600 rows, 512 x 2048: 74, 63; 1030, 640 x 2560: 91, 84) -- as long as they and what else passes between the launches (14 bytes for
 // each value of h) stay well inside the 256 MB last-level cache: at 4111 rows, 237 MB, dh takes 52 for 44 us and the shared launch gains 3.
-// bytes of the exponents of [rows, cols] values (Powers)
-size_t exp_bytes(int rows, int cols) { return ((size_t)cdiv(cols, 32) * cdiv(rows, 32) * 4 + 255) / 256 * 256; }
-size_t up256(size_t n) { return (n + 255) / 256 * 256; }
-
 struct BwdParts {
     size_t at[3] = {}, bytes = 0;
     bool together = false;

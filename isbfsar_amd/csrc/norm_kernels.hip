@@ -1,7 +1,8 @@
 // The norms around a block in one pass: r = x + scale o gate o N_post(y) (what leaves the block before) and z = N_pre(r) (what enters the
 // next one), with the gradients of everything. N: LayerNorm, RMS norm or none. Both are bound by HBM: every row is read once, kept in
 // registers and written once; r is normalised before it is rounded. 32704 rows of 1280, bf16: forward 81 us (4.1 TB/s), backward 120 us
-// (4.2 TB/s), the two small launches behind it 10.
+// (4.2 TB/s), the two small launches behind it 11. Widths that are no multiple of 8 are read a value at a time: 1279 instead of 1280 forward 242,
+// backward 411 us (f32 390, 684).
 //
 // A workgroup of ceil(D / 512) waves owns a row, eight neighbouring columns per lane. Backward, it walks the rows of one sample with four
 // column sums in registers -- dR, dR o y^, dz, dz o r^ -- from which all parameter gradients follow, because gate and scale do not vary

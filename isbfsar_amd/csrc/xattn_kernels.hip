@@ -534,7 +534,7 @@ __device__ __forceinline__ void scale_ds(f32x16& ds, f32x16 (&acc)[NA], float& s
     }
 }
 // dK, dV: S = Q K^T with the rows in the accumulator's rows and a state per lane; P and dS are then operands over the rows. 2 x 16 heads, 4096 rows
-// and states: 856 us 128 wide (642 TFLOP/s: dK, dV, K and V of a wave's 32 states need more than 256 registers, so a SIMD has one wave, and
+// and states: 743 us 128 wide (740 TFLOP/s: dK, dV, K and V of a wave's 32 states need more than 256 registers, so a SIMD has one wave, and
 // its products wait for LDS), 334 us 64 wide (823, two waves).
 constexpr int DKV_ROWS = 64;                                        // rows per barrier
 template <bool F16, int DT>

@@ -311,3 +311,81 @@ def test_xattn_an_infinity_stays_one(Lq, Lk, t):
     dout[0, Lq // 2, 0, 7] = math.inf
     dv = blocks().cross_attention_backward(dout, q, k, v, out, lse)[2]
     assert bool((dv[..., 7] == math.inf).all()) and int((~dv.isfinite()).sum()) == Lk
+
+
+# ------------------------------------------------------------------------------------------------ the powers of two in use
+def odd_ffn(M, D, F, seed=0):
+    """a block whose h, dG and dU need powers of two of every kind"""
+    g = gen(seed + M)
+    x = (normal(g, M, D) * 2.0 ** torch.randint(-9, 9, ((M + 8) // 9, 1), generator=g, device="cuda").repeat_interleave(9, 0)[:M]).to(FP16)
+    dy = (normal(g, M, D) * 2.0 ** torch.randint(-20, 0, ((M + 8) // 9, 1), generator=g, device="cuda").repeat_interleave(9, 0)[:M]).to(FP16)
+    w = [normal(g, F, D, type=FP16, std=4 * D ** -0.5) for _ in range(2)] + [normal(g, D, F, type=FP16, std=2.0 ** -8 * F ** -0.5)]
+    return x, w, dy
+
+
+@pytest.mark.parametrize("M,D,F", [(3, 64, 136), (45, 72, 264), (700, 136, 520)])
+def test_ffn_backward_again_in_a_graph_and_on_two_streams(M, D, F):
+    """the backward call may write the saved hidden values anew: a second call on them, replays and two calls at once give the same bits"""
+    x, w, dy = odd_ffn(M, D, F)
+
+    def forward():
+        return blocks().gated_ffn(x, *w, activation="gelu", save=True)
+
+    def backward(saved):
+        return list(blocks().gated_ffn_backward(dy, x, *w, saved, bias=True, activation="gelu").values())
+    y, saved = forward()
+    want = backward(saved)
+    assert all(torch.equal(a, b) for a, b in zip(backward(saved), want))
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [None, None]
+    for _ in range(3):
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                got[i] = backward(saved)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y2, s2 = forward()
+        res = backward(s2)
+    for i in range(3):
+        x2, _, dy2 = odd_ffn(M, D, F, seed=i)
+        x.copy_(x2)
+        dy.copy_(dy2)
+        graph.replay()
+        torch.cuda.synchronize()
+        y, saved = forward()
+        assert torch.equal(y, y2) and all(torch.equal(a, b) for a, b in zip(res, backward(saved)))
+
+
+@pytest.mark.parametrize("M,D,F", [(3, 72, 136), (45, 72, 136), (300, 136, 264)])
+def test_ffn_with_powers_writes_nothing_past_its_results(M, D, F):
+    import ctypes as C
+
+    from isbfsar_amd import _lib
+    lib = _lib.lib()
+    x, w, dy = odd_ffn(M, D, F)
+
+    def around(n, t=FP16):
+        b = torch.full((n + 1024,), 7.0, dtype=t, device="cuda")
+        return b, b.data_ptr() + 512 * b.element_size(), n
+    o = {"y": around(M * D), "pre_gate": around(M * F, F32), "pre_up": around(M * F, F32), "hidden": around(M * F), "dx": around(M * D),
+         "dw_gate_up": around(2 * F * D), "dw_down": around(D * F), "db_gate": around(F), "db_up": around(F), "db_down": around(D)}
+    args = _lib.isb_ffn_args(0, 1, M, D, F, 0, D, D, x.data_ptr(), *(v.data_ptr() for v in w))
+    args.dy = dy.data_ptr()
+    for name, v in o.items():
+        setattr(args, name, v[1])
+    st = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    for back, call in ((0, lib.isb_ffn_forward), (1, lib.isb_ffn_backward)):
+        n = C.c_size_t()
+        _lib.check(lib.isb_ffn_workspace(C.byref(args), back, C.byref(n)), "workspace")
+        ws = torch.full((n.value + 4096,), 0x55, dtype=torch.uint8, device="cuda")      # (also what the tables hold before they are written)
+        _lib.check(call(C.byref(args), ws.data_ptr(), n.value, st), "call")
+        assert bool((ws[n.value:] == 0x55).all())
+    for name, (b, _, n) in o.items():
+        assert bool((b[:512] == 7).all()) and bool((b[512 + n:] == 7).all()), name
+    y, saved = blocks().gated_ffn(x, *w, save=True)
+    d = blocks().gated_ffn_backward(dy, x, *w, saved, bias=True)
+    assert torch.equal(o["y"][0][512:512 + M * D].view(M, D), y)
+    for name, got in (("dx", d["dx"]), ("dw_down", d["dw_down"]), ("db_gate", d["db_gate"])):
+        assert torch.equal(o[name][0][512:512 + got.numel()].view(got.shape), got), name
