@@ -106,7 +106,7 @@ __device__ __forceinline__ uint4 pack8(const f32x16& x, int t) {
     return t == 0 ? make_uint4(T16<F16>::pack2(x[0], x[1]), T16<F16>::pack2(x[2], x[3]), T16<F16>::pack2(x[4], x[5]), T16<F16>::pack2(x[6], x[7]))
                   : make_uint4(T16<F16>::pack2(x[8], x[9]), T16<F16>::pack2(x[10], x[11]), T16<F16>::pack2(x[12], x[13]), T16<F16>::pack2(x[14], x[15]));
 }
-// What that rounds off, as a second operand. Where a sum has few terms (up to FEW_STATES states, up to 64 rows) the roundings of P and dS do not average
+// What that rounds off, as a second operand. Where a sum has few terms (up to FEW_STATES states; up to 32 rows for dQ, 64 for dK, dV) the roundings of P and dS do not average
 // out: they scale whole rows of V, K, dout or Q, and the results are as far off as with roundings of their own, or further. There both operands
 // enter (hi + lo: 2^-16 or better), which costs a few products of a launch that waits for its loads. An infinity of V or dout times a rest of 0 would be
 // a NaN: where one comes out (any_nan) the wave adds up once more without the rests.
@@ -820,7 +820,9 @@ __device__ __forceinline__ void add_dq(const unsigned char* ktile, const unsigne
 
 // dQ: as the forward kernel; dS^T has a row per lane, dQ^T += K^T dS^T reads the K tile a second time, transposed. 2 x 16 heads, 4096 rows and
 // states: 386 us 128 wide (1068 TFLOP/s), 259 us 64 wide (797).
-template <bool F16, int DT>
+// ROWS: REST for up to 32 rows of a group, whose products wait for the states anyway (single rows' dq was up to 1.56 times as far off as with f32
+// throughout, and few enough not to average out).
+template <bool F16, int DT, int ROWS>
 __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
     const int item = xcd_item(blockIdx.x, a.n_items);
     if (item >= a.n_items) return;
@@ -887,7 +889,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
         if (bits != 0) {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
-                add_dq<F16, DT>(ktile + 32 * b * DT * 2, vtile + 32 * b * DT * 2, g, acc, sc, a.c, bias + 32 * b, bits == ~0ull, lane);
+                add_dq<F16, DT, ROWS>(ktile + 32 * b * DT * 2, vtile + 32 * b * DT * 2, g, acc, sc, a.c, bias + 32 * b, bits == ~0ull, lane);
         }
         bits = next;
     }
@@ -906,7 +908,7 @@ __global__ __launch_bounds__(256, 2) void xattn_dq_kernel(XattnArgs a) {
 }
 
 // dQ in tiles of 32 rows, as the token kernel: eight waves walk their own blocks of 32 states, their sums meet in LDS and are added in wave order
-template <bool F16, int DT>
+template <bool F16, int DT, int ROWS>
 __global__ __launch_bounds__(TOKEN_WAVES * 64, TOKEN_WAVES / 4) void xattn_dq_few_kernel(XattnArgs a) {
     constexpr int NW = TOKEN_WAVES;
     const int item = xcd_item(blockIdx.x, a.n_items);
@@ -960,7 +962,7 @@ __global__ __launch_bounds__(TOKEN_WAVES * 64, TOKEN_WAVES / 4) void xattn_dq_fe
     }
     for (; t < nt; t += NW) {
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        if (bits != 0) add_dq<F16, DT>(own, own + TB, g, acc, sc, a.c, bias, bits == ~0u, lane);
+        if (bits != 0) add_dq<F16, DT, ROWS>(own, own + TB, g, acc, sc, a.c, bias, bits == ~0u, lane);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                    // the block is read before its place is requested again
         if (t + NW < nt) request(t + NW);
     }
@@ -1125,6 +1127,11 @@ int fwd(XattnArgs a, float* ws, hipStream_t st) {
     return ISB_OK;
 }
 
+template <bool F16, int DT, int ROWS>
+int run_dq(const XattnArgs& a, unsigned grid, hipStream_t st) {
+    if (few_dq(a)) return launch<xattn_dq_few_kernel<F16, DT, ROWS>>("xattn_dq_few", grid, TOKEN_WAVES * 64, TOKEN_WAVES * (2 * 32 * DT * 2 + 1024), a, st);
+    return launch<xattn_dq_kernel<F16, DT, ROWS>>("xattn_dq", grid, 256, 2 * (2 * KT * DT * 2 + KT * 4), a, st);
+}
 template <bool F16, int DT>
 int bwd(XattnArgs a, float* ws, hipStream_t st) {
     const int64_t rows = (int64_t)a.Bk * a.Hk * a.M, states = (int64_t)a.Bk * a.Hk * a.Lk;
@@ -1138,8 +1145,7 @@ int bwd(XattnArgs a, float* ws, hipStream_t st) {
     float* pv = pk + (int64_t)k.splits * states * DT;
     unsigned grid = items(a, q);
     a.part = pq;
-    if (few_dq(a)) ISB_TRY((launch<xattn_dq_few_kernel<F16, DT>>("xattn_dq_few", grid, TOKEN_WAVES * 64, TOKEN_WAVES * (2 * 32 * DT * 2 + 1024), a, st)));
-    else ISB_TRY((launch<xattn_dq_kernel<F16, DT>>("xattn_dq", grid, 256, 2 * (2 * KT * DT * 2 + KT * 4), a, st)));
+    ISB_TRY((a.M <= 32 ? run_dq<F16, DT, REST>(a, grid, st) : run_dq<F16, DT, MANY>(a, grid, st)));
     grid = items(a, k);
     a.part = pk;
     a.part2 = pv;

@@ -299,6 +299,34 @@ def test_xattn_few_states_or_rows(B, Bk, Lq, Lk, Hq, Hk, D, lens, t):
 
 
 @pytest.mark.parametrize("t", [BF16, FP16])
+@pytest.mark.parametrize("B,Lq,Lk,Hq,Hk,D", [(1, 1, 70, 1, 1, 64), (2, 1, 300, 4, 2, 128), (5, 3, 150, 8, 2, 72), (70, 4, 200, 4, 1, 64), (1, 32, 400, 1, 1, 64)])
+def test_xattn_few_rows_of_dq(B, Lq, Lk, Hq, Hk, D, t):
+    """up to 32 rows of a group: dS enters whole (two operands), whatever the states. delta is rowsum(dout o out) of the out that is handed in: with
+    that one in the formula, what is left is one rounding u of the result and f32's part (ep as in blocks_ref)"""
+    g = gen(Lk)
+    q, dout = normal(g, B, Lq, Hq, D, type=t), normal(g, B, Lq, Hq, D, type=t)
+    k, v = normal(g, B, Lk, Hk, D, type=t), normal(g, B, Lk, Hk, D, type=t)
+    out, lse = blocks().cross_attention(q, k, v)
+    dq = blocks().cross_attention_backward(dout, q, k, v, out, lse)[0]
+    u, G, scale = ref.half_step(t), Hq // Hk, 1 / math.sqrt(D)
+    rows = lambda x: x.double().unflatten(2, (Hk, G)).permute(0, 2, 1, 3, 4).reshape(B, Hk, Lq * G, D)     # noqa: E731
+    Q, dO, o, got = (rows(x) for x in (q, dout, out, dq))
+    K, V = (x.double().permute(0, 2, 1, 3).contiguous() for x in (k, v))
+    T = lambda x: x.transpose(-1, -2).contiguous()     # noqa: E731
+    s = Q @ T(K) * scale
+    P = torch.softmax(s, -1)
+    es = ((Q.abs() @ T(K.abs())) * scale * (D + 4) * E + s.abs() * 4 * E).amax(-1, keepdim=True)
+    ep = 2 * es + 8 * E + (Lk + 64) * E
+    abs_dP = dO.abs() @ T(V.abs())
+    dS = P * (dO @ T(V) - (dO * o).sum(-1, keepdim=True))
+    edS = dS.abs() * (ep + u * u + 2 * E) + P * ((D + 16) * E * (abs_dP + (dO * o).abs().sum(-1, keepdim=True))) * (1 + u)
+    if t == FP16:
+        edS = edS + 2.0 ** -34 * dS.abs().amax(-1, keepdim=True)
+    want = dS @ K * scale
+    held(got, want, u * want.abs() + scale * (edS @ K.abs() + (Lk + 64) * E * (dS.abs() @ K.abs())) * (1 + u) + 2.0 ** -25, "dq")
+
+
+@pytest.mark.parametrize("t", [BF16, FP16])
 @pytest.mark.parametrize("Lq,Lk", [(1, 5), (3, 40), (40, 60), (130, 20), (70, 300)])
 def test_xattn_an_infinity_stays_one(Lq, Lk, t):
     """an infinite value of a valid state makes that column of every row's result infinite (not NaN), an infinite gradient that column of dv"""
